@@ -7,8 +7,11 @@
 // Tensors are checked, made contiguous, and every launch goes to the caller's
 // current HIP stream; scratch comes from torch's caching allocator.
 #include <c10/hip/HIPStream.h>
+#include <ATen/MemoryOverlap.h>
 #include <torch/extension.h>
 
+#include <limits>
+#include <utility>
 #include <vector>
 
 #include "../../include/genie_tk.h"
@@ -579,6 +582,221 @@ at::Tensor tri_attn_forward(const at::Tensor& x, const c10::optional<at::Tensor>
   return out;
 }
 
+// ---------------------------------------------------------------------------
+// LayerNorm as training uses it
+// ---------------------------------------------------------------------------
+// x as rows of its last dimension, one stride apart and contiguous inside: x
+// itself where its strides allow it, else a contiguous copy.
+at::Tensor as_rows(const at::Tensor& x, int64_t* stride) {
+  const int64_t d = x.size(-1);
+  *stride = d;
+  if (x.is_contiguous()) return x;
+  bool ok = d == 1 || x.stride(-1) == 1;
+  int64_t step = -1, expect = -1;  // of the row index, from the innermost leading dimension outwards
+  for (int64_t k = x.dim() - 2; ok && k >= 0; --k) {
+    if (x.size(k) == 1) continue;
+    if (step < 0)
+      step = x.stride(k);
+    else
+      ok = x.stride(k) == expect;
+    expect = x.stride(k) * x.size(k);
+  }
+  if (!ok || x.numel() == 0) return x.contiguous();
+  if (step >= 0) *stride = step;
+  return x;
+}
+
+void check_ln(const at::Tensor& x, const c10::optional<at::Tensor>& p, const char* what) {
+  if (!p.has_value()) return;
+  check_on(*p, x, what);
+  TORCH_CHECK(p->dim() == 1 && p->size(0) == x.size(-1), what, " must be [", x.size(-1), "]");
+  gtk_dtype_of(*p, what);
+}
+
+at::Tensor layer_norm_forward(const at::Tensor& x, const c10::optional<at::Tensor>& weight,
+                              const c10::optional<at::Tensor>& bias, double eps) {
+  check_gpu(x, "x");
+  TORCH_CHECK(x.dim() >= 1, "x must have at least one dimension");
+  check_ln(x, weight, "weight");
+  check_ln(x, bias, "bias");
+  const at::DeviceGuard guard(x.device());
+  const int dt = gtk_dtype_of(x, "x");
+  const int64_t d = x.size(-1);
+  int64_t stride;
+  auto xc = as_rows(x, &stride);
+  // one type for both parameters
+  const bool mixed = weight.has_value() && bias.has_value() && weight->scalar_type() != bias->scalar_type();
+  at::Tensor w, b;
+  if (weight.has_value()) w = mixed ? f32c(*weight) : weight->contiguous();
+  if (bias.has_value()) b = mixed ? f32c(*bias) : bias->contiguous();
+  const int pdt = w.defined() ? gtk_dtype_of(w, "weight") : b.defined() ? gtk_dtype_of(b, "bias") : GTK_F32;
+  auto y = at::empty(x.sizes(), x.options());
+  check_rc(gtk_layer_norm_forward(xc.data_ptr(), stride, y.data_ptr(), ptr_or_null(w), ptr_or_null(b), pdt,
+                                  d ? x.numel() / d : 0, d, (float)eps, dt, cur_stream(x)));
+  return y;
+}
+
+// Returns [dx, dweight, dbias], the ones not asked for as None; dweight and
+// dbias in the weight's type (fp32 without a weight).
+std::vector<c10::optional<at::Tensor>> layer_norm_backward(const at::Tensor& x, const at::Tensor& dy,
+                                                           const c10::optional<at::Tensor>& weight, double eps,
+                                                           bool need_x, bool need_weight, bool need_bias) {
+  check_gpu(x, "x");
+  TORCH_CHECK(x.dim() >= 1, "x must have at least one dimension");
+  check_on(dy, x, "dy");
+  check_ln(x, weight, "weight");
+  TORCH_CHECK(dy.sizes() == x.sizes() && dy.scalar_type() == x.scalar_type(),
+              "dy must match x in shape and dtype");
+  const at::DeviceGuard guard(x.device());
+  const int dt = gtk_dtype_of(x, "x");
+  const int64_t d = x.size(-1), rows = d ? x.numel() / d : 0;
+  int64_t xs, ds;
+  auto xc = as_rows(x, &xs), dyc = as_rows(dy, &ds);
+  at::Tensor w;
+  if (weight.has_value()) w = weight->contiguous();
+  const auto popts = w.defined() ? w.options() : x.options().dtype(at::kFloat);
+  std::vector<c10::optional<at::Tensor>> out(3);
+  if (need_x) out[0] = at::empty(x.sizes(), x.options());
+  if (need_weight) out[1] = at::empty({d}, popts);
+  if (need_bias) out[2] = at::empty({d}, popts);
+  auto ptr = [&](int k) { return out[k].has_value() ? out[k]->data_ptr() : nullptr; };
+  auto ws = workspace(x, gtk_layer_norm_backward_workspace_size(rows, d, dt));
+  check_rc(gtk_layer_norm_backward(xc.data_ptr(), xs, dyc.data_ptr(), ds, ptr_or_null(w),
+                                   w.defined() ? gtk_dtype_of(w, "weight") : GTK_F32, ptr(0), ptr(1), ptr(2), rows, d,
+                                   (float)eps, dt, ws.data_ptr(), ws.numel(), cur_stream(x)));
+  return out;
+}
+
+// ---------------------------------------------------------------------------
+// Global gradient norm and clipping
+// ---------------------------------------------------------------------------
+// A list of tensors as the C functions take it.
+struct TensorList {
+  std::vector<void*> data;
+  std::vector<int64_t> numel;
+  std::vector<int> dtype;
+  void add(const at::Tensor& t) {
+    data.push_back(t.data_ptr());
+    numel.push_back(t.numel());
+    dtype.push_back(gtk_dtype_of(t, "a gradient"));
+  }
+  gtk_tensor_list list() const {
+    return {(int64_t)data.size(), data.data(), numel.data(), dtype.data()};
+  }
+};
+
+void check_grads(const std::vector<at::Tensor>& ts, const at::Tensor& like) {
+  for (const auto& t : ts) {
+    TORCH_CHECK(t.defined() && t.layout() == at::kStrided, "genie_tk._C: a gradient is not a dense tensor");
+    check_on(t, like, "a gradient");
+  }
+}
+
+int norm_kind(double p) {
+  if (p == 2.0) return GTK_NORM_2;
+  if (p == 1.0) return GTK_NORM_1;
+  TORCH_CHECK(p == std::numeric_limits<double>::infinity(), "genie_tk._C: norm_type must be 1, 2 or inf, got ", p);
+  return GTK_NORM_INF;
+}
+
+// The order of a norm's values does not matter: a tensor that fills its memory
+// is taken as it lies, any other is copied.
+at::Tensor as_run(const at::Tensor& t) {
+  return t.is_contiguous() || t.is_non_overlapping_and_dense() ? t : t.contiguous();
+}
+
+at::Tensor grad_norm(const std::vector<at::Tensor>& ts, double p) {
+  TORCH_CHECK(!ts.empty(), "grad_norm expects at least one tensor");
+  check_gpu(ts[0], "gradients");
+  check_grads(ts, ts[0]);
+  const int kind = norm_kind(p);
+  const at::DeviceGuard guard(ts[0].device());
+  std::vector<at::Tensor> copies;  // alive until the launch is enqueued
+  TensorList l;
+  for (const auto& t : ts) {
+    auto r = as_run(t);
+    l.add(r);
+    if (!r.is_same(t)) copies.push_back(r);
+  }
+  const auto g = l.list();
+  auto norm = at::empty({}, ts[0].options().dtype(at::kFloat));
+  auto ws = workspace(ts[0], gtk_grad_norm_workspace_size(&g));
+  check_rc(gtk_grad_norm(&g, kind, norm.data_ptr<float>(), ws.data_ptr(), ws.numel(), cur_stream(ts[0])));
+  return norm;
+}
+
+// Clips ts into outs (in place without them).  norm: given, or undefined:
+// computed, and returned.
+at::Tensor grad_clip_impl(const std::vector<at::Tensor>& ts, const c10::optional<std::vector<at::Tensor>>& outs,
+                          double max_norm, double p, at::Tensor norm) {
+  TORCH_CHECK(!ts.empty(), "grad_clip expects at least one tensor");
+  check_gpu(ts[0], "gradients");
+  check_grads(ts, ts[0]);
+  if (outs.has_value()) {
+    TORCH_CHECK(outs->size() == ts.size(), "genie_tk._C: ", outs->size(), " outputs for ", ts.size(), " gradients");
+    check_grads(*outs, ts[0]);
+  }
+  const bool given = norm.defined();
+  const int kind = given ? GTK_NORM_2 : norm_kind(p);
+  const at::DeviceGuard guard(ts[0].device());
+  // Tensors that are no run of memory in the other's order are clipped on
+  // copies, which are copied back at the end.
+  std::vector<std::pair<at::Tensor, at::Tensor>> back;
+  std::vector<at::Tensor> copies;
+  TensorList l, lo;
+  for (size_t i = 0; i < ts.size(); ++i) {
+    const auto& t = ts[i];
+    const auto& o = outs.has_value() ? (*outs)[i] : t;
+    TORCH_CHECK(o.sizes() == t.sizes(), "genie_tk._C: output ", i, " has another shape");
+    if ((t.is_contiguous() && o.is_contiguous()) ||
+        (t.strides() == o.strides() && t.is_non_overlapping_and_dense())) {
+      l.add(t);
+      if (outs.has_value()) lo.add(o);
+      continue;
+    }
+    at::assert_no_internal_overlap(o);
+    for (const auto& b : back)
+      TORCH_CHECK(o.numel() == 0 || b.first.data_ptr() != o.data_ptr(),
+                  "genie_tk._C: a tensor that is written is given twice");
+    copies.push_back(t.contiguous());
+    l.add(copies.back());
+    if (outs.has_value()) {
+      back.emplace_back(o, at::empty(o.sizes(), o.options().memory_format(at::MemoryFormat::Contiguous)));
+      lo.add(back.back().second);
+    } else {
+      back.emplace_back(o, copies.back());
+    }
+  }
+  const auto g = l.list(), go = lo.list();
+  const gtk_tensor_list* out = outs.has_value() ? &go : nullptr;
+  void* st = cur_stream(ts[0]);
+  if (given) {
+    check_rc(gtk_grad_clip_with_norm(&g, out, max_norm, norm.data_ptr<float>(), st));
+  } else {
+    norm = at::empty({}, ts[0].options().dtype(at::kFloat));
+    auto ws = workspace(ts[0], gtk_grad_norm_workspace_size(&g));
+    check_rc(gtk_grad_clip(&g, out, kind, max_norm, norm.data_ptr<float>(), ws.data_ptr(), ws.numel(), st));
+  }
+  for (auto& b : back) b.first.copy_(b.second);
+  // written behind autograd's back
+  for (const auto& t : outs.has_value() ? *outs : ts)
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+  return norm;
+}
+
+at::Tensor grad_clip(const std::vector<at::Tensor>& ts, const c10::optional<std::vector<at::Tensor>>& outs,
+                     double max_norm, double p) {
+  return grad_clip_impl(ts, outs, max_norm, p, at::Tensor());
+}
+
+void grad_clip_with_norm(const std::vector<at::Tensor>& ts, const c10::optional<std::vector<at::Tensor>>& outs,
+                         double max_norm, const at::Tensor& norm) {
+  TORCH_CHECK(!ts.empty(), "grad_clip_with_norm expects at least one tensor");
+  check_on(norm, ts[0], "norm");
+  TORCH_CHECK(norm.numel() == 1 && norm.scalar_type() == at::kFloat, "norm must be one float32 value");
+  grad_clip_impl(ts, outs, max_norm, 2.0, norm);
+}
+
 py::dict timing_report() {
   std::vector<char> buf(1 << 16);
   check_rc(gtk_timing_report(buf.data(), buf.size()));
@@ -659,6 +877,19 @@ PYBIND11_MODULE(_C, m) {
         py::arg("mask"), py::arg("packed"), py::arg("c_in"), py::arg("c_h"), py::arg("no_heads"),
         py::arg("starting"), py::arg("residual") = false, py::arg("eps") = 1e-5,
         py::arg("chunk_rows") = 0, py::arg("inf") = 1e9);
+  m.def("layer_norm_forward", &layer_norm_forward,
+        "LayerNorm over the last dimension, optional affine in either parameter type", py::arg("x"),
+        py::arg("weight") = py::none(), py::arg("bias") = py::none(), py::arg("eps") = 1e-5);
+  m.def("layer_norm_backward", &layer_norm_backward,
+        "layer_norm_forward's backward: [dx, dweight, dbias], None where not needed", py::arg("x"), py::arg("dy"),
+        py::arg("weight") = py::none(), py::arg("eps") = 1e-5, py::arg("need_x") = true,
+        py::arg("need_weight") = true, py::arg("need_bias") = true);
+  m.def("grad_norm", &grad_norm, "Norm over every value of the tensors (fp32 scalar; norm_type 1, 2 or inf)",
+        py::arg("tensors"), py::arg("norm_type") = 2.0);
+  m.def("grad_clip", &grad_clip, "Clip the tensors by their global norm into outs (None: in place); the norm",
+        py::arg("tensors"), py::arg("outs"), py::arg("max_norm"), py::arg("norm_type") = 2.0);
+  m.def("grad_clip_with_norm", &grad_clip_with_norm, "grad_clip by a given norm (one float32 value on the GPU)",
+        py::arg("tensors"), py::arg("outs"), py::arg("max_norm"), py::arg("norm"));
   m.def("version", []() { return gtk_version(); });
   m.def("timing_enable", [](bool on) { check_rc(gtk_timing_enable(on ? 1 : 0)); },
         "Record HIP events around every kernel launch (per-kernel timing)", py::arg("on"));

@@ -1,0 +1,158 @@
+"""The global norm of a set of gradients, and clipping by it.
+
+What a training loop does between the backward pass and the optimizer, with
+the names and arithmetic of ``torch.nn.utils``: the reference has no training
+loop (its users take torch's).  Kernel path (bf16 or fp32 GPU tensors, norms of
+order 1, 2 and inf): ``genie_tk._C.grad_norm``, ``grad_clip`` and
+``grad_clip_with_norm``; the squares and sums are 64-bit there, the norm is an
+fp32 value on the GPU, and nothing waits for the host.  Other tensors and
+orders run the same formulas in PyTorch.  All tensors of a call are on one
+device.
+"""
+from __future__ import annotations
+
+import math
+from typing import Iterable, List, Optional, Sequence, Tuple, Union
+
+import torch
+from torch import Tensor
+
+from genie_tk import _dispatch, _ext
+
+_EPS = 1e-6  # torch.nn.utils' addend of the norm
+
+
+def _on_kernels(tensors: Sequence[Tensor], norm_type: float) -> bool:
+    if not tensors[0].is_cuda:
+        return False
+    if _ext.C is None or not torch.cuda.is_available():
+        _ext.missing("gradients")
+        return False
+    return norm_type in (1.0, 2.0, math.inf) and all(t.dtype in _dispatch.SUPPORTED_DTYPES for t in tensors)
+
+
+def _check(tensors: Sequence[Tensor], what: str) -> None:
+    device = tensors[0].device
+    for t in tensors:
+        if t.layout != torch.strided:
+            raise ValueError(f"{what}: sparse gradients are not supported")
+        if t.is_complex() or not t.is_floating_point():
+            raise ValueError(f"{what}: gradients must be real floating-point tensors, got {t.dtype}")
+        if t.device != device:
+            raise ValueError(f"{what}: gradients on {device} and {t.device}")
+
+
+def _check_max_norm(max_norm: float, what: str) -> float:
+    max_norm = float(max_norm)
+    if not max_norm >= 0.0:
+        raise ValueError(f"{what}: max_norm must be >= 0, got {max_norm}")
+    return max_norm
+
+
+def _norm_pytorch(tensors: Sequence[Tensor], p: float) -> Tensor:
+    wide = [t.detach().double().abs().flatten() for t in tensors if t.numel()]
+    if not wide:
+        return tensors[0].new_zeros((), dtype=torch.float32)
+    each = torch.stack([torch.linalg.vector_norm(w, p) for w in wide])
+    return torch.linalg.vector_norm(each, p).float()
+
+
+def _clip_pytorch(tensors: Sequence[Tensor], outs: Sequence[Tensor], max_norm: float, norm: Tensor) -> None:
+    coef = (max_norm / (norm.double() + _EPS)).clamp(max=1.0)
+    with torch.no_grad():
+        for t, o in zip(tensors, outs):
+            # the product in 32 bits at least, rounded once
+            wide = t.double() if t.dtype == torch.float64 else t.float()
+            o.copy_(wide * coef.to(wide.dtype))
+
+
+def grad_norm(tensors: Iterable[Tensor], norm_type: float = 2.0) -> Tensor:
+    """``(sum |g|^p)^(1/p)`` over every value of ``tensors``, ``p = norm_type``
+    (the largest |g| for ``inf``): an fp32 scalar on their device.  No tensors
+    give 0."""
+    tensors = list(tensors)
+    norm_type = float(norm_type)
+    if not tensors:
+        return torch.zeros(())
+    _check(tensors, "grad_norm")
+    if _on_kernels(tensors, norm_type):
+        return _ext.C.grad_norm(tensors, norm_type)
+    return _norm_pytorch(tensors, norm_type)
+
+
+def clip_grads(grads: Iterable[Tensor], max_norm: float, norm_type: float = 2.0,
+               out: Optional[Sequence[Tensor]] = None) -> Tuple[Tensor, List[Tensor]]:
+    """``(norm, clipped)``: every gradient times ``min(1, max_norm / (norm +
+    1e-6))``.  ``grads`` are left as they are; the products are rounded once into
+    ``out``, tensors of the same shapes in bf16 or fp32 (fp32 ones hold the
+    gradients of fp32 master weights), or into new ones like ``grads``."""
+    grads = list(grads)
+    norm_type, max_norm = float(norm_type), _check_max_norm(max_norm, "clip_grads")
+    if out is not None and len(out) != len(grads):
+        raise ValueError(f"clip_grads: {len(out)} outputs for {len(grads)} gradients")
+    if not grads:
+        return torch.zeros(()), []
+    outs = [torch.empty_like(g) for g in grads] if out is None else list(out)
+    _check(grads, "clip_grads")
+    _check(outs, "clip_grads")
+    for g, o in zip(grads, outs):
+        if g.shape != o.shape or g.device != o.device:
+            raise ValueError(f"clip_grads: an output is {tuple(o.shape)} on {o.device} for a gradient "
+                             f"{tuple(g.shape)} on {g.device}")
+    if _on_kernels(grads + outs, norm_type):
+        return _ext.C.grad_clip(grads, outs, max_norm, norm_type), outs
+    norm = _norm_pytorch(grads, norm_type)
+    _clip_pytorch(grads, outs, max_norm, norm)
+    return norm, outs
+
+
+def clip_grad_norm_(parameters: Union[Tensor, Iterable[Tensor]], max_norm: float, norm_type: float = 2.0,
+                    error_if_nonfinite: bool = False) -> Tensor:
+    """Clips the gradients of ``parameters`` in place by their global norm and
+    returns the norm (fp32, before the clipping), as
+    ``torch.nn.utils.clip_grad_norm_``.  Parameters without a gradient are
+    passed over.  ``error_if_nonfinite`` looks at the norm on the host first (it
+    waits for the GPU) and raises RuntimeError with the gradients untouched."""
+    max_norm, norm_type = _check_max_norm(max_norm, "clip_grad_norm_"), float(norm_type)
+    grads = _grads_of(parameters)
+    if not grads:
+        return torch.zeros(())
+    _check(grads, "clip_grad_norm_")
+    if error_if_nonfinite:
+        norm = grad_norm(grads, norm_type)
+        if not math.isfinite(float(norm)):
+            raise RuntimeError(f"clip_grad_norm_: the gradients' norm of order {norm_type} is {float(norm)}")
+        _clip_with_norm(grads, max_norm, norm)
+        return norm
+    if _on_kernels(grads, norm_type):
+        return _ext.C.grad_clip(grads, None, max_norm, norm_type)
+    norm = _norm_pytorch(grads, norm_type)
+    _clip_pytorch(grads, grads, max_norm, norm)
+    return norm
+
+
+def clip_grads_with_norm_(parameters: Union[Tensor, Iterable[Tensor]], max_norm: float,
+                          total_norm: Tensor) -> None:
+    """Clips the gradients of ``parameters`` in place by a given norm: one over
+    the shards of several processes, say, joined from their ``grad_norm``."""
+    max_norm = _check_max_norm(max_norm, "clip_grads_with_norm_")
+    grads = _grads_of(parameters)
+    if not grads:
+        return
+    _check(grads, "clip_grads_with_norm_")
+    if total_norm.numel() != 1:
+        raise ValueError("clip_grads_with_norm_: total_norm must be one value")
+    _clip_with_norm(grads, max_norm, total_norm.detach().to(device=grads[0].device, dtype=torch.float32))
+
+
+def _clip_with_norm(grads: Sequence[Tensor], max_norm: float, total_norm: Tensor) -> None:
+    if _on_kernels(grads, 2.0):
+        _ext.C.grad_clip_with_norm(grads, None, max_norm, total_norm)
+    else:
+        _clip_pytorch(grads, grads, max_norm, total_norm)
+
+
+def _grads_of(parameters: Union[Tensor, Iterable[Tensor]]) -> List[Tensor]:
+    if isinstance(parameters, Tensor):
+        parameters = (parameters,)
+    return [p.grad for p in parameters if p.grad is not None]

@@ -1,7 +1,10 @@
-"""Linear layer with AlphaFold-style initialisers and gated multi-head attention.
+"""Linear layer with AlphaFold-style initialisers, gated multi-head attention
+and LayerNorm.
 
 API and semantics of ``src/genie_tk/primitives.py`` in the reference:
 ``_init_weights`` (:17-40), ``Linear`` (:43-62), ``Attention`` (:65-178).
+``LayerNorm`` and ``layer_norm`` are additions: torch's LayerNorm with the
+forward and the backward pass on the HIP kernels.
 """
 from __future__ import annotations
 
@@ -10,7 +13,11 @@ from typing import List, Optional
 
 import torch
 import torch.nn as nn
+import torch.nn.functional as F
 from torch import Tensor
+from torch.autograd.function import once_differentiable
+
+from genie_tk import _dispatch, _ext
 
 
 def _init_weights(linear: nn.Linear, init: str = "default", std: float = 0.02) -> None:
@@ -128,3 +135,74 @@ class Attention(nn.Module):
         if self.gating:
             o = o * self.sigmoid(self.linear_g(q_x))
         return self.linear_o(o)
+
+
+class _LayerNormFunction(torch.autograd.Function):
+    """LayerNorm on the HIP kernels, forward and backward.  Only x and the
+    weight are saved: the backward computes the rows' statistics again."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps):
+        ctx.save_for_backward(x, weight)
+        ctx.eps = eps
+        ctx.bias_dtype = None if bias is None else bias.dtype
+        return _ext.require().layer_norm_forward(x, weight, bias, eps)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, weight = ctx.saved_tensors
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        if need_b and weight is not None and ctx.bias_dtype != weight.dtype:
+            # both in fp32, each rounded once to its own type
+            dx, dw, db = _ext.require().layer_norm_backward(x, dy, weight.float(), ctx.eps, need_x,
+                                                            need_w, need_b)
+            return dx, dw if dw is None else dw.to(weight.dtype), db.to(ctx.bias_dtype), None
+        dx, dw, db = _ext.require().layer_norm_backward(x, dy, weight, ctx.eps, need_x, need_w, need_b)
+        return dx, dw, db if db is None else db.to(ctx.bias_dtype), None
+
+
+def layer_norm(x: Tensor, weight: Optional[Tensor] = None, bias: Optional[Tensor] = None,
+               eps: float = 1e-5) -> Tensor:
+    """LayerNorm over the last dimension of ``x`` with optional ``weight`` and
+    ``bias`` ([D]), differentiable once.
+
+    Kernel path (bf16 or fp32 GPU tensor, parameters in bf16 or fp32, also
+    mixed): ``genie_tk._C.layer_norm_forward`` / ``layer_norm_backward``.  The
+    output and dL/dx have the type of ``x``, the parameters' gradients their
+    own; statistics and sums are fp32.  Rows that lie one stride apart (a slice
+    of wider rows, a repeated row) are read as they are.  Other tensors run
+    torch's LayerNorm."""
+    params = [p for p in (weight, bias) if p is not None]
+    if x.is_cuda:
+        if _ext.C is None or not torch.cuda.is_available():
+            _ext.missing("layer_norm")
+        elif (x.dim() >= 1 and x.shape[-1] >= 1 and x.dtype in _dispatch.SUPPORTED_DTYPES
+              and all(p.dtype in _dispatch.SUPPORTED_DTYPES for p in params)):
+            if torch.is_grad_enabled() and (x.requires_grad or any(p.requires_grad for p in params)):
+                return _LayerNormFunction.apply(x, weight, bias, eps)
+            return _ext.C.layer_norm_forward(x, weight, bias, eps)
+    if any(p.dtype != x.dtype for p in params):  # in fp32, rounded once
+        wide = [None if p is None else p.float() for p in (weight, bias)]
+        return F.layer_norm(x.float(), x.shape[-1:], *wide, eps).to(x.dtype)
+    return F.layer_norm(x, x.shape[-1:], weight, bias, eps)
+
+
+class LayerNorm(nn.LayerNorm):
+    """``nn.LayerNorm`` (same constructor arguments, parameters and state_dict)
+    on ``layer_norm``; ``use_fused_kernel=False`` selects torch's."""
+
+    def __init__(self, normalized_shape, eps: float = 1e-5, elementwise_affine: bool = True,
+                 bias: bool = True, device=None, dtype=None, use_fused_kernel: bool = True):
+        super().__init__(normalized_shape, eps, elementwise_affine, bias, device=device, dtype=dtype)
+        self._fused_requested = use_fused_kernel
+
+    def forward(self, x: Tensor) -> Tensor:
+        shape = self.normalized_shape
+        if not self._fused_requested or tuple(x.shape[-len(shape):]) != tuple(shape):
+            return super().forward(x)  # torch's, or its error for the shape
+        if len(shape) == 1:
+            return layer_norm(x, self.weight, self.bias, self.eps)
+        # several dimensions are one: each row is contiguous in the flat view
+        flat = [None if p is None else p.flatten() for p in (self.weight, self.bias)]
+        return layer_norm(x.flatten(-len(shape)), *flat, self.eps).reshape(x.shape)

@@ -380,6 +380,66 @@ int gtk_pair_transition_backward(const void* p, const void* dy, const gtk_pair_t
                                  size_t workspace_bytes, void* stream);
 
 /* ------------------------------------------------------------------------
+ * LayerNorm as training uses it (no counterpart in the reference, whose
+ * LayerNorm gradients are torch autograd's).
+ * y[r][c] = (x[r][c] - mean_r) / sqrt(var_r + eps) * weight[c] + bias[c], with
+ * the biased variance.  x: [rows][d] of `dtype`, rows x_stride elements apart
+ * (0 repeats one row) and contiguous inside; y: [rows][d], contiguous.  weight,
+ * bias: [d] of `param_dtype`, each may be NULL (1 and 0).  Any alignment that
+ * the element type allows; d in [1, 2^24].  y may not alias x.
+ * ------------------------------------------------------------------------ */
+int gtk_layer_norm_forward(const void* x, int64_t x_stride, void* y, const void* weight, const void* bias,
+                           int param_dtype, int64_t rows, int64_t d, float eps, int dtype, void* stream);
+
+/* Its backward pass: given dL/dy (dy: [rows][d] of `dtype`, rows dy_stride
+ * elements apart), writes dL/dx (dx: [rows][d] of `dtype`, contiguous), dL/dweight
+ * and dL/dbias ([d] of `param_dtype`; the sums over the rows are held in fp32 and
+ * rounded once).  A NULL gradient pointer skips that output.  weight may be
+ * NULL (1).  Mean and variance are computed again from x.  Gradients are
+ * written, not accumulated; over no rows dweight and dbias are zero.  Equal
+ * inputs give equal bits.  dx may not alias x or dy.  The workspace size
+ * query returns 0 for a shape or type that the call refuses. */
+size_t gtk_layer_norm_backward_workspace_size(int64_t rows, int64_t d, int dtype);
+int gtk_layer_norm_backward(const void* x, int64_t x_stride, const void* dy, int64_t dy_stride, const void* weight,
+                            int param_dtype, void* dx, void* dweight, void* dbias, int64_t rows, int64_t d, float eps,
+                            int dtype, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------
+ * The global norm of a set of gradients, and clipping by it (no counterpart
+ * in the reference, which leaves both to torch).
+ *   n = (sum |g|^p)^(1/p) over every value of every tensor: p = 2, 1, or the
+ *       largest |g| (GTK_NORM_INF); 0 for no values
+ *   k = min(1, max_norm / (n + 1e-6)),  out = k * g
+ * Squares and sums are held in 64 bits, n is rounded once to fp32.  An
+ * infinite n gives k = 0 (0 * inf is NaN), a NaN n gives NaN everywhere, as the
+ * arithmetic has it.  k = 1 leaves every value's bits.
+ * Tensors: `count` of them, each a run of numel[i] values of dtype[i] at
+ * data[i], at any alignment that the type allows; the arrays are host memory
+ * and are read before the call returns.  Equal inputs give equal bits.
+ * gtk_grad_clip writes to `out` (NULL: in place): the same sizes, in either
+ * type.  No tensor that is written may overlap another one, or itself be
+ * given twice; out->data[i] may be grads->data[i] with the same type.
+ * max_norm >= 0.  norm: one fp32 value on the device, written first.
+ * gtk_grad_clip_with_norm takes n from there instead (a norm over several
+ * processes, or one that the host has looked at).
+ * ------------------------------------------------------------------------ */
+enum gtk_norm_kind { GTK_NORM_2 = 0, GTK_NORM_1 = 1, GTK_NORM_INF = 2 };
+typedef struct gtk_tensor_list {
+  int64_t count;
+  void* const* data;
+  const int64_t* numel;
+  const int* dtype;
+} gtk_tensor_list;
+
+size_t gtk_grad_norm_workspace_size(const gtk_tensor_list* grads);
+int gtk_grad_norm(const gtk_tensor_list* grads, int kind, float* norm, void* workspace, size_t workspace_bytes,
+                  void* stream);
+int gtk_grad_clip(const gtk_tensor_list* grads, const gtk_tensor_list* out, int kind, double max_norm, float* norm,
+                  void* workspace, size_t workspace_bytes, void* stream);
+int gtk_grad_clip_with_norm(const gtk_tensor_list* grads, const gtk_tensor_list* out, double max_norm,
+                            const float* norm, void* stream);
+
+/* ------------------------------------------------------------------------
  * Per-kernel timing (instrumentation; no counterpart in the reference).
  * gtk_timing_enable(1) makes every subsequent launch record a HIP event
  * before and after each kernel on its stream; gtk_timing_report() waits for
