@@ -27,60 +27,415 @@ struct ParamVec {
   }
 };
 
-__device__ __forceinline__ float wave_sum(float v) {
+// ---------------------------------------------------------------------------
+// Rows in registers.  W waves share a row, or W = 1 and L <= 64 lanes of a wave
+// do; lane t of a row's L * W lanes holds vectors of VE values (16 bytes), NV of
+// them, vector j at column (j * L * W + t) * VE.  A width that is no multiple
+// of VE ends with a vector that is moved back to end at column D: its first
+// `skip` values belong to the vector before it and count for nothing in the
+// row's sums (both lanes compute and store the same values there).  Rows of
+// any alignment are read with 16-byte accesses, which gfx950 does at any
+// address of the element's alignment.  VE = 1 is for rows shorter than one
+// vector.
+// ---------------------------------------------------------------------------
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef u32x4 u32x4_any __attribute__((aligned(2)));
+
+template <typename T, int VE> struct Vec {
+  u32x4 raw;
+  __device__ __forceinline__ void load(const T* p) { raw = __builtin_nontemporal_load((const u32x4_any*)p); }
+  __device__ __forceinline__ void store(T* p) const { *(u32x4_any*)p = raw; }
+  __device__ __forceinline__ void get(float* f) const {
+    if constexpr (sizeof(T) == 2) {
 #pragma unroll
-  for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
+      for (int i = 0; i < 4; ++i) {
+        f[2 * i] = __uint_as_float(raw[i] << 16);
+        f[2 * i + 1] = __uint_as_float(raw[i] & 0xffff0000u);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) f[i] = __uint_as_float(raw[i]);
+    }
+  }
+  __device__ __forceinline__ void set(const float* f) {
+    if constexpr (sizeof(T) == 2) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) raw[i] = pack_bf16x2(f[2 * i], f[2 * i + 1]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) raw[i] = __float_as_uint(f[i]);
+    }
+  }
+};
+template <typename T> struct Vec<T, 1> {
+  T v;
+  __device__ __forceinline__ void load(const T* p) { v = *p; }
+  __device__ __forceinline__ void store(T* p) const { *p = v; }
+  __device__ __forceinline__ void get(float* f) const { f[0] = to_f32(v); }
+  __device__ __forceinline__ void set(const float* f) { v = cvt<T>(f[0]); }
+};
+
+template <int CTRL> __device__ __forceinline__ float dpp(float v) {
+  return __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(v), CTRL, 0xf, 0xf, true));
+}
+// Sum over groups of L neighbouring lanes, the same bits in each of them.
+template <int L> __device__ __forceinline__ float lane_sum(float v) {
+  if (L >= 2) v += dpp<0xB1>(v);    // lane ^ 1
+  if (L >= 4) v += dpp<0x4E>(v);    // lane ^ 2
+  if (L >= 8) v += dpp<0x141>(v);   // the other four of eight
+  if (L >= 16) v += dpp<0x140>(v);  // the other eight of sixteen
+  if (L >= 32) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  }
+  if (L >= 64) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  }
   return v;
 }
 
-// One wave per row, three sweeps.
-template <typename T>
-__global__ __launch_bounds__(256) void ln_forward_kernel(const T* __restrict__ x, int64_t xs, T* __restrict__ y,
-                                                         ParamVec w, ParamVec b, int64_t rows, int D, float eps) {
-  const int lane = threadIdx.x & 63;
-  for (int64_t r = (int64_t)blockIdx.x * 4 + wave_id(); r < rows; r += (int64_t)gridDim.x * 4) {
-    const T* xr = x + r * xs;
-    float s = 0.f, q = 0.f;
-    for (int c = lane; c < D; c += 64) s += to_f32(xr[c]);
-    const float mean = wave_sum(s) / (float)D;
-    for (int c = lane; c < D; c += 64) {
-      const float d = to_f32(xr[c]) - mean;
-      q += d * d;
+// The launch shape of one kernel: see above; BT threads a block, U rows a lane
+// group in flight, EXACT: D = L * W * NV * VE.
+template <typename T_, int VE_, int NV_, int L_, int W_, int BT_, int U_, bool EXACT_> struct Shape {
+  typedef T_ T;
+  static constexpr int VE = VE_, NV = NV_, L = L_, W = W_, BT = BT_, U = U_;
+  static constexpr bool EXACT = EXACT_;
+  static constexpr int GROUPS = BT / (L * W);  // rows a block has in hand, times U
+  static constexpr int ROWS = GROUPS * U;      // rows a block step
+  static_assert(W == 1 || L == 64, "a row over several waves takes whole waves");
+};
+
+template <typename S> struct Columns {
+  int c[S::NV], skip[S::NV];
+  __device__ __forceinline__ Columns(int t, int D) {
+#pragma unroll
+    for (int j = 0; j < S::NV; ++j) {
+      const int nominal = (j * S::L * S::W + t) * S::VE;
+      c[j] = S::EXACT || nominal + S::VE <= D ? nominal : D - S::VE;
+      skip[j] = S::EXACT || nominal < D ? nominal - c[j] : S::VE;  // VE: no column
     }
-    const float rstd = 1.0f / sqrtf(wave_sum(q) / (float)D + eps);
-    for (int c = lane; c < D; c += 64)
+  }
+};
+
+// Sums of K values a lane over the row's lanes; red: K * (waves of a block)
+// floats that no other call uses before the next barrier of this kernel.
+template <typename S, int K> __device__ __forceinline__ void row_sums(float (&v)[K], float* red) {
+#pragma unroll
+  for (int k = 0; k < K; ++k) v[k] = lane_sum<S::L>(v[k]);
+  if constexpr (S::W > 1) {
+    const int wave = wave_id(), first = wave / S::W * S::W;
+    if ((threadIdx.x & 63) == 0) {
+#pragma unroll
+      for (int k = 0; k < K; ++k) red[k * (S::BT / 64) + wave] = v[k];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      v[k] = 0.f;
+#pragma unroll
+      for (int w = 0; w < S::W; ++w) v[k] += red[k * (S::BT / 64) + first + w];
+    }
+  }
+}
+
+// N consecutive values of a parameter vector (the branches are uniform).
+template <int N> __device__ __forceinline__ void load_run(float* f, const ParamVec& p, int c) {
+  if constexpr (N == 1) {
+    f[0] = p.get(c, 0.f);
+  } else if (p.bf) {
+    uint32_t raw[N / 2];
+    __builtin_memcpy(raw, (const bf16*)p.p + c, sizeof(raw));
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) {
+      f[2 * i] = __uint_as_float(raw[i] << 16);
+      f[2 * i + 1] = __uint_as_float(raw[i] & 0xffff0000u);
+    }
+  } else {
+    __builtin_memcpy(f, (const float*)p.p + c, N * sizeof(float));
+  }
+}
+template <typename S> __device__ __forceinline__ void load_param(float* f, const ParamVec& p, const Columns<S>& C, float none) {
+  if (p.p) {
+#pragma unroll
+    for (int j = 0; j < S::NV; ++j) load_run<S::VE>(f + j * S::VE, p, C.c[j]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < S::NV * S::VE; ++i) f[i] = none;
+  }
+}
+
+template <typename S>
+__global__ __launch_bounds__(S::BT) void ln_forward_kernel(const typename S::T* __restrict__ x, int64_t xs,
+                                                           typename S::T* __restrict__ y, ParamVec w, ParamVec b,
+                                                           int64_t rows, int D, float eps) {
+  typedef typename S::T T;
+  constexpr int U = S::U, NV = S::NV, VE = S::VE, N = NV * VE;
+  __shared__ float red[2][U * S::BT / 64];
+  const int t = threadIdx.x % (S::L * S::W), group = threadIdx.x / (S::L * S::W);
+  const Columns<S> C(t, D);
+  const float inv = 1.0f / (float)D;
+  float wf[N], bf[N];
+  bool first = true;
+  for (int64_t r0 = (int64_t)blockIdx.x * S::ROWS; r0 < rows; r0 += (int64_t)gridDim.x * S::ROWS) {
+    Vec<T, VE> in[U][NV];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      // rows past the last one read the last one and are not stored
+      const int64_t r = r0 + u * S::GROUPS + group, rc = r < rows ? r : rows - 1;
+#pragma unroll
+      for (int j = 0; j < NV; ++j) in[u][j].load(x + rc * xs + C.c[j]);
+    }
+    if (first) {  // behind the first rows' loads
+      load_param<S>(wf, w, C, 1.f);
+      load_param<S>(bf, b, C, 0.f);
+      first = false;
+    }
+    float s[U], q[U], f[U][N];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      s[u] = 0.f;
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        in[u][j].get(&f[u][j * VE]);
+#pragma unroll
+        for (int e = 0; e < VE; ++e) s[u] += S::EXACT || e >= C.skip[j] ? f[u][j * VE + e] : 0.f;
+      }
+    }
+    row_sums<S>(s, red[0]);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      q[u] = 0.f;
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int e = 0; e < VE; ++e) {
+          const float d = f[u][j * VE + e] - s[u] * inv;
+          f[u][j * VE + e] = d;
+          q[u] += S::EXACT || e >= C.skip[j] ? d * d : 0.f;
+        }
+    }
+    row_sums<S>(q, red[1]);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const float rstd = 1.0f / sqrtf(q[u] * inv + eps);
+      const int64_t r = r0 + u * S::GROUPS + group;
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        float o[VE];
+#pragma unroll
+        for (int e = 0; e < VE; ++e) o[e] = f[u][j * VE + e] * rstd * wf[j * VE + e] + bf[j * VE + e];
+        Vec<T, VE> out;
+        out.set(o);
+        if (r < rows && (S::EXACT || C.skip[j] < VE)) out.store(y + r * D + C.c[j]);
+      }
+    }
+  }
+}
+
+// dx of every row, and this block's sums of dy h and dy over its rows:
+// part[block][0][c], part[block][1][c].  The second reduction takes three sums
+// at once: with q = sum d^2 and s2 = sum g d, mean(g h) = r s2 / D.
+template <typename S>
+__global__ __launch_bounds__(S::BT) void ln_backward_kernel(const typename S::T* __restrict__ x, int64_t xs,
+                                                            const typename S::T* __restrict__ dy, int64_t ds,
+                                                            typename S::T* __restrict__ dx, ParamVec w,
+                                                            float* __restrict__ part, int64_t rows, int D, float eps) {
+  typedef typename S::T T;
+  constexpr int U = S::U, NV = S::NV, VE = S::VE, N = NV * VE;
+  __shared__ float red0[U * S::BT / 64], red1[3 * U * S::BT / 64];
+  extern __shared__ float sums[];  // [2][D], where a block has several groups
+  const int t = threadIdx.x % (S::L * S::W), group = threadIdx.x / (S::L * S::W);
+  const Columns<S> C(t, D);
+  const float inv = 1.0f / (float)D;
+  float wf[N], aw[N], ab[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) aw[i] = ab[i] = 0.f;
+  Vec<T, VE> xv[U][NV], gv[U][NV];
+  auto load_rows = [&](int64_t r0) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t r = r0 + u * S::GROUPS + group, rc = r < rows ? r : rows - 1;
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        xv[u][j].load(x + rc * xs + C.c[j]);
+        gv[u][j].load(dy + rc * ds + C.c[j]);
+      }
+    }
+  };
+  const int64_t stride = (int64_t)gridDim.x * S::ROWS;
+  int64_t r0 = (int64_t)blockIdx.x * S::ROWS;
+  load_rows(r0);
+  load_param<S>(wf, w, C, 1.f);
+  for (; r0 < rows; r0 += stride) {
+    float f[U][N], g[U][N], s[U], m[3 * U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      s[u] = 0.f;
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        xv[u][j].get(&f[u][j * VE]);
+        gv[u][j].get(&g[u][j * VE]);
+#pragma unroll
+        for (int e = 0; e < VE; ++e) s[u] += S::EXACT || e >= C.skip[j] ? f[u][j * VE + e] : 0.f;
+      }
+    }
+    load_rows(r0 + stride);  // the next step's rows; past the end the last row again
+    row_sums<S>(s, red0);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      float q = 0.f, s1 = 0.f, s2 = 0.f;
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const float d = f[u][i] - s[u] * inv;
+        const bool counts = S::EXACT || i % VE >= C.skip[i / VE];
+        const float gw = counts ? g[u][i] * wf[i] : 0.f;
+        f[u][i] = d;
+        q += counts ? d * d : 0.f;
+        s1 += gw;
+        s2 += gw * d;
+      }
+      m[3 * u] = q;
+      m[3 * u + 1] = s1;
+      m[3 * u + 2] = s2;
+    }
+    row_sums<S>(m, red1);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const float rstd = 1.0f / sqrtf(m[3 * u] * inv + eps);
+      const float c1 = m[3 * u + 1] * inv, c2 = m[3 * u + 2] * inv * rstd;
+      const int64_t r = r0 + u * S::GROUPS + group;
+      const bool live = r < rows;
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        float o[VE];
+#pragma unroll
+        for (int e = 0; e < VE; ++e) {
+          const int i = j * VE + e;
+          const float h = f[u][i] * rstd;
+          o[e] = (g[u][i] * wf[i] - c1 - h * c2) * rstd;
+          if (live) {
+            aw[i] += g[u][i] * h;
+            ab[i] += g[u][i];
+          }
+        }
+        Vec<T, VE> out;
+        out.set(o);
+        if (dx && live && (S::EXACT || C.skip[j] < VE)) out.store(dx + r * D + C.c[j]);
+      }
+    }
+  }
+  if (!part) return;
+  // the groups' sums: first those of a wave, then wave after wave in LDS
+  if constexpr (S::W == 1) {
+#pragma unroll
+    for (int off = S::L; off < 64; off <<= 1)
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        aw[i] += __shfl_xor(aw[i], off, 64);
+        ab[i] += __shfl_xor(ab[i], off, 64);
+      }
+  }
+  constexpr int TURNS = S::W == 1 ? S::BT / 64 : S::GROUPS;
+  const int turn = S::W == 1 ? wave_id() : group;
+  const bool holds = S::W > 1 || (threadIdx.x & 63) < S::L;
+  float* dst = part + (int64_t)blockIdx.x * 2 * D;
+#pragma unroll
+  for (int k = 0; k < TURNS; ++k) {
+    if (turn == k && holds) {
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int e = 0; e < VE; ++e) {
+          const int c = C.c[j] + e, i = j * VE + e;
+          if (!S::EXACT && e < C.skip[j]) continue;
+          const float vw = k == 0 ? aw[i] : sums[c] + aw[i], vb = k == 0 ? ab[i] : sums[D + c] + ab[i];
+          if (k == TURNS - 1) {
+            dst[c] = vw;
+            dst[D + c] = vb;
+          } else {
+            sums[c] = vw;
+            sums[D + c] = vb;
+          }
+        }
+    }
+    if (k < TURNS - 1) __syncthreads();
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Rows that registers do not hold: a block a row, several sweeps.
+// ---------------------------------------------------------------------------
+constexpr int kWideThreads = 1024;
+template <int K> __device__ __forceinline__ void block_sums(float (&v)[K], float* red) {
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    v[k] = lane_sum<64>(v[k]);
+    if ((threadIdx.x & 63) == 0) red[k * 16 + wave_id()] = v[k];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    v[k] = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWideThreads / 64; ++w) v[k] += red[k * 16 + w];
+  }
+}
+
+template <typename T>
+__global__ __launch_bounds__(kWideThreads) void ln_forward_wide_kernel(const T* __restrict__ x, int64_t xs,
+                                                                       T* __restrict__ y, ParamVec w, ParamVec b,
+                                                                       int64_t rows, int D, float eps) {
+  __shared__ float red[16];
+  for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
+    const T* xr = x + r * xs;
+    float s[1] = {0.f}, q[1] = {0.f};
+    for (int c = threadIdx.x; c < D; c += kWideThreads) s[0] += to_f32(xr[c]);
+    block_sums(s, red);
+    const float mean = s[0] / (float)D;
+    for (int c = threadIdx.x; c < D; c += kWideThreads) {
+      const float d = to_f32(xr[c]) - mean;
+      q[0] += d * d;
+    }
+    block_sums(q, red);
+    const float rstd = 1.0f / sqrtf(q[0] / (float)D + eps);
+    for (int c = threadIdx.x; c < D; c += kWideThreads)
       y[r * D + c] = cvt<T>((to_f32(xr[c]) - mean) * rstd * w.get(c, 1.f) + b.get(c, 0.f));
   }
 }
 
-// One wave per row: dx, and the row's mean and rstd for the column sums.
+// dx, and the row's mean and rstd for the column sums.
 template <typename T>
-__global__ __launch_bounds__(256) void ln_backward_rows_kernel(const T* __restrict__ x, int64_t xs,
-                                                               const T* __restrict__ dy, int64_t ds,
-                                                               T* __restrict__ dx, ParamVec w, float2* __restrict__ stats,
-                                                               int64_t rows, int D, float eps) {
-  const int lane = threadIdx.x & 63;
-  for (int64_t r = (int64_t)blockIdx.x * 4 + wave_id(); r < rows; r += (int64_t)gridDim.x * 4) {
+__global__ __launch_bounds__(kWideThreads) void ln_backward_wide_kernel(const T* __restrict__ x, int64_t xs,
+                                                                        const T* __restrict__ dy, int64_t ds,
+                                                                        T* __restrict__ dx, ParamVec w,
+                                                                        float2* __restrict__ stats, int64_t rows, int D,
+                                                                        float eps) {
+  __shared__ float red[48];
+  for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
     const T* xr = x + r * xs;
     const T* dr = dy + r * ds;
-    float s = 0.f, q = 0.f, s1 = 0.f, s2 = 0.f;
-    for (int c = lane; c < D; c += 64) s += to_f32(xr[c]);
-    const float mean = wave_sum(s) / (float)D;
-    for (int c = lane; c < D; c += 64) {
+    float s[1] = {0.f}, m[3] = {0.f, 0.f, 0.f};
+    for (int c = threadIdx.x; c < D; c += kWideThreads) s[0] += to_f32(xr[c]);
+    block_sums(s, red);
+    const float mean = s[0] / (float)D;
+    for (int c = threadIdx.x; c < D; c += kWideThreads) {
       const float d = to_f32(xr[c]) - mean;
       const float g = to_f32(dr[c]) * w.get(c, 1.f);
-      q += d * d;
-      s1 += g;
-      s2 += g * d;
+      m[0] += d * d;
+      m[1] += g;
+      m[2] += g * d;
     }
-    const float rstd = 1.0f / sqrtf(wave_sum(q) / (float)D + eps);
-    const float c1 = wave_sum(s1) / (float)D, c2 = wave_sum(s2) / (float)D * rstd;
+    block_sums(m, red);
+    const float rstd = 1.0f / sqrtf(m[0] / (float)D + eps);
+    const float c1 = m[1] / (float)D, c2 = m[2] / (float)D * rstd;
     if (dx)
-      for (int c = lane; c < D; c += 64) {
+      for (int c = threadIdx.x; c < D; c += kWideThreads) {
         const float h = (to_f32(xr[c]) - mean) * rstd;
         dx[r * D + c] = cvt<T>((to_f32(dr[c]) * w.get(c, 1.f) - c1 - h * c2) * rstd);
       }
-    if (stats && lane == 0) stats[r] = float2{mean, rstd};
+    if (threadIdx.x == 0) stats[r] = float2{mean, rstd};
   }
 }
 
@@ -109,52 +464,151 @@ __global__ __launch_bounds__(256) void ln_columns_kernel(const T* __restrict__ x
         (red[wave][0][lane] + red[wave][1][lane]) + (red[wave][2][lane] + red[wave][3][lane]);
 }
 
-// dst[c] = sum of the splits' partials (blockIdx.y: 0 the weight's, 1 the bias').
-__global__ __launch_bounds__(256) void ln_close_kernel(const float* __restrict__ part, int splits, int D,
-                                                       void* __restrict__ dw, void* __restrict__ db, int dst_bf) {
-  const int c = blockIdx.x * 256 + threadIdx.x;
-  void* dst = blockIdx.y ? db : dw;
-  if (c >= D || !dst) return;
-  float s = 0.f;
-  for (int k = 0; k < splits; ++k) s += part[((int64_t)k * 2 + blockIdx.y) * D + c];
+// dst[c] = sum over the partials (c < D: the weight's, else the bias'): 32 of
+// the 2 D sums a block, 16 threads each, eight loads in flight.
+constexpr int kCloseOuts = 32, kCloseChunks = 16;
+__global__ __launch_bounds__(kCloseOuts * kCloseChunks) void ln_close_kernel(const float* __restrict__ part, int parts,
+                                                                            int D, void* __restrict__ dw,
+                                                                            void* __restrict__ db, int dst_bf) {
+  __shared__ float red[kCloseChunks][kCloseOuts];
+  const int o = threadIdx.x % kCloseOuts, ch = threadIdx.x / kCloseOuts;
+  const int64_t i = (int64_t)blockIdx.x * kCloseOuts + o, n = 2 * (int64_t)D;
+  void* dst = i < D ? dw : db;
+  const bool live = i < n && dst;
+  float a[8] = {};
+  if (live)
+    for (int k = ch; k < parts; k += 8 * kCloseChunks)
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const int ku = k + u * kCloseChunks;
+        const float v = part[(ku < parts ? ku : parts - 1) * n + i];
+        a[u] += ku < parts ? v : 0.f;
+      }
+  red[ch][o] = ((a[0] + a[1]) + (a[2] + a[3])) + ((a[4] + a[5]) + (a[6] + a[7]));
+  __syncthreads();
+  if (ch != 0 || !live) return;
+  float s[kCloseChunks];
+#pragma unroll
+  for (int k = 0; k < kCloseChunks; ++k) s[k] = red[k][o];
+#pragma unroll
+  for (int w = kCloseChunks / 2; w > 0; w /= 2)
+#pragma unroll
+    for (int k = 0; k < w; ++k) s[k] += s[k + w];
+  const int c = (int)(i < D ? i : i - D);
   if (dst_bf)
-    ((bf16*)dst)[c] = cvt<bf16>(s);
+    ((bf16*)dst)[c] = cvt<bf16>(s[0]);
   else
-    ((float*)dst)[c] = s;
+    ((float*)dst)[c] = s[0];
+}
+
+static int launch_ln_close(const float* part, int parts, int D, void* dw, void* db, int dst_bf, hipStream_t st) {
+  StageTimer timer("layer_norm_close", st);
+  ln_close_kernel<<<(2 * D + kCloseOuts - 1) / kCloseOuts, kCloseOuts * kCloseChunks, 0, st>>>(part, parts, D, dw, db,
+                                                                                             dst_bf);
+  GTK_LAUNCH_CHECK();
+  return GTK_OK;
+}
+
+// ---------------------------------------------------------------------------
+// Shapes by width
+// ---------------------------------------------------------------------------
+// Calls run(Shape) for the narrowest shape that holds D.
+template <typename T, int VE, int NV, int L, int W, int BT, int U, typename F> static int with_shape(int D, F& run) {
+  if (D == VE * NV * L * W) return run(Shape<T, VE, NV, L, W, BT, U, true>());
+  return run(Shape<T, VE, NV, L, W, BT, U, false>());
+}
+
+template <typename T, bool BACKWARD, typename F> static int for_shape(int D, F run) {
+  constexpr int VE = 16 / sizeof(T);
+  constexpr int B1 = 256, U1 = 2;                        // a wave or less a row
+  constexpr int BW = BACKWARD ? 1024 : 0, U = 1;         // several waves a row
+  if (D < VE) return run(Shape<T, 1, 1, VE, 1, B1, U1, false>());
+  if (D <= 2 * VE) return with_shape<T, VE, 1, 2, 1, B1, U1>(D, run);
+  if (D <= 4 * VE) return with_shape<T, VE, 1, 4, 1, B1, U1>(D, run);
+  if (D <= 8 * VE) return with_shape<T, VE, 1, 8, 1, B1, U1>(D, run);
+  if (D <= 16 * VE) return with_shape<T, VE, 1, 16, 1, B1, U1>(D, run);
+  if (D <= 32 * VE) return with_shape<T, VE, 1, 32, 1, B1, U1>(D, run);
+  if (D <= 64 * VE) return with_shape<T, VE, 1, 64, 1, B1, U1>(D, run);
+  if (D <= 128 * VE) return with_shape<T, VE, 1, 64, 2, BW ? BW : 256, U>(D, run);
+  if (D <= 256 * VE) return with_shape<T, VE, 1, 64, 4, BW ? BW : 256, U>(D, run);
+  if (D <= 512 * VE) return with_shape<T, VE, 1, 64, 8, BW ? BW : 512, U>(D, run);
+  if (D <= 1024 * VE) return with_shape<T, VE, 1, 64, 16, 1024, U>(D, run);
+  return with_shape<T, VE, 2, 64, 16, 1024, U>(D, run);  // up to widest_in_registers
+}
+template <typename T> constexpr int widest_in_registers() { return 2048 * 16 / sizeof(T); }
+
+// Blocks of the backward kernel: each leaves 2 D partial sums, so no more than
+// fill the chip with `threads` threads a block.
+static int backward_blocks(int64_t rows, int rows_a_step, int threads) {
+  const int64_t steps = (rows + rows_a_step - 1) / rows_a_step;
+  return (int)std::min<int64_t>(steps, (int64_t)device_cus() * (1024 / threads));
 }
 
 static int column_splits(int64_t rows) { return (int)std::min<int64_t>(256, std::max<int64_t>(1, (rows + 15) / 16)); }
 
-static unsigned row_blocks(int64_t rows) { return (unsigned)std::min<int64_t>((rows + 3) / 4, 1 << 16); }
+// Partial sums that the backward pass leaves for its last launch.
+template <typename T> static int backward_parts(int64_t rows, int D) {
+  if (D > widest_in_registers<T>()) return column_splits(rows);
+  return for_shape<T, true>(D, [&](auto shape) {
+    typedef decltype(shape) S;
+    return backward_blocks(rows, S::ROWS, S::BT);
+  });
+}
 
-static int launch_ln_close(const float* part, int splits, int D, void* dw, void* db, int dst_bf, hipStream_t st) {
-  StageTimer timer("layer_norm_close", st);
-  ln_close_kernel<<<dim3((D + 255) / 256, 2), 256, 0, st>>>(part, splits, D, dw, db, dst_bf);
+template <typename T> static void carve_ln_backward(Carve& cv, int64_t rows, int64_t d, float2** stats, float** part) {
+  *stats = cv.take<float2>(d > widest_in_registers<T>() ? rows : 0);
+  *part = cv.take<float>(2 * d * backward_parts<T>(rows, (int)d));
+}
+
+template <typename T>
+static int launch_ln_forward(const T* x, int64_t xs, T* y, ParamVec w, ParamVec b, int64_t rows, int D, float eps,
+                             hipStream_t st) {
+  StageTimer timer("layer_norm_forward", st);
+  if (D > widest_in_registers<T>())
+    ln_forward_wide_kernel<T><<<(unsigned)std::min<int64_t>(rows, 1 << 20), kWideThreads, 0, st>>>(x, xs, y, w, b, rows, D, eps);
+  else
+    for_shape<T, false>(D, [&](auto shape) {
+      typedef decltype(shape) S;
+      const unsigned grid = (unsigned)std::min<int64_t>((rows + S::ROWS - 1) / S::ROWS, 1 << 20);
+      ln_forward_kernel<S><<<grid, S::BT, 0, st>>>(x, xs, y, w, b, rows, D, eps);
+      return 0;
+    });
   GTK_LAUNCH_CHECK();
   return GTK_OK;
 }
 
 template <typename T>
 static int launch_ln_backward(const T* x, int64_t xs, const T* dy, int64_t ds, T* dx, ParamVec w, void* dw, void* db,
-                              int dst_bf, int64_t rows, int D, float eps, float2* stats, float* part, hipStream_t st) {
-  {
+                              int dst_bf, int64_t rows, int D, float eps, void* ws, size_t ws_bytes, hipStream_t st) {
+  Carve cv(ws, ws_bytes);
+  float2* stats;
+  float* part;
+  carve_ln_backward<T>(cv, rows, D, &stats, &part);
+  const bool sums = dw || db;
+  const int parts = backward_parts<T>(rows, D);
+  if (D > widest_in_registers<T>()) {
+    {
+      StageTimer timer("layer_norm_backward", st);
+      ln_backward_wide_kernel<T><<<(unsigned)std::min<int64_t>(rows, 1 << 20), kWideThreads, 0, st>>>(
+          x, xs, dy, ds, dx, w, stats, rows, D, eps);
+      GTK_LAUNCH_CHECK();
+    }
+    if (sums) {
+      StageTimer timer("layer_norm_columns", st);
+      ln_columns_kernel<T><<<dim3((D + 63) / 64, parts), 256, 0, st>>>(x, xs, dy, ds, stats, part, rows, D);
+      GTK_LAUNCH_CHECK();
+    }
+  } else {
     StageTimer timer("layer_norm_backward", st);
-    ln_backward_rows_kernel<T><<<row_blocks(rows), 256, 0, st>>>(x, xs, dy, ds, dx, w, stats, rows, D, eps);
+    for_shape<T, true>(D, [&](auto shape) {
+      typedef decltype(shape) S;
+      const size_t lds = S::BT / 64 > S::W ? 2 * (size_t)D * sizeof(float) : 0;
+      ln_backward_kernel<S><<<(unsigned)parts, S::BT, lds, st>>>(x, xs, dy, ds, dx, w, sums ? part : nullptr, rows, D, eps);
+      return 0;
+    });
     GTK_LAUNCH_CHECK();
   }
-  if (!dw && !db) return GTK_OK;
-  const int splits = column_splits(rows);
-  {
-    StageTimer timer("layer_norm_columns", st);
-    ln_columns_kernel<T><<<dim3((D + 63) / 64, splits), 256, 0, st>>>(x, xs, dy, ds, stats, part, rows, D);
-    GTK_LAUNCH_CHECK();
-  }
-  return launch_ln_close(part, splits, D, dw, db, dst_bf, st);
-}
-
-static void carve_ln_backward(Carve& cv, int64_t rows, int64_t d, float2** stats, float** part) {
-  *stats = cv.take<float2>(rows);
-  *part = cv.take<float>(2 * d * column_splits(rows));
+  return sums ? launch_ln_close(part, parts, D, dw, db, dst_bf, st) : GTK_OK;
 }
 
 }  // namespace gtk
@@ -176,13 +630,8 @@ extern "C" int gtk_layer_norm_forward(const void* x, int64_t x_stride, void* y, 
   GTK_REQUIRE(x && y, GTK_EINVAL, "gtk_layer_norm_forward: null pointer");
   hipStream_t st = (hipStream_t)stream;
   const ParamVec w{weight, param_dtype == GTK_BF16}, b{bias, param_dtype == GTK_BF16};
-  StageTimer timer("layer_norm_forward", st);
-  if (dtype == GTK_F32)
-    ln_forward_kernel<float><<<row_blocks(rows), 256, 0, st>>>((const float*)x, x_stride, (float*)y, w, b, rows, (int)d, eps);
-  else
-    ln_forward_kernel<bf16><<<row_blocks(rows), 256, 0, st>>>((const bf16*)x, x_stride, (bf16*)y, w, b, rows, (int)d, eps);
-  GTK_LAUNCH_CHECK();
-  return GTK_OK;
+  if (dtype == GTK_F32) return launch_ln_forward<float>((const float*)x, x_stride, (float*)y, w, b, rows, (int)d, eps, st);
+  return launch_ln_forward<bf16>((const bf16*)x, x_stride, (bf16*)y, w, b, rows, (int)d, eps, st);
 }
 
 extern "C" size_t gtk_layer_norm_backward_workspace_size(int64_t rows, int64_t d, int dtype) {
@@ -190,7 +639,10 @@ extern "C" size_t gtk_layer_norm_backward_workspace_size(int64_t rows, int64_t d
   Carve cv(nullptr, SIZE_MAX);
   float2* stats;
   float* part;
-  carve_ln_backward(cv, rows, d, &stats, &part);
+  if (dtype == GTK_F32)
+    carve_ln_backward<float>(cv, rows, d, &stats, &part);
+  else
+    carve_ln_backward<bf16>(cv, rows, d, &stats, &part);
   return cv.off;
 }
 
@@ -210,13 +662,9 @@ extern "C" int gtk_layer_norm_backward(const void* x, int64_t x_stride, const vo
   GTK_REQUIRE(workspace_bytes >= need, GTK_EWORKSPACE, "gtk_layer_norm_backward: workspace %zu < %zu bytes",
               workspace_bytes, need);
   const ParamVec w{weight, pbf};
-  Carve cv(workspace, workspace_bytes);
-  float2* stats;
-  float* part;
-  carve_ln_backward(cv, rows, d, &stats, &part);
   if (dtype == GTK_F32)
     return launch_ln_backward<float>((const float*)x, x_stride, (const float*)dy, dy_stride, (float*)dx, w, dweight,
-                                     dbias, pbf, rows, (int)d, eps, stats, part, st);
+                                     dbias, pbf, rows, (int)d, eps, workspace, workspace_bytes, st);
   return launch_ln_backward<bf16>((const bf16*)x, x_stride, (const bf16*)dy, dy_stride, (bf16*)dx, w, dweight, dbias,
-                                  pbf, rows, (int)d, eps, stats, part, st);
+                                  pbf, rows, (int)d, eps, workspace, workspace_bytes, st);
 }
