@@ -8,8 +8,10 @@
 // current HIP stream; scratch comes from torch's caching allocator.
 #include <c10/hip/HIPStream.h>
 #include <ATen/MemoryOverlap.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
 
+#include <array>
 #include <limits>
 #include <utility>
 #include <vector>
@@ -636,11 +638,11 @@ at::Tensor layer_norm_forward(const at::Tensor& x, const c10::optional<at::Tenso
   return y;
 }
 
-// Returns [dx, dweight, dbias], the ones not asked for as None; dweight and
-// dbias in the weight's type (fp32 without a weight).
-std::vector<c10::optional<at::Tensor>> layer_norm_backward(const at::Tensor& x, const at::Tensor& dy,
-                                                           const c10::optional<at::Tensor>& weight, double eps,
-                                                           bool need_x, bool need_weight, bool need_bias) {
+// {dx, dweight, dbias}, the ones not asked for undefined; dweight and dbias in
+// the weight's type (fp32 without a weight).
+std::array<at::Tensor, 3> ln_backward(const at::Tensor& x, const at::Tensor& dy,
+                                      const c10::optional<at::Tensor>& weight, double eps, bool need_x,
+                                      bool need_weight, bool need_bias) {
   check_gpu(x, "x");
   TORCH_CHECK(x.dim() >= 1, "x must have at least one dimension");
   check_on(dy, x, "dy");
@@ -655,16 +657,83 @@ std::vector<c10::optional<at::Tensor>> layer_norm_backward(const at::Tensor& x, 
   at::Tensor w;
   if (weight.has_value()) w = weight->contiguous();
   const auto popts = w.defined() ? w.options() : x.options().dtype(at::kFloat);
-  std::vector<c10::optional<at::Tensor>> out(3);
+  std::array<at::Tensor, 3> out;
   if (need_x) out[0] = at::empty(x.sizes(), x.options());
   if (need_weight) out[1] = at::empty({d}, popts);
   if (need_bias) out[2] = at::empty({d}, popts);
-  auto ptr = [&](int k) { return out[k].has_value() ? out[k]->data_ptr() : nullptr; };
+  auto ptr = [&](int k) { return out[k].defined() ? out[k].data_ptr() : nullptr; };
   auto ws = workspace(x, gtk_layer_norm_backward_workspace_size(rows, d, dt));
   check_rc(gtk_layer_norm_backward(xc.data_ptr(), xs, dyc.data_ptr(), ds, ptr_or_null(w),
                                    w.defined() ? gtk_dtype_of(w, "weight") : GTK_F32, ptr(0), ptr(1), ptr(2), rows, d,
                                    (float)eps, dt, ws.data_ptr(), ws.numel(), cur_stream(x)));
   return out;
+}
+
+std::vector<c10::optional<at::Tensor>> layer_norm_backward(const at::Tensor& x, const at::Tensor& dy,
+                                                           const c10::optional<at::Tensor>& weight, double eps,
+                                                           bool need_x, bool need_weight, bool need_bias) {
+  std::vector<c10::optional<at::Tensor>> out(3);
+  auto g = ln_backward(x, dy, weight, eps, need_x, need_weight, need_bias);
+  for (int k = 0; k < 3; ++k)
+    if (g[k].defined()) out[k] = g[k];
+  return out;
+}
+
+// layer_norm_forward under autograd.  A node of C++ (a Python one takes some 30
+// us of host time a training pass, which is what a short one costs).  Only x
+// and the weight are saved: the backward computes the rows' statistics again.
+struct LayerNormFn : public torch::autograd::Function<LayerNormFn> {
+  static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x,
+                            const c10::optional<at::Tensor>& weight, const c10::optional<at::Tensor>& bias,
+                            double eps) {
+    ctx->save_for_backward({x, weight.has_value() ? *weight : at::Tensor()});
+    ctx->saved_data["eps"] = eps;
+    ctx->saved_data["bias"] = bias.has_value();
+    ctx->saved_data["bias_dtype"] = (int64_t)(bias.has_value() ? bias->scalar_type() : at::kFloat);
+    return layer_norm_forward(x, weight, bias, eps);
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const at::Tensor& x = saved[0];
+    c10::optional<at::Tensor> weight;
+    if (saved[1].defined()) weight = saved[1];
+    const auto bias_dtype = (at::ScalarType)ctx->saved_data["bias_dtype"].toInt();
+    const bool need_x = ctx->needs_input_grad(0), need_w = weight.has_value() && ctx->needs_input_grad(1);
+    // the edges of absent parameters are not counted
+    const bool need_b = ctx->saved_data["bias"].toBool() && ctx->needs_input_grad(weight.has_value() ? 2 : 1);
+    std::array<at::Tensor, 3> g;
+    {
+      at::NoGradGuard no_grad;
+      const auto weight_dtype = weight.has_value() ? weight->scalar_type() : at::kFloat;
+      // parameters of two types: both in fp32, each rounded once to its own
+      if (need_b && weight.has_value() && weight_dtype != bias_dtype) weight = weight->to(at::kFloat);
+      g = ln_backward(x, grads[0], weight, ctx->saved_data["eps"].toDouble(), need_x, need_w, need_b);
+      if (need_w) g[1] = g[1].to(weight_dtype);
+      if (need_b) g[2] = g[2].to(bias_dtype);
+    }
+    torch::autograd::variable_list out{g[0], g[1], g[2], at::Tensor()};
+    if (at::GradMode::is_enabled()) {  // create_graph: differentiating these again is an error
+      torch::autograd::variable_list some;
+      for (const auto& t : out)
+        if (t.defined()) some.push_back(t.detach().requires_grad_(true));
+      torch::autograd::DelayedError error("layer_norm's backward is once_differentiable: a second derivative is not "
+                                          "implemented", (int)some.size());
+      const auto guarded = error.apply(std::move(some));
+      size_t k = 0;
+      for (auto& t : out)
+        if (t.defined()) t = guarded[k++];
+    }
+    return out;
+  }
+};
+
+at::Tensor layer_norm(const at::Tensor& x, const c10::optional<at::Tensor>& weight,
+                      const c10::optional<at::Tensor>& bias, double eps) {
+  const bool grad = at::GradMode::is_enabled() &&
+                    (x.requires_grad() || (weight.has_value() && weight->requires_grad()) ||
+                     (bias.has_value() && bias->requires_grad()));
+  return grad ? LayerNormFn::apply(x, weight, bias, eps) : layer_norm_forward(x, weight, bias, eps);
 }
 
 // ---------------------------------------------------------------------------
@@ -877,6 +946,8 @@ PYBIND11_MODULE(_C, m) {
         py::arg("mask"), py::arg("packed"), py::arg("c_in"), py::arg("c_h"), py::arg("no_heads"),
         py::arg("starting"), py::arg("residual") = false, py::arg("eps") = 1e-5,
         py::arg("chunk_rows") = 0, py::arg("inf") = 1e9);
+  m.def("layer_norm", &layer_norm, "layer_norm_forward under autograd (differentiable once)", py::arg("x"),
+        py::arg("weight") = py::none(), py::arg("bias") = py::none(), py::arg("eps") = 1e-5);
   m.def("layer_norm_forward", &layer_norm_forward,
         "LayerNorm over the last dimension, optional affine in either parameter type", py::arg("x"),
         py::arg("weight") = py::none(), py::arg("bias") = py::none(), py::arg("eps") = 1e-5);

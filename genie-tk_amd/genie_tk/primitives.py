@@ -15,7 +15,6 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 from torch import Tensor
-from torch.autograd.function import once_differentiable
 
 from genie_tk import _dispatch, _ext
 
@@ -137,39 +136,14 @@ class Attention(nn.Module):
         return self.linear_o(o)
 
 
-class _LayerNormFunction(torch.autograd.Function):
-    """LayerNorm on the HIP kernels, forward and backward.  Only x and the
-    weight are saved: the backward computes the rows' statistics again."""
-
-    @staticmethod
-    def forward(ctx, x, weight, bias, eps):
-        ctx.save_for_backward(x, weight)
-        ctx.eps = eps
-        ctx.bias_dtype = None if bias is None else bias.dtype
-        return _ext.require().layer_norm_forward(x, weight, bias, eps)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        x, weight = ctx.saved_tensors
-        need_x, need_w, need_b = ctx.needs_input_grad[:3]
-        if need_b and weight is not None and ctx.bias_dtype != weight.dtype:
-            # both in fp32, each rounded once to its own type
-            dx, dw, db = _ext.require().layer_norm_backward(x, dy, weight.float(), ctx.eps, need_x,
-                                                            need_w, need_b)
-            return dx, dw if dw is None else dw.to(weight.dtype), db.to(ctx.bias_dtype), None
-        dx, dw, db = _ext.require().layer_norm_backward(x, dy, weight, ctx.eps, need_x, need_w, need_b)
-        return dx, dw, db if db is None else db.to(ctx.bias_dtype), None
-
-
 def layer_norm(x: Tensor, weight: Optional[Tensor] = None, bias: Optional[Tensor] = None,
                eps: float = 1e-5) -> Tensor:
     """LayerNorm over the last dimension of ``x`` with optional ``weight`` and
     ``bias`` ([D]), differentiable once.
 
     Kernel path (bf16 or fp32 GPU tensor, parameters in bf16 or fp32, also
-    mixed): ``genie_tk._C.layer_norm_forward`` / ``layer_norm_backward``.  The
-    output and dL/dx have the type of ``x``, the parameters' gradients their
+    mixed): ``genie_tk._C.layer_norm``, whose autograd node is the C++ one of
+    ``layer_norm_forward`` and ``layer_norm_backward``.  The output and dL/dx have the type of ``x``, the parameters' gradients their
     own; statistics and sums are fp32.  Rows that lie one stride apart (a slice
     of wider rows, a repeated row) are read as they are.  Other tensors run
     torch's LayerNorm."""
@@ -179,9 +153,7 @@ def layer_norm(x: Tensor, weight: Optional[Tensor] = None, bias: Optional[Tensor
             _ext.missing("layer_norm")
         elif (x.dim() >= 1 and x.shape[-1] >= 1 and x.dtype in _dispatch.SUPPORTED_DTYPES
               and all(p.dtype in _dispatch.SUPPORTED_DTYPES for p in params)):
-            if torch.is_grad_enabled() and (x.requires_grad or any(p.requires_grad for p in params)):
-                return _LayerNormFunction.apply(x, weight, bias, eps)
-            return _ext.C.layer_norm_forward(x, weight, bias, eps)
+            return _ext.C.layer_norm(x, weight, bias, eps)
     if any(p.dtype != x.dtype for p in params):  # in fp32, rounded once
         wide = [None if p is None else p.float() for p in (weight, bias)]
         return F.layer_norm(x.float(), x.shape[-1:], *wide, eps).to(x.dtype)
