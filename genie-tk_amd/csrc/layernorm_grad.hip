@@ -96,7 +96,7 @@ template <int L> __device__ __forceinline__ float lane_sum(float v) {
 }
 
 // The launch shape of one kernel: see above; BT threads a block, U rows a lane
-// group in flight, EXACT: D = L * W * NV * VE.
+// group at once, EXACT: D = L * W * NV * VE.
 template <typename T_, int VE_, int NV_, int L_, int W_, int BT_, int U_, bool EXACT_> struct Shape {
   typedef T_ T;
   static constexpr int VE = VE_, NV = NV_, L = L_, W = W_, BT = BT_, U = U_;
@@ -245,6 +245,8 @@ __global__ __launch_bounds__(S::BT) void ln_backward_kernel(const typename S::T*
   constexpr int U = S::U, NV = S::NV, VE = S::VE, N = NV * VE;
   __shared__ float red0[U * S::BT / 64], red1[3 * U * S::BT / 64];
   extern __shared__ float sums[];  // [2][D], where a block has several groups
+  // the widest rows read the weight again for each row: their registers hold no more
+  constexpr bool KEEP = NV == 1;
   const int t = threadIdx.x % (S::L * S::W), group = threadIdx.x / (S::L * S::W);
   const Columns<S> C(t, D);
   const float inv = 1.0f / (float)D;
@@ -252,6 +254,7 @@ __global__ __launch_bounds__(S::BT) void ln_backward_kernel(const typename S::T*
 #pragma unroll
   for (int i = 0; i < N; ++i) aw[i] = ab[i] = 0.f;
   Vec<T, VE> xv[U][NV], gv[U][NV];
+  // past the end the last row again
   auto load_rows = [&](int64_t r0) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -266,7 +269,7 @@ __global__ __launch_bounds__(S::BT) void ln_backward_kernel(const typename S::T*
   const int64_t stride = (int64_t)gridDim.x * S::ROWS;
   int64_t r0 = (int64_t)blockIdx.x * S::ROWS;
   load_rows(r0);
-  load_param<S>(wf, w, C, 1.f);
+  if constexpr (KEEP) load_param<S>(wf, w, C, 1.f);
   for (; r0 < rows; r0 += stride) {
     float f[U][N], g[U][N], s[U], m[3 * U];
 #pragma unroll
@@ -280,7 +283,10 @@ __global__ __launch_bounds__(S::BT) void ln_backward_kernel(const typename S::T*
         for (int e = 0; e < VE; ++e) s[u] += S::EXACT || e >= C.skip[j] ? f[u][j * VE + e] : 0.f;
       }
     }
-    load_rows(r0 + stride);  // the next step's rows; past the end the last row again
+    if constexpr (KEEP)
+      load_rows(r0 + stride);  // the next step's
+    else
+      load_param<S>(wf, w, C, 1.f);
     row_sums<S>(s, red0);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -324,6 +330,7 @@ __global__ __launch_bounds__(S::BT) void ln_backward_kernel(const typename S::T*
         if (dx && live && (S::EXACT || C.skip[j] < VE)) out.store(dx + r * D + C.c[j]);
       }
     }
+    if constexpr (!KEEP) load_rows(r0 + stride);
   }
   if (!part) return;
   // the groups' sums: first those of a wave, then wave after wave in LDS
@@ -344,20 +351,33 @@ __global__ __launch_bounds__(S::BT) void ln_backward_kernel(const typename S::T*
   for (int k = 0; k < TURNS; ++k) {
     if (turn == k && holds) {
 #pragma unroll
-      for (int j = 0; j < NV; ++j)
+      for (int j = 0; j < NV; ++j) {
+        const int c = C.c[j];
+        float *a = aw + j * VE, *b = ab + j * VE;
+        if (S::EXACT || C.skip[j] == 0) {  // whole vectors
+          if (k > 0) {
+            float v[2][VE];
+            __builtin_memcpy(v[0], sums + c, sizeof(v[0]));
+            __builtin_memcpy(v[1], sums + D + c, sizeof(v[1]));
 #pragma unroll
-        for (int e = 0; e < VE; ++e) {
-          const int c = C.c[j] + e, i = j * VE + e;
-          if (!S::EXACT && e < C.skip[j]) continue;
-          const float vw = k == 0 ? aw[i] : sums[c] + aw[i], vb = k == 0 ? ab[i] : sums[D + c] + ab[i];
-          if (k == TURNS - 1) {
-            dst[c] = vw;
-            dst[D + c] = vb;
-          } else {
-            sums[c] = vw;
-            sums[D + c] = vb;
+            for (int e = 0; e < VE; ++e) {
+              a[e] += v[0][e];
+              b[e] += v[1][e];
+            }
+          }
+          float* to = k == TURNS - 1 ? dst : sums;
+          __builtin_memcpy(to + c, a, VE * sizeof(float));
+          __builtin_memcpy(to + D + c, b, VE * sizeof(float));
+        } else {
+#pragma unroll
+          for (int e = 0; e < VE; ++e) {
+            if (e < C.skip[j]) continue;
+            const float vw = k == 0 ? a[e] : sums[c + e] + a[e], vb = k == 0 ? b[e] : sums[D + c + e] + b[e];
+            (k == TURNS - 1 ? dst : sums)[c + e] = vw;
+            (k == TURNS - 1 ? dst : sums)[D + c + e] = vb;
           }
         }
+      }
     }
     if (k < TURNS - 1) __syncthreads();
   }
@@ -464,47 +484,49 @@ __global__ __launch_bounds__(256) void ln_columns_kernel(const T* __restrict__ x
         (red[wave][0][lane] + red[wave][1][lane]) + (red[wave][2][lane] + red[wave][3][lane]);
 }
 
-// dst[c] = sum over the partials (c < D: the weight's, else the bias'): 32 of
-// the 2 D sums a block, 16 threads each, eight loads in flight.
-constexpr int kCloseOuts = 32, kCloseChunks = 16;
-__global__ __launch_bounds__(kCloseOuts * kCloseChunks) void ln_close_kernel(const float* __restrict__ part, int parts,
-                                                                            int D, void* __restrict__ dw,
-                                                                            void* __restrict__ db, int dst_bf) {
-  __shared__ float red[kCloseChunks][kCloseOuts];
-  const int o = threadIdx.x % kCloseOuts, ch = threadIdx.x / kCloseOuts;
-  const int64_t i = (int64_t)blockIdx.x * kCloseOuts + o, n = 2 * (int64_t)D;
+// dst[c] = sum over the partials (c < D: the weight's, else the bias'): OUTS of
+// the 2 D sums a block, CHUNKS threads each, eight loads in flight.
+template <int OUTS, int CHUNKS>
+__global__ __launch_bounds__(OUTS * CHUNKS) void ln_close_kernel(const float* __restrict__ part, int parts, int D,
+                                                                 void* __restrict__ dw, void* __restrict__ db,
+                                                                 int dst_bf) {
+  __shared__ float red[CHUNKS][OUTS];
+  const int o = threadIdx.x % OUTS, ch = threadIdx.x / OUTS;
+  const int64_t i = (int64_t)blockIdx.x * OUTS + o, n = 2 * (int64_t)D;
   void* dst = i < D ? dw : db;
   const bool live = i < n && dst;
   float a[8] = {};
   if (live)
-    for (int k = ch; k < parts; k += 8 * kCloseChunks)
+    for (int k = ch; k < parts; k += 8 * CHUNKS)
 #pragma unroll
       for (int u = 0; u < 8; ++u) {
-        const int ku = k + u * kCloseChunks;
+        const int ku = k + u * CHUNKS;
         const float v = part[(ku < parts ? ku : parts - 1) * n + i];
         a[u] += ku < parts ? v : 0.f;
       }
   red[ch][o] = ((a[0] + a[1]) + (a[2] + a[3])) + ((a[4] + a[5]) + (a[6] + a[7]));
-  __syncthreads();
+  // in pairs
+#pragma unroll
+  for (int w = CHUNKS / 2; w > 0; w /= 2) {
+    __syncthreads();
+    if (ch < w) red[ch][o] += red[ch + w][o];
+  }
   if (ch != 0 || !live) return;
-  float s[kCloseChunks];
-#pragma unroll
-  for (int k = 0; k < kCloseChunks; ++k) s[k] = red[k][o];
-#pragma unroll
-  for (int w = kCloseChunks / 2; w > 0; w /= 2)
-#pragma unroll
-    for (int k = 0; k < w; ++k) s[k] += s[k + w];
+  const float s = red[0][o];
   const int c = (int)(i < D ? i : i - D);
   if (dst_bf)
-    ((bf16*)dst)[c] = cvt<bf16>(s[0]);
+    ((bf16*)dst)[c] = cvt<bf16>(s);
   else
-    ((float*)dst)[c] = s[0];
+    ((float*)dst)[c] = s;
 }
 
 static int launch_ln_close(const float* part, int parts, int D, void* dw, void* db, int dst_bf, hipStream_t st) {
   StageTimer timer("layer_norm_close", st);
-  ln_close_kernel<<<(2 * D + kCloseOuts - 1) / kCloseOuts, kCloseOuts * kCloseChunks, 0, st>>>(part, parts, D, dw, db,
-                                                                                             dst_bf);
+  // narrow rows leave few sums, and many partials of each: more threads a sum
+  if (D <= 512)
+    ln_close_kernel<16, 64><<<(2 * D + 15) / 16, 1024, 0, st>>>(part, parts, D, dw, db, dst_bf);
+  else
+    ln_close_kernel<32, 32><<<(2 * D + 31) / 32, 1024, 0, st>>>(part, parts, D, dw, db, dst_bf);
   GTK_LAUNCH_CHECK();
   return GTK_OK;
 }
@@ -513,25 +535,27 @@ static int launch_ln_close(const float* part, int parts, int D, void* dw, void* 
 // Shapes by width
 // ---------------------------------------------------------------------------
 // Calls run(Shape) for the narrowest shape that holds D.
-template <typename T, int VE, int NV, int L, int W, int BT, int U, typename F> static int with_shape(int D, F& run) {
+template <typename T, int VE, int NV, int L, int W, int BT, int U, typename F>
+static int with_shape(int D, F& run) {
   if (D == VE * NV * L * W) return run(Shape<T, VE, NV, L, W, BT, U, true>());
   return run(Shape<T, VE, NV, L, W, BT, U, false>());
 }
 
 template <typename T, bool BACKWARD, typename F> static int for_shape(int D, F run) {
   constexpr int VE = 16 / sizeof(T);
-  constexpr int B1 = 256, U1 = 2;                        // a wave or less a row
-  constexpr int BW = BACKWARD ? 1024 : 0, U = 1;         // several waves a row
-  if (D < VE) return run(Shape<T, 1, 1, VE, 1, B1, U1, false>());
-  if (D <= 2 * VE) return with_shape<T, VE, 1, 2, 1, B1, U1>(D, run);
-  if (D <= 4 * VE) return with_shape<T, VE, 1, 4, 1, B1, U1>(D, run);
-  if (D <= 8 * VE) return with_shape<T, VE, 1, 8, 1, B1, U1>(D, run);
-  if (D <= 16 * VE) return with_shape<T, VE, 1, 16, 1, B1, U1>(D, run);
-  if (D <= 32 * VE) return with_shape<T, VE, 1, 32, 1, B1, U1>(D, run);
-  if (D <= 64 * VE) return with_shape<T, VE, 1, 64, 1, B1, U1>(D, run);
-  if (D <= 128 * VE) return with_shape<T, VE, 1, 64, 2, BW ? BW : 256, U>(D, run);
-  if (D <= 256 * VE) return with_shape<T, VE, 1, 64, 4, BW ? BW : 256, U>(D, run);
-  if (D <= 512 * VE) return with_shape<T, VE, 1, 64, 8, BW ? BW : 512, U>(D, run);
+  constexpr int U = BACKWARD ? 1 : 2;
+  constexpr int B1 = BACKWARD ? 512 : 256;                        // a wave or less a row
+  constexpr int B2 = BACKWARD ? 1024 : 256, B8 = BACKWARD ? 1024 : 512;  // two or four, eight waves a row
+  if (D < VE) return run(Shape<T, 1, 1, VE, 1, B1, U, false>());
+  if (D <= 2 * VE) return with_shape<T, VE, 1, 2, 1, B1, U>(D, run);
+  if (D <= 4 * VE) return with_shape<T, VE, 1, 4, 1, B1, U>(D, run);
+  if (D <= 8 * VE) return with_shape<T, VE, 1, 8, 1, B1, U>(D, run);
+  if (D <= 16 * VE) return with_shape<T, VE, 1, 16, 1, B1, U>(D, run);
+  if (D <= 32 * VE) return with_shape<T, VE, 1, 32, 1, B1, U>(D, run);
+  if (D <= 64 * VE) return with_shape<T, VE, 1, 64, 1, B1, U>(D, run);
+  if (D <= 128 * VE) return with_shape<T, VE, 1, 64, 2, B2, U>(D, run);
+  if (D <= 256 * VE) return with_shape<T, VE, 1, 64, 4, B2, U>(D, run);
+  if (D <= 512 * VE) return with_shape<T, VE, 1, 64, 8, B8, U>(D, run);
   if (D <= 1024 * VE) return with_shape<T, VE, 1, 64, 16, 1024, U>(D, run);
   return with_shape<T, VE, 2, 64, 16, 1024, U>(D, run);  // up to widest_in_registers
 }
