@@ -6,12 +6,14 @@
 // The values' squares and their sums are 64-bit: the square of a 32-bit float
 // fits a 64-bit one exactly, so neither gradients above 1.8e19 overflow nor
 // ones below 1e-23 vanish.  The tensors' addresses and sizes travel in the
-// kernel arguments, kMaxTensors a launch: no table is copied to the GPU, and a
-// captured launch keeps them.  Every block writes one partial sum and one
-// block adds them in a fixed order, so equal inputs give equal bits.
+// kernel arguments, kMaxIn or kMaxInOut tensors a launch: no table is copied to
+// the GPU, and a captured launch keeps them.  A block takes one chunk of one
+// tensor and leaves one partial sum; one block adds those in a fixed order, so
+// equal inputs give equal bits.
 #include <algorithm>
 #include <memory>
 #include <new>
+#include <type_traits>
 
 #include "capi_util.hpp"
 #include "common.hpp"
@@ -19,99 +21,170 @@
 
 namespace gtk {
 
-constexpr int kMaxTensors = 100;
-struct NormJobs {
-  const void* src[kMaxTensors];
-  void* dst[kMaxTensors];
-  int64_t n[kMaxTensors];
-  int first[kMaxTensors + 1];  // first block of each tensor
-  uint8_t src_bf[kMaxTensors], dst_bf[kMaxTensors];
-  int count;
-  int64_t chunk;  // values a block
+// One launch's tensors (or parts of one): src[k] of n[k] values, whose blocks
+// start at first[k].  The types are the two top bits of n.
+constexpr uint32_t kSrcBf = 1u << 31, kDstBf = 1u << 30, kCountMask = kDstBf - 1;
+constexpr int64_t kMaxPart = (int64_t)1 << 29;  // values an entry; a multiple of every chunk
+template <int MAX, bool OUT> struct Jobs {
+  static constexpr int kMax = MAX;
+  static constexpr bool kOut = OUT;
+  uint64_t src[MAX];
+  uint64_t dst[OUT ? MAX : 1];
+  uint32_t n[MAX];
+  uint32_t first[MAX];
+  uint32_t count, chunk;  // chunk: values a block
 };
-static_assert(sizeof(NormJobs) <= 4000, "kernel arguments");
+typedef Jobs<248, false> JobsIn;     // in place, or read alone
+typedef Jobs<165, true> JobsInOut;
+static_assert(sizeof(JobsIn) <= 4000 && sizeof(JobsInOut) <= 4000, "kernel arguments");
 
-__device__ __forceinline__ float grad_at(const void* p, int bf, int64_t i) {
-  return bf ? to_f32(((const bf16*)p)[i]) : ((const float*)p)[i];
-}
-
-// The tensor of this block, and its range of values.
-__device__ __forceinline__ int find_job(const NormJobs& J, int64_t& begin, int64_t& end) {
+// The entry that block blockIdx.x works on: every wave counts the entries that
+// start at or before it, 64 at a time.
+template <typename J> __device__ __forceinline__ int find_entry(const J& jobs) {
+  const uint32_t lane = threadIdx.x & 63;
   int k = 0;
-  while (k + 1 < J.count && (int)blockIdx.x >= J.first[k + 1]) ++k;
-  begin = (int64_t)((int)blockIdx.x - J.first[k]) * J.chunk;
-  end = begin + J.chunk < J.n[k] ? begin + J.chunk : J.n[k];
-  return k;
+#pragma unroll
+  for (uint32_t i = 0; i < (uint32_t)J::kMax; i += 64) {
+    const uint32_t at = i + lane;
+    const bool before = at < jobs.count && jobs.first[at < (uint32_t)J::kMax ? at : 0] <= blockIdx.x;
+    k += __popcll(__ballot(before));
+  }
+  return __builtin_amdgcn_readfirstlane(k - 1);
 }
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef u32x4 u32x4_any __attribute__((aligned(2)));  // 16 bytes at any address of the element's alignment
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef u32x2 u32x2_any __attribute__((aligned(2)));
+
+constexpr int kThreads = 256;
 
 // The largest |g| is found on the bits: the order of non-negative floats is
 // that of their bits, infinity and NaN (the largest) included.
-template <int KIND>
-__device__ __forceinline__ double block_join(double s, double* red) {
-  const int waves = blockDim.x >> 6;
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) {
-    const double o = __shfl_xor(s, off, 64);
-    if (KIND == GTK_NORM_INF) {
-      const uint64_t a = __builtin_bit_cast(uint64_t, s), b = __builtin_bit_cast(uint64_t, o);
-      s = __builtin_bit_cast(double, a > b ? a : b);
-    } else {
-      s += o;
-    }
-  }
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
-  __syncthreads();
-  s = red[0];
-  for (int w = 1; w < waves; ++w) {
-    if (KIND == GTK_NORM_INF) {
-      const uint64_t a = __builtin_bit_cast(uint64_t, s), b = __builtin_bit_cast(uint64_t, red[w]);
-      s = __builtin_bit_cast(double, a > b ? a : b);
-    } else {
-      s += red[w];
-    }
-  }
-  return s;
-}
-
-template <int KIND>
-__global__ __launch_bounds__(256) void grad_partials_kernel(NormJobs J, double* __restrict__ part) {
-  __shared__ double red[4];
-  int64_t begin, end;
-  const int k = find_job(J, begin, end);
-  double s = 0.0;
+template <int KIND> struct Sum {
+  double v = 0.0;
   uint32_t m = 0;
-  for (int64_t i = begin + threadIdx.x; i < end; i += 256) {
-    const float v = grad_at(J.src[k], J.src_bf[k], i);
-    if (KIND == GTK_NORM_2) s += (double)v * (double)v;
-    if (KIND == GTK_NORM_1) s += (double)fabsf(v);
+  __device__ __forceinline__ void add(float x) {
+    if (KIND == GTK_NORM_2) v = __builtin_fma((double)x, (double)x, v);
+    if (KIND == GTK_NORM_1) v += (double)fabsf(x);
     if (KIND == GTK_NORM_INF) {
-      const uint32_t a = __float_as_uint(v) & 0x7fffffffu;
+      const uint32_t a = __float_as_uint(x) & 0x7fffffffu;
       m = a > m ? a : m;
     }
   }
-  if (KIND == GTK_NORM_INF) s = __builtin_bit_cast(double, (uint64_t)m);
-  s = block_join<KIND>(s, red);
-  if (threadIdx.x == 0) part[blockIdx.x] = s;
+  __device__ __forceinline__ void join(const Sum& o) {
+    v += o.v;
+    m = o.m > m ? o.m : m;
+  }
+  // as 64 bits in memory
+  __device__ __forceinline__ void put(double* p) const {
+    *p = KIND == GTK_NORM_INF ? __builtin_bit_cast(double, (uint64_t)m) : v;
+  }
+  __device__ __forceinline__ static Sum of(double d) {
+    Sum s;
+    if (KIND == GTK_NORM_INF)
+      s.m = (uint32_t)__builtin_bit_cast(uint64_t, d);
+    else
+      s.v = d;
+    return s;
+  }
+};
+
+template <int KIND, int WAVES> __device__ __forceinline__ Sum<KIND> block_join(Sum<KIND> s, double* red) {
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) {
+    Sum<KIND> o;
+    o.v = __shfl_xor(s.v, off, 64);
+    o.m = __shfl_xor(s.m, off, 64);
+    s.join(o);
+  }
+  if ((threadIdx.x & 63) == 0) s.put(red + (threadIdx.x >> 6));
+  __syncthreads();
+  s = Sum<KIND>::of(red[0]);
+#pragma unroll
+  for (int w = 1; w < WAVES; ++w) s.join(Sum<KIND>::of(red[w]));
+  return s;
+}
+
+// 16 bytes of values as floats.
+template <bool BF> __device__ __forceinline__ void widen(u32x4 raw, float* f) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (BF) {
+      f[2 * i] = __uint_as_float(raw[i] << 16);
+      f[2 * i + 1] = __uint_as_float(raw[i] & 0xffff0000u);
+    } else {
+      f[i] = __uint_as_float(raw[i]);
+    }
+  }
+}
+
+// The sum over p[0 .. n): U vectors of 16 bytes in flight a thread, then the
+// last n % VE values one a thread.
+template <int KIND, bool BF> __device__ __forceinline__ Sum<KIND> sum_run(const void* base, int64_t begin, uint32_t n) {
+  typedef typename std::conditional<BF, bf16, float>::type T;
+  constexpr uint32_t VE = BF ? 8 : 4, U = 4;
+  const T* p = (const T*)base + begin;
+  Sum<KIND> s[2];
+  const uint32_t vecs = n / VE;
+  uint32_t v = threadIdx.x;
+  for (; v + (U - 1) * kThreads < vecs; v += U * kThreads) {
+    u32x4 raw[U];
+#pragma unroll
+    for (uint32_t u = 0; u < U; ++u)
+      raw[u] = __builtin_nontemporal_load((const u32x4_any*)(p + (uint64_t)(v + u * kThreads) * VE));
+#pragma unroll
+    for (uint32_t u = 0; u < U; ++u) {
+      float f[VE];
+      widen<BF>(raw[u], f);
+#pragma unroll
+      for (uint32_t e = 0; e < VE; ++e) s[e & 1].add(f[e]);
+    }
+  }
+  for (; v < vecs; v += kThreads) {
+    float f[VE];
+    widen<BF>(*(const u32x4_any*)(p + (uint64_t)v * VE), f);
+#pragma unroll
+    for (uint32_t e = 0; e < VE; ++e) s[e & 1].add(f[e]);
+  }
+  if (threadIdx.x < n % VE) s[0].add(to_f32(p[(uint64_t)vecs * VE + threadIdx.x]));
+  s[0].join(s[1]);
+  return s[0];
 }
 
 template <int KIND>
-__global__ __launch_bounds__(1024) void grad_norm_close_kernel(const double* __restrict__ part, int64_t parts,
-                                                               float* __restrict__ norm) {
-  __shared__ double red[16];
-  double s = 0.0;
-  for (int64_t i = threadIdx.x; i < parts; i += 1024) {
-    if (KIND == GTK_NORM_INF) {
-      const uint64_t a = __builtin_bit_cast(uint64_t, s), b = __builtin_bit_cast(uint64_t, part[i]);
-      s = __builtin_bit_cast(double, a > b ? a : b);
-    } else {
-      s += part[i];
+__global__ __launch_bounds__(kThreads) void grad_partials_kernel(JobsIn J, double* __restrict__ part) {
+  __shared__ double red[kThreads / 64];
+  const int k = find_entry(J);
+  const uint32_t count = J.n[k] & kCountMask, block = blockIdx.x - J.first[k];
+  const int64_t begin = (int64_t)block * J.chunk;
+  const uint32_t n = (uint32_t)(begin + J.chunk < count ? J.chunk : count - begin);
+  const void* p = (const void*)J.src[k];
+  Sum<KIND> s = J.n[k] & kSrcBf ? sum_run<KIND, true>(p, begin, n) : sum_run<KIND, false>(p, begin, n);
+  s = block_join<KIND, kThreads / 64>(s, red);
+  if (threadIdx.x == 0) s.put(part + blockIdx.x);
+}
+
+constexpr int kCloseThreads = 1024;
+template <int KIND>
+__global__ __launch_bounds__(kCloseThreads) void grad_norm_close_kernel(const double* __restrict__ part, int64_t parts,
+                                                                        float* __restrict__ norm) {
+  __shared__ double red[kCloseThreads / 64];
+  constexpr int U = 8;
+  Sum<KIND> s;
+  for (int64_t i = threadIdx.x; i < parts; i += U * kCloseThreads) {
+    double d[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t at = i + u * kCloseThreads;
+      d[u] = part[at < parts ? at : parts - 1];
     }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (i + u * kCloseThreads < parts) s.join(Sum<KIND>::of(d[u]));
   }
-  s = block_join<KIND>(s, red);
-  if (threadIdx.x == 0) {
-    if (KIND == GTK_NORM_2) s = sqrt(s);
-    *norm = KIND == GTK_NORM_INF ? __uint_as_float((uint32_t)__builtin_bit_cast(uint64_t, s)) : (float)s;
-  }
+  s = block_join<KIND, kCloseThreads / 64>(s, red);
+  if (threadIdx.x == 0) *norm = KIND == GTK_NORM_INF ? __uint_as_float(s.m) : (float)(KIND == GTK_NORM_2 ? sqrt(s.v) : s.v);
 }
 
 // The factor of the clipping, one rounding to 32 bits.  A norm of NaN makes it
@@ -121,63 +194,127 @@ __device__ __forceinline__ float clip_factor(float norm, double max_norm) {
   return f > 1.0 ? 1.f : (float)f;
 }
 
-__global__ __launch_bounds__(256) void grad_scale_kernel(NormJobs J, const float* __restrict__ norm, double max_norm) {
-  int64_t begin, end;
-  const int k = find_job(J, begin, end);
-  const float f = clip_factor(*norm, max_norm);
-  for (int64_t i = begin + threadIdx.x; i < end; i += 256) {
-    const float v = grad_at(J.src[k], J.src_bf[k], i) * f;
-    if (J.dst_bf[k])
-      ((bf16*)J.dst[k])[i] = cvt<bf16>(v);
+template <bool SRC_BF, bool DST_BF> __device__ __forceinline__ void put_vec(void* dst, const float* f) {
+  if constexpr (DST_BF) {
+    if constexpr (SRC_BF)
+      *(u32x4_any*)dst = u32x4{pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]),
+                               pack_bf16x2(f[6], f[7])};
     else
-      ((float*)J.dst[k])[i] = v;
+      *(u32x2_any*)dst = u32x2{pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3])};
+  } else {
+#pragma unroll
+    for (int h = 0; h < (SRC_BF ? 2 : 1); ++h)
+      ((u32x4_any*)dst)[h] = u32x4{__float_as_uint(f[4 * h]), __float_as_uint(f[4 * h + 1]),
+                                   __float_as_uint(f[4 * h + 2]), __float_as_uint(f[4 * h + 3])};
   }
 }
 
-constexpr int64_t kChunk = 8192;
+// dst[i] = src[i] * k for i in [begin, begin + n).  No thread writes what another
+// reads, so dst may be src.
+template <bool SRC_BF, bool DST_BF>
+__device__ __forceinline__ void scale_run(const void* src, void* dst, int64_t begin, uint32_t n, float k) {
+  typedef typename std::conditional<SRC_BF, bf16, float>::type S;
+  typedef typename std::conditional<DST_BF, bf16, float>::type D;
+  constexpr uint32_t VE = SRC_BF ? 8 : 4, U = 4;
+  const S* p = (const S*)src + begin;
+  D* q = (D*)dst + begin;
+  const uint32_t vecs = n / VE;
+  uint32_t v = threadIdx.x;
+  for (; v + (U - 1) * kThreads < vecs; v += U * kThreads) {
+    u32x4 raw[U];
+#pragma unroll
+    for (uint32_t u = 0; u < U; ++u) raw[u] = *(const u32x4_any*)(p + (uint64_t)(v + u * kThreads) * VE);
+#pragma unroll
+    for (uint32_t u = 0; u < U; ++u) {
+      float f[VE];
+      widen<SRC_BF>(raw[u], f);
+#pragma unroll
+      for (uint32_t e = 0; e < VE; ++e) f[e] *= k;
+      put_vec<SRC_BF, DST_BF>(q + (uint64_t)(v + u * kThreads) * VE, f);
+    }
+  }
+  for (; v < vecs; v += kThreads) {
+    float f[VE];
+    widen<SRC_BF>(*(const u32x4_any*)(p + (uint64_t)v * VE), f);
+#pragma unroll
+    for (uint32_t e = 0; e < VE; ++e) f[e] *= k;
+    put_vec<SRC_BF, DST_BF>(q + (uint64_t)v * VE, f);
+  }
+  if (threadIdx.x < n % VE) {
+    const uint64_t i = (uint64_t)vecs * VE + threadIdx.x;
+    q[i] = cvt<D>(to_f32(p[i]) * k);
+  }
+}
 
-static int64_t total_blocks(const gtk_tensor_list* g) {
+template <typename J>
+__global__ __launch_bounds__(kThreads) void grad_scale_kernel(J jobs, const float* __restrict__ norm, double max_norm) {
+  const float f = clip_factor(*norm, max_norm);
+  if (!J::kOut && f == 1.f) return;  // the product would leave every value's bits
+  const int k = find_entry(jobs);
+  const uint32_t flags = jobs.n[k], count = flags & kCountMask, block = blockIdx.x - jobs.first[k];
+  const int64_t begin = (int64_t)block * jobs.chunk;
+  const uint32_t n = (uint32_t)(begin + jobs.chunk < count ? jobs.chunk : count - begin);
+  const void* src = (const void*)jobs.src[k];
+  void* dst = J::kOut ? (void*)jobs.dst[J::kOut ? k : 0] : (void*)src;
+  if (flags & kSrcBf) {
+    if (flags & kDstBf)
+      scale_run<true, true>(src, dst, begin, n, f);
+    else if (J::kOut)
+      scale_run<true, false>(src, dst, begin, n, f);
+  } else {
+    if (!(flags & kDstBf))
+      scale_run<false, false>(src, dst, begin, n, f);
+    else if (J::kOut)
+      scale_run<false, true>(src, dst, begin, n, f);
+  }
+}
+
+// Values a block, the same for the whole call: what spreads the call over some
+// 16 blocks a CU, in whole rounds of a block's loads.
+constexpr int64_t kMinChunk = 4096;
+static int64_t chunk_of(const gtk_tensor_list* g) {
+  int64_t total = 0;
+  for (int64_t i = 0; i < g->count; ++i) total += g->numel[i];
+  int64_t chunk = kMinChunk;
+  while (chunk < kMaxPart && total / chunk > 4096) chunk *= 2;
+  return chunk;
+}
+
+static int64_t total_blocks(const gtk_tensor_list* g, int64_t chunk) {
   int64_t b = 0;
-  for (int64_t i = 0; i < g->count; ++i) b += (g->numel[i] + kChunk - 1) / kChunk;
+  for (int64_t i = 0; i < g->count; ++i) b += (g->numel[i] + chunk - 1) / chunk;
   return b;
 }
 
-// Calls launch(jobs, blocks, first partial) for every kMaxTensors tensors.
-template <typename F>
-static int for_each_launch(const gtk_tensor_list* g, const gtk_tensor_list* out, F launch) {
-  NormJobs J;
-  J.chunk = kChunk;
-  J.count = 0;
-  J.first[0] = 0;
+// Calls launch(jobs, blocks, first partial) for every J::kMax entries.
+template <typename J, typename F>
+static int for_each_launch(const gtk_tensor_list* g, const gtk_tensor_list* out, int64_t chunk, F launch) {
+  J jobs;
+  jobs.chunk = (uint32_t)chunk;
+  jobs.count = 0;
+  uint32_t blocks = 0;
   int64_t base = 0;
-  auto flush = [&]() -> int {
-    if (J.count == 0) return GTK_OK;
-    const int rc = launch(J, (unsigned)J.first[J.count], base);
-    base += J.first[J.count];
-    J.count = 0;
-    return rc;
-  };
+  const gtk_tensor_list* o = out ? out : g;
   for (int64_t i = 0; i < g->count; ++i) {
-    // a large tensor takes several entries: block counts stay in 32 bits
-    for (int64_t at = 0; at < g->numel[i];) {
-      const int64_t n = std::min<int64_t>(g->numel[i] - at, kChunk << 16);
-      const int k = J.count++;
-      const int64_t sb = g->dtype[i] == GTK_BF16 ? 2 : 4;
-      J.src[k] = (const char*)g->data[i] + at * sb;
-      J.src_bf[k] = g->dtype[i] == GTK_BF16;
-      const gtk_tensor_list* o = out ? out : g;
-      J.dst[k] = (char*)o->data[i] + at * (o->dtype[i] == GTK_BF16 ? 2 : 4);
-      J.dst_bf[k] = o->dtype[i] == GTK_BF16;
-      J.n[k] = n;
-      J.first[k + 1] = J.first[k] + (int)((n + kChunk - 1) / kChunk);
-      at += n;
-      if (J.count == kMaxTensors) {
-        const int rc = flush();
+    const bool sbf = g->dtype[i] == GTK_BF16, dbf = o->dtype[i] == GTK_BF16;
+    const uint32_t flags = (sbf ? kSrcBf : 0) | (dbf ? kDstBf : 0);
+    for (int64_t at = 0; at < g->numel[i]; at += kMaxPart) {
+      const int64_t n = std::min(g->numel[i] - at, kMaxPart);
+      const uint32_t k = jobs.count++;
+      jobs.src[k] = (uint64_t)(uintptr_t)g->data[i] + (uint64_t)at * (sbf ? 2 : 4);
+      if (J::kOut) jobs.dst[J::kOut ? k : 0] = (uint64_t)(uintptr_t)o->data[i] + (uint64_t)at * (dbf ? 2 : 4);
+      jobs.n[k] = (uint32_t)n | flags;
+      jobs.first[k] = blocks;
+      blocks += (uint32_t)((n + chunk - 1) / chunk);
+      if (jobs.count == (uint32_t)J::kMax || blocks >= 1u << 22) {
+        const int rc = launch(jobs, blocks, base);
         if (rc) return rc;
+        base += blocks;
+        jobs.count = blocks = 0;
       }
     }
   }
-  return flush();
+  return jobs.count ? launch(jobs, blocks, base) : GTK_OK;
 }
 
 static int check_list(const gtk_tensor_list* g, const char* name) {
@@ -230,17 +367,18 @@ static int check_overlap(const gtk_tensor_list* g, const gtk_tensor_list* out, c
 
 template <int KIND>
 static int launch_norm(const gtk_tensor_list* g, float* norm, double* part, hipStream_t st) {
+  const int64_t chunk = chunk_of(g);
   {
     StageTimer timer("grad_partials", st);
-    const int rc = for_each_launch(g, nullptr, [&](const NormJobs& J, unsigned blocks, int64_t base) -> int {
-      grad_partials_kernel<KIND><<<blocks, 256, 0, st>>>(J, part + base);
+    const int rc = for_each_launch<JobsIn>(g, nullptr, chunk, [&](const JobsIn& J, unsigned blocks, int64_t base) -> int {
+      grad_partials_kernel<KIND><<<blocks, kThreads, 0, st>>>(J, part + base);
       GTK_LAUNCH_CHECK();
       return GTK_OK;
     });
     if (rc) return rc;
   }
   StageTimer timer("grad_norm_close", st);
-  grad_norm_close_kernel<KIND><<<1, 1024, 0, st>>>(part, total_blocks(g), norm);
+  grad_norm_close_kernel<KIND><<<1, kCloseThreads, 0, st>>>(part, total_blocks(g, chunk), norm);
   GTK_LAUNCH_CHECK();
   return GTK_OK;
 }
@@ -253,14 +391,20 @@ static int launch_norm(int kind, const gtk_tensor_list* g, float* norm, double* 
   }
 }
 
+template <typename J>
 static int launch_scale(const gtk_tensor_list* g, const gtk_tensor_list* out, double max_norm, const float* norm,
                         hipStream_t st) {
   StageTimer timer("grad_scale", st);
-  return for_each_launch(g, out, [&](const NormJobs& J, unsigned blocks, int64_t) -> int {
-    grad_scale_kernel<<<blocks, 256, 0, st>>>(J, norm, max_norm);
+  return for_each_launch<J>(g, out, chunk_of(g), [&](const J& jobs, unsigned blocks, int64_t) -> int {
+    grad_scale_kernel<J><<<blocks, kThreads, 0, st>>>(jobs, norm, max_norm);
     GTK_LAUNCH_CHECK();
     return GTK_OK;
   });
+}
+
+static int launch_scale(const gtk_tensor_list* g, const gtk_tensor_list* out, double max_norm, const float* norm,
+                        hipStream_t st) {
+  return out ? launch_scale<JobsInOut>(g, out, max_norm, norm, st) : launch_scale<JobsIn>(g, out, max_norm, norm, st);
 }
 
 static int check_out(const gtk_tensor_list* g, const gtk_tensor_list* out, const char* name) {
@@ -292,7 +436,7 @@ using namespace gtk;
 
 extern "C" size_t gtk_grad_norm_workspace_size(const gtk_tensor_list* grads) {
   if (check_list(grads, "gtk_grad_norm_workspace_size")) return 0;
-  return sizeof(double) * (size_t)std::max<int64_t>(1, total_blocks(grads));
+  return sizeof(double) * (size_t)std::max<int64_t>(1, total_blocks(grads, chunk_of(grads)));
 }
 
 extern "C" int gtk_grad_norm(const gtk_tensor_list* grads, int kind, float* norm, void* workspace,

@@ -739,27 +739,53 @@ at::Tensor layer_norm(const at::Tensor& x, const c10::optional<at::Tensor>& weig
 // ---------------------------------------------------------------------------
 // Global gradient norm and clipping
 // ---------------------------------------------------------------------------
-// A list of tensors as the C functions take it.
-struct TensorList {
+// Gradients as the C functions take them.  The tensors are those of a Python
+// sequence, or with `grads_of` their .grad (ones without are passed over), and
+// are not copied: a net has hundreds of small ones, and the host time of a call
+// is theirs.
+struct GradList {
+  std::vector<const at::Tensor*> t;
   std::vector<void*> data;
   std::vector<int64_t> numel;
   std::vector<int> dtype;
-  void add(const at::Tensor& t) {
-    data.push_back(t.data_ptr());
-    numel.push_back(t.numel());
-    dtype.push_back(gtk_dtype_of(t, "a gradient"));
-  }
-  gtk_tensor_list list() const {
-    return {(int64_t)data.size(), data.data(), numel.data(), dtype.data()};
-  }
-};
+  py::object items;  // holds the tensors
 
-void check_grads(const std::vector<at::Tensor>& ts, const at::Tensor& like) {
-  for (const auto& t : ts) {
-    TORCH_CHECK(t.defined() && t.layout() == at::kStrided, "genie_tk._C: a gradient is not a dense tensor");
-    check_on(t, like, "a gradient");
+  // What the kernels take: bf16 or fp32, strided, on one GPU.  Otherwise false
+  // without `strict`, and an error with it.
+  bool collect(const py::handle& seq, bool grads_of, bool strict) {
+    items = py::reinterpret_steal<py::object>(PySequence_Fast(seq.ptr(), "expected a sequence of tensors"));
+    if (!items) throw py::error_already_set();
+    const Py_ssize_t n = PySequence_Fast_GET_SIZE(items.ptr());
+    PyObject** it = PySequence_Fast_ITEMS(items.ptr());
+    t.reserve(n);
+    for (Py_ssize_t i = 0; i < n; ++i) {
+      TORCH_CHECK_TYPE(THPVariable_Check(it[i]), "genie_tk._C: item ", i, " is not a tensor");
+      const at::Tensor* v = &THPVariable_Unpack(it[i]);
+      if (grads_of) v = &v->grad();
+      if (v->defined()) t.push_back(v);
+    }
+    for (const auto* v : t) {
+      const bool ok = v->is_cuda() && v->layout() == at::kStrided && v->device() == t[0]->device() &&
+                      (v->scalar_type() == at::kFloat || v->scalar_type() == at::kBFloat16);
+      if (ok) continue;
+      if (!strict) return false;
+      check_gpu(*v, "gradients");
+      TORCH_CHECK(v->layout() == at::kStrided, "genie_tk._C: a gradient is not a dense tensor");
+      check_on(*v, *t[0], "a gradient");
+      gtk_dtype_of(*v, "a gradient");
+    }
+    data.reserve(t.size());
+    numel.reserve(t.size());
+    dtype.reserve(t.size());
+    return true;
   }
-}
+  void add(const at::Tensor& v) {
+    data.push_back(v.data_ptr());
+    numel.push_back(v.numel());
+    dtype.push_back(v.scalar_type() == at::kFloat ? GTK_F32 : GTK_BF16);
+  }
+  gtk_tensor_list list() const { return {(int64_t)data.size(), data.data(), numel.data(), dtype.data()}; }
+};
 
 int norm_kind(double p) {
   if (p == 2.0) return GTK_NORM_2;
@@ -768,59 +794,51 @@ int norm_kind(double p) {
   return GTK_NORM_INF;
 }
 
-// The order of a norm's values does not matter: a tensor that fills its memory
-// is taken as it lies, any other is copied.
-at::Tensor as_run(const at::Tensor& t) {
-  return t.is_contiguous() || t.is_non_overlapping_and_dense() ? t : t.contiguous();
-}
-
-at::Tensor grad_norm(const std::vector<at::Tensor>& ts, double p) {
-  TORCH_CHECK(!ts.empty(), "grad_norm expects at least one tensor");
-  check_gpu(ts[0], "gradients");
-  check_grads(ts, ts[0]);
+// The norm of the tensors; without `strict`, None where a tensor is not one for
+// the kernels.
+c10::optional<at::Tensor> grad_norm(const py::handle& tensors, double p, bool strict) {
+  GradList l;
   const int kind = norm_kind(p);
-  const at::DeviceGuard guard(ts[0].device());
+  if (!l.collect(tensors, false, strict)) return c10::nullopt;
+  TORCH_CHECK(!l.t.empty(), "grad_norm expects at least one tensor");
+  const at::Tensor& like = *l.t[0];
+  const at::DeviceGuard guard(like.device());
   std::vector<at::Tensor> copies;  // alive until the launch is enqueued
-  TensorList l;
-  for (const auto& t : ts) {
-    auto r = as_run(t);
-    l.add(r);
-    if (!r.is_same(t)) copies.push_back(r);
+  for (const auto* t : l.t) {
+    // the order of the values does not matter: a tensor that fills its memory
+    // is taken as it lies, any other is copied
+    if (t->is_contiguous() || t->is_non_overlapping_and_dense()) {
+      l.add(*t);
+    } else {
+      copies.push_back(t->contiguous());
+      l.add(copies.back());
+    }
   }
   const auto g = l.list();
-  auto norm = at::empty({}, ts[0].options().dtype(at::kFloat));
-  auto ws = workspace(ts[0], gtk_grad_norm_workspace_size(&g));
-  check_rc(gtk_grad_norm(&g, kind, norm.data_ptr<float>(), ws.data_ptr(), ws.numel(), cur_stream(ts[0])));
+  auto norm = at::empty({}, like.options().dtype(at::kFloat));
+  auto ws = workspace(like, gtk_grad_norm_workspace_size(&g));
+  check_rc(gtk_grad_norm(&g, kind, norm.data_ptr<float>(), ws.data_ptr(), ws.numel(), cur_stream(like)));
   return norm;
 }
 
-// Clips ts into outs (in place without them).  norm: given, or undefined:
-// computed, and returned.
-at::Tensor grad_clip_impl(const std::vector<at::Tensor>& ts, const c10::optional<std::vector<at::Tensor>>& outs,
-                          double max_norm, double p, at::Tensor norm) {
-  TORCH_CHECK(!ts.empty(), "grad_clip expects at least one tensor");
-  check_gpu(ts[0], "gradients");
-  check_grads(ts, ts[0]);
-  if (outs.has_value()) {
-    TORCH_CHECK(outs->size() == ts.size(), "genie_tk._C: ", outs->size(), " outputs for ", ts.size(), " gradients");
-    check_grads(*outs, ts[0]);
-  }
+// Clips l into lo (in place without it).  norm: given, or undefined: computed,
+// and returned.
+at::Tensor clip_list(GradList& l, GradList* lo, double max_norm, double p, at::Tensor norm) {
+  const at::Tensor& like = *l.t[0];
   const bool given = norm.defined();
   const int kind = given ? GTK_NORM_2 : norm_kind(p);
-  const at::DeviceGuard guard(ts[0].device());
+  const at::DeviceGuard guard(like.device());
   // Tensors that are no run of memory in the other's order are clipped on
   // copies, which are copied back at the end.
   std::vector<std::pair<at::Tensor, at::Tensor>> back;
   std::vector<at::Tensor> copies;
-  TensorList l, lo;
-  for (size_t i = 0; i < ts.size(); ++i) {
-    const auto& t = ts[i];
-    const auto& o = outs.has_value() ? (*outs)[i] : t;
-    TORCH_CHECK(o.sizes() == t.sizes(), "genie_tk._C: output ", i, " has another shape");
+  for (size_t i = 0; i < l.t.size(); ++i) {
+    const at::Tensor &t = *l.t[i], &o = lo ? *lo->t[i] : t;
+    TORCH_CHECK(!lo || o.sizes() == t.sizes(), "genie_tk._C: output ", i, " has another shape");
     if ((t.is_contiguous() && o.is_contiguous()) ||
         (t.strides() == o.strides() && t.is_non_overlapping_and_dense())) {
       l.add(t);
-      if (outs.has_value()) lo.add(o);
+      if (lo) lo->add(o);
       continue;
     }
     at::assert_no_internal_overlap(o);
@@ -829,41 +847,66 @@ at::Tensor grad_clip_impl(const std::vector<at::Tensor>& ts, const c10::optional
                   "genie_tk._C: a tensor that is written is given twice");
     copies.push_back(t.contiguous());
     l.add(copies.back());
-    if (outs.has_value()) {
+    if (lo) {
       back.emplace_back(o, at::empty(o.sizes(), o.options().memory_format(at::MemoryFormat::Contiguous)));
-      lo.add(back.back().second);
+      lo->add(back.back().second);
     } else {
       back.emplace_back(o, copies.back());
     }
   }
-  const auto g = l.list(), go = lo.list();
-  const gtk_tensor_list* out = outs.has_value() ? &go : nullptr;
-  void* st = cur_stream(ts[0]);
+  const auto g = l.list(), go = lo ? lo->list() : gtk_tensor_list{};
+  const gtk_tensor_list* out = lo ? &go : nullptr;
+  void* st = cur_stream(like);
   if (given) {
     check_rc(gtk_grad_clip_with_norm(&g, out, max_norm, norm.data_ptr<float>(), st));
   } else {
-    norm = at::empty({}, ts[0].options().dtype(at::kFloat));
-    auto ws = workspace(ts[0], gtk_grad_norm_workspace_size(&g));
+    norm = at::empty({}, like.options().dtype(at::kFloat));
+    auto ws = workspace(like, gtk_grad_norm_workspace_size(&g));
     check_rc(gtk_grad_clip(&g, out, kind, max_norm, norm.data_ptr<float>(), ws.data_ptr(), ws.numel(), st));
   }
   for (auto& b : back) b.first.copy_(b.second);
   // written behind autograd's back
-  for (const auto& t : outs.has_value() ? *outs : ts)
-    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+  for (const auto* t : lo ? lo->t : l.t)
+    if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
   return norm;
 }
 
-at::Tensor grad_clip(const std::vector<at::Tensor>& ts, const c10::optional<std::vector<at::Tensor>>& outs,
-                     double max_norm, double p) {
-  return grad_clip_impl(ts, outs, max_norm, p, at::Tensor());
+c10::optional<at::Tensor> grad_clip(const py::handle& tensors, const py::handle& outs, double max_norm, double p,
+                                    bool strict) {
+  GradList l, lo;
+  norm_kind(p);
+  if (!l.collect(tensors, false, strict)) return c10::nullopt;
+  TORCH_CHECK(!l.t.empty(), "grad_clip expects at least one tensor");
+  if (outs.is_none()) return clip_list(l, nullptr, max_norm, p, at::Tensor());
+  if (!lo.collect(outs, false, strict)) return c10::nullopt;
+  TORCH_CHECK(lo.t.size() == l.t.size(), "genie_tk._C: ", lo.t.size(), " outputs for ", l.t.size(), " gradients");
+  check_on(*lo.t[0], *l.t[0], "an output");
+  return clip_list(l, &lo, max_norm, p, at::Tensor());
 }
 
-void grad_clip_with_norm(const std::vector<at::Tensor>& ts, const c10::optional<std::vector<at::Tensor>>& outs,
-                         double max_norm, const at::Tensor& norm) {
-  TORCH_CHECK(!ts.empty(), "grad_clip_with_norm expects at least one tensor");
-  check_on(norm, ts[0], "norm");
+// grad_clip in place on the gradients of `parameters`: the norm, or None where
+// there is no gradient or one that is not for the kernels.
+c10::optional<at::Tensor> grad_clip_parameters(const py::handle& parameters, double max_norm, double p) {
+  GradList l;
+  norm_kind(p);
+  if (!l.collect(parameters, true, false) || l.t.empty()) return c10::nullopt;
+  return clip_list(l, nullptr, max_norm, p, at::Tensor());
+}
+
+void grad_clip_with_norm(const py::handle& tensors, const py::handle& outs, double max_norm, const at::Tensor& norm) {
+  GradList l, lo;
+  l.collect(tensors, false, true);
+  TORCH_CHECK(!l.t.empty(), "grad_clip_with_norm expects at least one tensor");
+  check_on(norm, *l.t[0], "norm");
   TORCH_CHECK(norm.numel() == 1 && norm.scalar_type() == at::kFloat, "norm must be one float32 value");
-  grad_clip_impl(ts, outs, max_norm, 2.0, norm);
+  if (outs.is_none()) {
+    clip_list(l, nullptr, max_norm, 2.0, norm);
+    return;
+  }
+  lo.collect(outs, false, true);
+  TORCH_CHECK(lo.t.size() == l.t.size(), "genie_tk._C: ", lo.t.size(), " outputs for ", l.t.size(), " gradients");
+  check_on(*lo.t[0], *l.t[0], "an output");
+  clip_list(l, &lo, max_norm, 2.0, norm);
 }
 
 py::dict timing_report() {
@@ -955,10 +998,15 @@ PYBIND11_MODULE(_C, m) {
         "layer_norm_forward's backward: [dx, dweight, dbias], None where not needed", py::arg("x"), py::arg("dy"),
         py::arg("weight") = py::none(), py::arg("eps") = 1e-5, py::arg("need_x") = true,
         py::arg("need_weight") = true, py::arg("need_bias") = true);
-  m.def("grad_norm", &grad_norm, "Norm over every value of the tensors (fp32 scalar; norm_type 1, 2 or inf)",
-        py::arg("tensors"), py::arg("norm_type") = 2.0);
+  m.def("grad_norm", &grad_norm,
+        "Norm over every value of the tensors (fp32 scalar; norm_type 1, 2 or inf).  Without strict, None where a "
+        "tensor is not bf16 or fp32 on one GPU",
+        py::arg("tensors"), py::arg("norm_type") = 2.0, py::arg("strict") = true);
   m.def("grad_clip", &grad_clip, "Clip the tensors by their global norm into outs (None: in place); the norm",
-        py::arg("tensors"), py::arg("outs"), py::arg("max_norm"), py::arg("norm_type") = 2.0);
+        py::arg("tensors"), py::arg("outs"), py::arg("max_norm"), py::arg("norm_type") = 2.0, py::arg("strict") = true);
+  m.def("grad_clip_parameters", &grad_clip_parameters,
+        "grad_clip in place on the parameters' gradients; None where there is none, or one not for the kernels",
+        py::arg("parameters"), py::arg("max_norm"), py::arg("norm_type") = 2.0);
   m.def("grad_clip_with_norm", &grad_clip_with_norm, "grad_clip by a given norm (one float32 value on the GPU)",
         py::arg("tensors"), py::arg("outs"), py::arg("max_norm"), py::arg("norm"));
   m.def("version", []() { return gtk_version(); });

@@ -22,13 +22,14 @@ from genie_tk import _dispatch, _ext
 _EPS = 1e-6  # torch.nn.utils' addend of the norm
 
 
-def _on_kernels(tensors: Sequence[Tensor], norm_type: float) -> bool:
-    if not tensors[0].is_cuda:
-        return False
-    if _ext.C is None or not torch.cuda.is_available():
+def _kernels(like: Tensor, norm_type: float):
+    """The extension, where the kernels have this norm and ``like`` is on a GPU
+    (whether every tensor is one for them is for the extension to see)."""
+    if not like.is_cuda or norm_type not in (1.0, 2.0, math.inf):
+        return None
+    if _ext.C is None:
         _ext.missing("gradients")
-        return False
-    return norm_type in (1.0, 2.0, math.inf) and all(t.dtype in _dispatch.SUPPORTED_DTYPES for t in tensors)
+    return _ext.C
 
 
 def _check(tensors: Sequence[Tensor], what: str) -> None:
@@ -74,9 +75,11 @@ def grad_norm(tensors: Iterable[Tensor], norm_type: float = 2.0) -> Tensor:
     norm_type = float(norm_type)
     if not tensors:
         return torch.zeros(())
+    C = _kernels(tensors[0], norm_type)
+    norm = None if C is None else C.grad_norm(tensors, norm_type, False)
+    if norm is not None:
+        return norm
     _check(tensors, "grad_norm")
-    if _on_kernels(tensors, norm_type):
-        return _ext.C.grad_norm(tensors, norm_type)
     return _norm_pytorch(tensors, norm_type)
 
 
@@ -93,14 +96,16 @@ def clip_grads(grads: Iterable[Tensor], max_norm: float, norm_type: float = 2.0,
     if not grads:
         return torch.zeros(()), []
     outs = [torch.empty_like(g) for g in grads] if out is None else list(out)
+    C = _kernels(grads[0], norm_type)
+    norm = None if C is None else C.grad_clip(grads, outs, max_norm, norm_type, False)
+    if norm is not None:
+        return norm, outs
     _check(grads, "clip_grads")
     _check(outs, "clip_grads")
     for g, o in zip(grads, outs):
         if g.shape != o.shape or g.device != o.device:
             raise ValueError(f"clip_grads: an output is {tuple(o.shape)} on {o.device} for a gradient "
                              f"{tuple(g.shape)} on {g.device}")
-    if _on_kernels(grads + outs, norm_type):
-        return _ext.C.grad_clip(grads, outs, max_norm, norm_type), outs
     norm = _norm_pytorch(grads, norm_type)
     _clip_pytorch(grads, outs, max_norm, norm)
     return norm, outs
@@ -114,20 +119,19 @@ def clip_grad_norm_(parameters: Union[Tensor, Iterable[Tensor]], max_norm: float
     passed over.  ``error_if_nonfinite`` looks at the norm on the host first (it
     waits for the GPU) and raises RuntimeError with the gradients untouched."""
     max_norm, norm_type = _check_max_norm(max_norm, "clip_grad_norm_"), float(norm_type)
+    parameters = [parameters] if isinstance(parameters, Tensor) else list(parameters)
+    if parameters and not error_if_nonfinite:
+        C = _kernels(parameters[0], norm_type)
+        norm = None if C is None else C.grad_clip_parameters(parameters, max_norm, norm_type)
+        if norm is not None:
+            return norm
     grads = _grads_of(parameters)
     if not grads:
         return torch.zeros(())
-    _check(grads, "clip_grad_norm_")
-    if error_if_nonfinite:
-        norm = grad_norm(grads, norm_type)
-        if not math.isfinite(float(norm)):
-            raise RuntimeError(f"clip_grad_norm_: the gradients' norm of order {norm_type} is {float(norm)}")
-        _clip_with_norm(grads, max_norm, norm)
-        return norm
-    if _on_kernels(grads, norm_type):
-        return _ext.C.grad_clip(grads, None, max_norm, norm_type)
-    norm = _norm_pytorch(grads, norm_type)
-    _clip_pytorch(grads, grads, max_norm, norm)
+    norm = grad_norm(grads, norm_type)
+    if error_if_nonfinite and not math.isfinite(float(norm)):
+        raise RuntimeError(f"clip_grad_norm_: the gradients' norm of order {norm_type} is {float(norm)}")
+    _clip_with_norm(grads, max_norm, norm)
     return norm
 
 
@@ -146,10 +150,12 @@ def clip_grads_with_norm_(parameters: Union[Tensor, Iterable[Tensor]], max_norm:
 
 
 def _clip_with_norm(grads: Sequence[Tensor], max_norm: float, total_norm: Tensor) -> None:
-    if _on_kernels(grads, 2.0):
-        _ext.C.grad_clip_with_norm(grads, None, max_norm, total_norm)
-    else:
-        _clip_pytorch(grads, grads, max_norm, total_norm)
+    if all(g.is_cuda and g.dtype in _dispatch.SUPPORTED_DTYPES for g in grads):
+        C = _kernels(grads[0], 2.0)
+        if C is not None:
+            C.grad_clip_with_norm(grads, None, max_norm, total_norm)
+            return
+    _clip_pytorch(grads, grads, max_norm, total_norm)
 
 
 def _grads_of(parameters: Union[Tensor, Iterable[Tensor]]) -> List[Tensor]:
