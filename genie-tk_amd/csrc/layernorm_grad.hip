@@ -44,7 +44,7 @@ typedef u32x4 u32x4_any __attribute__((aligned(2)));
 template <typename T, int VE> struct Vec {
   u32x4 raw;
   __device__ __forceinline__ void load(const T* p) { raw = __builtin_nontemporal_load((const u32x4_any*)p); }
-  __device__ __forceinline__ void store(T* p) const { *(u32x4_any*)p = raw; }
+  __device__ __forceinline__ void store(T* p) const { __builtin_nontemporal_store(raw, (u32x4_any*)p); }
   __device__ __forceinline__ void get(float* f) const {
     if constexpr (sizeof(T) == 2) {
 #pragma unroll
@@ -403,25 +403,67 @@ template <int K> __device__ __forceinline__ void block_sums(float (&v)[K], float
   }
 }
 
+// Calls f(c, skip) for this thread's vectors of a row: at column c, of which
+// the first `skip` values belong to another thread's vector (the last one ends
+// at the row's end).
+template <typename T, typename F> __device__ __forceinline__ void for_vectors(int D, F f) {
+  constexpr int VE = 16 / sizeof(T);
+#pragma unroll 4
+  for (int c = threadIdx.x * VE; c < D; c += kWideThreads * VE) {
+    const int at = c + VE <= D ? c : D - VE;
+    f(at, c - at);
+  }
+}
+
 template <typename T>
 __global__ __launch_bounds__(kWideThreads) void ln_forward_wide_kernel(const T* __restrict__ x, int64_t xs,
                                                                        T* __restrict__ y, ParamVec w, ParamVec b,
                                                                        int64_t rows, int D, float eps) {
+  constexpr int VE = 16 / sizeof(T);
   __shared__ float red[16];
   for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
     const T* xr = x + r * xs;
     float s[1] = {0.f}, q[1] = {0.f};
-    for (int c = threadIdx.x; c < D; c += kWideThreads) s[0] += to_f32(xr[c]);
+    for_vectors<T>(D, [&](int c, int skip) {
+      Vec<T, VE> v;
+      float f[VE];
+      v.load(xr + c);
+      v.get(f);
+#pragma unroll
+      for (int e = 0; e < VE; ++e) s[0] += e >= skip ? f[e] : 0.f;
+    });
     block_sums(s, red);
     const float mean = s[0] / (float)D;
-    for (int c = threadIdx.x; c < D; c += kWideThreads) {
-      const float d = to_f32(xr[c]) - mean;
-      q[0] += d * d;
-    }
+    for_vectors<T>(D, [&](int c, int skip) {
+      Vec<T, VE> v;
+      float f[VE];
+      v.load(xr + c);
+      v.get(f);
+#pragma unroll
+      for (int e = 0; e < VE; ++e) {
+        const float d = f[e] - mean;
+        q[0] += e >= skip ? d * d : 0.f;
+      }
+    });
     block_sums(q, red);
     const float rstd = 1.0f / sqrtf(q[0] / (float)D + eps);
-    for (int c = threadIdx.x; c < D; c += kWideThreads)
-      y[r * D + c] = cvt<T>((to_f32(xr[c]) - mean) * rstd * w.get(c, 1.f) + b.get(c, 0.f));
+    for_vectors<T>(D, [&](int c, int) {
+      Vec<T, VE> v;
+      float f[VE], wf[VE], bf[VE];
+      v.load(xr + c);
+      v.get(f);
+#pragma unroll
+      for (int e = 0; e < VE; ++e) {
+        wf[e] = 1.f;
+        bf[e] = 0.f;
+      }
+      if (w.p) load_run<VE>(wf, w, c);
+      if (b.p) load_run<VE>(bf, b, c);
+#pragma unroll
+      for (int e = 0; e < VE; ++e) f[e] = (f[e] - mean) * rstd * wf[e] + bf[e];
+      v.set(f);
+      v.store(y + r * D + c);
+    });
   }
 }
 
@@ -432,29 +474,62 @@ __global__ __launch_bounds__(kWideThreads) void ln_backward_wide_kernel(const T*
                                                                         T* __restrict__ dx, ParamVec w,
                                                                         float2* __restrict__ stats, int64_t rows, int D,
                                                                         float eps) {
+  constexpr int VE = 16 / sizeof(T);
   __shared__ float red[48];
   for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
     const T* xr = x + r * xs;
     const T* dr = dy + r * ds;
     float s[1] = {0.f}, m[3] = {0.f, 0.f, 0.f};
-    for (int c = threadIdx.x; c < D; c += kWideThreads) s[0] += to_f32(xr[c]);
+    for_vectors<T>(D, [&](int c, int skip) {
+      Vec<T, VE> v;
+      float f[VE];
+      v.load(xr + c);
+      v.get(f);
+#pragma unroll
+      for (int e = 0; e < VE; ++e) s[0] += e >= skip ? f[e] : 0.f;
+    });
     block_sums(s, red);
     const float mean = s[0] / (float)D;
-    for (int c = threadIdx.x; c < D; c += kWideThreads) {
-      const float d = to_f32(xr[c]) - mean;
-      const float g = to_f32(dr[c]) * w.get(c, 1.f);
-      m[0] += d * d;
-      m[1] += g;
-      m[2] += g * d;
-    }
+    // x - mean and dy w at column c
+    auto load = [&](int c, float* d, float* g) {
+      Vec<T, VE> xv, gv;
+      float wf[VE];
+      xv.load(xr + c);
+      gv.load(dr + c);
+      xv.get(d);
+      gv.get(g);
+      if (w.p) {
+        load_run<VE>(wf, w, c);
+#pragma unroll
+        for (int e = 0; e < VE; ++e) g[e] *= wf[e];
+      }
+#pragma unroll
+      for (int e = 0; e < VE; ++e) d[e] -= mean;
+    };
+    for_vectors<T>(D, [&](int c, int skip) {
+      float d[VE], g[VE];
+      load(c, d, g);
+#pragma unroll
+      for (int e = 0; e < VE; ++e) {
+        const float dm = e >= skip ? d[e] : 0.f, gm = e >= skip ? g[e] : 0.f;
+        m[0] += dm * dm;
+        m[1] += gm;
+        m[2] += gm * dm;
+      }
+    });
     block_sums(m, red);
     const float rstd = 1.0f / sqrtf(m[0] / (float)D + eps);
     const float c1 = m[1] / (float)D, c2 = m[2] / (float)D * rstd;
     if (dx)
-      for (int c = threadIdx.x; c < D; c += kWideThreads) {
-        const float h = (to_f32(xr[c]) - mean) * rstd;
-        dx[r * D + c] = cvt<T>((to_f32(dr[c]) * w.get(c, 1.f) - c1 - h * c2) * rstd);
-      }
+      for_vectors<T>(D, [&](int c, int) {
+        float d[VE], g[VE];
+        load(c, d, g);
+#pragma unroll
+        for (int e = 0; e < VE; ++e) d[e] = (g[e] - c1 - d[e] * rstd * c2) * rstd;
+        Vec<T, VE> v;
+        v.set(d);
+        v.store(dx + r * D + c);
+      });
     if (threadIdx.x == 0) stats[r] = float2{mean, rstd};
   }
 }
@@ -534,32 +609,37 @@ static int launch_ln_close(const float* part, int parts, int D, void* dw, void* 
 // ---------------------------------------------------------------------------
 // Shapes by width
 // ---------------------------------------------------------------------------
-// Calls run(Shape) for the narrowest shape that holds D.
-template <typename T, int VE, int NV, int L, int W, int BT, int U, typename F>
+// Calls run(Shape) for the narrowest shape that holds D: U rows a lane group at
+// once where the shape is filled, UM where it is not.
+template <typename T, int VE, int NV, int L, int W, int BT, int U, int UM, typename F>
 static int with_shape(int D, F& run) {
   if (D == VE * NV * L * W) return run(Shape<T, VE, NV, L, W, BT, U, true>());
-  return run(Shape<T, VE, NV, L, W, BT, U, false>());
+  return run(Shape<T, VE, NV, L, W, BT, UM, false>());
 }
 
 template <typename T, bool BACKWARD, typename F> static int for_shape(int D, F run) {
   constexpr int VE = 16 / sizeof(T);
-  constexpr int U = BACKWARD ? 1 : 2;
-  constexpr int B1 = BACKWARD ? 512 : 256;                        // a wave or less a row
-  constexpr int B2 = BACKWARD ? 1024 : 256, B8 = BACKWARD ? 1024 : 512;  // two or four, eight waves a row
-  if (D < VE) return run(Shape<T, 1, 1, VE, 1, B1, U, false>());
-  if (D <= 2 * VE) return with_shape<T, VE, 1, 2, 1, B1, U>(D, run);
-  if (D <= 4 * VE) return with_shape<T, VE, 1, 4, 1, B1, U>(D, run);
-  if (D <= 8 * VE) return with_shape<T, VE, 1, 8, 1, B1, U>(D, run);
-  if (D <= 16 * VE) return with_shape<T, VE, 1, 16, 1, B1, U>(D, run);
-  if (D <= 32 * VE) return with_shape<T, VE, 1, 32, 1, B1, U>(D, run);
-  if (D <= 64 * VE) return with_shape<T, VE, 1, 64, 1, B1, U>(D, run);
-  if (D <= 128 * VE) return with_shape<T, VE, 1, 64, 2, B2, U>(D, run);
-  if (D <= 256 * VE) return with_shape<T, VE, 1, 64, 4, B2, U>(D, run);
-  if (D <= 512 * VE) return with_shape<T, VE, 1, 64, 8, B8, U>(D, run);
-  if (D <= 1024 * VE) return with_shape<T, VE, 1, 64, 16, 1024, U>(D, run);
-  return with_shape<T, VE, 2, 64, 16, 1024, U>(D, run);  // up to widest_in_registers
+  // a wave or less a row
+  constexpr int B = BACKWARD ? 512 : 256, UM = BACKWARD ? 1 : 2;
+  if (D < VE) return run(Shape<T, 1, 1, VE, 1, B, UM, false>());
+  if (D <= 2 * VE) return with_shape<T, VE, 1, 2, 1, B, 2, UM>(D, run);
+  if (D <= 4 * VE) return with_shape<T, VE, 1, 4, 1, B, 2, UM>(D, run);
+  if (D <= 8 * VE) return with_shape<T, VE, 1, 8, 1, B, 2, UM>(D, run);
+  if (D <= 16 * VE) return with_shape<T, VE, 1, 16, 1, B, 2, UM>(D, run);
+  if (D <= 32 * VE) return with_shape<T, VE, 1, 32, 1, B, 2, UM>(D, run);
+  if (D <= 64 * VE) return with_shape<T, VE, 1, 64, 1, B, 2, UM>(D, run);
+  // several waves: the backward's registers hold one row, and one block a CU
+  // leaves the fewest partial sums
+  constexpr int U = BACKWARD ? 1 : 2, BW = BACKWARD ? 1024 : 0;
+  if (D <= 128 * VE) return with_shape<T, VE, 1, 64, 2, BW ? BW : 256, U, U>(D, run);
+  if (D <= 256 * VE) return with_shape<T, VE, 1, 64, 4, BW ? BW : 256, U, U>(D, run);
+  if (D <= 512 * VE) return with_shape<T, VE, 1, 64, 8, BW ? BW : 512, U, U>(D, run);
+  if (D <= 1024 * VE) return with_shape<T, VE, 1, 64, 16, 1024, U, U>(D, run);
+  if constexpr (sizeof(T) == 4)
+    if (D > 2048 * VE) return with_shape<T, VE, 4, 64, 16, 1024, 1, 1>(D, run);
+  return with_shape<T, VE, 2, 64, 16, 1024, U, U>(D, run);
 }
-template <typename T> constexpr int widest_in_registers() { return 2048 * 16 / sizeof(T); }
+constexpr int kWidestInRegisters = 16384;
 
 // Blocks of the backward kernel: each leaves 2 D partial sums, so no more than
 // fill the chip with `threads` threads a block.
@@ -572,7 +652,7 @@ static int column_splits(int64_t rows) { return (int)std::min<int64_t>(256, std:
 
 // Partial sums that the backward pass leaves for its last launch.
 template <typename T> static int backward_parts(int64_t rows, int D) {
-  if (D > widest_in_registers<T>()) return column_splits(rows);
+  if (D > kWidestInRegisters) return column_splits(rows);
   return for_shape<T, true>(D, [&](auto shape) {
     typedef decltype(shape) S;
     return backward_blocks(rows, S::ROWS, S::BT);
@@ -580,7 +660,7 @@ template <typename T> static int backward_parts(int64_t rows, int D) {
 }
 
 template <typename T> static void carve_ln_backward(Carve& cv, int64_t rows, int64_t d, float2** stats, float** part) {
-  *stats = cv.take<float2>(d > widest_in_registers<T>() ? rows : 0);
+  *stats = cv.take<float2>(d > kWidestInRegisters ? rows : 0);
   *part = cv.take<float>(2 * d * backward_parts<T>(rows, (int)d));
 }
 
@@ -588,7 +668,7 @@ template <typename T>
 static int launch_ln_forward(const T* x, int64_t xs, T* y, ParamVec w, ParamVec b, int64_t rows, int D, float eps,
                              hipStream_t st) {
   StageTimer timer("layer_norm_forward", st);
-  if (D > widest_in_registers<T>())
+  if (D > kWidestInRegisters)
     ln_forward_wide_kernel<T><<<(unsigned)std::min<int64_t>(rows, 1 << 20), kWideThreads, 0, st>>>(x, xs, y, w, b, rows, D, eps);
   else
     for_shape<T, false>(D, [&](auto shape) {
@@ -610,7 +690,7 @@ static int launch_ln_backward(const T* x, int64_t xs, const T* dy, int64_t ds, T
   carve_ln_backward<T>(cv, rows, D, &stats, &part);
   const bool sums = dw || db;
   const int parts = backward_parts<T>(rows, D);
-  if (D > widest_in_registers<T>()) {
+  if (D > kWidestInRegisters) {
     {
       StageTimer timer("layer_norm_backward", st);
       ln_backward_wide_kernel<T><<<(unsigned)std::min<int64_t>(rows, 1 << 20), kWideThreads, 0, st>>>(
