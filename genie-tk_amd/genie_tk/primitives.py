@@ -154,9 +154,12 @@ def layer_norm(x: Tensor, weight: Optional[Tensor] = None, bias: Optional[Tensor
         elif (x.dim() >= 1 and x.shape[-1] >= 1 and x.dtype in _dispatch.SUPPORTED_DTYPES
               and all(p.dtype in _dispatch.SUPPORTED_DTYPES for p in params)):
             return _ext.C.layer_norm(x, weight, bias, eps)
-    if any(p.dtype != x.dtype for p in params):  # in fp32, rounded once
-        wide = [None if p is None else p.float() for p in (weight, bias)]
-        return F.layer_norm(x.float(), x.shape[-1:], *wide, eps).to(x.dtype)
+    wide = x.dtype
+    for p in params:
+        wide = torch.promote_types(wide, p.dtype)
+    if any(p.dtype != x.dtype for p in params):  # in the widest of the types, rounded once
+        weight, bias = (None if p is None else p.to(wide) for p in (weight, bias))
+        return F.layer_norm(x.to(wide), x.shape[-1:], weight, bias, eps).to(x.dtype)
     return F.layer_norm(x, x.shape[-1:], weight, bias, eps)
 
 

@@ -292,6 +292,22 @@ def test_sizes_at_the_edges_of_fp32():
 
 
 @gpu
+def test_products_among_the_smallest_values():
+    """Products below the normal range are rounded to its steps (2^-149 fp32,
+    2^-133 bf16), not flushed to zero."""
+    g = torch.tensor([1e-38, 5e-39, 7e-41, 3e-45, -2e-39] * 20, device="cuda")
+    for t in (g, g.bfloat16()):
+        for out in (torch.float32, torch.bfloat16):
+            step = 2.0 ** -149 if out == torch.float32 else 2.0 ** -133
+            o = torch.empty(100, device="cuda", dtype=out)
+            _ext.require().grad_clip_with_norm([t], [o], 0.25, torch.ones(1, device="cuda"))
+            ref = np64(t) * train_ops.clip_factor(1.0, 0.25)
+            # half a step, and twice where the product is rounded to fp32 before bf16
+            assert (np.abs(np64(o) - ref) <= 0.5 * step + 2.0 ** -150 + 4 * U * np.abs(ref)).all()
+            assert (np64(o)[np.abs(ref) > step] != 0).all()
+
+
+@gpu
 @pytest.mark.parametrize("p", [2.0, 1.0, INF])
 @pytest.mark.parametrize("dt", ["fp32", "bf16"])
 def test_not_finite(dt, p):

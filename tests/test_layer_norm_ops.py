@@ -131,6 +131,13 @@ def test_pytorch_path(dt, pdt):
     np.testing.assert_allclose(np64(y), ref, rtol=half(DT[dt]), atol=1e-5)
 
 
+def test_pytorch_path_keeps_64_bits():
+    x = rows(5, 33, 0, torch.float64)
+    w, b = params(33, 1, torch.float32)
+    ref = train_ops.layer_norm(np64(x), np64(w), np64(b))[0]
+    np.testing.assert_allclose(np64(layer_norm(x, w, b)), ref, rtol=0, atol=1e-13)
+
+
 def test_module_is_a_drop_in():
     a, b = torch.nn.LayerNorm((3, 8), eps=1e-4), LayerNorm((3, 8), eps=1e-4)
     b.load_state_dict(a.state_dict())
@@ -363,6 +370,37 @@ def test_captured_and_replayed():
         for out in outs:
             for a, c in zip(out, ref):
                 assert torch.equal(a, c), k
+
+
+@gpu
+def test_captured_through_autograd():
+    """The public path captured, as torch asks for it: warmed up on a side
+    stream, with no eager graph of the leaves alive."""
+    x = rows(700, 128, 0, torch.float32, "cuda").requires_grad_(True)
+    w, b = (t.requires_grad_(True) for t in params(128, 2, torch.float32, "cuda"))
+    dy = rows(700, 128, 1, torch.float32, "cuda")
+
+    def step():
+        y = layer_norm(x, w, b)
+        return (y.detach(), *torch.autograd.grad(y, (x, w, b), dy))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for k in range(3):
+        with torch.no_grad():
+            x.copy_(rows(700, 128, 30 + k, torch.float32, "cuda"))
+        ref = step()
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, c in zip(out, ref):
+            assert torch.equal(a, c), k
 
 
 @gpu
