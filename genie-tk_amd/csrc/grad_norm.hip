@@ -9,7 +9,7 @@
 // kernel arguments, kMaxIn or kMaxInOut tensors a launch: no table is copied to
 // the GPU, and a captured launch keeps them.  A block takes one chunk of one
 // tensor and leaves one partial sum; one block adds those in a fixed order, so
-// equal inputs give equal bits.
+// equal inputs in equal places give equal bits.
 #include <algorithm>
 #include <memory>
 #include <new>
@@ -285,13 +285,17 @@ static int64_t chunk_of(const gtk_tensor_list* g, int64_t most) {
   return chunk;
 }
 
-static int64_t total_blocks(const gtk_tensor_list* g, int64_t chunk) {
+// Most blocks that the list takes: runs that are joined take fewer.
+static int64_t most_blocks(const gtk_tensor_list* g, int64_t chunk) {
   int64_t b = 0;
   for (int64_t i = 0; i < g->count; ++i) b += (g->numel[i] + chunk - 1) / chunk;
   return b;
 }
 
 // Calls launch(jobs, blocks, first partial) for every J::kMax entries.
+// Tensors that lie one behind the other in memory (a module's gradients are
+// views of one buffer) are one run, and so one entry: the 1392 gradients of 24
+// layers in one buffer take one launch a pass instead of six.
 template <typename J, typename F>
 static int for_each_launch(const gtk_tensor_list* g, const gtk_tensor_list* out, int64_t chunk, F launch) {
   J jobs;
@@ -300,14 +304,26 @@ static int for_each_launch(const gtk_tensor_list* g, const gtk_tensor_list* out,
   uint32_t blocks = 0;
   int64_t base = 0;
   const gtk_tensor_list* o = out ? out : g;
-  for (int64_t i = 0; i < g->count; ++i) {
+  for (int64_t i = 0; i < g->count;) {
+    const int64_t i0 = i;
     const bool sbf = g->dtype[i] == GTK_BF16, dbf = o->dtype[i] == GTK_BF16;
     const uint32_t flags = (sbf ? kSrcBf : 0) | (dbf ? kDstBf : 0);
-    for (int64_t at = 0; at < g->numel[i]; at += kMaxPart) {
-      const int64_t n = std::min(g->numel[i] - at, kMaxPart);
+    const char* src = (const char*)g->data[i];
+    char* dst = (char*)o->data[i];
+    int64_t run = g->numel[i];
+    const int64_t se = sbf ? 2 : 4, de = dbf ? 2 : 4;
+    for (++i; i < g->count; ++i) {
+      if (g->numel[i] == 0) continue;
+      if (run == 0 || g->data[i] != src + run * se || g->dtype[i] != g->dtype[i0] || o->data[i] != dst + run * de ||
+          o->dtype[i] != o->dtype[i0])
+        break;
+      run += g->numel[i];
+    }
+    for (int64_t at = 0; at < run; at += kMaxPart) {
+      const int64_t n = std::min(run - at, kMaxPart);
       const uint32_t k = jobs.count++;
-      jobs.src[k] = (uint64_t)(uintptr_t)g->data[i] + (uint64_t)at * (sbf ? 2 : 4);
-      if (J::kOut) jobs.dst[J::kOut ? k : 0] = (uint64_t)(uintptr_t)o->data[i] + (uint64_t)at * (dbf ? 2 : 4);
+      jobs.src[k] = (uint64_t)(uintptr_t)(src + at * se);
+      if (J::kOut) jobs.dst[J::kOut ? k : 0] = (uint64_t)(uintptr_t)(dst + at * de);
       jobs.n[k] = (uint32_t)n | flags;
       jobs.first[k] = blocks;
       blocks += (uint32_t)((n + chunk - 1) / chunk);
@@ -372,18 +388,19 @@ static int check_overlap(const gtk_tensor_list* g, const gtk_tensor_list* out, c
 
 template <int KIND>
 static int launch_norm(const gtk_tensor_list* g, float* norm, double* part, hipStream_t st) {
-  const int64_t chunk = chunk_of(g, kNormChunk);
+  int64_t parts = 0;
   {
     StageTimer timer("grad_partials", st);
-    const int rc = for_each_launch<JobsIn>(g, nullptr, chunk, [&](const JobsIn& J, unsigned blocks, int64_t base) -> int {
+    const int rc = for_each_launch<JobsIn>(g, nullptr, chunk_of(g, kNormChunk), [&](const JobsIn& J, unsigned blocks, int64_t base) -> int {
       grad_partials_kernel<KIND><<<blocks, kThreads, 0, st>>>(J, part + base);
       GTK_LAUNCH_CHECK();
+      parts = base + blocks;
       return GTK_OK;
     });
     if (rc) return rc;
   }
   StageTimer timer("grad_norm_close", st);
-  grad_norm_close_kernel<KIND><<<1, kCloseThreads, 0, st>>>(part, total_blocks(g, chunk), norm);
+  grad_norm_close_kernel<KIND><<<1, kCloseThreads, 0, st>>>(part, parts, norm);
   GTK_LAUNCH_CHECK();
   return GTK_OK;
 }
@@ -441,7 +458,7 @@ using namespace gtk;
 
 extern "C" size_t gtk_grad_norm_workspace_size(const gtk_tensor_list* grads) {
   if (check_list(grads, "gtk_grad_norm_workspace_size")) return 0;
-  return sizeof(double) * (size_t)std::max<int64_t>(1, total_blocks(grads, chunk_of(grads, kNormChunk)));
+  return sizeof(double) * (size_t)std::max<int64_t>(1, most_blocks(grads, chunk_of(grads, kNormChunk)));
 }
 
 extern "C" int gtk_grad_norm(const gtk_tensor_list* grads, int kind, float* norm, void* workspace,

@@ -415,7 +415,8 @@ int gtk_layer_norm_backward(const void* x, int64_t x_stride, const void* dy, int
  * arithmetic has it.  k = 1 leaves every value's bits.
  * Tensors: `count` of them, each a run of numel[i] values of dtype[i] at
  * data[i], at any alignment that the type allows; the arrays are host memory
- * and are read before the call returns.  Equal inputs give equal bits.
+ * and are read before the call returns.  Equal inputs in equal places give
+ * equal bits (tensors that lie one behind the other are summed as one run).
  * gtk_grad_clip writes to `out` (NULL: in place): the same sizes, in either
  * type.  No tensor that is written may overlap another one, or itself be
  * given twice; out->data[i] may be grads->data[i] with the same type.

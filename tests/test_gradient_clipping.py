@@ -255,6 +255,30 @@ def test_packed_at_any_alignment(dt):
 
 
 @gpu
+def test_one_behind_the_other():
+    """Neighbours are one run only where both sides are neighbours of one type."""
+    raw = torch.randn(40_000, device="cuda")
+    a, b, c, d = raw[:9000], raw[9000:9000], raw[9000:9003], raw[9003:20_000]
+    e = raw[20_000:20_500].view(torch.bfloat16)  # right behind d, another type
+    e.copy_(torch.randn(1000))
+    f = raw[20_500:30_000]
+    every = [a, b, c, d, e, f]
+    before = [g.clone() for g in every]
+    ref = check_norm(grad_norm(every), every, 2.0)
+    apart = [torch.full_like(g, math.nan) for g in every]
+    together = torch.full((40_000,), 7.0, device="cuda")
+    ends = [0, 9000, 9000, 9003, 20_000, 21_000, 30_500]
+    fp32 = [together[lo:hi] for lo, hi in zip(ends, ends[1:])]
+    for outs in (apart, fp32, fp32[:3] + apart[3:]):
+        clip_grads(every, 0.5 * ref, out=outs)
+        check_clipped(outs, before, 0.5 * ref, ref)
+    assert (together[30_500:] == 7.0).all()
+    order = [5, 3, 0, 4, 2, 1]
+    clip_grad_norm_(as_params([every[k] for k in order]), 0.5 * ref)
+    check_clipped(every, before, 0.5 * ref, ref)
+
+
+@gpu
 def test_strides():
     base = torch.randn(40, 60, device="cuda")
     dense, gapped, repeated = base.t(), torch.randn(50, 70, device="cuda")[:, 5:23], torch.randn(9, 1, device="cuda").expand(9, 30)
