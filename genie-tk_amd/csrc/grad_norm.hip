@@ -6,10 +6,19 @@
 // The values' squares and their sums are 64-bit: the square of a 32-bit float
 // fits a 64-bit one exactly, so neither gradients above 1.8e19 overflow nor
 // ones below 1e-23 vanish.  The tensors' addresses and sizes travel in the
-// kernel arguments, kMaxIn or kMaxInOut tensors a launch: no table is copied to
-// the GPU, and a captured launch keeps them.  A block takes one chunk of one
-// tensor and leaves one partial sum; one block adds those in a fixed order, so
-// equal inputs in equal places give equal bits.
+// kernel arguments, 248 runs of memory a launch (165 with outputs): no table is
+// copied to the GPU, and a captured launch keeps them.  A block takes one chunk
+// of one run and leaves one partial sum; one block adds those in a fixed order,
+// so equal inputs in equal places give equal bits.
+//
+// The norm reads every value once, the product reads and writes it once more:
+// memory, or for small sets the launches.  On MI355X 4e8 bf16 values take 122 us
+// (6.5 TB/s; conversion to 64 bits and the product-sum are hidden), 1.5e8 fp32
+// values clipped into fp32 masters 308 us (1.8 GB moved, 5.8 TB/s; a copy of
+// 1 GiB runs at 5.15).  464 gradients of one buffer into masters: 5 + 3 + 8 us
+// on the GPU in 34 us of host time; 1392 separate ones in place 116 us.
+// Reading the values in reverse for the product, to find the last of them still
+// in the Infinity Cache, gained nothing (432 us forwards, 451 backwards).
 #include <algorithm>
 #include <memory>
 #include <new>

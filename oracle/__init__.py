@@ -10,6 +10,8 @@ implementation of this path in the reference):
   pair_ops.contract                 src/genie_tk/triangle_mul.py:77-101
   pair_ops.attention_core           kernels/bindings.cpp:82-90 semantics
   pair_ops.pair_block               src/genie_tk/pair_transform.py:162-195 (eval mode)
+  train_ops.*                       torch.nn.LayerNorm with its gradients and
+                                    torch.nn.utils.clip_grad_norm_, in 64 bits
   brute.*                           scalar-loop versions of the above for tiny
                                     inputs, used to pin pair_ops
 
