@@ -648,13 +648,13 @@ template <typename T, bool BACKWARD, typename F> static int for_shape(int D, F r
   if (D <= 32 * VE) return with_shape<T, VE, 1, 32, 1, B, 2, UM>(D, run);
   if (D <= 64 * VE) return with_shape<T, VE, 1, 64, 1, B, 2, UM>(D, run);
   // Several waves: forward, two rows a group wait for each barrier once (4096
-  // rows of 4096: 16.4 us, with one 18.2).  The backward's registers hold one
-  // row (two spill: 45 us against 32), and one block a CU leaves the fewest
-  // partial sums.
-  constexpr int U = BACKWARD ? 1 : 2, BW = BACKWARD ? 1024 : 0;
-  if (D <= 128 * VE) return with_shape<T, VE, 1, 64, 2, BW ? BW : 256, U, U>(D, run);
-  if (D <= 256 * VE) return with_shape<T, VE, 1, 64, 4, BW ? BW : 256, U, U>(D, run);
-  if (D <= 512 * VE) return with_shape<T, VE, 1, 64, 8, BW ? BW : 512, U, U>(D, run);
+  // rows of 4096: 16.4 us, with one 18.2).  The backward's one block a CU leaves
+  // the fewest partial sums; 512 threads hold enough loads in flight (16384 rows
+  // of 1024: 25 us, of 1024 threads 27; two rows a group 27.5).
+  constexpr int U = BACKWARD ? 1 : 2, BW = BACKWARD ? 512 : 256;
+  if (D <= 128 * VE) return with_shape<T, VE, 1, 64, 2, BW, U, U>(D, run);
+  if (D <= 256 * VE) return with_shape<T, VE, 1, 64, 4, BW, U, U>(D, run);
+  if (D <= 512 * VE) return with_shape<T, VE, 1, 64, 8, 512, U, U>(D, run);
   if (D <= 1024 * VE) return with_shape<T, VE, 1, 64, 16, 1024, U, U>(D, run);
   if constexpr (sizeof(T) == 4)
     if (D > 2048 * VE) return with_shape<T, VE, 4, 64, 16, 1024, 1, 1>(D, run);
@@ -663,11 +663,10 @@ template <typename T, bool BACKWARD, typename F> static int for_shape(int D, F r
 // 3000 fp32 rows of 16384: backward 131 us in registers, 293 by sweeps.
 constexpr int kWidestInRegisters = 16384;
 
-// Blocks of the backward kernel: each leaves 2 D partial sums, so no more than
-// fill the chip with `threads` threads a block.
-static int backward_blocks(int64_t rows, int rows_a_step, int threads) {
+// Blocks of the backward kernel: each leaves 2 D partial sums, so few.
+static int backward_blocks(int64_t rows, int rows_a_step, int blocks_a_cu) {
   const int64_t steps = (rows + rows_a_step - 1) / rows_a_step;
-  return (int)std::min<int64_t>(steps, (int64_t)device_cus() * (1024 / threads));
+  return (int)std::min<int64_t>(steps, (int64_t)device_cus() * blocks_a_cu);
 }
 
 static int column_splits(int64_t rows) { return (int)std::min<int64_t>(256, std::max<int64_t>(1, (rows + 15) / 16)); }
@@ -677,7 +676,7 @@ template <typename T> static int backward_parts(int64_t rows, int D) {
   if (D > kWidestInRegisters) return column_splits(rows);
   return for_shape<T, true>(D, [&](auto shape) {
     typedef decltype(shape) S;
-    return backward_blocks(rows, S::ROWS, S::BT);
+    return backward_blocks(rows, S::ROWS, S::W == 1 ? 2 : 1);
   });
 }
 

@@ -275,6 +275,12 @@ def test_each_gradient_alone():
         y = layer_norm(*leaves)
         for k, g in zip(keep, torch.autograd.grad(y, [leaves[k] for k in keep], dy)):
             assert torch.equal(g, every[k]), (keep, k)
+    # all three differentiable, one asked for
+    leaves = [t.clone().requires_grad_(True) for t in (x, w, b)]
+    y = layer_norm(*leaves)
+    for k in (2, 0, 1):
+        g, = torch.autograd.grad(y, leaves[k], dy, retain_graph=True)
+        assert torch.equal(g, every[k]), k
     C = _ext.require()
     assert C.layer_norm_backward(x, dy, w, EPS, False, False, False) == [None, None, None]
 
