@@ -362,35 +362,45 @@ static int check_list(const gtk_tensor_list* g, const char* name) {
 
 struct Span {
   const char *begin, *end;
-  bool written;
+};
+
+// The memory of a list's tensors, in ascending order.
+struct Spans {
+  std::unique_ptr<Span[]> v;
+  int64_t n = 0;
+  bool sorted = true;
+  explicit Spans(int64_t most) : v(new (std::nothrow) Span[(size_t)most + 1]) {}
+  void add(const gtk_tensor_list* l, int64_t i) {
+    if (l->numel[i] == 0) return;
+    const char* p = (const char*)l->data[i];
+    if (n && p < v[n - 1].begin) sorted = false;
+    v[n++] = {p, p + l->numel[i] * (int64_t)dtype_size(l->dtype[i])};
+  }
+  void sort() {
+    if (!sorted) std::sort(v.get(), v.get() + n, [](const Span& a, const Span& b) { return a.begin < b.begin; });
+  }
 };
 
 // Nothing that is written is written twice or read by another tensor's block:
 // blocks run in any order.
 static int check_overlap(const gtk_tensor_list* g, const gtk_tensor_list* out, const char* name) {
-  const gtk_tensor_list* o = out ? out : g;
-  const std::unique_ptr<Span[]> v(new (std::nothrow) Span[2 * (size_t)g->count + 1]);
-  GTK_REQUIRE(v, GTK_EINVAL, "%s: out of host memory", name);
-  int64_t spans = 0;
-  bool sorted = true;
-  auto add = [&](const gtk_tensor_list* l, int64_t i, bool written) {
-    if (l->numel[i] == 0) return;
-    const char* p = (const char*)l->data[i];
-    if (spans && p < v[spans - 1].begin) sorted = false;
-    v[spans++] = {p, p + l->numel[i] * (int64_t)dtype_size(l->dtype[i]), written};
-  };
-  for (int64_t i = 0; i < g->count; ++i) add(o, i, true);
-  for (int64_t i = 0; out && i < g->count; ++i)
+  Spans w(g->count), r(out ? g->count : 0);
+  GTK_REQUIRE(w.v && r.v, GTK_EINVAL, "%s: out of host memory", name);
+  for (int64_t i = 0; i < g->count; ++i) {
+    w.add(out ? out : g, i);
     // a tensor clipped onto itself is read and written by the same thread
-    if (!(out->data[i] == g->data[i] && out->dtype[i] == g->dtype[i])) add(g, i, false);
-  if (!sorted) std::sort(v.get(), v.get() + spans, [](const Span& a, const Span& b) { return a.begin < b.begin; });
+    if (out && !(out->data[i] == g->data[i] && out->dtype[i] == g->dtype[i])) r.add(g, i);
+  }
+  w.sort();
+  r.sort();
   const char *any = nullptr, *written = nullptr;  // the furthest ends so far
-  for (int64_t i = 0; i < spans; ++i) {
-    const Span& s = v[i];
-    GTK_REQUIRE(s.begin >= written && (!s.written || s.begin >= any), GTK_EINVAL,
+  for (int64_t i = 0, j = 0; i < w.n || j < r.n;) {
+    const bool write = j == r.n || (i < w.n && w.v[i].begin <= r.v[j].begin);
+    const Span& s = write ? w.v[i++] : r.v[j++];
+    GTK_REQUIRE(s.begin >= (write ? any : written), GTK_EINVAL,
                 "%s: a tensor that is written overlaps another (or is given twice)", name);
     any = std::max(any, s.end);
-    if (s.written) written = std::max(written, s.end);
+    if (write) written = std::max(written, s.end);
   }
   return GTK_OK;
 }
