@@ -50,12 +50,16 @@ def _check_max_norm(max_norm: float, what: str) -> float:
     return max_norm
 
 
+def _norm_dtype(tensors: Sequence[Tensor]) -> torch.dtype:
+    return torch.float64 if any(t.dtype == torch.float64 for t in tensors) else torch.float32
+
+
 def _norm_pytorch(tensors: Sequence[Tensor], p: float) -> Tensor:
-    wide = [t.detach().double().abs().flatten() for t in tensors if t.numel()]
+    wide = [t.detach().double().flatten() for t in tensors if t.numel()]
     if not wide:
-        return tensors[0].new_zeros((), dtype=torch.float32)
+        return tensors[0].new_zeros((), dtype=_norm_dtype(tensors))
     each = torch.stack([torch.linalg.vector_norm(w, p) for w in wide])
-    return torch.linalg.vector_norm(each, p).float()
+    return torch.linalg.vector_norm(each, p).to(_norm_dtype(tensors))
 
 
 def _clip_pytorch(tensors: Sequence[Tensor], outs: Sequence[Tensor], max_norm: float, norm: Tensor) -> None:
@@ -69,8 +73,8 @@ def _clip_pytorch(tensors: Sequence[Tensor], outs: Sequence[Tensor], max_norm: f
 
 def grad_norm(tensors: Iterable[Tensor], norm_type: float = 2.0) -> Tensor:
     """``(sum |g|^p)^(1/p)`` over every value of ``tensors``, ``p = norm_type``
-    (the largest |g| for ``inf``): an fp32 scalar on their device.  No tensors
-    give 0."""
+    (the largest |g| for ``inf``): a scalar on their device, fp32 (fp64 where one
+    of them is).  No tensors give 0."""
     tensors = list(tensors)
     norm_type = float(norm_type)
     if not tensors:
@@ -146,7 +150,7 @@ def clip_grads_with_norm_(parameters: Union[Tensor, Iterable[Tensor]], max_norm:
     _check(grads, "clip_grads_with_norm_")
     if total_norm.numel() != 1:
         raise ValueError("clip_grads_with_norm_: total_norm must be one value")
-    _clip_with_norm(grads, max_norm, total_norm.detach().to(device=grads[0].device, dtype=torch.float32))
+    _clip_with_norm(grads, max_norm, total_norm.detach().to(device=grads[0].device, dtype=_norm_dtype(grads)))
 
 
 def _clip_with_norm(grads: Sequence[Tensor], max_norm: float, total_norm: Tensor) -> None:

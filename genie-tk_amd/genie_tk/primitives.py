@@ -151,7 +151,7 @@ def layer_norm(x: Tensor, weight: Optional[Tensor] = None, bias: Optional[Tensor
     if x.is_cuda:
         if _ext.C is None or not torch.cuda.is_available():
             _ext.missing("layer_norm")
-        elif (x.dim() >= 1 and x.shape[-1] >= 1 and x.dtype in _dispatch.SUPPORTED_DTYPES
+        elif (x.dim() >= 1 and 1 <= x.shape[-1] <= 1 << 24 and x.dtype in _dispatch.SUPPORTED_DTYPES
               and all(p.dtype in _dispatch.SUPPORTED_DTYPES for p in params)):
             return _ext.C.layer_norm(x, weight, bias, eps)
     wide = x.dtype

@@ -100,6 +100,18 @@ def test_pytorch_path_forms():
     assert [float(grad_norm([torch.empty(0)], q)) for q in (1.0, 2.0, INF)] == [0.0] * 3
 
 
+def test_pytorch_path_keeps_64_bits():
+    grads = make([40, 7], 1, [torch.float64])
+    before = [g.clone() for g in grads]
+    norm, outs = clip_grads(grads, 0.01)
+    ref = train_ops.global_norm([np64(g) for g in grads])
+    assert norm.dtype == torch.float64 and abs(float(norm) - ref) < 1e-14
+    clip_grads_with_norm_(as_params(grads), 0.01, norm)
+    for a, o, b in zip(grads, outs, before):
+        np.testing.assert_allclose(np64(a), np64(b) * train_ops.clip_factor(ref, 0.01), rtol=1e-13)
+        np.testing.assert_allclose(np64(o), np64(a), rtol=1e-15)
+
+
 def test_refusals():
     g = [torch.ones(3), torch.ones(2, 2)]
     for call in (lambda: clip_grads(g, -1.0), lambda: clip_grads(g, math.nan), lambda: clip_grads(g, 1.0, out=g[:1]),
