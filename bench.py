@@ -772,12 +772,19 @@ def config_table(torch, C, dev: str) -> int:
 
 def fwd_bwd_run(torch, mods, z, mask, steps: int, warmup: int) -> int:
     """Forward + backward (the input's and every parameter's gradient) of
-    tri-mul outgoing and tri-attn starting node, `steps` times each after
-    `warmup`; prints their median times as one JSON line."""
+    tri-mul outgoing, tri-attn starting node and LayerNorm, and the clipping of
+    their gradients by the global norm, `steps` times each after `warmup`;
+    prints their median times as one JSON line."""
+    from genie_tk.gradients import clip_grad_norm_
+    from genie_tk.primitives import LayerNorm
+
     maskb = mask.to(torch.bfloat16)
+    norm = LayerNorm(z.shape[-1]).to(z.device)
+    calls = {"tri_mul_out": (mods["tri_mul_out"], lambda zg: mods["tri_mul_out"](zg, maskb)),
+             "tri_att_start": (mods["tri_att_start"], lambda zg: mods["tri_att_start"](zg, maskb)),
+             "layer_norm": (norm, norm)}
     out = {}
-    for name in ("tri_mul_out", "tri_att_start"):
-        mod = mods[name]
+    for name, (mod, fwd) in calls.items():
         zg = z.detach().clone().requires_grad_(True)
         dy = torch.randn_like(z)
 
@@ -785,12 +792,14 @@ def fwd_bwd_run(torch, mods, z, mask, steps: int, warmup: int) -> int:
             zg.grad = None
             for p in mod.parameters():
                 p.grad = None
-            mod(zg, maskb).backward(dy)
+            fwd(zg).backward(dy)
         for _ in range(warmup):
             run()
         out[name] = round(statistics.median(event_time_ms(torch, run, steps)), 4)
         print(f"[bench] {name} forward+backward {out[name]:.3f} ms", file=sys.stderr, flush=True)
-    print(json.dumps({"fwd_bwd_ms": out}))
+    params = [p for mod, _ in calls.values() for p in mod.parameters()]
+    clip = statistics.median(event_time_ms(torch, lambda: clip_grad_norm_(params, 1.0), steps))
+    print(json.dumps({"fwd_bwd_ms": out, "clip_grad_norm_ms": round(clip, 4)}))
     return 0
 
 
@@ -816,8 +825,9 @@ def main() -> int:
     ap.add_argument("--only-step", action="store_true",
                     help="time the step and its kernels only (for counter collection)")
     ap.add_argument("--only-fwd-bwd", action="store_true",
-                    help="no bench line: forward + backward of tri-mul outgoing and tri-attn "
-                         "starting at N (for a kernel trace of the backward kernels)")
+                    help="no bench line: forward + backward of tri-mul outgoing, tri-attn starting "
+                         "and LayerNorm at N, and the clipping of their gradients (for a kernel "
+                         "trace of the backward kernels)")
     ap.add_argument("--only-ln", action="store_true",
                     help="no bench line: LayerNorm launches over rotating inputs at N=1024 and "
                          "N=512 (for HBM byte counters and a kernel trace), then --calibrate-copy")
