@@ -473,3 +473,59 @@ def test_module_on_the_kernels():
     check_all(x.flatten(1), dy.flatten(1), m.weight.flatten(), m.bias.flatten(), m(x).flatten(1), None,
               m.weight.grad.flatten(), m.bias.grad.flatten())
     assert torch.equal(m.weight.grad.flatten(), dw) and torch.equal(m.bias.grad.flatten(), db)
+
+
+# ---------------------------------------------------------------------------
+# Rows whose spread is small against their offset
+# ---------------------------------------------------------------------------
+def spread_bounds(x, dy, w, eps=EPS):
+    """`bounds` with S, the row's largest |x - mean|, in the place of M: the sums
+    are taken of p = x - x_0, which is at most 2 S and off by u times that.  The
+    mean of p is off by 2 (adds + 3) u S (with the roundings of 1 / D and of the
+    product), so d by a = (2 adds + 9) u S; the relative error of r is a r + (adds
+    / 2 + 8) u, as sd / (sd^2 + eps) <= r; both go into h = d r.  With |c1|, |c2|
+    <= G, c1 is off by (adds + 3) u G, c2 by G max(eh) + (adds + 5) u G, and dx by
+    those, its own roundings and the error of r."""
+    D, R = x.shape[-1], x.shape[0]
+    adds = D / 64 + 16
+    _, h, r = train_ops.layer_norm(x, None, None, eps)
+    ah = np.abs(h)
+    ar = (2 * adds + 9) * U * np.abs(x - x.mean(-1, keepdims=True)).max(-1, keepdims=True) * r
+    er = ar + (adds / 2 + 8) * U
+    eh = (1 + ar) * (ar + er * ah)
+    g = np.abs(dy if w is None else dy * w).max(-1, keepdims=True)
+    edx = (1 + ar) * r * g * ((2 * adds + 13) * U * (1 + ah) + eh.max(-1, keepdims=True) * (1 + ah) + er * (2 + ah))
+    chain = R / 16 + 64
+    ew = (np.abs(dy) * eh).sum(0) + chain * U * np.abs(dy * h).sum(0)
+    return eh, edx, ew, chain * U * np.abs(dy).sum(0)
+
+
+@gpu
+@pytest.mark.parametrize("dt", ["fp32", "bf16"])
+@pytest.mark.parametrize("D", [3, 7, 8, 15, 31, 64, 77, 128, 301, 512, 1023, 1100, 2048, 5001, 8200, 16383, 20001])
+def test_small_spread_far_from_zero(D, dt):
+    """The error follows the spread, not the offset; a row of one value gives the bias."""
+    print(f"small spread D={D} {dt}", flush=True)
+    gen = torch.Generator().manual_seed(D)
+    x = torch.zeros(11, D, dtype=torch.float64)
+    x[:4] = torch.tensor([1000.1, 1e5 + 0.1, -7654321.0, 1e30], dtype=torch.float64)[:, None]  # one value
+    near = torch.randn(5, D, generator=gen, dtype=torch.float64)
+    x[4:9] = near * torch.tensor([1e-2, 0.05, 3.0, 1e-4, 1.0])[:, None].double()
+    x[4:9] += torch.tensor([1000.1, 1e5, -1e6, 1.0, 3e5], dtype=torch.float64)[:, None]
+    x[8, 0] = -3e5           # an outlier in the first place
+    x[9] = 1e8
+    x[9, D // 2] += 8        # one value, one step of fp32 higher
+    x[10] = near[0]          # around zero
+    x = x.to(DT[dt]).cuda()
+    dy = rows(11, D, 1, DT[dt], "cuda")
+    w, b = params(D, 2, DT[dt], "cuda")
+    y, dx, dw, db = run(x, w, b, dy)
+    xn, dn, wn, bn = (np64(t) for t in (x, dy, w, b))
+    eh, edx, ew, eb = spread_bounds(xn, dn, wn)
+    yr, h, _ = train_ops.layer_norm(xn, wn, bn)
+    dxr, dwr, dbr = train_ops.layer_norm_grads(xn, dn, wn)
+    assert (h[:4] == 0).all() and torch.equal(y[:4], b.expand(4, D))
+    check(y, yr, eh * np.abs(wn) + 2 * U * (np.abs(h * wn) + np.abs(bn)), "y")
+    check(dx, dxr, edx, "dx")
+    check(dw, dwr, ew, "dweight")
+    check(db, dbr, eb, "dbias")
