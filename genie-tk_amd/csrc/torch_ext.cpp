@@ -728,8 +728,15 @@ struct LayerNormFn : public torch::autograd::Function<LayerNormFn> {
   }
 };
 
-at::Tensor layer_norm(const at::Tensor& x, const c10::optional<at::Tensor>& weight,
-                      const c10::optional<at::Tensor>& bias, double eps) {
+// Without `strict`, None where an input carries a forward-mode tangent, which
+// the kernels do not propagate (a dual tensor need not require a gradient).
+c10::optional<at::Tensor> layer_norm(const at::Tensor& x, const c10::optional<at::Tensor>& weight,
+                                     const c10::optional<at::Tensor>& bias, double eps, bool strict) {
+  auto dual = [](const at::Tensor& t) { return t._fw_grad(/*level=*/0).defined(); };
+  if (dual(x) || (weight.has_value() && dual(*weight)) || (bias.has_value() && dual(*bias))) {
+    TORCH_CHECK_NOT_IMPLEMENTED(!strict, "genie_tk._C: layer_norm has no forward-mode derivative");
+    return c10::nullopt;
+  }
   const bool grad = at::GradMode::is_enabled() &&
                     (x.requires_grad() || (weight.has_value() && weight->requires_grad()) ||
                      (bias.has_value() && bias->requires_grad()));
@@ -989,8 +996,11 @@ PYBIND11_MODULE(_C, m) {
         py::arg("mask"), py::arg("packed"), py::arg("c_in"), py::arg("c_h"), py::arg("no_heads"),
         py::arg("starting"), py::arg("residual") = false, py::arg("eps") = 1e-5,
         py::arg("chunk_rows") = 0, py::arg("inf") = 1e9);
-  m.def("layer_norm", &layer_norm, "layer_norm_forward under autograd (differentiable once)", py::arg("x"),
-        py::arg("weight") = py::none(), py::arg("bias") = py::none(), py::arg("eps") = 1e-5);
+  m.def("layer_norm", &layer_norm,
+        "layer_norm_forward under autograd (differentiable once, in reverse mode).  Without strict, None where an "
+        "input has a forward-mode tangent",
+        py::arg("x"), py::arg("weight") = py::none(), py::arg("bias") = py::none(), py::arg("eps") = 1e-5,
+        py::arg("strict") = true);
   m.def("layer_norm_forward", &layer_norm_forward,
         "LayerNorm over the last dimension, optional affine in either parameter type", py::arg("x"),
         py::arg("weight") = py::none(), py::arg("bias") = py::none(), py::arg("eps") = 1e-5);

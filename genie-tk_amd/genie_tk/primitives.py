@@ -143,17 +143,20 @@ def layer_norm(x: Tensor, weight: Optional[Tensor] = None, bias: Optional[Tensor
 
     Kernel path (bf16 or fp32 GPU tensor, parameters in bf16 or fp32, also
     mixed): ``genie_tk._C.layer_norm``, whose autograd node is the C++ one of
-    ``layer_norm_forward`` and ``layer_norm_backward``.  The output and dL/dx have the type of ``x``, the parameters' gradients their
-    own; statistics and sums are fp32.  Rows that lie one stride apart (a slice
-    of wider rows, a repeated row) are read as they are.  Other tensors run
-    torch's LayerNorm."""
+    ``layer_norm_forward`` and ``layer_norm_backward``.  The output and dL/dx
+    have the type of ``x``, the parameters' gradients their own; statistics and
+    sums are fp32.  Rows that lie one stride apart (a slice of wider rows, a
+    repeated row) are read as they are.  Other tensors, and those with a
+    forward-mode tangent, run torch's LayerNorm."""
     params = [p for p in (weight, bias) if p is not None]
     if x.is_cuda:
         if _ext.C is None or not torch.cuda.is_available():
             _ext.missing("layer_norm")
         elif (x.dim() >= 1 and 1 <= x.shape[-1] <= 1 << 24 and x.dtype in _dispatch.SUPPORTED_DTYPES
               and all(p.dtype in _dispatch.SUPPORTED_DTYPES for p in params)):
-            return _ext.C.layer_norm(x, weight, bias, eps)
+            y = _ext.C.layer_norm(x, weight, bias, eps, False)
+            if y is not None:
+                return y
     wide = x.dtype
     for p in params:
         wide = torch.promote_types(wide, p.dtype)

@@ -529,3 +529,55 @@ def test_small_spread_far_from_zero(D, dt):
     check(dx, dxr, edx, "dx")
     check(dw, dwr, ew, "dweight")
     check(db, dbr, eb, "dbias")
+
+
+# ---------------------------------------------------------------------------
+# Forward-mode derivatives
+# ---------------------------------------------------------------------------
+def check_tangents(device, dt, pdt):
+    """The tangent of y along (vx, vw, vb), each alone and all together, against
+    64 bits: r (vx - mean(vx) - h mean(vx h)) w + h vw + vb.  The first term is a
+    dx (g = vx) times w and the second an h times vw, so they are off by `bounds`'
+    edx |w| and eh |vw|, three times that as torch's sums of 48 terms may be one
+    chain (adds is 16.75).  In types narrower than fp32 torch rounds up to eight
+    steps on the way, each by half a step of the sizes that edx and eh hold."""
+    import torch.autograd.forward_ad as fwAD
+
+    D = 48
+    x, vx = rows(9, D, 0, DT[dt], device), rows(9, D, 1, DT[dt], device, 0.0)
+    w, b = params(D, 2, DT[pdt], device)
+    vw, vb = params(D, 3, DT[pdt], device)
+    _, h, r = train_ops.layer_norm(np64(x))
+    v, wn = np64(vx), np64(w)
+    part = (r * (v - v.mean(-1, keepdims=True) - h * (v * h).mean(-1, keepdims=True)) * wn, h * np64(vw),
+            np64(vb) + 0 * h)
+    eh, edx, _, _ = bounds(np64(x), v, None)
+    adds, step = D / 64 + 16, half(DT[dt])
+    u = 3 * U + 8 * step / (2 * adds) if dt != "fp32" else 3 * U
+    err = (edx * np.abs(wn) * u / U, eh * np.abs(np64(vw)) * u / U, 8 * step * np.abs(np64(vb)))
+    for duals in ((0,), (1,), (2,), (0, 1, 2)):
+        for grad in (False, True):
+            with fwAD.dual_level():
+                args = [t.clone().requires_grad_(grad) for t in (x, w, b)]
+                args = [fwAD.make_dual(t, tv) if k in duals else t for k, (t, tv) in enumerate(zip(args, (vx, vw, vb)))]
+                y, t = fwAD.unpack_dual(layer_norm(*args))
+            assert t is not None, f"tangent of {duals} lost"
+            assert y.dtype == x.dtype  # the tangent's is torch's: fp32 where its statistics are
+            ref = sum(part[k] for k in duals)
+            check(t, ref, sum(err[k] for k in duals) + 4 * U * sum(np.abs(part[k]) for k in duals), f"tangent {duals}")
+
+
+@pytest.mark.parametrize("dt,pdt", [("fp32", "fp32"), ("bf16", "fp32")])
+def test_pytorch_path_forward_mode(dt, pdt):
+    check_tangents("cpu", dt, pdt)
+
+
+@gpu
+@pytest.mark.parametrize("dt,pdt", [("fp32", "fp32"), ("bf16", "bf16"), ("bf16", "fp32")])
+def test_forward_mode_is_not_dropped(dt, pdt):
+    import torch.autograd.forward_ad as fwAD
+
+    check_tangents("cuda", dt, pdt)
+    x = rows(3, 16, 0, DT[dt], "cuda")
+    with fwAD.dual_level(), pytest.raises(NotImplementedError, match="forward-mode"):
+        _ext.require().layer_norm(fwAD.make_dual(x, x))
