@@ -147,7 +147,12 @@ def layer_norm(x: Tensor, weight: Optional[Tensor] = None, bias: Optional[Tensor
     have the type of ``x``, the parameters' gradients their own; statistics and
     sums are fp32.  Rows that lie one stride apart (a slice of wider rows, a
     repeated row) are read as they are.  Other tensors, and those with a
-    forward-mode tangent, run torch's LayerNorm."""
+    forward-mode tangent, run torch's LayerNorm.  Under autocast GPU tensors
+    narrower than fp32 are taken to fp32 first, as torch's LayerNorm takes them,
+    and so is the output."""
+    if x.is_cuda and torch.is_autocast_enabled("cuda"):
+        x, weight, bias = (t.float() if t is not None and t.is_floating_point() and t.dtype != torch.float64 else t
+                           for t in (x, weight, bias))
     params = [p for p in (weight, bias) if p is not None]
     if x.is_cuda:
         if _ext.C is None or not torch.cuda.is_available():

@@ -581,3 +581,25 @@ def test_forward_mode_is_not_dropped(dt, pdt):
     x = rows(3, 16, 0, DT[dt], "cuda")
     with fwAD.dual_level(), pytest.raises(NotImplementedError, match="forward-mode"):
         _ext.require().layer_norm(fwAD.make_dual(x, x))
+
+
+@gpu
+@pytest.mark.parametrize("dt,pdt", [("bf16", "fp32"), ("bf16", "bf16"), ("fp32", "fp32"), ("fp32", "bf16"),
+                                    ("bf16", None)])
+def test_autocast_gives_fp32(dt, pdt):
+    """As torch's LayerNorm: computed and returned in fp32, gradients in the
+    leaves' own types."""
+    x, dy = rows(50, 96, 0, DT[dt], "cuda"), rows(50, 96, 1, torch.float32, "cuda")
+    w, b = (None, None) if pdt is None else params(96, 2, DT[pdt], "cuda")
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        want = F.layer_norm(x, (96,), w, b, EPS)
+        got = run(x, w, b, dy)
+        with torch.autocast("cuda", enabled=False):
+            assert layer_norm(x, w, b).dtype == x.dtype
+        m = LayerNorm((4, 24), elementwise_affine=False)
+        assert m(x.view(50, 4, 24)).dtype == torch.float32
+        assert layer_norm(x.half()).dtype == torch.float32
+        assert layer_norm(x.double()).dtype == F.layer_norm(x.double(), (96,)).dtype == torch.float64
+    assert got[0].dtype == want.dtype == torch.float32 and got[1].dtype == x.dtype
+    assert w is None or got[2].dtype == got[3].dtype == w.dtype
+    check_all(x, dy, w, b, *got)
