@@ -182,7 +182,7 @@ class LayerNorm(nn.LayerNorm):
 
     def forward(self, x: Tensor) -> Tensor:
         shape = self.normalized_shape
-        if not self._fused_requested or tuple(x.shape[-len(shape):]) != tuple(shape):
+        if not self._fused_requested or not shape or tuple(x.shape[-len(shape):]) != tuple(shape):
             return super().forward(x)  # torch's, or its error for the shape
         if len(shape) == 1:
             return layer_norm(x, self.weight, self.bias, self.eps)

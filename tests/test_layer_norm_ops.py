@@ -603,3 +603,8 @@ def test_autocast_gives_fp32(dt, pdt):
     assert got[0].dtype == want.dtype == torch.float32 and got[1].dtype == x.dtype
     assert w is None or got[2].dtype == got[3].dtype == w.dtype
     check_all(x, dy, w, b, *got)
+
+
+def test_module_without_dimensions_is_refused():
+    with pytest.raises(RuntimeError, match="normalized_shape"):
+        LayerNorm(())(torch.ones(()))
