@@ -11,7 +11,9 @@
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
 
+#include <algorithm>
 #include <array>
+#include <functional>
 #include <limits>
 #include <utility>
 #include <vector>
@@ -828,6 +830,91 @@ c10::optional<at::Tensor> grad_norm(const py::handle& tensors, double p, bool st
   return norm;
 }
 
+// Whether two strided tensors share a byte.  A value of a tensor lies at its
+// address + the sum of i_k stride_k, so they do if the distance of their addresses
+// is a sum of c_s s over the distinct strides s (1 for the bytes of a value), each
+// c_s in a range that the sizes give.  Searched from the largest stride down: what
+// the smaller ones can still reach leaves few c_s to try where strides nest, as
+// slices' do.  Past 2^16 tries the answer is yes.
+bool share_memory(const at::Tensor& a, const at::Tensor& b) {
+  struct Axis {
+    int64_t stride, lo, hi;
+  };
+  std::vector<Axis> axes;
+  auto add = [&](int64_t stride, int64_t lo, int64_t hi) {
+    for (auto& x : axes)
+      if (x.stride == stride) {
+        x.lo += lo;
+        x.hi += hi;
+        return;
+      }
+    if (stride) axes.push_back({stride, lo, hi});
+  };
+  const int64_t ea = a.element_size(), eb = b.element_size();
+  for (int64_t k = 0; k < a.dim(); ++k) add(a.stride(k) * ea, 0, a.size(k) - 1);
+  for (int64_t k = 0; k < b.dim(); ++k) add(b.stride(k) * eb, 1 - b.size(k), 0);
+  add(1, 0, ea - 1);
+  add(1, 1 - eb, 0);
+  std::sort(axes.begin(), axes.end(), [](const Axis& x, const Axis& y) { return x.stride > y.stride; });
+  std::vector<int64_t> low(axes.size() + 1, 0), high(axes.size() + 1, 0);  // of the sum from axis k on
+  for (size_t k = axes.size(); k-- > 0;) {
+    low[k] = low[k + 1] + axes[k].lo * axes[k].stride;
+    high[k] = high[k + 1] + axes[k].hi * axes[k].stride;
+  }
+  int tries = 1 << 16;
+  std::function<bool(size_t, int64_t)> reach = [&](size_t k, int64_t to) {
+    if (to < low[k] || to > high[k]) return false;
+    if (k == axes.size()) return true;
+    const Axis& x = axes[k];
+    // the first c that the rest can complete
+    const int64_t need = to - high[k + 1];
+    int64_t c = std::max(x.lo, need >= 0 ? (need + x.stride - 1) / x.stride : -(-need / x.stride));
+    for (; c <= x.hi && c * x.stride <= to - low[k + 1]; ++c)
+      if (--tries < 0 || reach(k + 1, to - c * x.stride)) return true;
+    return false;
+  };
+  return reach(0, (const char*)b.data_ptr() - (const char*)a.data_ptr());
+}
+
+// No written tensor may overlap another tensor of the call.  The C functions see
+// to that for those that they are given; here, for those that are clipped on
+// copies (`copied`).
+void check_apart(const GradList& l, const GradList* lo, const std::vector<bool>& copied) {
+  struct Piece {
+    const char *begin, *end;
+    const at::Tensor* t;
+    size_t index;
+    bool written;
+  };
+  std::vector<Piece> pieces;
+  auto add = [&](const at::Tensor& t, size_t i, bool written) {
+    if (t.numel() == 0) return;
+    int64_t last = 0;
+    for (int64_t k = 0; k < t.dim(); ++k) last += (t.size(k) - 1) * t.stride(k);
+    const char* p = (const char*)t.data_ptr();
+    pieces.push_back({p, p + (last + 1) * t.element_size(), &t, i, written});
+  };
+  for (size_t i = 0; i < l.t.size(); ++i) {
+    add(*l.t[i], i, !lo);
+    if (lo) add(*lo->t[i], i, true);
+  }
+  std::sort(pieces.begin(), pieces.end(), [](const Piece& a, const Piece& b) { return a.begin < b.begin; });
+  std::vector<const Piece*> open;  // those that reach past the current one's begin
+  for (const auto& p : pieces) {
+    size_t kept = 0;
+    for (const Piece* q : open)
+      if (q->end > p.begin) open[kept++] = q;
+    open.resize(kept);
+    for (const Piece* q : open) {
+      // a tensor and its own output: the copy is whole before anything is written
+      if (q->index == p.index || !(p.written || q->written) || !(copied[p.index] || copied[q->index])) continue;
+      TORCH_CHECK(!share_memory(*p.t, *q->t),
+                  "genie_tk._C: a tensor that is written overlaps another (or is given twice)");
+    }
+    open.push_back(&p);
+  }
+}
+
 // Clips l into lo (in place without it).  norm: given, or undefined: computed,
 // and returned.
 at::Tensor clip_list(GradList& l, GradList* lo, double max_norm, double p, at::Tensor norm) {
@@ -839,6 +926,7 @@ at::Tensor clip_list(GradList& l, GradList* lo, double max_norm, double p, at::T
   // copies, which are copied back at the end.
   std::vector<std::pair<at::Tensor, at::Tensor>> back;
   std::vector<at::Tensor> copies;
+  std::vector<bool> copied(l.t.size(), false);
   for (size_t i = 0; i < l.t.size(); ++i) {
     const at::Tensor &t = *l.t[i], &o = lo ? *lo->t[i] : t;
     TORCH_CHECK(!lo || o.sizes() == t.sizes(), "genie_tk._C: output ", i, " has another shape");
@@ -849,9 +937,7 @@ at::Tensor clip_list(GradList& l, GradList* lo, double max_norm, double p, at::T
       continue;
     }
     at::assert_no_internal_overlap(o);
-    for (const auto& b : back)
-      TORCH_CHECK(o.numel() == 0 || b.first.data_ptr() != o.data_ptr(),
-                  "genie_tk._C: a tensor that is written is given twice");
+    copied[i] = true;
     copies.push_back(t.contiguous());
     l.add(copies.back());
     if (lo) {
@@ -861,6 +947,7 @@ at::Tensor clip_list(GradList& l, GradList* lo, double max_norm, double p, at::T
       back.emplace_back(o, copies.back());
     }
   }
+  if (!copies.empty()) check_apart(l, lo, copied);
   const auto g = l.list(), go = lo ? lo->list() : gtk_tensor_list{};
   const gtk_tensor_list* out = lo ? &go : nullptr;
   void* st = cur_stream(like);

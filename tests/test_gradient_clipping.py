@@ -509,3 +509,92 @@ def test_training_step_with_the_pair_stack(dt):
     norm = clip_grad_norm_(every, 0.25 * ref)
     check_norm(norm, before, 2.0)
     check_clipped([q.grad for q in every], before, 0.25 * ref, ref)
+
+
+# ---------------------------------------------------------------------------
+# Written tensors that overlap
+# ---------------------------------------------------------------------------
+def view_pairs(count, seed, device):
+    """Pairs of views of one buffer of distinct values, each without overlap in
+    itself, with the answer whether they share a value: by their elements'
+    places.  Strides nest or not, dimensions in any order."""
+    rng = np.random.default_rng(seed)
+    for _ in range(count):
+        base = torch.arange(1.0, 4001.0, device=device)
+        places = torch.arange(4000)
+        pair = []
+        strides = [int(rng.choice([1, 1, 2, 3]))]
+        for _ in range(2):
+            while True:
+                if rng.random() < 0.5:  # each its own
+                    strides = [int(rng.choice([1, 1, 2, 3]))]
+                sizes, mine = [], []
+                for k in range(int(rng.integers(1, 4))):
+                    if k == len(strides):
+                        strides.append(int(strides[-1] * sizes[-1] + rng.integers(0, 9)))
+                    sizes.append(int(rng.integers(1, 7)))
+                    mine.append(strides[k])
+                order = rng.permutation(len(sizes))
+                shape, step = [sizes[k] for k in order], [mine[k] for k in order]
+                room = 1 + sum((n - 1) * s for n, s in zip(shape, step))
+                at = int(rng.integers(0, 60))
+                if room + at <= 4000:
+                    where = torch.as_strided(places, shape, step, at)
+                    if where.unique().numel() == where.numel():
+                        break
+            pair.append((torch.as_strided(base, shape, step, at), set(where.flatten().tolist())))
+        (a, ia), (b, ib) = pair
+        yield base, a, b, bool(ia & ib)
+
+
+def check_view_pairs(device):
+    met = apart = 0
+    for base, a, b, share in view_pairs(300, 11, device):
+        before = base.clone()
+        if share:
+            met += 1
+            with pytest.raises(RuntimeError, match="overlaps another"):
+                clip_grad_norm_(as_params([a, b]), 0.5)
+            assert torch.equal(base, before)
+            continue
+        apart += 1
+        ga, gb = a.clone(), b.clone()
+        norm = clip_grad_norm_(as_params([a, b]), 0.5)
+        ref = check_norm(norm, [ga, gb], 2.0)
+        check_clipped([a, b], [ga, gb], 0.5, ref)
+        assert int((base != before).sum()) == a.numel() + b.numel()  # and nothing between them
+    assert met > 60 and apart > 60
+
+
+def check_overlap_refusals(device):
+    """Overlapping written tensors in each of the calls; their neighbours pass."""
+    base = torch.arange(1.0, 49.0, device=device).view(6, 8)
+    other = torch.arange(1.0, 49.0, device=device).view(6, 8)
+    before = base.clone()
+    wide = base[:, 0:5]
+    half_words = base.view(torch.bfloat16)[:, 7:9]  # the upper half of column 3 and the lower of column 4
+    bad = [[wide, base[:, 3:8]], [base, wide], [wide, base.flatten()[17:19]], [wide, wide], [base[::2], base[4:, :3]],
+           [base[1:, ::2], base[:3, ::4]], [wide, half_words], [base.t()[2:5], base[5:]]]
+    for pair in bad:
+        total = torch.ones((), device=device)
+        for call in (lambda: clip_grad_norm_(as_params(pair), 0.5), lambda: clip_grads_with_norm_(as_params(pair), 0.5, total),
+                     lambda: clip_grad_norm_(as_params(pair), 0.5, 3.0),
+                     lambda: clip_grads([other[:t.shape[0], :t.shape[1]] if t.dim() == 2 else other.flatten()[:t.numel()]
+                                         for t in pair], 0.5, out=pair)):
+            with pytest.raises(RuntimeError, match="overlaps another"):
+                call()
+    # onto another gradient of the call
+    with pytest.raises(RuntimeError, match="overlaps another"):
+        clip_grads([wide, other[:, 1:3]], 0.5, out=[other[:, 2:7], torch.empty(6, 2, device=device)])
+    assert torch.equal(base, before)
+    # read twice, and written onto themselves
+    clip_grads([wide, wide, base], 0.5)
+    clip_grads([wide, base[:, 5:]], 0.5, out=[wide, base[:, 5:]])
+    ref = train_ops.global_norm([np64(before)])
+    check_clipped([base], [before], 0.5, ref)
+
+
+@gpu
+def test_overlapping_views_on_the_kernels():
+    check_view_pairs("cuda")
+    check_overlap_refusals("cuda")
