@@ -12,7 +12,7 @@ device.
 from __future__ import annotations
 
 import math
-from typing import Iterable, List, Optional, Sequence, Tuple, Union
+from typing import Dict, Iterable, List, Optional, Sequence, Tuple, Union
 
 import torch
 from torch import Tensor
@@ -62,7 +62,62 @@ def _norm_pytorch(tensors: Sequence[Tensor], p: float) -> Tensor:
     return torch.linalg.vector_norm(each, p).to(_norm_dtype(tensors))
 
 
+def _share_memory(a: Tensor, b: Tensor) -> bool:
+    """Whether two strided tensors share a byte: whether the distance of their
+    addresses is a sum of c_s s over the distinct strides s (1 for the bytes of a
+    value), each c_s in a range that the sizes give.  Searched from the largest
+    stride down, which leaves few c_s to try where strides nest; past 2^16 tries
+    the answer is yes."""
+    axes: Dict[int, List[int]] = {}
+    for t, sign in ((a, 1), (b, -1)):
+        size = t.element_size()
+        for n, stride in [(n, s * size) for n, s in zip(t.shape, t.stride()) if s] + [(size, 1)]:
+            bounds = axes.setdefault(stride, [0, 0])
+            bounds[sign > 0] += sign * (n - 1)
+    order = sorted(axes.items(), reverse=True)
+    low, high = [0], [0]  # of the sum from each axis on
+    for stride, (lo, hi) in reversed(order):
+        low.insert(0, low[0] + lo * stride)
+        high.insert(0, high[0] + hi * stride)
+    tries = 1 << 16
+
+    def reach(k: int, to: int) -> bool:
+        nonlocal tries
+        if not low[k] <= to <= high[k]:
+            return False
+        if k == len(order):
+            return True
+        stride, (lo, hi) = order[k]
+        for c in range(max(lo, -((high[k + 1] - to) // stride)), min(hi, (to - low[k + 1]) // stride) + 1):
+            tries -= 1
+            if tries < 0 or reach(k + 1, to - c * stride):
+                return True
+        return False
+
+    return reach(0, b.data_ptr() - a.data_ptr())
+
+
+def _check_apart(tensors: Sequence[Tensor], outs: Sequence[Tensor]) -> None:
+    """Raises RuntimeError where a tensor of ``outs``, which are written, shares
+    memory with another one or with another one's gradient, as the kernels do."""
+    pieces = []  # (begin, end, tensor, index, written)
+    for i, (t, o) in enumerate(zip(tensors, outs)):
+        for v, written in ((o, True),) if t is o else ((o, True), (t, False)):
+            if v.numel() and v.device.type != "meta":
+                end = 1 + sum((n - 1) * s for n, s in zip(v.shape, v.stride()))
+                pieces.append((v.data_ptr(), v.data_ptr() + end * v.element_size(), v, i, written))
+    pieces.sort(key=lambda p: p[0])
+    reaching: list = []
+    for p in pieces:
+        reaching = [q for q in reaching if q[1] > p[0]]
+        for q in reaching:
+            if q[3] != p[3] and (q[4] or p[4]) and _share_memory(q[2], p[2]):
+                raise RuntimeError("a tensor that is written overlaps another (or is given twice)")
+        reaching.append(p)
+
+
 def _clip_pytorch(tensors: Sequence[Tensor], outs: Sequence[Tensor], max_norm: float, norm: Tensor) -> None:
+    _check_apart(tensors, outs)
     coef = (max_norm / (norm.double() + _EPS)).clamp(max=1.0)
     with torch.no_grad():
         for t, o in zip(tensors, outs):

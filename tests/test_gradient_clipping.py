@@ -598,3 +598,24 @@ def check_overlap_refusals(device):
 def test_overlapping_views_on_the_kernels():
     check_view_pairs("cuda")
     check_overlap_refusals("cuda")
+
+
+def test_overlapping_views_on_the_pytorch_path():
+    check_view_pairs("cpu")
+    check_overlap_refusals("cpu")
+    p = torch.nn.Parameter(torch.zeros(4))  # a shared parameter listed twice
+    p.grad = torch.ones(4)
+    for call in (lambda: clip_grad_norm_([p, p], 0.5), lambda: clip_grads_with_norm_([p, p], 0.5, torch.tensor(2.0))):
+        with pytest.raises(RuntimeError, match="given twice"):
+            call()
+    assert torch.equal(p.grad, torch.ones(4))
+
+
+@gpu
+def test_overlapping_views_in_types_beyond_the_kernels():
+    base = torch.ones(6, 8, device="cuda", dtype=torch.float16)
+    with pytest.raises(RuntimeError, match="overlaps another"):
+        clip_grad_norm_(as_params([base[:, :5], base[:, 3:]]), 0.5)
+    assert (base == 1).all()
+    clip_grad_norm_(as_params([base[:, :5], base[:, 5:]]), 0.5)
+    assert (base < 0.1).all()
