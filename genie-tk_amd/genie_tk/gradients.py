@@ -99,10 +99,13 @@ def _share_memory(a: Tensor, b: Tensor) -> bool:
 
 def _check_apart(tensors: Sequence[Tensor], outs: Sequence[Tensor]) -> None:
     """Raises RuntimeError where a tensor of ``outs``, which are written, shares
-    memory with another one or with another one's gradient, as the kernels do."""
+    memory with another one or with another one's gradient, or is expanded, as
+    the kernels' calls do: before anything is written."""
     pieces = []  # (begin, end, tensor, index, written)
     for i, (t, o) in enumerate(zip(tensors, outs)):
         for v, written in ((o, True),) if t is o else ((o, True), (t, False)):
+            if written and any(s == 0 and n > 1 for n, s in zip(v.shape, v.stride())):
+                raise RuntimeError("a tensor that is written is expanded: several of its values are one")
             if v.numel() and v.device.type != "meta":
                 end = 1 + sum((n - 1) * s for n, s in zip(v.shape, v.stride()))
                 pieces.append((v.data_ptr(), v.data_ptr() + end * v.element_size(), v, i, written))

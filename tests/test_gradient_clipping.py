@@ -619,3 +619,14 @@ def test_overlapping_views_in_types_beyond_the_kernels():
     assert (base == 1).all()
     clip_grad_norm_(as_params([base[:, :5], base[:, 5:]]), 0.5)
     assert (base < 0.1).all()
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+def test_an_expanded_gradient_leaves_the_others_alone(device):
+    first = torch.ones(4, device=device)
+    grads = [first, torch.ones(3, 1, device=device).expand(3, 5)]
+    with pytest.raises(RuntimeError):
+        clip_grad_norm_(as_params(grads), 0.5)
+    with pytest.raises(RuntimeError):
+        clip_grads_with_norm_(as_params(grads), 0.5, torch.tensor(4.0))
+    assert torch.equal(first, torch.ones(4, device=device))
