@@ -806,6 +806,7 @@ int norm_kind(double p) {
 // The norm of the tensors; without `strict`, None where a tensor is not one for
 // the kernels.
 c10::optional<at::Tensor> grad_norm(const py::handle& tensors, double p, bool strict) {
+  const at::NoGradGuard no_grad;
   GradList l;
   const int kind = norm_kind(p);
   if (!l.collect(tensors, false, strict)) return c10::nullopt;
@@ -918,6 +919,7 @@ void check_apart(const GradList& l, const GradList* lo, const std::vector<bool>&
 // Clips l into lo (in place without it).  norm: given, or undefined: computed,
 // and returned.
 at::Tensor clip_list(GradList& l, GradList* lo, double max_norm, double p, at::Tensor norm) {
+  const at::NoGradGuard no_grad;  // of the copies: a gradient may require one itself
   const at::Tensor& like = *l.t[0];
   const bool given = norm.defined();
   const int kind = given ? GTK_NORM_2 : norm_kind(p);

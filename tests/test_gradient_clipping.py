@@ -630,3 +630,24 @@ def test_an_expanded_gradient_leaves_the_others_alone(device):
     with pytest.raises(RuntimeError):
         clip_grads_with_norm_(as_params(grads), 0.5, torch.tensor(4.0))
     assert torch.equal(first, torch.ones(4, device=device))
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+def test_gradients_that_require_gradients(device):
+    """Clipping is not recorded by autograd (as torch's is not), whatever the strides."""
+    for cols in (slice(0, 8), slice(0, 5)):
+        leaf = torch.empty_strided((6, 8), (8, 1), device=device)[:, cols].fill_(2.0).requires_grad_(True)
+        x = torch.ones(6, 8, device=device, requires_grad=True)
+        whole = x * 3.0  # as with create_graph
+        graph = whole[:, cols]
+        out = torch.empty(6, 8, device=device)[:, cols]
+        norm, outs = clip_grads([leaf, graph], 0.5)
+        n2, _ = clip_grads([leaf], 0.5, out=[out])
+        assert not any(t.requires_grad for t in (norm, n2, out, *outs)) and not grad_norm([graph]).requires_grad
+        before = [leaf.detach().clone(), graph.detach().clone()]
+        p, q = as_params([before[0], before[1]])  # their gradients are set below
+        p.grad, q.grad = leaf, graph
+        ref = train_ops.global_norm([np64(b) for b in before])
+        clip_grad_norm_([p, q], 0.5)
+        check_clipped([leaf, graph], before, 0.5, ref)
+        assert leaf.is_leaf and whole.grad_fn.name() == "MulBackward0"  # a recorded copy would be CopySlices
