@@ -174,12 +174,14 @@ def clip_grads(grads: Iterable[Tensor], max_norm: float, norm_type: float = 2.0,
 
 
 def clip_grad_norm_(parameters: Union[Tensor, Iterable[Tensor]], max_norm: float, norm_type: float = 2.0,
-                    error_if_nonfinite: bool = False) -> Tensor:
+                    error_if_nonfinite: bool = False, foreach: Optional[bool] = None) -> Tensor:
     """Clips the gradients of ``parameters`` in place by their global norm and
     returns the norm (fp32, before the clipping), as
     ``torch.nn.utils.clip_grad_norm_``.  Parameters without a gradient are
     passed over.  ``error_if_nonfinite`` looks at the norm on the host first (it
-    waits for the GPU) and raises RuntimeError with the gradients untouched."""
+    waits for the GPU) and raises RuntimeError with the gradients untouched.
+    ``foreach`` is accepted for torch's signature and changes nothing: the kernels
+    take all gradients in one launch."""
     max_norm, norm_type = _check_max_norm(max_norm, "clip_grad_norm_"), float(norm_type)
     parameters = [parameters] if isinstance(parameters, Tensor) else list(parameters)
     if parameters and not error_if_nonfinite:
@@ -198,9 +200,10 @@ def clip_grad_norm_(parameters: Union[Tensor, Iterable[Tensor]], max_norm: float
 
 
 def clip_grads_with_norm_(parameters: Union[Tensor, Iterable[Tensor]], max_norm: float,
-                          total_norm: Tensor) -> None:
+                          total_norm: Tensor, foreach: Optional[bool] = None) -> None:
     """Clips the gradients of ``parameters`` in place by a given norm: one over
-    the shards of several processes, say, joined from their ``grad_norm``."""
+    the shards of several processes, say, joined from their ``grad_norm``.
+    ``foreach`` as in ``clip_grad_norm_``."""
     max_norm = _check_max_norm(max_norm, "clip_grads_with_norm_")
     grads = _grads_of(parameters)
     if not grads:

@@ -651,3 +651,19 @@ def test_gradients_that_require_gradients(device):
         clip_grad_norm_([p, q], 0.5)
         check_clipped([leaf, graph], before, 0.5, ref)
         assert leaf.is_leaf and whole.grad_fn.name() == "MulBackward0"  # a recorded copy would be CopySlices
+
+
+def test_calls_take_torchs_arguments():
+    import inspect
+
+    for ours, theirs in ((clip_grad_norm_, torch.nn.utils.clip_grad_norm_),
+                         (clip_grads_with_norm_, torch.nn.utils.clip_grads_with_norm_)):
+        ours, theirs = ([(p.name, p.default) for p in inspect.signature(f).parameters.values()] for f in (ours, theirs))
+        assert ours == theirs
+    for foreach in (True, False, None):
+        ps = as_params([torch.full((4,), 2.0)])
+        assert float(clip_grad_norm_(ps, 1.0, foreach=foreach)) == 4.0
+        before = [ps[0].grad.clone()]
+        check_clipped(before, [torch.full((4,), 2.0)], 1.0, 4.0)
+        clip_grads_with_norm_(ps, 0.5, torch.tensor(1.0), foreach=foreach)
+        check_clipped([ps[0].grad], before, 0.5, 1.0)
