@@ -667,3 +667,19 @@ def test_calls_take_torchs_arguments():
         check_clipped(before, [torch.full((4,), 2.0)], 1.0, 4.0)
         clip_grads_with_norm_(ps, 0.5, torch.tensor(1.0), foreach=foreach)
         check_clipped([ps[0].grad], before, 0.5, 1.0)
+
+
+def test_timed_clipping_does_the_same_work_in_every_call():
+    import bench
+
+    grads = make([40, 7, 300], 2, [torch.float32, torch.bfloat16])
+    before = [g.clone() for g in grads]
+    params = [*as_params(grads), torch.nn.Parameter(torch.zeros(2))]
+    ref = train_ops.global_norm([np64(g) for g in before])
+    above, below = bench.clip_calls(params).values()
+    for _ in range(12):
+        norm, outs = above()
+        check_norm(norm, before, 2.0)
+        check_clipped(outs, before, 0.5 * float(norm), ref)
+        check_norm(below(), before, 2.0)
+        assert all(torch.equal(a, b) for a, b in zip(grads, before))
