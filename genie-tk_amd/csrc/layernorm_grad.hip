@@ -16,7 +16,9 @@
 // the row's spread and not its offset.  (77 values of 1000.1 summed as they are
 // give a mean 6e-5 away, which with eps = 1e-5 makes h 0.02 instead of 0; the
 // subtraction costs nothing beside the row's loads: 2^20 bf16 rows of 128, both
-// passes, 227 us against 224.)
+// passes, 227 us against 224.)  Each difference is divided by D before it is
+// added, so that a row with the type's lowest value in it, in a masked place, has
+// a finite mean; its variance is infinite in 32 bits, r and h are 0.
 //
 // Some twenty operations a value of 2 or 4 bytes: memory bounds both passes.  A
 // row therefore stays in the registers of its threads from its one load to its
@@ -245,7 +247,7 @@ __global__ __launch_bounds__(S::BT) void ln_forward_kernel(const typename S::T* 
 #pragma unroll
       for (int i = 0; i < N; ++i) {
         f[u][i] -= x0;
-        s[u] += S::EXACT || i % VE >= C.skip[i / VE] ? f[u][i] : 0.f;
+        s[u] += (S::EXACT || i % VE >= C.skip[i / VE] ? f[u][i] : 0.f) * inv;
       }
     }
     row_sums<S>(s, red[0]);
@@ -256,7 +258,7 @@ __global__ __launch_bounds__(S::BT) void ln_forward_kernel(const typename S::T* 
       for (int j = 0; j < NV; ++j)
 #pragma unroll
         for (int e = 0; e < VE; ++e) {
-          const float d = f[u][j * VE + e] - s[u] * inv;
+          const float d = f[u][j * VE + e] - s[u];
           f[u][j * VE + e] = d;
           q[u] += S::EXACT || e >= C.skip[j] ? d * d : 0.f;
         }
@@ -335,7 +337,7 @@ __global__ __launch_bounds__(S::BT) void ln_backward_kernel(const typename S::T*
 #pragma unroll
       for (int i = 0; i < N; ++i) {
         f[u][i] -= x0;
-        s[u] += S::EXACT || i % VE >= C.skip[i / VE] ? f[u][i] : 0.f;
+        s[u] += (S::EXACT || i % VE >= C.skip[i / VE] ? f[u][i] : 0.f) * inv;
       }
     }
     if constexpr (KEEP)
@@ -348,7 +350,7 @@ __global__ __launch_bounds__(S::BT) void ln_backward_kernel(const typename S::T*
       float q = 0.f, s1 = 0.f, s2 = 0.f;
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        const float d = f[u][i] - s[u] * inv;
+        const float d = f[u][i] - s[u];
         const bool counts = S::EXACT || i % VE >= C.skip[i / VE];
         const float gw = counts ? g[u][i] * wf[i] : 0.f;
         f[u][i] = d;
@@ -479,6 +481,7 @@ __global__ __launch_bounds__(kWideThreads) void ln_forward_wide_kernel(const T* 
   __shared__ float red[16];
   for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
     const T* xr = x + r * xs;
+    const float inv = 1.0f / (float)D;
     const float x0 = to_f32(xr[0]);
     float s[1] = {0.f}, q[1] = {0.f};
     for_vectors<T>(D, [&](int c, int skip) {
@@ -487,10 +490,10 @@ __global__ __launch_bounds__(kWideThreads) void ln_forward_wide_kernel(const T* 
       v.load(xr + c);
       v.get(f);
 #pragma unroll
-      for (int e = 0; e < VE; ++e) s[0] += e >= skip ? f[e] - x0 : 0.f;
+      for (int e = 0; e < VE; ++e) s[0] += (e >= skip ? f[e] - x0 : 0.f) * inv;
     });
     block_sums(s, red);
-    const float mean = s[0] / (float)D;  // of x - x_0
+    const float mean = s[0];  // of x - x_0
     for_vectors<T>(D, [&](int c, int skip) {
       Vec<T, VE> v;
       float f[VE];
@@ -503,7 +506,7 @@ __global__ __launch_bounds__(kWideThreads) void ln_forward_wide_kernel(const T* 
       }
     });
     block_sums(q, red);
-    const float rstd = 1.0f / sqrtf(q[0] / (float)D + eps);
+    const float rstd = 1.0f / sqrtf(q[0] * inv + eps);
     for_vectors<T>(D, [&](int c, int) {
       Vec<T, VE> v;
       float f[VE], wf[VE], bf[VE];
@@ -536,6 +539,7 @@ __global__ __launch_bounds__(kWideThreads) void ln_backward_wide_kernel(const T*
   for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
     const T* xr = x + r * xs;
     const T* dr = dy + r * ds;
+    const float inv = 1.0f / (float)D;
     const float x0 = to_f32(xr[0]);
     float s[1] = {0.f}, m[3] = {0.f, 0.f, 0.f};
     for_vectors<T>(D, [&](int c, int skip) {
@@ -544,10 +548,10 @@ __global__ __launch_bounds__(kWideThreads) void ln_backward_wide_kernel(const T*
       v.load(xr + c);
       v.get(f);
 #pragma unroll
-      for (int e = 0; e < VE; ++e) s[0] += e >= skip ? f[e] - x0 : 0.f;
+      for (int e = 0; e < VE; ++e) s[0] += (e >= skip ? f[e] - x0 : 0.f) * inv;
     });
     block_sums(s, red);
-    const float mean = s[0] / (float)D;  // of x - x_0
+    const float mean = s[0];  // of x - x_0
     // d and g at column c
     auto load = [&](int c, float* d, float* g) {
       Vec<T, VE> xv, gv;
@@ -576,8 +580,8 @@ __global__ __launch_bounds__(kWideThreads) void ln_backward_wide_kernel(const T*
       }
     });
     block_sums(m, red);
-    const float rstd = 1.0f / sqrtf(m[0] / (float)D + eps);
-    const float c1 = m[1] / (float)D, c2 = m[2] / (float)D * rstd;
+    const float rstd = 1.0f / sqrtf(m[0] * inv + eps);
+    const float c1 = m[1] * inv, c2 = m[2] * inv * rstd;
     if (dx)
       for_vectors<T>(D, [&](int c, int) {
         float d[VE], g[VE];

@@ -608,3 +608,20 @@ def test_autocast_gives_fp32(dt, pdt):
 def test_module_without_dimensions_is_refused():
     with pytest.raises(RuntimeError, match="normalized_shape"):
         LayerNorm(())(torch.ones(()))
+
+
+@gpu
+@pytest.mark.parametrize("dt", ["fp32", "bf16"])
+@pytest.mark.parametrize("D", [5, 64, 100, 1023, 4096, 20001])
+def test_lowest_values_in_masked_places(D, dt):
+    """The variance is past fp32's range: r = 0 and h = 0, not NaN, wherever the
+    lowest values stand; in every place they are a row of one value."""
+    x = rows(6, D, 0, DT[dt], "cuda")
+    w, b = params(D, 2, DT[dt], "cuda")
+    low = torch.finfo(DT[dt]).min
+    x[0, 0] = x[1, D // 2] = x[2, D - 1] = low
+    x[3, : D // 2] = low
+    x[4, D // 2:] = low
+    x[5] = low
+    assert torch.equal(layer_norm(x, w, b), b.expand(6, D))
+    assert torch.equal(run(x, w, b, torch.zeros_like(x))[1], torch.zeros_like(x))
