@@ -12,11 +12,14 @@
 // so equal inputs in equal places give equal bits.
 //
 // The norm reads every value once, the product reads and writes it once more:
-// memory, or for small sets the launches.  On MI355X 4e8 bf16 values take 122 us
-// (6.5 TB/s; conversion to 64 bits and the product-sum are hidden), 1.5e8 fp32
-// values clipped into fp32 masters 308 us (1.8 GB moved, 5.8 TB/s; a copy of
-// 1 GiB runs at 5.15).  464 gradients of one buffer into masters: 5 + 3 + 8 us
-// on the GPU in 34 us of host time; 1392 separate ones in place 116 us.
+// memory, or for small sets the launches.  On MI355X 4e8 bf16 values take 123 us
+// (6.5 TB/s, reading alone reaches 7.0; conversion to 64 bits and the product-sum
+// are hidden), in norms of order 1 and inf too.  1.5e8 fp32 values clipped into
+// fp32 masters take 309 us (1.8 GB moved, 5.8 TB/s; a copy reaches 6.3), in place
+// 321 us, and bf16 ones in place 167 us (5.6 and 5.4 TB/s).  The 464 gradients of
+// an 8-layer net, as its backward pass leaves them: 33 us in place, 44 into
+// masters, of which the GPU works 16; the 1392 of 24 layers 71 to 80 and 106 to
+// 120.  Those are the host's: it touches every tensor.
 // Reading the values in reverse for the product, to find the last of them still
 // in the Infinity Cache, gained nothing (432 us forwards, 451 backwards).
 #include <algorithm>
@@ -302,9 +305,11 @@ static int64_t most_blocks(const gtk_tensor_list* g, int64_t chunk) {
 }
 
 // Calls launch(jobs, blocks, first partial) for every J::kMax entries.
-// Tensors that lie one behind the other in memory (a module's gradients are
-// views of one buffer) are one run, and so one entry: the 1392 gradients of 24
-// layers in one buffer take one launch a pass instead of six.
+// Tensors that lie one behind the other in memory are one run, and so one entry.
+// An operator's backward pass leaves its gradients in one buffer, but partly in
+// another order than the module's parameters: a pair-stack layer's 58 gradients
+// are 15 runs, the 1392 of 24 layers 360, two launches a pass (apart: six; in one
+// buffer in the list's order: one.  In place 71, 89 and 63 us).
 template <typename J, typename F>
 static int for_each_launch(const gtk_tensor_list* g, const gtk_tensor_list* out, int64_t chunk, F launch) {
   J jobs;

@@ -14,20 +14,20 @@
 // lies far from zero and close together that difference is exact, and in any
 // row |x - x_0| is at most twice the largest |d|, so what 32 bits lose follows
 // the row's spread and not its offset.  (77 values of 1000.1 summed as they are
-// give a mean 6e-5 away, which with eps = 1e-5 makes h 0.02 instead of 0; the
-// subtraction costs nothing beside the row's loads: 2^20 bf16 rows of 128, both
-// passes, 227 us against 224.)  Each difference is divided by D before it is
-// added, so that a row with the type's lowest value in it, in a masked place, has
-// a finite mean; its variance is infinite in 32 bits, r and h are 0.
+// give a mean 6e-5 away, which with eps = 1e-5 makes h 0.02 instead of 0.  The
+// subtraction costs 1 to 2 %: 2^20 bf16 rows of 128, both passes, 226 us against
+// 224; 3000 of 16384, 122 against 120.)  Each difference is divided by D before
+// it is added, so that a row with the type's lowest value in it, in a masked
+// place, has a finite mean; its variance is infinite in 32 bits, r and h are 0.
 //
 // Some twenty operations a value of 2 or 4 bytes: memory bounds both passes.  A
-// row therefore stays in the registers of its threads from its one load to its
-// one store, whatever its width, and only rows of more than kWidestInRegisters
-// values are swept several times.  On MI355X, inputs in rotation: 2^20 bf16
-// rows of 128 take 84 us forward (6.4 TB/s) and 140 us backward (5.8 TB/s),
-// 2^18 take 23 and 41 us, 4096 of 4096 16 and 28 us, 10007 fp32 rows of 1023
-// 17 and 29 us; a copy of 1 GiB runs at 5.15 TB/s.  Short launches are bound by
-// their latency: 4096 fp32 rows of 128 take 3 us forward and 5 + 3 us backward.
+// row of up to kWidestInRegisters values therefore stays in the registers of its
+// threads from its one load to its one store; wider ones are swept several times.
+// On MI355X, inputs in rotation: 2^20 bf16 rows of 128 take 86 us forward (6.3
+// TB/s) and 145 us backward (5.6 TB/s), 2^18 take 24 and 41 us, 4096 of 4096 17
+// and 31 us, 10007 fp32 rows of 1023 17 and 31 us (backward: both launches); a
+// copy beyond the caches runs at 6.3 TB/s.  Short launches are bound by their
+// latency: 4096 fp32 rows of 128 take 3 us forward and 5 + 3 us backward.
 #include <algorithm>
 
 #include "capi_util.hpp"
@@ -285,8 +285,9 @@ __global__ __launch_bounds__(S::BT) void ln_forward_kernel(const typename S::T* 
 // part[block][0][c], part[block][1][c].  The second reduction takes three sums
 // at once: with q = sum d^2 and s2 = sum g d, mean(g h) = r s2 / D.  A thread
 // keeps its columns over all its rows, so the column sums cost two registers a
-// value and no traffic until the end; blocks are few and long-lived for that,
-// and the next step's rows are on their way while this one is reduced.
+// value and no traffic until the end; blocks are few and long-lived for that.
+// With one vector a thread (NV = 1) the next step's rows are on their way while
+// this one is reduced; with more the registers hold one step's only.
 template <typename S>
 __global__ __launch_bounds__(S::BT) void ln_backward_kernel(const typename S::T* __restrict__ x, int64_t xs,
                                                             const typename S::T* __restrict__ dy, int64_t ds,

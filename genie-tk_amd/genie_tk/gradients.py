@@ -124,7 +124,7 @@ def _clip_pytorch(tensors: Sequence[Tensor], outs: Sequence[Tensor], max_norm: f
     coef = (max_norm / (norm.double() + _EPS)).clamp(max=1.0)
     with torch.no_grad():
         for t, o in zip(tensors, outs):
-            # the product in 32 bits at least, rounded once
+            # the product in 32 bits at least, then rounded to the output's type
             wide = t.double() if t.dtype == torch.float64 else t.float()
             o.copy_(wide * coef.to(wide.dtype))
 
@@ -148,9 +148,9 @@ def grad_norm(tensors: Iterable[Tensor], norm_type: float = 2.0) -> Tensor:
 def clip_grads(grads: Iterable[Tensor], max_norm: float, norm_type: float = 2.0,
                out: Optional[Sequence[Tensor]] = None) -> Tuple[Tensor, List[Tensor]]:
     """``(norm, clipped)``: every gradient times ``min(1, max_norm / (norm +
-    1e-6))``.  ``grads`` are left as they are; the products are rounded once into
-    ``out``, tensors of the same shapes in bf16 or fp32 (fp32 ones hold the
-    gradients of fp32 master weights), or into new ones like ``grads``."""
+    1e-6))``.  ``grads`` are left as they are; the products, formed in fp32, are
+    rounded to ``out``, tensors of the same shapes in bf16 or fp32 (fp32 ones hold
+    the gradients of fp32 master weights), or to new ones like ``grads``."""
     grads = list(grads)
     norm_type, max_norm = float(norm_type), _check_max_norm(max_norm, "clip_grads")
     if out is not None and len(out) != len(grads):
