@@ -26,7 +26,7 @@ ARCH = "gfx950"
 
 HIP_SOURCES = ["layernorm.hip", "tri_mul.hip", "tri_mul_bwd.hip", "tri_attn.hip", "tri_attn_bwd.hip",
                "pair_transition.hip", "layernorm_grad.hip", "grad_norm.hip",
-               "capi.cpp"]
+               "dropout.hip", "group_norm.hip", "capi.cpp"]
 HIP_FLAGS = [
     f"--offload-arch={ARCH}",
     "-O3",

@@ -681,6 +681,23 @@ std::vector<c10::optional<at::Tensor>> layer_norm_backward(const at::Tensor& x, 
   return out;
 }
 
+// What a backward pass returns under create_graph: differentiating it again is an
+// error that names the operator.
+void once_differentiable(torch::autograd::variable_list& out, const char* what) {
+  if (!at::GradMode::is_enabled()) return;
+  torch::autograd::variable_list some;
+  for (const auto& t : out)
+    if (t.defined()) some.push_back(t.detach().requires_grad_(true));
+  if (some.empty()) return;
+  torch::autograd::DelayedError error(
+      std::string(what) + "'s backward is once_differentiable: a second derivative is not implemented",
+      (int)some.size());
+  const auto guarded = error.apply(std::move(some));
+  size_t k = 0;
+  for (auto& t : out)
+    if (t.defined()) t = guarded[k++];
+}
+
 // layer_norm_forward under autograd.  A node of C++: a training pass over 4096
 // rows of 128 takes 71 us of host time with it, 87 with a Python one.  Only x and
 // the weight are saved: the backward computes the rows' statistics again.
@@ -715,17 +732,7 @@ struct LayerNormFn : public torch::autograd::Function<LayerNormFn> {
       if (need_b) g[2] = g[2].to(bias_dtype);
     }
     torch::autograd::variable_list out{g[0], g[1], g[2], at::Tensor()};
-    if (at::GradMode::is_enabled()) {  // create_graph: differentiating these again is an error
-      torch::autograd::variable_list some;
-      for (const auto& t : out)
-        if (t.defined()) some.push_back(t.detach().requires_grad_(true));
-      torch::autograd::DelayedError error("layer_norm's backward is once_differentiable: a second derivative is not "
-                                          "implemented", (int)some.size());
-      const auto guarded = error.apply(std::move(some));
-      size_t k = 0;
-      for (auto& t : out)
-        if (t.defined()) t = guarded[k++];
-    }
+    once_differentiable(out, "layer_norm");
     return out;
   }
 };
@@ -743,6 +750,266 @@ c10::optional<at::Tensor> layer_norm(const at::Tensor& x, const c10::optional<at
                     (x.requires_grad() || (weight.has_value() && weight->requires_grad()) ||
                      (bias.has_value() && bias->requires_grad()));
   return grad ? LayerNormFn::apply(x, weight, bias, eps) : layer_norm_forward(x, weight, bias, eps);
+}
+
+// ---------------------------------------------------------------------------
+// Dropout with a counter-based generator
+// ---------------------------------------------------------------------------
+// What fixes a mask: the view of x, the share that is dropped and the key.
+struct DropoutMask {
+  int64_t outer, shared, inner;
+  double p;
+  uint64_t seed, offset;
+};
+
+at::Tensor dropout_forward(const at::Tensor& x, const at::Tensor& residual, at::ScalarType out_type,
+                           const at::Tensor& seed_device, const DropoutMask& k) {
+  const at::DeviceGuard guard(x.device());
+  const auto xc = x.contiguous(), rc = residual.defined() ? residual.contiguous() : residual;
+  auto out = at::empty(x.sizes(), x.options().dtype(out_type));
+  check_rc(gtk_dropout(xc.data_ptr(), gtk_dtype_of(xc, "x"), ptr_or_null(rc),
+                       rc.defined() ? gtk_dtype_of(rc, "residual") : GTK_F32, out.data_ptr(),
+                       gtk_dtype_of(out, "the output"), k.outer, k.shared, k.inner, k.p, k.seed,
+                       (const uint64_t*)ptr_or_null(seed_device), k.offset, cur_stream(x)));
+  return out;
+}
+
+using MaybeTensor = c10::optional<at::Tensor>;
+at::Tensor or_undefined(const MaybeTensor& t) { return t.value_or(at::Tensor()); }
+
+at::Tensor dropout_or_grad(const at::Tensor& x, const MaybeTensor& residual, at::ScalarType out_type,
+                           const MaybeTensor& seed_device, const DropoutMask& k);
+
+// Linear in x and in the residual: dL/dx is the same call on dL/dout, of which
+// any number of derivatives may be taken.  Nothing is saved but the key.
+struct DropoutFn : public torch::autograd::Function<DropoutFn> {
+  static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x, const MaybeTensor& residual,
+                            int64_t out_type, const MaybeTensor& seed_device, const DropoutMask& k) {
+    ctx->save_for_backward({or_undefined(seed_device)});
+    ctx->saved_data["key"] = std::vector<int64_t>{k.outer, k.shared, k.inner, (int64_t)k.seed, (int64_t)k.offset,
+                                                  (int64_t)x.scalar_type()};
+    ctx->saved_data["p"] = k.p;
+    ctx->saved_data["has_residual"] = residual.has_value();
+    ctx->saved_data["residual_type"] = (int64_t)(residual.has_value() ? residual->scalar_type() : at::kFloat);
+    return dropout_forward(x, or_undefined(residual), (at::ScalarType)out_type, or_undefined(seed_device), k);
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grads) {
+    const at::Tensor& dy = grads[0];
+    const auto v = ctx->saved_data["key"].toIntVector();
+    const DropoutMask k{v[0], v[1], v[2], ctx->saved_data["p"].toDouble(), (uint64_t)v[3], (uint64_t)v[4]};
+    const auto seed = ctx->get_saved_variables()[0];
+    torch::autograd::variable_list out(5);
+    if (ctx->needs_input_grad(0))
+      out[0] = dropout_or_grad(dy, c10::nullopt, (at::ScalarType)v[5], seed.defined() ? MaybeTensor(seed) : c10::nullopt, k);
+    // an absent residual has no edge to ask about
+    const bool residual = ctx->saved_data["has_residual"].toBool();
+    if (residual && ctx->needs_input_grad(1))
+      out[1] = dy.to((at::ScalarType)ctx->saved_data["residual_type"].toInt());
+    return out;
+  }
+};
+
+at::Tensor dropout_or_grad(const at::Tensor& x, const MaybeTensor& residual, at::ScalarType out_type,
+                           const MaybeTensor& seed_device, const DropoutMask& k) {
+  const bool grad =
+      at::GradMode::is_enabled() && (x.requires_grad() || (residual.has_value() && residual->requires_grad()));
+  return grad ? DropoutFn::apply(x, residual, (int64_t)out_type, seed_device, k)
+              : dropout_forward(x, or_undefined(residual), out_type, or_undefined(seed_device), k);
+}
+
+// x seen as [outer, size of shared_dim, inner] (no shared_dim: one decision a
+// value).  Without `strict`, None where an input has a forward-mode tangent.
+c10::optional<at::Tensor> dropout(const at::Tensor& x, double p, uint64_t seed, uint64_t offset,
+                                  c10::optional<int64_t> shared_dim, const c10::optional<at::Tensor>& residual,
+                                  const c10::optional<at::Tensor>& seed_device, bool strict) {
+  check_gpu(x, "x");
+  check_on(residual, x, "residual");
+  check_on(seed_device, x, "seed");
+  TORCH_CHECK(p >= 0.0 && p <= 1.0, "dropout probability has to be between 0 and 1, but got ", p);
+  TORCH_CHECK(!residual.has_value() || residual->sizes() == x.sizes(), "genie_tk._C: residual must have x's shape");
+  TORCH_CHECK(!seed_device.has_value() || (seed_device->numel() == 1 && seed_device->scalar_type() == at::kLong),
+              "genie_tk._C: a seed tensor is one int64 value");
+  if (x._fw_grad(0).defined() || (residual.has_value() && residual->_fw_grad(0).defined())) {
+    TORCH_CHECK_NOT_IMPLEMENTED(!strict, "genie_tk._C: dropout has no forward-mode derivative");
+    return c10::nullopt;
+  }
+  DropoutMask k{1, 1, x.numel(), p, seed, offset};
+  if (shared_dim.has_value()) {
+    const int64_t dim = at::maybe_wrap_dim(*shared_dim, x.dim());
+    k.inner = 1;
+    for (int64_t i = 0; i < x.dim(); ++i) (i < dim ? k.outer : i == dim ? k.shared : k.inner) *= x.size(i);
+  }
+  return dropout_or_grad(x, residual, residual.has_value() ? residual->scalar_type() : x.scalar_type(), seed_device, k);
+}
+
+// ---------------------------------------------------------------------------
+// Group norm with an activation, channels last
+// ---------------------------------------------------------------------------
+// Checked arguments: x [B, ..., C] as rows, the mask as floats, one type for both
+// parameters.
+struct GroupNormArgs {
+  int64_t B, P, C, groups, stride;
+  int dtype, param_dtype;
+  at::Tensor x, mask, weight, bias;
+
+  GroupNormArgs(const at::Tensor& in, int64_t groups_, const at::Tensor& w, const at::Tensor& b, const at::Tensor& m)
+      : groups(groups_) {
+    check_gpu(in, "x");
+    TORCH_CHECK(in.dim() >= 2, "x must be [B, ..., C]");
+    C = in.size(-1);
+    B = in.size(0);
+    P = 1;
+    for (int64_t k = 1; k < in.dim() - 1; ++k) P *= in.size(k);
+    TORCH_CHECK(groups >= 1 && C >= 1 && C % groups == 0, "genie_tk._C: ", C, " channels in ", groups, " groups");
+    dtype = gtk_dtype_of(in, "x");
+    c10::optional<at::Tensor> ow, ob;
+    if (w.defined()) ow = w;
+    if (b.defined()) ob = b;
+    check_ln(in, ow, "weight");
+    check_ln(in, ob, "bias");
+    check_on(m, in, "mask");
+    const bool mixed = w.defined() && b.defined() && w.scalar_type() != b.scalar_type();
+    if (w.defined()) weight = mixed ? f32c(w) : w.contiguous();
+    if (b.defined()) bias = mixed ? f32c(b) : b.contiguous();
+    param_dtype = weight.defined() ? gtk_dtype_of(weight, "weight")
+                  : bias.defined() ? gtk_dtype_of(bias, "bias")
+                                   : GTK_F32;
+    if (m.defined()) {
+      TORCH_CHECK(m.sizes() == in.sizes().slice(0, in.dim() - 1), "mask must be x's shape without its channels");
+      mask = f32c(m);
+    }
+    x = as_rows(in, &stride);
+  }
+  const float* mask_ptr() const { return mask.defined() ? mask.data_ptr<float>() : nullptr; }
+};
+
+// {y, stats}
+std::array<at::Tensor, 2> gn_forward(const at::Tensor& x, int64_t groups, const at::Tensor& weight,
+                                     const at::Tensor& bias, double eps, int64_t act, const at::Tensor& mask) {
+  const at::DeviceGuard guard(x.device());
+  const GroupNormArgs a(x, groups, weight, bias, mask);
+  auto y = at::empty(x.sizes(), x.options());
+  auto stats = at::empty({a.B, groups, 4}, x.options().dtype(at::kFloat));
+  if (a.B && a.P) {
+    at::Tensor ws;
+    const size_t need = gtk_group_norm_workspace_size(a.B, a.P, a.C, groups, a.dtype);
+    if (need) ws = workspace(x, need);
+    check_rc(gtk_group_norm_forward(a.x.data_ptr(), a.stride, a.mask_ptr(), y.data_ptr(), stats.data_ptr<float>(),
+                                    ptr_or_null(a.weight), ptr_or_null(a.bias), a.param_dtype, a.B, a.P, a.C, groups,
+                                    (float)eps, (int)act, a.dtype, need ? ws.data_ptr() : nullptr, need,
+                                    cur_stream(x)));
+  }
+  return {y, stats};
+}
+
+// {dx, dweight, dbias}, the ones not asked for undefined; dweight and dbias in
+// their parameters' types (fp32 without).
+std::array<at::Tensor, 3> gn_backward(const at::Tensor& x, const at::Tensor& dy, const at::Tensor& stats,
+                                      int64_t groups, const at::Tensor& weight, const at::Tensor& bias, int64_t act,
+                                      const at::Tensor& mask, std::array<bool, 3> need) {
+  const at::DeviceGuard guard(x.device());
+  const GroupNormArgs a(x, groups, weight, bias, mask);
+  check_on(dy, x, "dy");
+  check_on(stats, x, "stats");
+  TORCH_CHECK(dy.sizes() == x.sizes() && dy.scalar_type() == x.scalar_type(), "dy must match x in shape and dtype");
+  TORCH_CHECK(stats.scalar_type() == at::kFloat && stats.is_contiguous() && stats.numel() == a.B * groups * 4,
+              "stats are those that the forward pass returned");
+  int64_t ds;
+  const auto dyc = as_rows(dy, &ds);
+  const auto popts = x.options().dtype(a.param_dtype == GTK_F32 ? at::kFloat : at::kBFloat16);
+  std::array<at::Tensor, 3> out;
+  if (need[0]) out[0] = at::empty(x.sizes(), x.options());
+  for (int k = 1; k < 3; ++k)
+    if (need[k]) out[k] = at::empty({a.C}, popts);
+  if (a.P) {
+    at::Tensor ws;
+    const size_t bytes = gtk_group_norm_backward_workspace_size(a.B, a.P, a.C, groups, a.dtype);
+    if (bytes) ws = workspace(x, bytes);
+    auto ptr = [&](int k) { return out[k].defined() ? out[k].data_ptr() : nullptr; };
+    check_rc(gtk_group_norm_backward(a.x.data_ptr(), a.stride, a.mask_ptr(), dyc.data_ptr(), ds,
+                                     stats.data_ptr<float>(), ptr_or_null(a.weight), ptr_or_null(a.bias),
+                                     a.param_dtype, ptr(0), ptr(1), ptr(2), a.B, a.P, a.C, groups, (int)act, a.dtype,
+                                     bytes ? ws.data_ptr() : nullptr, bytes, cur_stream(x)));
+  } else {
+    for (int k = 1; k < 3; ++k)
+      if (need[k]) out[k].zero_();
+  }
+  // parameters of two types were taken in fp32
+  if (out[1].defined() && weight.defined()) out[1] = out[1].to(weight.scalar_type());
+  if (out[2].defined() && bias.defined()) out[2] = out[2].to(bias.scalar_type());
+  return out;
+}
+
+std::vector<at::Tensor> group_norm_forward(const at::Tensor& x, int64_t groups, const c10::optional<at::Tensor>& weight,
+                                           const c10::optional<at::Tensor>& bias, double eps, int64_t act,
+                                           const c10::optional<at::Tensor>& mask) {
+  const auto r = gn_forward(x, groups, or_undefined(weight), or_undefined(bias), eps, act, or_undefined(mask));
+  return {r[0], r[1]};
+}
+
+std::vector<c10::optional<at::Tensor>> group_norm_backward(const at::Tensor& x, const at::Tensor& dy,
+                                                           const at::Tensor& stats, int64_t groups,
+                                                           const c10::optional<at::Tensor>& weight,
+                                                           const c10::optional<at::Tensor>& bias, int64_t act,
+                                                           const c10::optional<at::Tensor>& mask, bool need_x,
+                                                           bool need_weight, bool need_bias) {
+  const auto g = gn_backward(x, dy, stats, groups, or_undefined(weight), or_undefined(bias), act, or_undefined(mask),
+                             {need_x, need_weight, need_bias});
+  std::vector<c10::optional<at::Tensor>> out(3);
+  for (int k = 0; k < 3; ++k)
+    if (g[k].defined()) out[k] = g[k];
+  return out;
+}
+
+struct GroupNormFn : public torch::autograd::Function<GroupNormFn> {
+  static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x, const MaybeTensor& weight,
+                            const MaybeTensor& bias, int64_t groups, double eps, int64_t act,
+                            const MaybeTensor& mask) {
+    const auto w = or_undefined(weight), b = or_undefined(bias), m = or_undefined(mask);
+    const auto r = gn_forward(x, groups, w, b, eps, act, m);
+    ctx->save_for_backward({x, w, b, m, r[1]});
+    ctx->saved_data["groups"] = groups;
+    ctx->saved_data["act"] = act;
+    return r[0];
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    torch::autograd::variable_list out(7);
+    {
+      at::NoGradGuard no_grad;
+      // the edges of absent parameters are not counted
+      const bool has_w = saved[1].defined(), has_b = saved[2].defined();
+      const auto g = gn_backward(saved[0], grads[0], saved[4], ctx->saved_data["groups"].toInt(), saved[1], saved[2],
+                                 ctx->saved_data["act"].toInt(), saved[3],
+                                 {ctx->needs_input_grad(0), has_w && ctx->needs_input_grad(1),
+                                  has_b && ctx->needs_input_grad(has_w ? 2 : 1)});
+      for (int k = 0; k < 3; ++k) out[k] = g[k];
+    }
+    once_differentiable(out, "group_norm");
+    return out;
+  }
+};
+
+// Without `strict`, None where an input has a forward-mode tangent.
+c10::optional<at::Tensor> group_norm(const at::Tensor& x, int64_t groups, const c10::optional<at::Tensor>& weight,
+                                     const c10::optional<at::Tensor>& bias, double eps, int64_t act,
+                                     const c10::optional<at::Tensor>& mask, bool strict) {
+  bool grad = false;
+  auto dual = [&](const at::Tensor& t) {
+    grad = grad || t.requires_grad();
+    return t._fw_grad(/*level=*/0).defined();
+  };
+  bool any = dual(x);
+  if (weight.has_value()) any = dual(*weight) || any;
+  if (bias.has_value()) any = dual(*bias) || any;
+  if (any) {
+    TORCH_CHECK_NOT_IMPLEMENTED(!strict, "genie_tk._C: group_norm has no forward-mode derivative");
+    return c10::nullopt;
+  }
+  if (grad && at::GradMode::is_enabled()) return GroupNormFn::apply(x, weight, bias, groups, eps, act, mask);
+  return gn_forward(x, groups, or_undefined(weight), or_undefined(bias), eps, act, or_undefined(mask))[0];
 }
 
 // ---------------------------------------------------------------------------
@@ -1096,6 +1363,25 @@ PYBIND11_MODULE(_C, m) {
   m.def("layer_norm_backward", &layer_norm_backward,
         "layer_norm_forward's backward: [dx, dweight, dbias], None where not needed", py::arg("x"), py::arg("dy"),
         py::arg("weight") = py::none(), py::arg("eps") = 1e-5, py::arg("need_x") = true,
+        py::arg("need_weight") = true, py::arg("need_bias") = true);
+  m.def("dropout", &dropout,
+        "residual + dropout(x) with the mask of a counter-based generator (shared along shared_dim), under autograd.  "
+        "Without strict, None where an input has a forward-mode tangent",
+        py::arg("x"), py::arg("p"), py::arg("seed"), py::arg("offset") = 0, py::arg("shared_dim") = py::none(),
+        py::arg("residual") = py::none(), py::arg("seed_device") = py::none(), py::arg("strict") = true);
+  m.def("group_norm", &group_norm,
+        "group_norm_forward under autograd (differentiable once, in reverse mode).  Without strict, None where an "
+        "input has a forward-mode tangent",
+        py::arg("x"), py::arg("groups"), py::arg("weight") = py::none(), py::arg("bias") = py::none(),
+        py::arg("eps") = 1e-5, py::arg("activation") = 0, py::arg("mask") = py::none(), py::arg("strict") = true);
+  m.def("group_norm_forward", &group_norm_forward,
+        "Group norm over channels-last x [B, ..., C] with an activation (0 none, 1 silu, 2 gelu): [y, stats]",
+        py::arg("x"), py::arg("groups"), py::arg("weight") = py::none(), py::arg("bias") = py::none(),
+        py::arg("eps") = 1e-5, py::arg("activation") = 0, py::arg("mask") = py::none());
+  m.def("group_norm_backward", &group_norm_backward,
+        "group_norm_forward's backward: [dx, dweight, dbias], None where not needed", py::arg("x"), py::arg("dy"),
+        py::arg("stats"), py::arg("groups"), py::arg("weight") = py::none(), py::arg("bias") = py::none(),
+        py::arg("activation") = 0, py::arg("mask") = py::none(), py::arg("need_x") = true,
         py::arg("need_weight") = true, py::arg("need_bias") = true);
   m.def("grad_norm", &grad_norm,
         "Norm over every value of the tensors (fp32 scalar; norm_type 1, 2 or inf).  Without strict, None where a "

@@ -5,10 +5,15 @@ API of ``src/genie_tk/pair_transform.py`` in the reference (DropoutRowwise
 :87-195, PairTransformNet :198-258).  Update order per layer (:180-193):
 tri-mul out, tri-mul in, tri-attn start, tri-attn end (each added to p with
 row/column-shared dropout), pair transition, then p * mask.
+
+An addition: given a ``dropout_seed``, the layers draw their masks from the
+counter-based generator of ``genie_tk.primitives.dropout``, which applies the mask
+and adds the residual in one kernel and stores no mask.  Without one they draw
+from torch's generator.
 """
 from __future__ import annotations
 
-from typing import Optional, Tuple
+from typing import Optional, Tuple, Union
 
 import torch
 import torch.nn as nn
@@ -16,13 +21,16 @@ from torch import Tensor
 
 from genie_tk import _dispatch, _ext
 
-from genie_tk.primitives import Linear
+from genie_tk.primitives import Linear, dropout
 from genie_tk.triangle_attention import TriangleAttentionEndingNode, TriangleAttentionStartingNode
 from genie_tk.triangle_mul import TriangleMultiplicationIncoming, TriangleMultiplicationOutgoing
 
 
 class _SharedDropout(nn.Module):
-    """Dropout whose mask is shared along one spatial axis of [*, L, L, C]."""
+    """Dropout whose mask is shared along one spatial axis of [*, L, L, C].
+
+    ``forward(x, seed, offset, residual)`` is ``genie_tk.primitives.dropout``;
+    without a seed the mask comes from torch's generator."""
 
     def __init__(self, p: float, shared_dim: int):
         super().__init__()
@@ -30,12 +38,15 @@ class _SharedDropout(nn.Module):
         self.dropout = nn.Dropout(p)
         self._shared_dim = shared_dim
 
-    def forward(self, x: Tensor) -> Tensor:
-        if not self.training or self.p == 0:
-            return x
-        shape = list(x.shape)
-        shape[self._shared_dim] = 1
-        return x * self.dropout(x.new_ones(shape))
+    def forward(self, x: Tensor, seed: Union[int, Tensor, None] = None, offset: int = 0,
+                residual: Optional[Tensor] = None) -> Tensor:
+        if self.training and self.p != 0:
+            if seed is not None:
+                return dropout(x, self.p, seed, offset, self._shared_dim, residual)
+            shape = list(x.shape)
+            shape[self._shared_dim] = 1
+            x = x * self.dropout(x.new_ones(shape))
+        return x if residual is None else residual + x
 
 
 class DropoutRowwise(_SharedDropout):
@@ -149,7 +160,12 @@ class PairTransition(nn.Module):
 
 
 class PairTransformLayer(nn.Module):
-    """One pair-stack block; forward((p, p_mask)) -> (p, p_mask)."""
+    """One pair-stack block; forward((p, p_mask)) -> (p, p_mask).
+
+    ``dropout_seed`` (an int, or one int64 value on p's device) with
+    ``dropout_offset`` to ``dropout_offset + 3`` chooses the four dropout masks."""
+
+    DROPOUTS = 4  # offsets that a layer takes
 
     def __init__(self, c_p: int, include_mul_update: bool = True, include_tri_att: bool = True,
                  c_hidden_mul: int = 128, c_hidden_tri_att: int = 32, n_head_tri: int = 4,
@@ -175,7 +191,8 @@ class PairTransformLayer(nn.Module):
         self.dropout_row = DropoutRowwise(tri_dropout)
         self.dropout_col = DropoutColumnwise(tri_dropout)
 
-    def forward(self, inputs: Tuple[Tensor, Tensor]) -> Tuple[Tensor, Tensor]:
+    def forward(self, inputs: Tuple[Tensor, Tensor], dropout_seed: Union[int, Tensor, None] = None,
+                dropout_offset: int = 0) -> Tuple[Tensor, Tensor]:
         p, p_mask = inputs
         if not self.training or self.dropout_row.p == 0:
             # dropout is the identity: every residual add and the final mask
@@ -187,19 +204,26 @@ class PairTransformLayer(nn.Module):
                 p = self.tri_att_start.forward_residual(p, p_mask)
                 p = self.tri_att_end.forward_residual(p, p_mask)
             return self.pair_transition.forward_residual_masked(p, p_mask), p_mask
+
+        def add(p: Tensor, drop: nn.Module, update: Tensor, place: int) -> Tensor:
+            if dropout_seed is None:
+                return p + drop(update)
+            return drop(update, dropout_seed, dropout_offset + place, p)
+
         if self.include_mul_update:
-            p = p + self.dropout_row(self.tri_mul_out(p, p_mask))
-            p = p + self.dropout_row(self.tri_mul_in(p, p_mask))
+            p = add(p, self.dropout_row, self.tri_mul_out(p, p_mask), 0)
+            p = add(p, self.dropout_row, self.tri_mul_in(p, p_mask), 1)
         if self.include_tri_att:
-            p = p + self.dropout_row(self.tri_att_start(p, p_mask))
-            p = p + self.dropout_col(self.tri_att_end(p, p_mask))
+            p = add(p, self.dropout_row, self.tri_att_start(p, p_mask), 2)
+            p = add(p, self.dropout_col, self.tri_att_end(p, p_mask), 3)
         p = p + self.pair_transition(p, p_mask)
         p = p * p_mask.unsqueeze(-1)
         return p, p_mask
 
 
 class PairTransformNet(nn.Module):
-    """``n_layers`` PairTransformLayers applied in sequence."""
+    """``n_layers`` PairTransformLayers applied in sequence; with a ``dropout_seed``
+    (PairTransformLayer's) layer k takes the offsets 4 k to 4 k + 3."""
 
     def __init__(self, c_p: int, n_layers: int, include_mul_update: bool = True,
                  include_tri_att: bool = True, c_hidden_mul: int = 128,
@@ -215,7 +239,8 @@ class PairTransformNet(nn.Module):
             for _ in range(n_layers)
         ])
 
-    def forward(self, p: Tensor, p_mask: Tensor) -> Tensor:
-        for layer in self.layers:
-            p, p_mask = layer((p, p_mask))
+    def forward(self, p: Tensor, p_mask: Tensor, dropout_seed: Union[int, Tensor, None] = None) -> Tensor:
+        for k, layer in enumerate(self.layers):
+            seeded = () if dropout_seed is None else (dropout_seed, k * PairTransformLayer.DROPOUTS)
+            p, p_mask = layer((p, p_mask), *seeded)
         return p

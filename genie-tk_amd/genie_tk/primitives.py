@@ -1,15 +1,17 @@
-"""Linear layer with AlphaFold-style initialisers, gated multi-head attention
-and LayerNorm.
+"""Linear layer with AlphaFold-style initialisers, gated multi-head attention,
+LayerNorm, group norm and dropout.
 
 API and semantics of ``src/genie_tk/primitives.py`` in the reference:
 ``_init_weights`` (:17-40), ``Linear`` (:43-62), ``Attention`` (:65-178).
 ``LayerNorm`` and ``layer_norm`` are additions: torch's LayerNorm with the
-forward and the backward pass on the HIP kernels.
+forward and the backward pass on the HIP kernels.  So are ``GroupNorm`` and
+``group_norm`` (channels last, with an activation and a mask) and ``dropout``
+(the mask of a counter-based generator, never stored).
 """
 from __future__ import annotations
 
 import math
-from typing import List, Optional
+from typing import List, Optional, Union
 
 import torch
 import torch.nn as nn
@@ -189,3 +191,205 @@ class LayerNorm(nn.LayerNorm):
         # several dimensions are one: each row is contiguous in the flat view
         flat = [None if p is None else p.flatten() for p in (self.weight, self.bias)]
         return layer_norm(x.flatten(-len(shape)), *flat, self.eps).reshape(x.shape)
+
+
+# the codes of genie_tk._C's group norm
+_ACTIVATIONS = {None: 0, "silu": 1, "gelu": 2}
+
+
+def _group_norm_pytorch(x: Tensor, num_groups: int, weight: Optional[Tensor], bias: Optional[Tensor], eps: float,
+                        activation: Optional[str], mask: Optional[Tensor]) -> Tensor:
+    """In the widest of the types and at least fp32, rounded once."""
+    wide = torch.promote_types(x.dtype, torch.float32)
+    for p in (weight, bias):
+        if p is not None:
+            wide = torch.promote_types(wide, p.dtype)
+    B, C = x.shape[0], x.shape[-1]
+    P = math.prod(x.shape[1:-1])  # also where another size is 0
+    xf = x.to(wide).reshape(B, P, num_groups, C // num_groups)
+    if mask is None:
+        var, mean = torch.var_mean(xf, (1, 3), correction=0, keepdim=True)
+        d = xf - mean
+    else:
+        live = (mask != 0).reshape(B, P, 1, 1)
+        zero = xf.new_zeros(())
+        xf = torch.where(live, xf, zero)
+        count = (live.sum((1, 2, 3), keepdim=True) * xf.shape[3]).clamp(min=1).to(wide)
+        d = torch.where(live, xf - xf.sum((1, 3), keepdim=True) / count, zero)
+        var = d.square().sum((1, 3), keepdim=True) / count
+    y = d * torch.rsqrt(var + eps)
+    if weight is not None:
+        y = y * weight.to(wide).view(num_groups, -1)
+    if bias is not None:
+        y = y + bias.to(wide).view(num_groups, -1)
+    if activation is not None:
+        y = F.silu(y) if activation == "silu" else F.gelu(y)
+    if mask is not None:
+        y = torch.where(live, y, zero)
+    return y.to(x.dtype).reshape(x.shape)
+
+
+def group_norm(x: Tensor, num_groups: int, weight: Optional[Tensor] = None, bias: Optional[Tensor] = None,
+               eps: float = 1e-5, activation: Optional[str] = None, mask: Optional[Tensor] = None) -> Tensor:
+    """Group norm of channels-last ``x`` ([B, ..., C]) with optional ``weight`` and
+    ``bias`` ([C]) and an ``activation`` behind it (None, "silu" or "gelu", the exact
+    one), differentiable once.
+
+    A sample's group of C / ``num_groups`` channels is normalised over all of the
+    sample's positions; [B, C] normalises each row's groups by themselves, and
+    ``num_groups`` = C each channel (instance norm).  With a ``mask`` (broadcast to
+    x's shape without its channels; no gradient) only positions where it is not 0
+    count: elsewhere the output and dL/dx are 0, whatever x and dL/dy hold there.  A
+    sample without any is all 0.
+
+    Kernel path (bf16 or fp32 GPU tensor, parameters in bf16 or fp32, also mixed):
+    ``genie_tk._C.group_norm``.  The output and dL/dx have the type of ``x``, the
+    parameters' gradients their own; sums and statistics are held in fp32 or more.
+    Positions that lie one stride apart (a slice of wider channels) are read as they
+    are.  Other tensors, and those with a forward-mode tangent, run the same formula
+    in PyTorch.  Under autocast GPU tensors narrower than fp32 are taken to fp32
+    first, as torch's group norm takes them, and so is the output."""
+    if x.dim() < 2:
+        raise ValueError(f"group_norm: x must be [B, ..., C], got {tuple(x.shape)}")
+    C = x.shape[-1]
+    if num_groups < 1 or C < 1 or C % num_groups:
+        raise ValueError(f"group_norm: {C} channels in {num_groups} groups")
+    if activation not in _ACTIVATIONS:
+        raise ValueError(f"group_norm: activation must be None, 'silu' or 'gelu', got {activation!r}")
+    for name, p in (("weight", weight), ("bias", bias)):
+        if p is not None and p.shape != (C,):
+            raise ValueError(f"group_norm: {name} must be [{C}], got {tuple(p.shape)}")
+    if mask is not None:
+        mask = mask.detach().expand(x.shape[:-1])
+    if x.is_cuda and torch.is_autocast_enabled("cuda"):
+        x, weight, bias = (t.float() if t is not None and t.is_floating_point() and t.dtype != torch.float64 else t
+                           for t in (x, weight, bias))
+    if x.is_cuda:
+        if _ext.C is None or not torch.cuda.is_available():
+            _ext.missing("group_norm")
+        elif (x.dtype in _dispatch.SUPPORTED_DTYPES
+              and all(p is None or p.dtype in _dispatch.SUPPORTED_DTYPES for p in (weight, bias))):
+            y = _ext.C.group_norm(x, num_groups, weight, bias, eps, _ACTIVATIONS[activation], mask, False)
+            if y is not None:
+                return y
+    return _group_norm_pytorch(x, num_groups, weight, bias, eps, activation, mask)
+
+
+class GroupNorm(nn.GroupNorm):
+    """``nn.GroupNorm`` (same parameters and state_dict) over channels-last tensors
+    on ``group_norm``, with its ``activation`` and ``forward(x, mask=None)``;
+    ``use_fused_kernel=False`` selects the PyTorch path."""
+
+    def __init__(self, num_groups: int, num_channels: int, eps: float = 1e-5, affine: bool = True,
+                 device=None, dtype=None, activation: Optional[str] = None, use_fused_kernel: bool = True):
+        super().__init__(num_groups, num_channels, eps, affine, device=device, dtype=dtype)
+        if activation not in _ACTIVATIONS:
+            raise ValueError(f"GroupNorm: activation must be None, 'silu' or 'gelu', got {activation!r}")
+        self.activation = activation
+        self._fused_requested = use_fused_kernel
+
+    def extra_repr(self) -> str:
+        return super().extra_repr() + f", activation={self.activation!r}"
+
+    def forward(self, x: Tensor, mask: Optional[Tensor] = None) -> Tensor:
+        if x.dim() < 2 or x.shape[-1] != self.num_channels:
+            raise ValueError(f"GroupNorm: x must be [B, ..., {self.num_channels}], got {tuple(x.shape)}")
+        if self._fused_requested:
+            return group_norm(x, self.num_groups, self.weight, self.bias, self.eps, self.activation, mask)
+        if mask is not None:
+            mask = mask.detach().expand(x.shape[:-1])
+        return _group_norm_pytorch(x, self.num_groups, self.weight, self.bias, self.eps, self.activation, mask)
+
+
+_U32 = 0xFFFFFFFF
+_U64 = 0xFFFFFFFFFFFFFFFF
+
+
+def _signed(value: int) -> int:
+    """The int64 with the low 64 bits of ``value``."""
+    value &= _U64
+    return value - (1 << 64) if value >> 63 else value
+
+
+def dropout_mask(shape, p: float, seed: Union[int, Tensor], offset: int = 0, shared_dim: Optional[int] = None,
+                 device=None) -> Tensor:
+    """The mask that ``dropout`` applies to an x of ``shape``: True where a value is
+    kept, of size 1 along ``shared_dim``.  In PyTorch, on any device.
+
+    x is seen as [outer, shared, inner].  Value r of outer index o has 16 bits of
+    its own, half r % 2 (low first) of word r % 8 // 2 of Philox4x32-10 (J. Salmon,
+    M. Moraes, R. Dror, D. Shaw, "Parallel random numbers: as easy as 1, 2, 3", SC
+    2011) at counter o * ceil(inner / 8) + r // 8 (low 64 bits) and ``offset`` (high
+    64 bits) under the key ``seed``; it is kept where they are at least
+    round(65536 p)."""
+    shape = list(shape)
+    outer, inner = 1, math.prod(shape)
+    if shared_dim is not None:
+        dim = range(len(shape))[shared_dim]
+        outer, inner = math.prod(shape[:dim]), math.prod(shape[dim + 1:])
+        shape[dim] = 1
+    if isinstance(seed, Tensor):
+        device = seed.device if device is None else device
+        key = seed.detach().reshape(1).to(device)
+    else:
+        key = torch.tensor([_signed(seed)], device=device)
+    blocks = (inner + 7) // 8
+    c0 = torch.arange(outer * blocks, device=device)
+    c1 = c0 >> 32
+    c0 = c0 & _U32
+    c2, c3 = torch.full_like(c0, offset & _U32), torch.full_like(c0, offset >> 32 & _U32)
+    k0, k1 = key & _U32, key >> 32 & _U32
+    for _ in range(10):  # products wrap at 64 bits, whose halves are those of unsigned ones
+        p0, p1 = c0 * 0xD2511F53, c2 * 0xCD9E8D57
+        c0, c1, c2, c3 = (p1 >> 32 & _U32) ^ c1 ^ k0, p1 & _U32, (p0 >> 32 & _U32) ^ c3 ^ k1, p0 & _U32
+        k0, k1 = k0 + 0x9E3779B9 & _U32, k1 + 0xBB67AE85 & _U32
+    bits = torch.stack([h for w in (c0, c1, c2, c3) for h in (w & 0xFFFF, w >> 16)], -1)
+    keep = bits.view(outer, blocks * 8)[:, :inner] >= round(65536 * p)
+    return keep.reshape(shape)
+
+
+def dropout(x: Tensor, p: float, seed: Union[int, Tensor], offset: int = 0, shared_dim: Optional[int] = None,
+            residual: Optional[Tensor] = None) -> Tensor:
+    """``residual + dropout(x)`` (without ``residual``: ``dropout(x)``), the mask drawn
+    from a counter-based generator and never stored: the backward pass draws it
+    again.  ``dropout_mask`` is the mask.
+
+    ``seed`` (64 bits) and ``offset`` (64 bits: the layer, the place in it) choose the
+    mask; equal ones give equal masks on every device and in every type.  A ``seed``
+    tensor (one int64 value on x's device) is read when the kernel runs, so that a
+    captured graph draws another mask when the tensor has changed; it must not change
+    between a forward pass and its backward.  With ``shared_dim`` one mask holds for
+    all indices of that dimension.  Each value is dropped with probability t / 65536,
+    t = round(65536 p), and what is kept is scaled by 65536 / (65536 - t).  Dropped
+    values count for nothing, also where they are not finite.  The result has the
+    wider of the types of x and residual and is rounded once.
+
+    Kernel path (bf16 and fp32 GPU tensors): ``genie_tk._C.dropout``, differentiable
+    any number of times.  Other tensors, and those with a forward-mode tangent, run
+    the same formula in PyTorch.  Whether a module is training is the caller's to
+    ask."""
+    if not 0.0 <= p <= 1.0:
+        raise ValueError(f"dropout probability has to be between 0 and 1, but got {p}")
+    if shared_dim is not None and not -x.dim() <= shared_dim < x.dim():
+        raise IndexError(f"dropout: shared_dim {shared_dim} of {x.dim()} dimensions")
+    if residual is not None and residual.shape != x.shape:
+        raise ValueError(f"dropout: residual {tuple(residual.shape)} for x {tuple(x.shape)}")
+    drawn = isinstance(seed, Tensor)
+    if drawn and (seed.dtype != torch.int64 or seed.numel() != 1 or seed.device != x.device):
+        raise ValueError("dropout: a seed tensor is one int64 value on x's device")
+    kind = x.dtype if residual is None else torch.promote_types(x.dtype, residual.dtype)
+    if x.is_cuda:
+        if _ext.C is None or not torch.cuda.is_available():
+            _ext.missing("dropout")
+        elif (x.dtype in _dispatch.SUPPORTED_DTYPES
+              and (residual is None or residual.dtype in _dispatch.SUPPORTED_DTYPES)):
+            wide = None if residual is None else residual.to(kind)
+            y = _ext.C.dropout(x, p, 0 if drawn else seed & _U64, offset & _U64, shared_dim, wide,
+                               seed if drawn else None, False)
+            if y is not None:
+                return y
+    wide = torch.promote_types(kind, torch.float32)
+    t = round(65536 * p)
+    keep = dropout_mask(x.shape, p, seed, offset, shared_dim, x.device)
+    y = torch.where(keep, x.to(wide) * (65536 / (65536 - t) if t < 65536 else 0.0), torch.zeros((), dtype=wide, device=x.device))
+    return (y if residual is None else y + residual.to(wide)).to(kind)

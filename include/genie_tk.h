@@ -441,6 +441,69 @@ int gtk_grad_clip_with_norm(const gtk_tensor_list* grads, const gtk_tensor_list*
                             const float* norm, void* stream);
 
 /* ------------------------------------------------------------------------
+ * Dropout whose mask comes from a counter-based generator and is never stored
+ * (the reference's DropoutRowwise / DropoutColumnwise
+ * src/genie_tk/pair_transform.py:26-61 and the addition around them :180-193,
+ * which it leaves to torch).
+ *   out = residual + (kept ? x * 65536 / (65536 - t) : 0),  t = round(65536 p)
+ * x, residual (NULL: 0), out: [outer][shared][inner], contiguous; one mask for
+ * all `shared` indices (1: a decision for each value).  Value r < inner of outer
+ * index o is kept where its 16 bits are >= t: half r % 2 (low first) of word
+ * r % 8 / 2 of Philox4x32-10 at counter o * ceil(inner / 8) + r / 8 (low 64 bits)
+ * and `offset` (high 64 bits) under the key `seed`.  So p is taken to a multiple
+ * of 2^-16, and the scale is that multiple's; t = 65536 drops everything.  A
+ * dropped value counts for nothing, also where it is not finite.  The product
+ * and the sum are fp32, rounded once to out's type.  The backward pass is the
+ * same call without residual on dL/dout.
+ * seed_device: NULL, or one value on the device that replaces `seed` when the
+ * kernel runs (a captured graph draws a new mask at each replay).
+ * Types (x, residual, out): without residual any pair of GTK_F32 and GTK_BF16;
+ * with it all three alike, or (GTK_BF16, GTK_F32, GTK_F32).  p in [0, 1];
+ * outer * shared * inner and outer * inner rounded up to eights <= 2^48.  out may
+ * not alias x or residual.
+ * ------------------------------------------------------------------------ */
+int gtk_dropout(const void* x, int dtype, const void* residual, int residual_dtype, void* out, int out_dtype,
+                int64_t outer, int64_t shared, int64_t inner, double p, uint64_t seed, const uint64_t* seed_device,
+                uint64_t offset, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Group norm with an activation, channels last (no counterpart in the
+ * reference).  x: [B][positions][c] of `dtype`, positions x_stride elements apart
+ * throughout (also from one sample to the next; 0 repeats one) and contiguous
+ * inside; y the same, contiguous; channels in `groups` runs of c / groups.
+ *   y = act((x - mean) / sqrt(var + eps) * weight[ch] + bias[ch])
+ * mean and (biased) var are those of a sample's group over all positions that
+ * count: mask ([B][positions], NULL: all) is not 0 there.  Elsewhere y is 0, and
+ * x (and dy) may hold anything.  weight, bias: [c] of `param_dtype`, each may be
+ * NULL (1 and 0).  Sums and statistics are fp64.  Any alignment that the element
+ * type allows; equal inputs give equal bits.  y may not alias x.
+ * stats: [B][groups][4] floats, written for the backward pass: the mean (rounded,
+ * and what the rounding left), 1 / sqrt(var + eps), and 1 / (counted values), 0
+ * where there are none.  c in [1, 2^24], positions >= 1 and B >= 0,
+ * B * positions * c <= 2^48.  The workspace size queries return 0 for a shape or
+ * type that the call refuses; a call whose size is 0 otherwise takes NULL.
+ * ------------------------------------------------------------------------ */
+enum gtk_activation { GTK_ACT_NONE = 0, GTK_ACT_SILU = 1, GTK_ACT_GELU = 2 }; /* z, z / (1 + e^-z), z Phi(z) */
+
+size_t gtk_group_norm_workspace_size(int64_t B, int64_t positions, int64_t c, int64_t groups, int dtype);
+int gtk_group_norm_forward(const void* x, int64_t x_stride, const float* mask, void* y, float* stats,
+                           const void* weight, const void* bias, int param_dtype, int64_t B, int64_t positions,
+                           int64_t c, int64_t groups, float eps, int activation, int dtype, void* workspace,
+                           size_t workspace_bytes, void* stream);
+
+/* Its backward pass: given dL/dy (dy: as x, positions dy_stride apart) and the
+ * forward's stats, writes dL/dx ([B][positions][c] of `dtype`, contiguous, 0
+ * where the mask is), dL/dweight and dL/dbias ([c] of `param_dtype`, sums in fp32
+ * or more, rounded once).  A NULL gradient pointer skips that output.  Gradients
+ * are written, not accumulated; over no samples dweight and dbias are zero.  dx
+ * may not alias x or dy. */
+size_t gtk_group_norm_backward_workspace_size(int64_t B, int64_t positions, int64_t c, int64_t groups, int dtype);
+int gtk_group_norm_backward(const void* x, int64_t x_stride, const float* mask, const void* dy, int64_t dy_stride,
+                            const float* stats, const void* weight, const void* bias, int param_dtype, void* dx,
+                            void* dweight, void* dbias, int64_t B, int64_t positions, int64_t c, int64_t groups,
+                            int activation, int dtype, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------
  * Per-kernel timing (instrumentation; no counterpart in the reference).
  * gtk_timing_enable(1) makes every subsequent launch record a HIP event
  * before and after each kernel on its stream; gtk_timing_report() waits for
