@@ -16,8 +16,8 @@ struct ParamVec {
   }
 };
 
-// VE values of T: 16 bytes, or one.  Loads and stores are non-temporal: each value is
-// used once.
+// VE values of T: 16 bytes, or one.  Loads and stores are non-temporal where each
+// value is used once.
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef u32x4 u32x4_any __attribute__((aligned(2)));
 
@@ -25,6 +25,8 @@ template <typename T, int VE> struct Vec {
   u32x4 raw;
   __device__ __forceinline__ void load(const T* p) { raw = __builtin_nontemporal_load((const u32x4_any*)p); }
   __device__ __forceinline__ void store(T* p) const { __builtin_nontemporal_store(raw, (u32x4_any*)p); }
+  __device__ __forceinline__ void load_plain(const T* p) { raw = *(const u32x4_any*)p; }
+  __device__ __forceinline__ void store_plain(T* p) const { *(u32x4_any*)p = raw; }
   __device__ __forceinline__ void get(float* f) const {
     if constexpr (sizeof(T) == 2) {
 #pragma unroll
@@ -51,6 +53,8 @@ template <typename T> struct Vec<T, 1> {
   T v;
   __device__ __forceinline__ void load(const T* p) { v = *p; }
   __device__ __forceinline__ void store(T* p) const { *p = v; }
+  __device__ __forceinline__ void load_plain(const T* p) { v = *p; }
+  __device__ __forceinline__ void store_plain(T* p) const { *p = v; }
   __device__ __forceinline__ void get(float* f) const { f[0] = to_f32(v); }
   __device__ __forceinline__ void set(const float* f) { v = cvt<T>(f[0]); }
 };
