@@ -8,13 +8,22 @@
 // is exact there, so far from zero as a value lies, the variance loses nothing
 // that matters.  The mean is kept as a sum of two floats, so that d is off by its
 // own rounding only.
+//
+// Memory bounds it: some 15 to 40 operations a value of 2 or 4 bytes.  A sample's
+// group has to be read whole before its first result.  Where a slice of a sample
+// (all its positions, some whole groups) fits the registers of one block, a block
+// holds it from its one load to its one store.  Larger samples are streamed twice:
+// one launch sums, the next one applies, in the opposite order, so that what was read
+// last, and is still in the caches, comes first.
 #include <math.h>
 
 #include <algorithm>
 
 #include "capi_util.hpp"
+#include "column_sums.hpp"
 #include "common.hpp"
 #include "pack.hpp"
+#include "row_vec.hpp"
 
 namespace gtk {
 
@@ -31,44 +40,629 @@ __device__ __forceinline__ GroupStats close_stats(double s, double q, double cou
     g.low = (float)(mean - (double)g.mean);
     g.rstd = (float)(1.0 / sqrt(var + (double)eps));
     g.inv = (float)(1.0 / count);
+    // fmax takes the other operand of a NaN
+    if (!(q - q == 0.0)) g.mean = g.low = g.rstd = __builtin_nanf("");
   }
   return g;
 }
 
-// The value of the standard normal distribution's function and density at z.
+// ---------------------------------------------------------------------------
+// Activations.  The quotients are v_rcp_f32 (1 ulp); a division would take ten
+// instructions.
+// ---------------------------------------------------------------------------
+__device__ __forceinline__ float logistic(float z) { return __builtin_amdgcn_rcpf(1.f + __expf(-z)); }
+
+// The standard normal distribution's function at z, and its density.  For z < 0
+// the function is e^(-z^2/2) t P(t), t = 1 / (1 + 0.3 |z|), which keeps its
+// relative accuracy to the end; P was fitted to erfcx (weighted least squares on
+// |z| <= 14, iterated towards equal errors): 1.5e-7 of the value, 4.4e-7 with fp32's
+// roundings.
 __device__ __forceinline__ float normal_below(float z, float& density) {
-  density = 0.3989422804f * expf(-0.5f * z * z);
-  return 0.5f * erfcf(-0.70710678f * z);
+  const float e = __expf(-0.5f * z * z), t = __builtin_amdgcn_rcpf(fmaf(0.3f, fabsf(z), 1.f));
+  float p = 0.03567477342812997f;
+  p = fmaf(p, t, -0.1572030800704706f);
+  p = fmaf(p, t, 0.20635350232969402f);
+  p = fmaf(p, t, -0.05368364104385134f);
+  p = fmaf(p, t, 0.1285616251824942f);
+  p = fmaf(p, t, 0.09991349247240931f);
+  p = fmaf(p, t, 0.12075395598321578f);
+  p = fmaf(p, t, 0.11962929883230777f);
+  density = 0.3989422804f * e;
+  const float below = e * t * p;
+  return z < 0.f ? below : 1.f - below;
 }
 
 __device__ __forceinline__ float activate(float z, int act) {
   float density;
-  if (act == GTK_ACT_SILU) return z * sigmoidf_(z);
+  if (act == GTK_ACT_SILU) return z * logistic(z);
   if (act == GTK_ACT_GELU) return z * normal_below(z, density);
   return z;
 }
 __device__ __forceinline__ float activate_slope(float z, int act) {
   if (act == GTK_ACT_SILU) {
-    const float s = sigmoidf_(z);
-    return s * (1.f + z * (1.f - s));
+    const float s = logistic(z);
+    return s * fmaf(z, 1.f - s, 1.f);
   }
   if (act == GTK_ACT_GELU) {
     float density;
     const float below = normal_below(z, density);
-    return below + z * density;
+    return fmaf(z, density, below);
   }
   return 1.f;
 }
 
-struct ParamVector {
-  const void* p;
-  int bf;
-  __device__ __forceinline__ float get(int64_t c, float none) const {
-    if (!p) return none;
-    return bf ? to_f32(((const bf16*)p)[c]) : ((const float*)p)[c];
+// ---------------------------------------------------------------------------
+// Threads over positions and channels.  A team of `threads` has `across` vectors of
+// VE channels side by side and `rows` positions at once.  A vector's channels fall
+// into SL slots, each within one group.  Where the width is no multiple of VE the
+// last vector is moved back to end with it, and its first `skip` channels count for
+// nothing in sums (both threads store the same results there).
+// ---------------------------------------------------------------------------
+template <typename T_, int VE_, int SL_> struct Form {
+  typedef T_ T;
+  static constexpr int VE = VE_, SL = SL_, CPS = VE / SL;  // channels a slot
+};
+
+struct Team {
+  int threads, across, rows;
+  int pitch;  // of a slot's (channel's) partial sums in LDS
+  int lanes;  // that share one group's sum, a power of two
+  int channel_lanes;
+};
+
+struct Shape {
+  int64_t B, P;
+  int C, G, cg;
+};
+
+template <typename F> struct Place {
+  int at, row, skip;  // first channel within the slice
+  bool on, first;
+  __device__ __forceinline__ Place(int t, const Team& g, int width) {
+    row = t / g.across;
+    const int nominal = (t - row * g.across) * F::VE;
+    on = row < g.rows;
+    first = nominal == 0;
+    at = nominal + F::VE <= width ? nominal : width - F::VE;
+    skip = nominal - at;
   }
 };
 
+// Partial sums of N runs of channels each, [run][row of the team].
+template <int N, int VE, typename S>
+__device__ __forceinline__ void put_sums(S* sums, const S (&v)[N], int at, int skip, int row, bool on, const Team& g) {
+  if (!on) return;
+  constexpr int RUN = VE / N;
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    if (j * RUN < skip) continue;
+    S* to = sums + (at / RUN + j) * g.pitch;
+    to[row] = v[j];
+    if (row == g.rows - 1 && g.pitch > g.rows) to[g.rows] = S{0, 0};
+  }
+}
+
+template <typename S> __device__ __forceinline__ S lanes_sum(S a, int lanes) {
+  for (int off = lanes / 2; off; off /= 2) {
+    a.x += __shfl_xor(a.x, off, 64);
+    a.y += __shfl_xor(a.y, off, 64);
+  }
+  return a;
+}
+
+// f(o, sum of the o-th `len` entries) for o < outs, by one lane of each `lanes`.
+template <typename S, typename Fn>
+__device__ __forceinline__ void sum_runs(const S* sums, int outs, int len, int t, int threads, int lanes, Fn f) {
+  const int l = t & (lanes - 1);
+  for (int o = t / lanes; o < outs; o += threads / lanes) {
+    const S* from = sums + (int64_t)o * len;
+    S a{0, 0};
+#pragma unroll 4
+    for (int e = l; e < len; e += lanes) {
+      a.x += from[e].x;
+      a.y += from[e].y;
+    }
+    a = lanes_sum(a, lanes);
+    if (l == 0) f(o, a);
+  }
+}
+
+// Positions that count, of `n` counts; the sum in each lane.
+__device__ __forceinline__ int64_t sum_counts(const int* counts, int n, int t, int lanes) {
+  int64_t a = 0;
+  for (int e = t & (lanes - 1); e < n; e += lanes) a += counts[e];
+  for (int off = lanes / 2; off; off /= 2) a += __shfl_xor(a, off, 64);
+  return a;
+}
+
+template <typename F> __device__ __forceinline__ void load_params(float* f, const ParamVec& p, int c, float none) {
+  if (p.p) {
+    load_run<F::VE>(f, p, c);
+  } else {
+#pragma unroll
+    for (int e = 0; e < F::VE; ++e) f[e] = none;
+  }
+}
+
+// sum += (f, f^2), slot by slot
+template <typename F> __device__ __forceinline__ void add_squares(double2 (&sum)[F::SL], const float* f) {
+#pragma unroll
+  for (int e = 0; e < F::VE; ++e) {
+    const double v = f[e];
+    sum[e / F::CPS].x += v;
+    sum[e / F::CPS].y = fma(v, v, sum[e / F::CPS].y);
+  }
+}
+
+// What a thread needs of its groups and channels.
+template <typename F> struct Coefs {
+  float mean[F::SL], low[F::SL], rstd[F::SL], w[F::VE], b[F::VE];
+  __device__ __forceinline__ void set(const GroupStats* stats, const ParamVec& wp, const ParamVec& bp, int c, int at, int cg) {
+#pragma unroll
+    for (int j = 0; j < F::SL; ++j) {
+      const GroupStats g = stats[(at + j * F::CPS) / cg];
+      mean[j] = g.mean;
+      low[j] = g.low;
+      rstd[j] = g.rstd;
+    }
+    load_params<F>(w, wp, c, 1.f);
+    load_params<F>(b, bp, c, 0.f);
+  }
+  __device__ __forceinline__ float h(float x, int e) const {
+    const int j = e / F::CPS;
+    return ((x - mean[j]) - low[j]) * rstd[j];
+  }
+  // f = act(h w + b), or 0
+  __device__ __forceinline__ void forward(float* f, bool live, int act) const {
+#pragma unroll
+    for (int e = 0; e < F::VE; ++e) f[e] = live ? activate(fmaf(h(f[e], e), w[e], b[e]), act) : 0.f;
+  }
+  // f = h, g = dL/dz, 0 where the position does not count
+  __device__ __forceinline__ void backward(float* f, float* g, bool live, int act) const {
+#pragma unroll
+    for (int e = 0; e < F::VE; ++e) {
+      const float v = h(f[e], e);
+      f[e] = live ? v : 0.f;
+      g[e] = live ? g[e] * activate_slope(fmaf(v, w[e], b[e]), act) : 0.f;
+    }
+  }
+};
+
+struct Inputs {
+  const void* x;
+  int64_t xs;
+  const float* mask;
+  ParamVec w, b;
+};
+
+// ---------------------------------------------------------------------------
+// Resident: a team a slice of `groups` whole groups of one sample.
+// ---------------------------------------------------------------------------
+struct ResidentPlan {
+  Team team;
+  int held;    // vectors a thread
+  int groups;  // a slice
+  int slices;
+  int64_t per_slice;  // teams of a slice in the backward pass: each takes several samples
+  size_t lds;         // of a team
+};
+
+__device__ __forceinline__ int64_t row_of(int64_t b, int64_t P, int64_t pos) { return b * P + (pos < P ? pos : P - 1); }
+
+template <typename F, int NV>
+__global__ __launch_bounds__(1024) void gn_resident_forward_kernel(Inputs in, typename F::T* __restrict__ y,
+                                                                   GroupStats* __restrict__ stats, Shape s,
+                                                                   ResidentPlan p, float eps, int act) {
+  typedef typename F::T T;
+  extern __shared__ double2 gn_lds[];
+  const Team& g = p.team;
+  const int t = threadIdx.x % g.threads, team = threadIdx.x / g.threads, teams = blockDim.x / g.threads;
+  const int width = p.groups * s.cg;
+  const Place<F> at(t, g, width);
+  char* lds = (char*)gn_lds + team * p.lds;
+  double2* sums = (double2*)lds;
+  GroupStats* mine = (GroupStats*)(sums + (int64_t)width / F::CPS * g.pitch);
+  int* counts = (int*)(mine + p.groups);
+  const int64_t units = s.B * p.slices;
+  for (int64_t u0 = (int64_t)blockIdx.x * teams; u0 < units; u0 += (int64_t)gridDim.x * teams) {
+    const bool any = u0 + team < units;
+    const int64_t u = any ? u0 + team : units - 1, b = u / p.slices;
+    const int slice = (int)(u - b * p.slices), c = slice * width + at.at;
+    Vec<T, F::VE> v[NV];
+    bool live[NV];
+    int n = 0;
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int64_t pos = at.row + (int64_t)k * g.rows, row = row_of(b, s.P, pos);
+      v[k].load((const T*)in.x + row * in.xs + c);
+      live[k] = at.on && pos < s.P && (!in.mask || in.mask[row] != 0.f);
+      n += live[k];
+    }
+    double2 sum[F::SL];
+#pragma unroll
+    for (int j = 0; j < F::SL; ++j) sum[j] = double2{0, 0};
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      float f[F::VE];
+      v[k].get(f);
+      if (live[k]) add_squares<F>(sum, f);
+    }
+    put_sums<F::SL, F::VE>(sums, sum, at.at, at.skip, at.row, at.on, g);
+    if (at.first && at.on) counts[at.row] = n;
+    __syncthreads();
+    const double count = (double)s.cg * (double)(in.mask ? sum_counts(counts, g.rows, t, g.lanes) : s.P);
+    sum_runs(sums, p.groups, s.cg / F::CPS * g.pitch, t, g.threads, g.lanes, [&](int o, double2 a) {
+      mine[o] = close_stats(a.x, a.y, count, eps);
+      if (any) stats[b * s.G + slice * p.groups + o] = mine[o];
+    });
+    __syncthreads();
+    Coefs<F> co;
+    co.set(mine, in.w, in.b, c, at.at, s.cg);
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int64_t pos = at.row + (int64_t)k * g.rows;
+      float f[F::VE];
+      v[k].get(f);
+      co.forward(f, live[k], act);
+      v[k].set(f);
+      if (any && at.on && pos < s.P) v[k].store(y + (b * s.P + pos) * s.C + c);
+    }
+  }
+}
+
+// dx, and this team's sums of dz h and dz over its samples, part[team][0 and 1][c].
+template <typename F, int NV>
+__global__ __launch_bounds__(1024) void gn_resident_backward_kernel(Inputs in, const typename F::T* __restrict__ dy,
+                                                                    int64_t ds, const GroupStats* __restrict__ stats,
+                                                                    typename F::T* __restrict__ dx,
+                                                                    float* __restrict__ part, Shape s, ResidentPlan p,
+                                                                    int act) {
+  typedef typename F::T T;
+  extern __shared__ double2 gn_lds[];
+  const Team& g = p.team;
+  const int t = threadIdx.x % g.threads, team = threadIdx.x / g.threads, teams = blockDim.x / g.threads;
+  const int width = p.groups * s.cg;
+  const Place<F> at(t, g, width);
+  char* lds = (char*)gn_lds + team * p.lds;
+  float2* means = (float2*)lds;
+  float2* sums = means + p.groups;
+  const int64_t id = (int64_t)blockIdx.x * teams + team, index = id / p.slices;
+  const int slice = (int)(id - index * p.slices), c = slice * width + at.at;
+  float2 channel[F::VE];
+#pragma unroll
+  for (int e = 0; e < F::VE; ++e) channel[e] = float2{0.f, 0.f};
+  for (int64_t b0 = 0; b0 < s.B; b0 += p.per_slice) {
+    const bool any = index < p.per_slice && b0 + index < s.B;
+    const int64_t b = any ? b0 + index : s.B - 1;
+    Vec<T, F::VE> xv[NV], gv[NV];
+    bool live[NV];
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int64_t pos = at.row + (int64_t)k * g.rows, row = row_of(b, s.P, pos);
+      xv[k].load((const T*)in.x + row * in.xs + c);
+      gv[k].load(dy + row * ds + c);
+      live[k] = any && at.on && pos < s.P && (!in.mask || in.mask[row] != 0.f);
+    }
+    const GroupStats* of = stats + b * s.G + slice * p.groups;
+    Coefs<F> co;
+    co.set(of, in.w, in.b, c, at.at, s.cg);
+    float2 sum[F::SL];
+#pragma unroll
+    for (int j = 0; j < F::SL; ++j) sum[j] = float2{0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      float f[F::VE], d[F::VE];
+      xv[k].get(f);
+      gv[k].get(d);
+      co.backward(f, d, live[k], act);
+#pragma unroll
+      for (int e = 0; e < F::VE; ++e) {
+        const float gw = d[e] * co.w[e];
+        sum[e / F::CPS].x += gw;
+        sum[e / F::CPS].y += gw * f[e];
+        channel[e].x += d[e] * f[e];
+        channel[e].y += d[e];
+      }
+    }
+    if (!dx) continue;
+    put_sums<F::SL, F::VE>(sums, sum, at.at, at.skip, at.row, at.on, g);
+    __syncthreads();
+    sum_runs(sums, p.groups, s.cg / F::CPS * g.pitch, t, g.threads, g.lanes, [&](int o, float2 a) {
+      const float inv = of[o].inv;
+      means[o] = float2{a.x * inv, a.y * inv};
+    });
+    __syncthreads();
+    float2 mean[F::SL];
+#pragma unroll
+    for (int j = 0; j < F::SL; ++j) mean[j] = means[(at.at + j * F::CPS) / s.cg];
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int64_t pos = at.row + (int64_t)k * g.rows;
+      float f[F::VE], d[F::VE];
+      xv[k].get(f);
+      gv[k].get(d);
+      co.backward(f, d, live[k], act);
+#pragma unroll
+      for (int e = 0; e < F::VE; ++e) {
+        const int j = e / F::CPS;
+        f[e] = live[k] ? (d[e] * co.w[e] - mean[j].x - f[e] * mean[j].y) * co.rstd[j] : 0.f;
+      }
+      xv[k].set(f);
+      if (any && at.on && pos < s.P) xv[k].store(dx + (b * s.P + pos) * s.C + c);
+    }
+  }
+  if (!part) return;
+  __syncthreads();
+  put_sums<F::VE, F::VE>(sums, channel, at.at, at.skip, at.row, at.on, g);
+  __syncthreads();
+  float* dst = part + index * 2 * s.C + slice * width;
+  sum_runs(sums, width, g.pitch, t, g.threads, g.channel_lanes, [&](int o, float2 a) {
+    if (index >= p.per_slice) return;
+    dst[o] = a.x;
+    dst[s.C + o] = a.y;
+  });
+}
+
+// ---------------------------------------------------------------------------
+// Streamed: a team is a block, and has a chunk of a sample's positions, `steps` times
+// the team's rows.
+// ---------------------------------------------------------------------------
+constexpr int kStreamThreads = 1024;
+
+struct StreamPlan {
+  Team team;
+  int chunks, steps;
+};
+
+// The team's rows of steps [first, last) of sample b, U at once.
+template <typename F, int U> struct Rows {
+  Vec<typename F::T, F::VE> v[U];
+  // past the last step that one again
+  __device__ __forceinline__ void load(const typename F::T* p, int64_t stride, const Shape& s, int64_t b, int64_t step,
+                                       int64_t last, const Place<F>& at, const Team& g, bool keep) {
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+      const int64_t at_step = step + j < last ? step + j : last - 1;
+      const auto* from = p + row_of(b, s.P, at_step * g.rows + at.row) * stride + at.at;
+      if (keep)
+        v[j].load_plain(from);
+      else
+        v[j].load(from);
+    }
+  }
+};
+template <typename F, int U> struct Live {
+  bool live[U];
+  __device__ __forceinline__ void load(const float* mask, const Shape& s, int64_t b, int64_t step, int64_t last,
+                                       const Place<F>& at, const Team& g) {
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+      const int64_t pos = (step + j) * g.rows + at.row;
+      live[j] = at.on && step + j < last && pos < s.P && (!mask || mask[row_of(b, s.P, pos)] != 0.f);
+    }
+  }
+};
+
+// part[b][group][chunk], counts[b][chunk]
+template <typename F>
+__global__ __launch_bounds__(kStreamThreads) void gn_stats_kernel(Inputs in, double2* __restrict__ part,
+                                                                  int* __restrict__ counts, Shape s, StreamPlan p) {
+  constexpr int U = 4;
+  extern __shared__ double2 gn_lds[];
+  __shared__ int row_counts[kStreamThreads];
+  const Team& g = p.team;
+  const int t = threadIdx.x;
+  const Place<F> at(t, g, s.C);
+  const int64_t all = (s.P + g.rows - 1) / g.rows;
+  for (int64_t item = blockIdx.x; item < s.B * p.chunks; item += gridDim.x) {
+    const int64_t b = item / p.chunks;
+    const int chunk = (int)(item - b * p.chunks);
+    const int64_t first = (int64_t)chunk * p.steps, last = std::min<int64_t>(first + p.steps, all);
+    double2 sum[F::SL];
+#pragma unroll
+    for (int j = 0; j < F::SL; ++j) sum[j] = double2{0, 0};
+    int n = 0;
+    for (int64_t step = first; step < last; step += U) {
+      Rows<F, U> x;
+      Live<F, U> m;
+      x.load((const typename F::T*)in.x, in.xs, s, b, step, last, at, g, true);
+      m.load(in.mask, s, b, step, last, at, g);
+#pragma unroll
+      for (int j = 0; j < U; ++j) {
+        float f[F::VE];
+        x.v[j].get(f);
+        n += m.live[j];
+        if (m.live[j]) add_squares<F>(sum, f);
+      }
+    }
+    put_sums<F::SL, F::VE>(gn_lds, sum, at.at, at.skip, at.row, at.on, g);
+    if (at.first && at.on) row_counts[at.row] = n;
+    __syncthreads();
+    sum_runs(gn_lds, s.G, s.cg / F::CPS * g.pitch, t, kStreamThreads, g.lanes,
+             [&](int o, double2 a) { part[(b * s.G + o) * p.chunks + chunk] = a; });
+    if (in.mask && t < 64) {
+      const int64_t count = sum_counts(row_counts, g.rows, t, 64);
+      if (t == 0) counts[item] = (int)count;
+    }
+    __syncthreads();
+  }
+}
+
+template <typename F>
+__global__ __launch_bounds__(kStreamThreads) void gn_apply_kernel(Inputs in, const double2* __restrict__ part,
+                                                                  const int* __restrict__ counts,
+                                                                  typename F::T* __restrict__ y,
+                                                                  GroupStats* __restrict__ stats, Shape s, StreamPlan p,
+                                                                  float eps, int act) {
+  constexpr int U = 4;
+  extern __shared__ double2 gn_lds[];
+  GroupStats* mine = (GroupStats*)gn_lds;
+  const Team& g = p.team;
+  const int t = threadIdx.x;
+  const Place<F> at(t, g, s.C);
+  const int64_t all = (s.P + g.rows - 1) / g.rows;
+  for (int64_t item = blockIdx.x; item < s.B * p.chunks; item += gridDim.x) {
+    const int64_t b = item / p.chunks;
+    const int chunk = (int)(item - b * p.chunks);
+    const int64_t first = (int64_t)chunk * p.steps, last = std::min<int64_t>(first + p.steps, all);
+    Rows<F, U> x;
+    Live<F, U> m;
+    int64_t step = first + (last - 1 - first) / U * U;  // backwards
+    x.load((const typename F::T*)in.x, in.xs, s, b, step, last, at, g, false);
+    m.load(in.mask, s, b, step, last, at, g);
+    const double count =
+        (double)s.cg * (double)(in.mask ? sum_counts(counts + b * p.chunks, p.chunks, t, g.lanes) : s.P);
+    sum_runs(part + b * s.G * p.chunks, s.G, p.chunks, t, kStreamThreads, g.lanes, [&](int o, double2 a) {
+      mine[o] = close_stats(a.x, a.y, count, eps);
+      if (chunk == 0) stats[b * s.G + o] = mine[o];
+    });
+    __syncthreads();
+    Coefs<F> co;
+    co.set(mine, in.w, in.b, at.at, at.at, s.cg);
+    for (;;) {
+#pragma unroll
+      for (int j = 0; j < U; ++j) {
+        const int64_t pos = (step + j) * g.rows + at.row;
+        float f[F::VE];
+        x.v[j].get(f);
+        co.forward(f, m.live[j], act);
+        Vec<typename F::T, F::VE> o;
+        o.set(f);
+        if (at.on && step + j < last && pos < s.P) o.store(y + (b * s.P + pos) * s.C + at.at);
+      }
+      step -= U;
+      if (step < first) break;
+      x.load((const typename F::T*)in.x, in.xs, s, b, step, last, at, g, false);
+      m.load(in.mask, s, b, step, last, at, g);
+    }
+    __syncthreads();
+  }
+}
+
+// The chunk's sums of dz h and dz, channels[b][chunk][0 and 1][c], and of g and g h,
+// part[b][group][chunk].
+template <typename F>
+__global__ __launch_bounds__(kStreamThreads) void gn_backward_sums_kernel(Inputs in, const typename F::T* __restrict__ dy,
+                                                                          int64_t ds, const GroupStats* __restrict__ stats,
+                                                                          float2* __restrict__ part,
+                                                                          float* __restrict__ channels, Shape s,
+                                                                          StreamPlan p, int act) {
+  constexpr int U = 2;
+  extern __shared__ double2 gn_lds[];
+  float2* weighted = (float2*)gn_lds;  // [C]: a channel's part of its group's sums
+  float2* sums = weighted + s.C;
+  const Team& g = p.team;
+  const int t = threadIdx.x;
+  const Place<F> at(t, g, s.C);
+  const int64_t all = (s.P + g.rows - 1) / g.rows;
+  for (int64_t item = blockIdx.x; item < s.B * p.chunks; item += gridDim.x) {
+    const int64_t b = item / p.chunks;
+    const int chunk = (int)(item - b * p.chunks);
+    const int64_t first = (int64_t)chunk * p.steps, last = std::min<int64_t>(first + p.steps, all);
+    Coefs<F> co;
+    co.set(stats + b * s.G, in.w, in.b, at.at, at.at, s.cg);
+    float2 sum[F::VE];
+#pragma unroll
+    for (int e = 0; e < F::VE; ++e) sum[e] = float2{0.f, 0.f};
+    for (int64_t step = first; step < last; step += U) {
+      Rows<F, U> x, d;
+      Live<F, U> m;
+      x.load((const typename F::T*)in.x, in.xs, s, b, step, last, at, g, true);
+      d.load(dy, ds, s, b, step, last, at, g, true);
+      m.load(in.mask, s, b, step, last, at, g);
+#pragma unroll
+      for (int j = 0; j < U; ++j) {
+        float f[F::VE], dz[F::VE];
+        x.v[j].get(f);
+        d.v[j].get(dz);
+        co.backward(f, dz, m.live[j], act);
+#pragma unroll
+        for (int e = 0; e < F::VE; ++e) {
+          sum[e].x += dz[e] * f[e];
+          sum[e].y += dz[e];
+        }
+      }
+    }
+    put_sums<F::VE, F::VE>(sums, sum, at.at, at.skip, at.row, at.on, g);
+    __syncthreads();
+    sum_runs(sums, s.C, g.pitch, t, kStreamThreads, g.channel_lanes, [&](int c, float2 a) {
+      if (channels) {
+        channels[item * 2 * s.C + c] = a.x;
+        channels[(item * 2 + 1) * s.C + c] = a.y;
+      }
+      const float w = in.w.get(c, 1.f);
+      weighted[c] = float2{a.y * w, a.x * w};
+    });
+    __syncthreads();
+    if (part)
+      sum_runs(weighted, s.G, s.cg, t, kStreamThreads, g.lanes,
+               [&](int o, float2 a) { part[(b * s.G + o) * p.chunks + chunk] = a; });
+    __syncthreads();
+  }
+}
+
+template <typename F>
+__global__ __launch_bounds__(kStreamThreads) void gn_backward_apply_kernel(
+    Inputs in, const typename F::T* __restrict__ dy, int64_t ds, const GroupStats* __restrict__ stats,
+    const float2* __restrict__ part, typename F::T* __restrict__ dx, Shape s, StreamPlan p, int act) {
+  constexpr int U = 2;
+  extern __shared__ double2 gn_lds[];
+  float2* means = (float2*)gn_lds;
+  const Team& g = p.team;
+  const int t = threadIdx.x;
+  const Place<F> at(t, g, s.C);
+  const int64_t all = (s.P + g.rows - 1) / g.rows;
+  for (int64_t item = blockIdx.x; item < s.B * p.chunks; item += gridDim.x) {
+    const int64_t b = item / p.chunks;
+    const int chunk = (int)(item - b * p.chunks);
+    const int64_t first = (int64_t)chunk * p.steps, last = std::min<int64_t>(first + p.steps, all);
+    Rows<F, U> x, d;
+    Live<F, U> m;
+    int64_t step = first + (last - 1 - first) / U * U;  // backwards
+    x.load((const typename F::T*)in.x, in.xs, s, b, step, last, at, g, false);
+    d.load(dy, ds, s, b, step, last, at, g, false);
+    m.load(in.mask, s, b, step, last, at, g);
+    sum_runs(part + b * s.G * p.chunks, s.G, p.chunks, t, kStreamThreads, g.lanes, [&](int o, float2 a) {
+      const float inv = stats[b * s.G + o].inv;
+      means[o] = float2{a.x * inv, a.y * inv};
+    });
+    Coefs<F> co;
+    co.set(stats + b * s.G, in.w, in.b, at.at, at.at, s.cg);
+    __syncthreads();
+    float2 mean[F::SL];
+#pragma unroll
+    for (int j = 0; j < F::SL; ++j) mean[j] = means[(at.at + j * F::CPS) / s.cg];
+    for (;;) {
+#pragma unroll
+      for (int j = 0; j < U; ++j) {
+        const int64_t pos = (step + j) * g.rows + at.row;
+        float f[F::VE], dz[F::VE];
+        x.v[j].get(f);
+        d.v[j].get(dz);
+        co.backward(f, dz, m.live[j], act);
+#pragma unroll
+        for (int e = 0; e < F::VE; ++e) {
+          const int k = e / F::CPS;
+          f[e] = m.live[j] ? (dz[e] * co.w[e] - mean[k].x - f[e] * mean[k].y) * co.rstd[k] : 0.f;
+        }
+        Vec<typename F::T, F::VE> o;
+        o.set(f);
+        if (at.on && step + j < last && pos < s.P) o.store(dx + (b * s.P + pos) * s.C + at.at);
+      }
+      step -= U;
+      if (step < first) break;
+      x.load((const typename F::T*)in.x, in.xs, s, b, step, last, at, g, false);
+      d.load(dy, ds, s, b, step, last, at, g, false);
+      m.load(in.mask, s, b, step, last, at, g);
+    }
+    __syncthreads();
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Swept: rows of channels that a block's threads do not span.  A block a sample's
+// group, and for the parameters a block a channel.
+// ---------------------------------------------------------------------------
 template <typename T> __device__ __forceinline__ void block_add(T (&v)[3], T (*red)[4]) {
   __syncthreads();
 #pragma unroll
@@ -81,95 +675,315 @@ template <typename T> __device__ __forceinline__ void block_add(T (&v)[3], T (*r
   for (int k = 0; k < 3; ++k) v[k] = red[k][0] + red[k][1] + red[k][2] + red[k][3];
 }
 
-// A block a sample's group.
+// Calls f(position, channel) for this thread's values of a group that starts at
+// channel c0.
+template <typename Fn> __device__ __forceinline__ void for_values(const Shape& s, int c0, Fn f) {
+  for (int64_t pos = 0; pos < s.P; ++pos)
+    for (int k = threadIdx.x; k < s.cg; k += 256) f(pos, c0 + k);
+}
+
 template <typename T>
-__global__ __launch_bounds__(256) void gn_forward_kernel(const T* __restrict__ x, int64_t xs,
-                                                         const float* __restrict__ mask, T* __restrict__ y,
-                                                         GroupStats* __restrict__ stats, ParamVector w, ParamVector b,
-                                                         int64_t P, int64_t C, int64_t G, float eps, int act) {
+__global__ __launch_bounds__(256) void gn_swept_forward_kernel(Inputs in, T* __restrict__ y,
+                                                               GroupStats* __restrict__ stats, Shape s, float eps,
+                                                               int act) {
   __shared__ double red[3][4];
-  const int64_t bg = blockIdx.x, n = bg / G, cg = C / G, c0 = bg % G * cg;
-  double v[3] = {0, 0, 0};
-  for (int64_t i = threadIdx.x; i < P * cg; i += 256) {
-    const int64_t row = n * P + i / cg;
-    if (mask && mask[row] == 0.f) continue;
-    const double f = to_f32(x[row * xs + c0 + i % cg]);
-    v[0] += f;
-    v[1] += f * f;
-    v[2] += 1;
+  const T* x = (const T*)in.x;
+  for (int64_t bg = blockIdx.x; bg < s.B * s.G; bg += gridDim.x) {
+    const int64_t first = bg / s.G * s.P;
+    const int c0 = (int)(bg % s.G) * s.cg;
+    double v[3] = {0, 0, 0};
+    for_values(s, c0, [&](int64_t pos, int c) {
+      if (in.mask && in.mask[first + pos] == 0.f) return;
+      const double f = to_f32(x[(first + pos) * in.xs + c]);
+      v[0] += f;
+      v[1] += f * f;
+      v[2] += 1;
+    });
+    block_add(v, red);
+    const GroupStats g = close_stats(v[0], v[1], v[2], eps);
+    if (threadIdx.x == 0) stats[bg] = g;
+    for_values(s, c0, [&](int64_t pos, int c) {
+      const bool live = !in.mask || in.mask[first + pos] != 0.f;
+      const float h = ((to_f32(x[(first + pos) * in.xs + c]) - g.mean) - g.low) * g.rstd;
+      y[(first + pos) * s.C + c] = cvt<T>(live ? activate(fmaf(h, in.w.get(c, 1.f), in.b.get(c, 0.f)), act) : 0.f);
+    });
   }
-  block_add(v, red);
-  const GroupStats g = close_stats(v[0], v[1], v[2], eps);
-  if (threadIdx.x == 0) stats[bg] = g;
-  for (int64_t i = threadIdx.x; i < P * cg; i += 256) {
-    const int64_t row = n * P + i / cg, c = c0 + i % cg;
-    const bool live = !mask || mask[row] != 0.f;
-    const float h = ((to_f32(x[row * xs + c]) - g.mean) - g.low) * g.rstd;
-    y[row * C + c] = cvt<T>(live ? activate(h * w.get(c, 1.f) + b.get(c, 0.f), act) : 0.f);
+}
+
+// h and dz of a value; false where it does not count.
+template <typename T>
+__device__ __forceinline__ bool swept_backward(const Inputs& in, const T* dy, int64_t ds, const GroupStats& g,
+                                               int64_t row, int c, int act, float& h, float& dz) {
+  h = dz = 0.f;
+  if (in.mask && in.mask[row] == 0.f) return false;
+  h = ((to_f32(((const T*)in.x)[row * in.xs + c]) - g.mean) - g.low) * g.rstd;
+  dz = to_f32(dy[row * ds + c]) * activate_slope(fmaf(h, in.w.get(c, 1.f), in.b.get(c, 0.f)), act);
+  return true;
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void gn_swept_backward_kernel(Inputs in, const T* __restrict__ dy, int64_t ds,
+                                                                const GroupStats* __restrict__ stats,
+                                                                T* __restrict__ dx, Shape s, int act) {
+  __shared__ double red[3][4];
+  for (int64_t bg = blockIdx.x; bg < s.B * s.G; bg += gridDim.x) {
+    const int64_t first = bg / s.G * s.P;
+    const int c0 = (int)(bg % s.G) * s.cg;
+    const GroupStats g = stats[bg];
+    float h, dz;
+    double v[3] = {0, 0, 0};
+    for_values(s, c0, [&](int64_t pos, int c) {
+      swept_backward(in, dy, ds, g, first + pos, c, act, h, dz);
+      const float gw = dz * in.w.get(c, 1.f);
+      v[0] += gw;
+      v[1] += (double)gw * h;
+    });
+    block_add(v, red);
+    const float c1 = (float)(v[0] * g.inv), c2 = (float)(v[1] * g.inv);
+    for_values(s, c0, [&](int64_t pos, int c) {
+      const bool live = swept_backward(in, dy, ds, g, first + pos, c, act, h, dz);
+      dx[(first + pos) * s.C + c] = cvt<T>(live ? (dz * in.w.get(c, 1.f) - c1 - h * c2) * g.rstd : 0.f);
+    });
   }
 }
 
 template <typename T>
-__global__ __launch_bounds__(256) void gn_backward_kernel(const T* __restrict__ x, int64_t xs,
-                                                          const float* __restrict__ mask, const T* __restrict__ dy,
-                                                          int64_t ds, const GroupStats* __restrict__ stats,
-                                                          ParamVector w, ParamVector b, T* __restrict__ dx, int64_t P,
-                                                          int64_t C, int64_t G, int act) {
+__global__ __launch_bounds__(256) void gn_swept_params_kernel(Inputs in, const T* __restrict__ dy, int64_t ds,
+                                                              const GroupStats* __restrict__ stats,
+                                                              void* __restrict__ dw, void* __restrict__ db, int dst_bf,
+                                                              Shape s, int act) {
   __shared__ double red[3][4];
-  const int64_t bg = blockIdx.x, n = bg / G, cg = C / G, c0 = bg % G * cg;
-  const GroupStats st = stats[bg];
-  auto at = [&](int64_t i, float& h, float& g) {
-    const int64_t row = n * P + i / cg, c = c0 + i % cg;
-    h = g = 0.f;
-    if (mask && mask[row] == 0.f) return false;
-    h = ((to_f32(x[row * xs + c]) - st.mean) - st.low) * st.rstd;
-    g = to_f32(dy[row * ds + c]) * activate_slope(h * w.get(c, 1.f) + b.get(c, 0.f), act) * w.get(c, 1.f);
-    return true;
-  };
-  double v[3] = {0, 0, 0};
-  float h, g;
-  for (int64_t i = threadIdx.x; i < P * cg; i += 256) {
-    at(i, h, g);
-    v[0] += g;
-    v[1] += (double)g * h;
-  }
-  block_add(v, red);
-  const float c1 = (float)(v[0] * st.inv), c2 = (float)(v[1] * st.inv);
-  for (int64_t i = threadIdx.x; i < P * cg; i += 256) {
-    const bool live = at(i, h, g);
-    dx[(n * P + i / cg) * C + c0 + i % cg] = cvt<T>(live ? (g - c1 - h * c2) * st.rstd : 0.f);
+  for (int c = blockIdx.x; c < s.C; c += gridDim.x) {
+    double v[3] = {0, 0, 0};
+    for (int64_t row = threadIdx.x; row < s.B * s.P; row += 256) {
+      float h, dz;
+      swept_backward(in, dy, ds, stats[row / s.P * s.G + c / s.cg], row, c, act, h, dz);
+      v[0] += (double)dz * h;
+      v[1] += dz;
+    }
+    block_add(v, red);
+    if (threadIdx.x) continue;
+    for (int k = 0; k < 2; ++k) {
+      void* dst = k ? db : dw;
+      if (!dst) continue;
+      if (dst_bf)
+        ((bf16*)dst)[c] = (bf16)(float)v[k];
+      else
+        ((float*)dst)[c] = (float)v[k];
+    }
   }
 }
 
-// A block a channel.
-template <typename T>
-__global__ __launch_bounds__(256) void gn_params_kernel(const T* __restrict__ x, int64_t xs,
-                                                        const float* __restrict__ mask, const T* __restrict__ dy,
-                                                        int64_t ds, const GroupStats* __restrict__ stats, ParamVector w,
-                                                        ParamVector b, void* __restrict__ dw, void* __restrict__ db,
-                                                        int dst_bf, int64_t B, int64_t P, int64_t C, int64_t G,
-                                                        int act) {
-  __shared__ double red[3][4];
-  const int64_t c = blockIdx.x;
-  double v[3] = {0, 0, 0};
-  for (int64_t row = threadIdx.x; row < B * P; row += 256) {
-    if (mask && mask[row] == 0.f) continue;
-    const GroupStats st = stats[row / P * G + c / (C / G)];
-    const float h = ((to_f32(x[row * xs + c]) - st.mean) - st.low) * st.rstd;
-    const float dz = to_f32(dy[row * ds + c]) * activate_slope(h * w.get(c, 1.f) + b.get(c, 0.f), act);
-    v[0] += (double)dz * h;
-    v[1] += dz;
+// ---------------------------------------------------------------------------
+// Plans
+// ---------------------------------------------------------------------------
+constexpr size_t kMostLds = 156 * 1024;
+constexpr int kMostBlocks = 1 << 20;  // the kernels loop past that
+
+static int pow2_up(int64_t v) {
+  int p = 1;
+  while (p < v) p *= 2;
+  return p;
+}
+// A power of two of lanes for each of `outs` sums.
+static int lanes_for(int threads, int64_t outs) {
+  int l = 64;
+  while (l > 1 && (l > threads || l * outs > threads)) l /= 2;
+  return l;
+}
+static Team make_team(int threads, int across, int64_t groups, int64_t channels) {
+  Team t;
+  t.threads = threads;
+  t.across = across;
+  t.rows = threads / across;
+  // an odd pitch, or neighbouring slots' sums would lie in the same banks
+  t.pitch = t.rows >= 8 ? t.rows | 1 : t.rows;
+  t.lanes = lanes_for(threads, groups);
+  t.channel_lanes = lanes_for(threads, channels);
+  return t;
+}
+
+// The narrowest slices of whole groups that fill 64-byte pieces of memory, wider
+// ones as long as they leave four teams a CU.
+template <typename F> static bool plan_resident(const Shape& s, bool backward, ResidentPlan* plan) {
+  const int most = backward ? 4 : 8;
+  bool found = false;
+  for (int groups = 1; groups <= s.G; ++groups) {
+    if (s.G % groups) continue;
+    const int64_t width = (int64_t)groups * s.cg;
+    if (width < F::VE || (groups < s.G && width * (int64_t)sizeof(typename F::T) < 64)) continue;
+    const int64_t across = (width + F::VE - 1) / F::VE;
+    if (across > 1024 || s.P > 1024 * most) break;
+    const int64_t units = s.B * (s.G / groups);
+    if (found && units < 4 * (int64_t)device_cus()) break;
+    int threads = pow2_up(across);
+    auto held = [&](int n) { return (s.P + n / across - 1) / (n / across); };
+    while (threads < 1024 && held(threads) > most) threads *= 2;
+    if (held(threads) > most) break;
+    // more threads where there are few teams
+    while (threads < 1024 && held(threads) > 1 && units * threads < 512 * (int64_t)device_cus()) threads *= 2;
+    ResidentPlan p;
+    p.team = make_team(threads, (int)across, groups, width);
+    p.held = (int)held(threads);
+    p.groups = groups;
+    p.slices = s.G / groups;
+    p.per_slice = std::min<int64_t>(s.B, std::max<int64_t>(1, 2048 * (int64_t)device_cus() / threads / p.slices));
+    p.lds = backward ? groups * sizeof(float2) + width * p.team.pitch * sizeof(float2)
+                     : width / F::CPS * p.team.pitch * sizeof(double2) + groups * sizeof(GroupStats) +
+                           p.team.rows * sizeof(int);
+    p.lds = (p.lds + 15) & ~size_t(15);
+    if (p.lds * std::max(1, 256 / threads) > kMostLds) break;
+    *plan = p;
+    found = true;
   }
-  block_add(v, red);
-  if (threadIdx.x) return;
-  for (int k = 0; k < 2; ++k) {
-    void* dst = k ? db : dw;
-    if (!dst) continue;
-    if (dst_bf)
-      ((bf16*)dst)[c] = (bf16)(float)v[k];
-    else
-      ((float*)dst)[c] = (float)v[k];
+  return found;
+}
+
+// A chunk a CU, two where there are several samples (each block of the second
+// launch adds its sample's partial sums up).
+template <typename F> static bool plan_streamed(const Shape& s, StreamPlan* p) {
+  const int64_t across = ((int64_t)s.C + F::VE - 1) / F::VE;
+  if (across > kStreamThreads) return false;
+  p->team = make_team(kStreamThreads, (int)across, s.G, s.C);
+  const int64_t all = (s.P + p->team.rows - 1) / p->team.rows;
+  const int64_t want = std::max<int64_t>(1, (s.B == 1 ? 1 : 2) * (int64_t)device_cus() / s.B);
+  const int64_t steps = std::max<int64_t>((all + want - 1) / want, (all + (1 << 30) - 1) >> 30);
+  if (steps > 1 << 30) return false;
+  p->steps = (int)steps;
+  p->chunks = (int)((all + steps - 1) / steps);
+  return true;
+}
+
+template <typename F> struct Plan {
+  bool resident, streamed;
+  ResidentPlan r;
+  StreamPlan t;
+  Plan(const Shape& s, bool backward) {
+    resident = plan_resident<F>(s, backward, &r);
+    streamed = !resident && plan_streamed<F>(s, &t);
   }
+  int64_t parts(const Shape& s) const { return resident ? r.per_slice : streamed ? s.B * t.chunks : 0; }
+};
+
+// Calls run(Form) for the types and the width of a slot.
+template <typename T, typename Fn> static auto for_form(const Shape& s, Fn run) {
+  constexpr int VE = 16 / sizeof(T);
+  if (s.C < VE) return run(Form<T, 1, 1>());
+  if (s.cg % VE == 0) return run(Form<T, VE, 1>());
+  if (s.cg % (VE / 2) == 0) return run(Form<T, VE, 2>());
+  return run(Form<T, VE, VE>());
+}
+// Calls run(number) for the smallest number of held vectors that is enough.
+template <int MOST, typename Fn> static void for_held(int held, Fn run) {
+  if constexpr (MOST > 4)
+    if (held > 4) return run(std::integral_constant<int, 8>());
+  if (held > 2) return run(std::integral_constant<int, 4>());
+  if (held > 1) return run(std::integral_constant<int, 2>());
+  run(std::integral_constant<int, 1>());
+}
+
+static unsigned blocks_for(int64_t items) { return (unsigned)std::min<int64_t>(items, kMostBlocks); }
+
+template <typename F> struct ForwardWork {
+  double2* part;
+  int* counts;
+  ForwardWork(Carve& cv, const Shape& s, const Plan<F>& p) {
+    part = cv.take<double2>(p.streamed ? s.B * s.G * p.t.chunks : 0);
+    counts = cv.take<int>(p.streamed ? s.B * p.t.chunks : 0);
+  }
+};
+template <typename F> struct BackwardWork {
+  float2* part;
+  float* channels;
+  BackwardWork(Carve& cv, const Shape& s, const Plan<F>& p) {
+    part = cv.take<float2>(p.streamed ? s.B * s.G * p.t.chunks : 0);
+    channels = cv.take<float>(2 * (int64_t)s.C * p.parts(s));
+  }
+};
+
+template <typename F>
+static int launch_gn_forward(const Inputs& in, void* yp, GroupStats* stats, const Shape& s, float eps, int act, void* ws,
+                             size_t ws_bytes, hipStream_t st) {
+  typedef typename F::T T;
+  T* y = (T*)yp;
+  const Plan<F> p(s, false);
+  if (p.resident) {
+    StageTimer timer("group_norm_forward", st);
+    const int threads = std::max(256, p.r.team.threads), teams = threads / p.r.team.threads;
+    for_held<8>(p.r.held, [&](auto nv) {
+      gn_resident_forward_kernel<F, decltype(nv)::value>
+          <<<blocks_for((s.B * p.r.slices + teams - 1) / teams), threads, teams * p.r.lds, st>>>(in, y, stats, s, p.r, eps,
+                                                                                               act);
+    });
+  } else if (p.streamed) {
+    Carve cv(ws, ws_bytes);
+    const ForwardWork<F> work(cv, s, p);
+    const unsigned blocks = blocks_for(s.B * p.t.chunks);
+    {
+      StageTimer timer("group_norm_stats", st);
+      gn_stats_kernel<F><<<blocks, kStreamThreads, (size_t)(s.C / F::CPS) * p.t.team.pitch * sizeof(double2), st>>>(
+          in, work.part, work.counts, s, p.t);
+      GTK_LAUNCH_CHECK();
+    }
+    StageTimer timer("group_norm_apply", st);
+    gn_apply_kernel<F><<<blocks, kStreamThreads, s.G * sizeof(GroupStats), st>>>(in, work.part, work.counts, y, stats, s,
+                                                                                p.t, eps, act);
+  } else {
+    StageTimer timer("group_norm_forward", st);
+    gn_swept_forward_kernel<T><<<blocks_for(s.B * s.G), 256, 0, st>>>(in, y, stats, s, eps, act);
+  }
+  GTK_LAUNCH_CHECK();
+  return GTK_OK;
+}
+
+template <typename F>
+static int launch_gn_backward(const Inputs& in, const void* dyp, int64_t ds, const GroupStats* stats, void* dxp, void* dw,
+                              void* db, int dst_bf, const Shape& s, int act, void* ws, size_t ws_bytes, hipStream_t st) {
+  typedef typename F::T T;
+  const T* dy = (const T*)dyp;
+  T* dx = (T*)dxp;
+  const Plan<F> p(s, true);
+  Carve cv(ws, ws_bytes);
+  const BackwardWork<F> work(cv, s, p);
+  const bool sums = dw || db;
+  if (p.resident) {
+    StageTimer timer("group_norm_backward", st);
+    const int threads = std::max(256, p.r.team.threads), teams = threads / p.r.team.threads;
+    for_held<4>(p.r.held, [&](auto nv) {
+      gn_resident_backward_kernel<F, decltype(nv)::value>
+          <<<(unsigned)((p.r.per_slice * p.r.slices + teams - 1) / teams), threads, teams * p.r.lds, st>>>(
+              in, dy, ds, stats, dx, sums ? work.channels : nullptr, s, p.r, act);
+    });
+    GTK_LAUNCH_CHECK();
+  } else if (p.streamed) {
+    const unsigned blocks = blocks_for(s.B * p.t.chunks);
+    {
+      StageTimer timer("group_norm_backward_sums", st);
+      const size_t lds = (size_t)s.C * (1 + p.t.team.pitch) * sizeof(float2);
+      gn_backward_sums_kernel<F><<<blocks, kStreamThreads, lds, st>>>(
+          in, dy, ds, stats, dx ? work.part : nullptr, sums ? work.channels : nullptr, s, p.t, act);
+      GTK_LAUNCH_CHECK();
+    }
+    if (dx) {
+      StageTimer timer("group_norm_backward_apply", st);
+      gn_backward_apply_kernel<F><<<blocks, kStreamThreads, s.G * sizeof(float2), st>>>(in, dy, ds, stats, work.part, dx,
+                                                                                       s, p.t, act);
+      GTK_LAUNCH_CHECK();
+    }
+  } else {
+    if (dx) {
+      StageTimer timer("group_norm_backward", st);
+      gn_swept_backward_kernel<T><<<blocks_for(s.B * s.G), 256, 0, st>>>(in, dy, ds, stats, dx, s, act);
+      GTK_LAUNCH_CHECK();
+    }
+    if (sums) {
+      StageTimer timer("group_norm_params", st);
+      gn_swept_params_kernel<T><<<blocks_for(s.C), 256, 0, st>>>(in, dy, ds, stats, dw, db, dst_bf, s, act);
+      GTK_LAUNCH_CHECK();
+    }
+    return GTK_OK;
+  }
+  return sums ? launch_column_close("group_norm_close", work.channels, (int)p.parts(s), s.C, dw, db, dst_bf, st) : GTK_OK;
 }
 
 static bool gn_shape_ok(int64_t B, int64_t P, int64_t C, int64_t G, int dtype) {
@@ -178,34 +992,15 @@ static bool gn_shape_ok(int64_t B, int64_t P, int64_t C, int64_t G, int dtype) {
          B <= most / (P * C) && (dtype == GTK_F32 || dtype == GTK_BF16);
 }
 
-template <typename T>
-static int launch_gn_forward(const void* x, int64_t xs, const float* mask, void* y, float* stats, ParamVector w,
-                             ParamVector b, int64_t B, int64_t P, int64_t C, int64_t G, float eps, int act,
-                             hipStream_t st) {
-  StageTimer timer("group_norm_forward", st);
-  gn_forward_kernel<T><<<(unsigned)(B * G), 256, 0, st>>>((const T*)x, xs, mask, (T*)y, (GroupStats*)stats, w, b, P, C,
-                                                          G, eps, act);
-  GTK_LAUNCH_CHECK();
-  return GTK_OK;
-}
-
-template <typename T>
-static int launch_gn_backward(const void* x, int64_t xs, const float* mask, const void* dy, int64_t ds,
-                              const float* stats, ParamVector w, ParamVector b, void* dx, void* dw, void* db, int pbf,
-                              int64_t B, int64_t P, int64_t C, int64_t G, int act, hipStream_t st) {
-  if (dx && B) {
-    StageTimer timer("group_norm_backward", st);
-    gn_backward_kernel<T><<<(unsigned)(B * G), 256, 0, st>>>((const T*)x, xs, mask, (const T*)dy, ds,
-                                                             (const GroupStats*)stats, w, b, (T*)dx, P, C, G, act);
-    GTK_LAUNCH_CHECK();
-  }
-  if (dw || db) {
-    StageTimer timer("group_norm_params", st);
-    gn_params_kernel<T><<<(unsigned)C, 256, 0, st>>>((const T*)x, xs, mask, (const T*)dy, ds, (const GroupStats*)stats,
-                                                     w, b, dw, db, pbf, B, P, C, G, act);
-    GTK_LAUNCH_CHECK();
-  }
-  return GTK_OK;
+template <template <typename> class Work> static size_t work_size(const Shape& s, int dtype, bool backward) {
+  auto size = [&](auto form) {
+    typedef decltype(form) F;
+    Carve cv(nullptr, SIZE_MAX);
+    const Plan<F> p(s, backward);
+    const Work<F> work(cv, s, p);
+    return cv.off;
+  };
+  return dtype == GTK_F32 ? for_form<float>(s, size) : for_form<bf16>(s, size);
 }
 
 }  // namespace gtk
@@ -223,7 +1018,8 @@ using namespace gtk;
   GTK_REQUIRE(x_stride >= 0, GTK_EINVAL, name ": negative stride")
 
 extern "C" size_t gtk_group_norm_workspace_size(int64_t B, int64_t positions, int64_t c, int64_t groups, int dtype) {
-  return 0;
+  if (!gn_shape_ok(B, positions, c, groups, dtype) || B == 0) return 0;
+  return work_size<ForwardWork>(Shape{B, positions, (int)c, (int)groups, (int)(c / groups)}, dtype, false);
 }
 
 extern "C" int gtk_group_norm_forward(const void* x, int64_t x_stride, const float* mask, void* y, float* stats,
@@ -236,14 +1032,20 @@ extern "C" int gtk_group_norm_forward(const void* x, int64_t x_stride, const flo
   const size_t need = gtk_group_norm_workspace_size(B, positions, c, groups, dtype);
   GTK_REQUIRE(workspace_bytes >= need && (workspace || !need), GTK_EWORKSPACE,
               "gtk_group_norm_forward: workspace %zu < %zu bytes", workspace ? workspace_bytes : 0, need);
-  const ParamVector w{weight, param_dtype == GTK_BF16}, b{bias, param_dtype == GTK_BF16};
-  return (dtype == GTK_F32 ? launch_gn_forward<float> : launch_gn_forward<bf16>)(
-      x, x_stride, mask, y, stats, w, b, B, positions, c, groups, eps, activation, (hipStream_t)stream);
+  const int pbf = param_dtype == GTK_BF16;
+  const Inputs in{x, x_stride, mask, {weight, pbf}, {bias, pbf}};
+  const Shape s{B, positions, (int)c, (int)groups, (int)(c / groups)};
+  auto run = [&](auto form) {
+    return launch_gn_forward<decltype(form)>(in, y, (GroupStats*)stats, s, eps, activation, workspace, workspace_bytes,
+                                             (hipStream_t)stream);
+  };
+  return dtype == GTK_F32 ? for_form<float>(s, run) : for_form<bf16>(s, run);
 }
 
 extern "C" size_t gtk_group_norm_backward_workspace_size(int64_t B, int64_t positions, int64_t c, int64_t groups,
                                                          int dtype) {
-  return 0;
+  if (!gn_shape_ok(B, positions, c, groups, dtype) || B == 0) return 0;
+  return work_size<BackwardWork>(Shape{B, positions, (int)c, (int)groups, (int)(c / groups)}, dtype, true);
 }
 
 extern "C" int gtk_group_norm_backward(const void* x, int64_t x_stride, const float* mask, const void* dy,
@@ -258,8 +1060,16 @@ extern "C" int gtk_group_norm_backward(const void* x, int64_t x_stride, const fl
   const size_t need = gtk_group_norm_backward_workspace_size(B, positions, c, groups, dtype);
   GTK_REQUIRE(workspace_bytes >= need && (workspace || !need), GTK_EWORKSPACE,
               "gtk_group_norm_backward: workspace %zu < %zu bytes", workspace ? workspace_bytes : 0, need);
-  const ParamVector w{weight, param_dtype == GTK_BF16}, b{bias, param_dtype == GTK_BF16};
-  return (dtype == GTK_F32 ? launch_gn_backward<float> : launch_gn_backward<bf16>)(
-      x, x_stride, mask, dy, dy_stride, stats, w, b, dx, dweight, dbias, param_dtype == GTK_BF16, B, positions, c,
-      groups, activation, (hipStream_t)stream);
+  const int pbf = param_dtype == GTK_BF16;
+  if (B == 0)  // no samples: the sums are zero
+    return dweight || dbias
+               ? launch_column_close("group_norm_close", nullptr, 0, (int)c, dweight, dbias, pbf, (hipStream_t)stream)
+               : GTK_OK;
+  const Inputs in{x, x_stride, mask, {weight, pbf}, {bias, pbf}};
+  const Shape s{B, positions, (int)c, (int)groups, (int)(c / groups)};
+  auto run = [&](auto form) {
+    return launch_gn_backward<decltype(form)>(in, dy, dy_stride, (const GroupStats*)stats, dx, dweight, dbias, pbf, s,
+                                              activation, workspace, workspace_bytes, (hipStream_t)stream);
+  };
+  return dtype == GTK_F32 ? for_form<float>(s, run) : for_form<bf16>(s, run);
 }

@@ -31,6 +31,7 @@
 #include <algorithm>
 
 #include "capi_util.hpp"
+#include "column_sums.hpp"
 #include "common.hpp"
 #include "pack.hpp"
 #include "row_vec.hpp"
@@ -540,55 +541,6 @@ __global__ __launch_bounds__(256) void ln_columns_kernel(const T* __restrict__ x
         (red[wave][0][lane] + red[wave][1][lane]) + (red[wave][2][lane] + red[wave][3][lane]);
 }
 
-// dst[c] = sum over the partials (c < D: the weight's, else the bias'): OUTS of
-// the 2 D sums a block, CHUNKS threads each, eight loads in flight.
-template <int OUTS, int CHUNKS>
-__global__ __launch_bounds__(OUTS * CHUNKS) void ln_close_kernel(const float* __restrict__ part, int parts, int D,
-                                                                 void* __restrict__ dw, void* __restrict__ db,
-                                                                 int dst_bf) {
-  __shared__ float red[CHUNKS][OUTS];
-  const int o = threadIdx.x % OUTS, ch = threadIdx.x / OUTS;
-  const int64_t i = (int64_t)blockIdx.x * OUTS + o, n = 2 * (int64_t)D;
-  void* dst = i < D ? dw : db;
-  const bool live = i < n && dst;
-  float a[8] = {};
-  if (live)
-    for (int k = ch; k < parts; k += 8 * CHUNKS)
-#pragma unroll
-      for (int u = 0; u < 8; ++u) {
-        const int ku = k + u * CHUNKS;
-        const float v = part[(ku < parts ? ku : parts - 1) * n + i];
-        a[u] += ku < parts ? v : 0.f;
-      }
-  red[ch][o] = ((a[0] + a[1]) + (a[2] + a[3])) + ((a[4] + a[5]) + (a[6] + a[7]));
-  // in pairs
-#pragma unroll
-  for (int w = CHUNKS / 2; w > 0; w /= 2) {
-    __syncthreads();
-    if (ch < w) red[ch][o] += red[ch + w][o];
-  }
-  if (ch != 0 || !live) return;
-  const float s = red[0][o];
-  const int c = (int)(i < D ? i : i - D);
-  if (dst_bf)
-    ((bf16*)dst)[c] = cvt<bf16>(s);
-  else
-    ((float*)dst)[c] = s;
-}
-
-static int launch_ln_close(const float* part, int parts, int D, void* dw, void* db, int dst_bf, hipStream_t st) {
-  StageTimer timer("layer_norm_close", st);
-  // narrow rows leave few sums, and many partials of each: more threads a sum
-  // (backward, 2^18 rows of 128: 40.5 us against 44.2 with 32 x 32; 2048 rows of
-  // 8192: 34.0 against 31.4)
-  if (D <= 512)
-    ln_close_kernel<16, 64><<<(2 * D + 15) / 16, 1024, 0, st>>>(part, parts, D, dw, db, dst_bf);
-  else
-    ln_close_kernel<32, 32><<<(2 * D + 31) / 32, 1024, 0, st>>>(part, parts, D, dw, db, dst_bf);
-  GTK_LAUNCH_CHECK();
-  return GTK_OK;
-}
-
 // ---------------------------------------------------------------------------
 // Shapes by width
 // ---------------------------------------------------------------------------
@@ -700,7 +652,7 @@ static int launch_ln_backward(const T* x, int64_t xs, const T* dy, int64_t ds, T
     });
     GTK_LAUNCH_CHECK();
   }
-  return sums ? launch_ln_close(part, parts, D, dw, db, dst_bf, st) : GTK_OK;
+  return sums ? launch_column_close("layer_norm_close", part, parts, D, dw, db, dst_bf, st) : GTK_OK;
 }
 
 }  // namespace gtk
@@ -748,7 +700,7 @@ extern "C" int gtk_layer_norm_backward(const void* x, int64_t x_stride, const vo
   hipStream_t st = (hipStream_t)stream;
   const int pbf = param_dtype == GTK_BF16;
   if (rows == 0)  // no rows: the sums are zero
-    return dweight || dbias ? launch_ln_close(nullptr, 0, (int)d, dweight, dbias, pbf, st) : GTK_OK;
+    return dweight || dbias ? launch_column_close("layer_norm_close", nullptr, 0, (int)d, dweight, dbias, pbf, st) : GTK_OK;
   GTK_REQUIRE(x && dy && workspace, GTK_EINVAL, "gtk_layer_norm_backward: null pointer");
   const size_t need = gtk_layer_norm_backward_workspace_size(rows, d, dtype);
   GTK_REQUIRE(workspace_bytes >= need, GTK_EWORKSPACE, "gtk_layer_norm_backward: workspace %zu < %zu bytes",
