@@ -52,41 +52,46 @@ __device__ __forceinline__ GroupStats close_stats(double s, double q, double cou
 // ---------------------------------------------------------------------------
 __device__ __forceinline__ float logistic(float z) { return __builtin_amdgcn_rcpf(1.f + __expf(-z)); }
 
-// The standard normal distribution's function at z, and its density.  For z < 0
-// the function is e^(-z^2/2) t P(t), t = 1 / (1 + 0.3 |z|), which keeps its
-// relative accuracy to the end; P was fitted to erfcx (weighted least squares on
-// |z| <= 14, iterated towards equal errors): 1.5e-7 of the value, 4.4e-7 with fp32's
-// roundings.
-__device__ __forceinline__ float normal_below(float z, float& density) {
-  const float e = __expf(-0.5f * z * z), t = __builtin_amdgcn_rcpf(fmaf(0.3f, fabsf(z), 1.f));
-  float p = 0.03567477342812997f;
-  p = fmaf(p, t, -0.1572030800704706f);
-  p = fmaf(p, t, 0.20635350232969402f);
-  p = fmaf(p, t, -0.05368364104385134f);
-  p = fmaf(p, t, 0.1285616251824942f);
-  p = fmaf(p, t, 0.09991349247240931f);
-  p = fmaf(p, t, 0.12075395598321578f);
-  p = fmaf(p, t, 0.11962929883230777f);
-  density = 0.3989422804f * e;
-  const float below = e * t * p;
-  return z < 0.f ? below : 1.f - below;
-}
+// The standard normal distribution's function below -|z| is e^(-z^2/2) t P(t) with t =
+// 1 / (1 + 0.3 |z|), which keeps its relative accuracy to the end; P was fitted to
+// erfcx (weighted least squares on |z| <= 14, iterated towards equal errors): 1.5e-7
+// of the value, 4.4e-7 with fp32's roundings.
+struct Tail {
+  float e, tp;  // e^(-z^2/2), t P(t)
+  __device__ __forceinline__ explicit Tail(float z) {
+    e = __builtin_amdgcn_exp2f(z * z * -0.7213475204f);  // log2(e) / 2
+    const float t = __builtin_amdgcn_rcpf(fmaf(0.3f, fabsf(z), 1.f));
+    float p = 0.03567477342812997f;
+    p = fmaf(p, t, -0.1572030800704706f);
+    p = fmaf(p, t, 0.20635350232969402f);
+    p = fmaf(p, t, -0.05368364104385134f);
+    p = fmaf(p, t, 0.1285616251824942f);
+    p = fmaf(p, t, 0.09991349247240931f);
+    p = fmaf(p, t, 0.12075395598321578f);
+    p = fmaf(p, t, 0.11962929883230777f);
+    tp = t * p;
+  }
+};
 
-__device__ __forceinline__ float activate(float z, int act) {
-  float density;
-  if (act == GTK_ACT_SILU) return z * logistic(z);
-  if (act == GTK_ACT_GELU) return z * normal_below(z, density);
+// silu(z) = z s(z); gelu(z) = z Phi(z) = max(z, 0) - |z| Phi(-|z|)
+template <int ACT> __device__ __forceinline__ float activate(float z) {
+  if constexpr (ACT == GTK_ACT_SILU) return z * logistic(z);
+  if constexpr (ACT == GTK_ACT_GELU) {
+    const Tail a(z);
+    return fmaf(-fabsf(z), a.e * a.tp, fmaxf(z, 0.f));
+  }
   return z;
 }
-__device__ __forceinline__ float activate_slope(float z, int act) {
-  if (act == GTK_ACT_SILU) {
+// silu' = s + z s (1 - s); gelu' = Phi(z) + z phi(z), 1 - that of -z
+template <int ACT> __device__ __forceinline__ float activate_slope(float z) {
+  if constexpr (ACT == GTK_ACT_SILU) {
     const float s = logistic(z);
     return s * fmaf(z, 1.f - s, 1.f);
   }
-  if (act == GTK_ACT_GELU) {
-    float density;
-    const float below = normal_below(z, density);
-    return fmaf(z, density, below);
+  if constexpr (ACT == GTK_ACT_GELU) {
+    const Tail a(z);
+    const float below = a.e * fmaf(-fabsf(z), 0.3989422804f, a.tp);
+    return z < 0.f ? below : 1.f - below;
   }
   return 1.f;
 }
@@ -117,11 +122,12 @@ struct Shape {
 
 template <typename F> struct Place {
   int at, row, skip;  // first channel within the slice
-  bool on, first;
+  bool on, first;     // threads past the last whole row repeat that one, and are off
   __device__ __forceinline__ Place(int t, const Team& g, int width) {
     row = t / g.across;
     const int nominal = (t - row * g.across) * F::VE;
     on = row < g.rows;
+    if (!on) row = g.rows - 1;
     first = nominal == 0;
     at = nominal + F::VE <= width ? nominal : width - F::VE;
     skip = nominal - at;
@@ -150,14 +156,15 @@ template <typename S> __device__ __forceinline__ S lanes_sum(S a, int lanes) {
   return a;
 }
 
-// f(o, sum of the o-th `len` entries) for o < outs, by one lane of each `lanes`.
-template <typename S, typename Fn>
+// f(o, sum of the o-th `len` entries) for o < outs, by one lane of each `lanes`; U
+// loads in flight.
+template <int U = 4, typename S, typename Fn>
 __device__ __forceinline__ void sum_runs(const S* sums, int outs, int len, int t, int threads, int lanes, Fn f) {
   const int l = t & (lanes - 1);
   for (int o = t / lanes; o < outs; o += threads / lanes) {
     const S* from = sums + (int64_t)o * len;
     S a{0, 0};
-#pragma unroll 4
+#pragma unroll U
     for (int e = l; e < len; e += lanes) {
       a.x += from[e].x;
       a.y += from[e].y;
@@ -194,36 +201,66 @@ template <typename F> __device__ __forceinline__ void add_squares(double2 (&sum)
   }
 }
 
-// What a thread needs of its groups and channels.
-template <typename F> struct Coefs {
-  float mean[F::SL], low[F::SL], rstd[F::SL], w[F::VE], b[F::VE];
-  __device__ __forceinline__ void set(const GroupStats* stats, const ParamVec& wp, const ParamVec& bp, int c, int at, int cg) {
+// What a thread needs of its groups and channels.  With d = x - mean, exact where x
+// is near the mean: z = d (r w) + (b - low r w), and in the backward pass h = d r -
+// low r, z = h w + b.
+template <typename F> struct Params {
+  float w[F::VE], b[F::VE];
+  __device__ __forceinline__ Params(const ParamVec& wp, const ParamVec& bp, int c) {
+    load_params<F>(w, wp, c, 1.f);
+    load_params<F>(b, bp, c, 0.f);
+  }
+};
+template <typename F> struct ForwardCoefs {
+  float mean[F::SL], a[F::VE], b[F::VE];
+  __device__ __forceinline__ void set(const GroupStats* stats, const Params<F>& p, int at, int cg) {
 #pragma unroll
     for (int j = 0; j < F::SL; ++j) {
       const GroupStats g = stats[(at + j * F::CPS) / cg];
       mean[j] = g.mean;
-      low[j] = g.low;
-      rstd[j] = g.rstd;
-    }
-    load_params<F>(w, wp, c, 1.f);
-    load_params<F>(b, bp, c, 0.f);
-  }
-  __device__ __forceinline__ float h(float x, int e) const {
-    const int j = e / F::CPS;
-    return ((x - mean[j]) - low[j]) * rstd[j];
-  }
-  // f = act(h w + b), or 0
-  __device__ __forceinline__ void forward(float* f, bool live, int act) const {
 #pragma unroll
-    for (int e = 0; e < F::VE; ++e) f[e] = live ? activate(fmaf(h(f[e], e), w[e], b[e]), act) : 0.f;
+      for (int e = j * F::CPS; e < (j + 1) * F::CPS; ++e) {
+        a[e] = g.rstd * p.w[e];
+        b[e] = fmaf(-g.low, a[e], p.b[e]);
+      }
+    }
   }
-  // f = h, g = dL/dz, 0 where the position does not count
-  __device__ __forceinline__ void backward(float* f, float* g, bool live, int act) const {
+  template <int ACT> __device__ __forceinline__ void apply(float* f) const {
+#pragma unroll
+    for (int e = 0; e < F::VE; ++e) f[e] = activate<ACT>(fmaf(f[e] - mean[e / F::CPS], a[e], b[e]));
+  }
+};
+template <typename F> struct BackwardCoefs {
+  float mean[F::SL], rstd[F::SL], shift[F::SL], w[F::VE], b[F::VE];
+  __device__ __forceinline__ void set(const GroupStats* stats, const Params<F>& p, int at, int cg) {
+#pragma unroll
+    for (int j = 0; j < F::SL; ++j) {
+      const GroupStats g = stats[(at + j * F::CPS) / cg];
+      mean[j] = g.mean;
+      rstd[j] = g.rstd;
+      shift[j] = -g.low * g.rstd;
+    }
 #pragma unroll
     for (int e = 0; e < F::VE; ++e) {
-      const float v = h(f[e], e);
-      f[e] = live ? v : 0.f;
-      g[e] = live ? g[e] * activate_slope(fmaf(v, w[e], b[e]), act) : 0.f;
+      w[e] = p.w[e];
+      b[e] = p.b[e];
+    }
+  }
+  // f = h, g = dL/dz
+  template <int ACT> __device__ __forceinline__ void apply(float* f, float* g) const {
+#pragma unroll
+    for (int e = 0; e < F::VE; ++e) {
+      const int j = e / F::CPS;
+      f[e] = fmaf(f[e] - mean[j], rstd[j], shift[j]);
+      g[e] *= activate_slope<ACT>(fmaf(f[e], w[e], b[e]));
+    }
+  }
+  // f = dL/dx of h = f and dz = g; means: of g w and g w h over the group
+  __device__ __forceinline__ void finish(float* f, const float* g, const float2 (&means)[F::SL]) const {
+#pragma unroll
+    for (int e = 0; e < F::VE; ++e) {
+      const int j = e / F::CPS;
+      f[e] = fmaf(-f[e], means[j].y, fmaf(g[e], w[e], -means[j].x)) * rstd[j];
     }
   }
 };
@@ -247,12 +284,12 @@ struct ResidentPlan {
   size_t lds;         // of a team
 };
 
-__device__ __forceinline__ int64_t row_of(int64_t b, int64_t P, int64_t pos) { return b * P + (pos < P ? pos : P - 1); }
+constexpr int kThreads = 512;  // of a block, at most: 256 registers a thread
 
-template <typename F, int NV>
-__global__ __launch_bounds__(1024) void gn_resident_forward_kernel(Inputs in, typename F::T* __restrict__ y,
+template <typename F, int NV, int ACT>
+__global__ __launch_bounds__(kThreads) void gn_resident_forward_kernel(Inputs in, typename F::T* __restrict__ y,
                                                                    GroupStats* __restrict__ stats, Shape s,
-                                                                   ResidentPlan p, float eps, int act) {
+                                                                   ResidentPlan p, float eps) {
   typedef typename F::T T;
   extern __shared__ double2 gn_lds[];
   const Team& g = p.team;
@@ -262,61 +299,68 @@ __global__ __launch_bounds__(1024) void gn_resident_forward_kernel(Inputs in, ty
   char* lds = (char*)gn_lds + team * p.lds;
   double2* sums = (double2*)lds;
   GroupStats* mine = (GroupStats*)(sums + (int64_t)width / F::CPS * g.pitch);
-  int* counts = (int*)(mine + p.groups);
-  const int64_t units = s.B * p.slices;
-  for (int64_t u0 = (int64_t)blockIdx.x * teams; u0 < units; u0 += (int64_t)gridDim.x * teams) {
-    const bool any = u0 + team < units;
-    const int64_t u = any ? u0 + team : units - 1, b = u / p.slices;
+  int* row_counts = (int*)(mine + p.groups);
+  const int64_t units = s.B * p.slices, steps = (units + teams - 1) / teams;
+  for (int64_t step = blockIdx.x; step < steps; step += gridDim.x) {
+    // slices of a sample share lines of memory: on one die
+    const int64_t unit = xcd_remap_any(step, steps) * teams + team;
+    const bool any = unit < units;
+    const int64_t u = any ? unit : units - 1, b = u / p.slices;
     const int slice = (int)(u - b * p.slices), c = slice * width + at.at;
-    Vec<T, F::VE> v[NV];
+    const int P = (int)s.P;
+    Vec<T, F::VE> x[NV];
     bool live[NV];
     int n = 0;
 #pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      const int64_t pos = at.row + (int64_t)k * g.rows, row = row_of(b, s.P, pos);
-      v[k].load((const T*)in.x + row * in.xs + c);
-      live[k] = at.on && pos < s.P && (!in.mask || in.mask[row] != 0.f);
+    for (int k = 0; k < NV; ++k) {  // past the last position that one again
+      const int pos = at.row + k * g.rows;
+      const int64_t row = b * P + (pos < P ? pos : P - 1);
+      x[k].load((const T*)in.x + row * in.xs + c);
+      live[k] = at.on && pos < P && (!in.mask || in.mask[row] != 0.f);
       n += live[k];
     }
+    const Params<F> params(in.w, in.b, c);
     double2 sum[F::SL];
 #pragma unroll
     for (int j = 0; j < F::SL; ++j) sum[j] = double2{0, 0};
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
       float f[F::VE];
-      v[k].get(f);
+      x[k].get(f);
       if (live[k]) add_squares<F>(sum, f);
     }
     put_sums<F::SL, F::VE>(sums, sum, at.at, at.skip, at.row, at.on, g);
-    if (at.first && at.on) counts[at.row] = n;
+    if (at.first && at.on) row_counts[at.row] = n;
     __syncthreads();
-    const double count = (double)s.cg * (double)(in.mask ? sum_counts(counts, g.rows, t, g.lanes) : s.P);
+    const double count = (double)s.cg * (double)(in.mask ? sum_counts(row_counts, g.rows, t, g.lanes) : s.P);
     sum_runs(sums, p.groups, s.cg / F::CPS * g.pitch, t, g.threads, g.lanes, [&](int o, double2 a) {
       mine[o] = close_stats(a.x, a.y, count, eps);
       if (any) stats[b * s.G + slice * p.groups + o] = mine[o];
     });
     __syncthreads();
-    Coefs<F> co;
-    co.set(mine, in.w, in.b, c, at.at, s.cg);
+    ForwardCoefs<F> co;
+    co.set(mine, params, at.at, s.cg);
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      const int64_t pos = at.row + (int64_t)k * g.rows;
-      float f[F::VE];
-      v[k].get(f);
-      co.forward(f, live[k], act);
-      v[k].set(f);
-      if (any && at.on && pos < s.P) v[k].store(y + (b * s.P + pos) * s.C + c);
+      const int pos = at.row + k * g.rows;
+      float f[F::VE] = {};
+      x[k].forget_unpacked();
+      if (live[k]) {
+        x[k].get(f);
+        co.template apply<ACT>(f);
+      }
+      x[k].set(f);
+      if (any && at.on && pos < P) x[k].store(y + (b * P + pos) * s.C + c);
     }
   }
 }
 
 // dx, and this team's sums of dz h and dz over its samples, part[team][0 and 1][c].
-template <typename F, int NV>
-__global__ __launch_bounds__(1024) void gn_resident_backward_kernel(Inputs in, const typename F::T* __restrict__ dy,
+template <typename F, int NV, int ACT>
+__global__ __launch_bounds__(kThreads) void gn_resident_backward_kernel(Inputs in, const typename F::T* __restrict__ dy,
                                                                     int64_t ds, const GroupStats* __restrict__ stats,
                                                                     typename F::T* __restrict__ dx,
-                                                                    float* __restrict__ part, Shape s, ResidentPlan p,
-                                                                    int act) {
+                                                                    float* __restrict__ part, Shape s, ResidentPlan p) {
   typedef typename F::T T;
   extern __shared__ double2 gn_lds[];
   const Team& g = p.team;
@@ -326,7 +370,7 @@ __global__ __launch_bounds__(1024) void gn_resident_backward_kernel(Inputs in, c
   char* lds = (char*)gn_lds + team * p.lds;
   float2* means = (float2*)lds;
   float2* sums = means + p.groups;
-  const int64_t id = (int64_t)blockIdx.x * teams + team, index = id / p.slices;
+  const int64_t id = xcd_remap_any(blockIdx.x, gridDim.x) * teams + team, index = id / p.slices;
   const int slice = (int)(id - index * p.slices), c = slice * width + at.at;
   float2 channel[F::VE];
 #pragma unroll
@@ -334,34 +378,37 @@ __global__ __launch_bounds__(1024) void gn_resident_backward_kernel(Inputs in, c
   for (int64_t b0 = 0; b0 < s.B; b0 += p.per_slice) {
     const bool any = index < p.per_slice && b0 + index < s.B;
     const int64_t b = any ? b0 + index : s.B - 1;
-    Vec<T, F::VE> xv[NV], gv[NV];
+    const int P = (int)s.P;
+    Vec<T, F::VE> x[NV], d[NV];
     bool live[NV];
 #pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      const int64_t pos = at.row + (int64_t)k * g.rows, row = row_of(b, s.P, pos);
-      xv[k].load((const T*)in.x + row * in.xs + c);
-      gv[k].load(dy + row * ds + c);
-      live[k] = any && at.on && pos < s.P && (!in.mask || in.mask[row] != 0.f);
+    for (int k = 0; k < NV; ++k) {  // past the last position that one again
+      const int pos = at.row + k * g.rows;
+      const int64_t row = b * P + (pos < P ? pos : P - 1);
+      x[k].load((const T*)in.x + row * in.xs + c);
+      d[k].load(dy + row * ds + c);
+      live[k] = any && at.on && pos < P && (!in.mask || in.mask[row] != 0.f);
     }
     const GroupStats* of = stats + b * s.G + slice * p.groups;
-    Coefs<F> co;
-    co.set(of, in.w, in.b, c, at.at, s.cg);
+    BackwardCoefs<F> co;
+    co.set(of, Params<F>(in.w, in.b, c), at.at, s.cg);
     float2 sum[F::SL];
 #pragma unroll
     for (int j = 0; j < F::SL; ++j) sum[j] = float2{0.f, 0.f};
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      float f[F::VE], d[F::VE];
-      xv[k].get(f);
-      gv[k].get(d);
-      co.backward(f, d, live[k], act);
+      if (!live[k]) continue;
+      float f[F::VE], dz[F::VE];
+      x[k].get(f);
+      d[k].get(dz);
+      co.template apply<ACT>(f, dz);
 #pragma unroll
       for (int e = 0; e < F::VE; ++e) {
-        const float gw = d[e] * co.w[e];
+        const float gw = dz[e] * co.w[e];
         sum[e / F::CPS].x += gw;
-        sum[e / F::CPS].y += gw * f[e];
-        channel[e].x += d[e] * f[e];
-        channel[e].y += d[e];
+        sum[e / F::CPS].y = fmaf(gw, f[e], sum[e / F::CPS].y);
+        channel[e].x = fmaf(dz[e], f[e], channel[e].x);
+        channel[e].y += dz[e];
       }
     }
     if (!dx) continue;
@@ -377,18 +424,19 @@ __global__ __launch_bounds__(1024) void gn_resident_backward_kernel(Inputs in, c
     for (int j = 0; j < F::SL; ++j) mean[j] = means[(at.at + j * F::CPS) / s.cg];
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      const int64_t pos = at.row + (int64_t)k * g.rows;
-      float f[F::VE], d[F::VE];
-      xv[k].get(f);
-      gv[k].get(d);
-      co.backward(f, d, live[k], act);
-#pragma unroll
-      for (int e = 0; e < F::VE; ++e) {
-        const int j = e / F::CPS;
-        f[e] = live[k] ? (d[e] * co.w[e] - mean[j].x - f[e] * mean[j].y) * co.rstd[j] : 0.f;
+      const int pos = at.row + k * g.rows;
+      float f[F::VE] = {};
+      x[k].forget_unpacked();
+      d[k].forget_unpacked();
+      if (live[k]) {
+        float dz[F::VE];
+        x[k].get(f);
+        d[k].get(dz);
+        co.template apply<ACT>(f, dz);
+        co.finish(f, dz, mean);
       }
-      xv[k].set(f);
-      if (any && at.on && pos < s.P) xv[k].store(dx + (b * s.P + pos) * s.C + c);
+      x[k].set(f);
+      if (any && at.on && pos < P) x[k].store(dx + (b * P + pos) * s.C + c);
     }
   }
   if (!part) return;
@@ -404,188 +452,223 @@ __global__ __launch_bounds__(1024) void gn_resident_backward_kernel(Inputs in, c
 }
 
 // ---------------------------------------------------------------------------
-// Streamed: a team is a block, and has a chunk of a sample's positions, `steps` times
+// Streamed: a team is a block, and has a chunk of a sample's positions: `steps` times
 // the team's rows.
 // ---------------------------------------------------------------------------
-constexpr int kStreamThreads = 1024;
-
 struct StreamPlan {
   Team team;
-  int chunks, steps;
+  int chunks;
+  int64_t steps, all, whole;  // of a chunk; of a sample; those of them that have all their rows
 };
 
-// The team's rows of steps [first, last) of sample b, U at once.
-template <typename F, int U> struct Rows {
-  Vec<typename F::T, F::VE> v[U];
-  // past the last step that one again
-  __device__ __forceinline__ void load(const typename F::T* p, int64_t stride, const Shape& s, int64_t b, int64_t step,
-                                       int64_t last, const Place<F>& at, const Team& g, bool keep) {
-#pragma unroll
-    for (int j = 0; j < U; ++j) {
-      const int64_t at_step = step + j < last ? step + j : last - 1;
-      const auto* from = p + row_of(b, s.P, at_step * g.rows + at.row) * stride + at.at;
-      if (keep)
-        v[j].load_plain(from);
-      else
-        v[j].load(from);
-    }
+// A block's chunk: steps [first, last) of sample b, of which those before `whole` have
+// all their rows.
+struct Chunk {
+  int64_t b, first, last, whole;
+  int chunk;
+  __device__ __forceinline__ Chunk(int64_t item, const StreamPlan& p) {
+    b = item / p.chunks;
+    chunk = (int)(item - b * p.chunks);
+    first = chunk * p.steps;
+    last = first + p.steps < p.all ? first + p.steps : p.all;
+    whole = last < p.whole ? last : p.whole;
   }
 };
-template <typename F, int U> struct Live {
+
+// A thread's vectors of one tensor or two, and whether their positions count.
+template <typename F, int U, bool TWO> struct Held {
+  Vec<typename F::T, F::VE> x[U], d[TWO ? U : 1];
   bool live[U];
-  __device__ __forceinline__ void load(const float* mask, const Shape& s, int64_t b, int64_t step, int64_t last,
-                                       const Place<F>& at, const Team& g) {
+};
+
+// A thread's place in the tensors, at a step of its chunk's sample.  KEEP: a second
+// launch reads the values again.
+template <typename F, bool TWO, bool KEEP> struct Cursor {
+  typedef typename F::T T;
+  const T *x, *d;
+  const float* mask;
+  int64_t x_step, d_step;
+  int rows, row;
+  int64_t left;  // positions behind the sample's first one
+  __device__ __forceinline__ Cursor(const Inputs& in, const T* dy, int64_t ds, const Shape& s, const Team& g, int64_t b,
+                                    const Place<F>& at)
+      : x_step(g.rows * in.xs), d_step(g.rows * ds), rows(g.rows), row(at.row), left(s.P) {
+    x = (const T*)in.x + (b * s.P + at.row) * in.xs + at.at;
+    d = TWO ? dy + (b * s.P + at.row) * ds + at.at : nullptr;
+    mask = in.mask ? in.mask + b * s.P + at.row : nullptr;
+  }
+  template <int U> __device__ __forceinline__ void load(Held<F, U, TWO>& v, int64_t step) const {
 #pragma unroll
     for (int j = 0; j < U; ++j) {
-      const int64_t pos = (step + j) * g.rows + at.row;
-      live[j] = at.on && step + j < last && pos < s.P && (!mask || mask[row_of(b, s.P, pos)] != 0.f);
+      get(v.x[j], x + (step + j) * x_step);
+      if constexpr (TWO) get(v.d[j], d + (step + j) * d_step);
     }
+#pragma unroll
+    for (int j = 0; j < U; ++j) v.live[j] = !mask || mask[(step + j) * rows] != 0.f;
+  }
+  // The sample's last step, which not all threads have a position in: the others
+  // read the last one.
+  __device__ __forceinline__ void load_part(Held<F, 1, TWO>& v, int64_t step) const {
+    const int64_t over = step * rows + row - (left - 1), back = over > 0 ? over : 0;
+    get(v.x[0], x + step * x_step - back * (x_step / rows));
+    if constexpr (TWO) get(v.d[0], d + step * d_step - back * (d_step / rows));
+    v.live[0] = over <= 0 && (!mask || mask[step * rows] != 0.f);
+  }
+  __device__ __forceinline__ bool inside(int64_t step) const { return step * rows + row < left; }
+
+ private:
+  static __device__ __forceinline__ void get(Vec<T, F::VE>& v, const T* p) {
+    if constexpr (KEEP)
+      v.load_plain(p);
+    else
+      v.load(p);
   }
 };
+
+// Calls use(held, j, step) for the chunk's steps, forwards or backwards, U whole ones at
+// a time while the next U are on their way; start() runs behind the first loads.
+template <int U, bool BACK, typename F, bool TWO, bool KEEP, typename Start, typename Use>
+__device__ __forceinline__ void for_steps(const Cursor<F, TWO, KEEP>& at, const Chunk& k, Start start, Use use) {
+  const int64_t whole = k.whole > k.first ? k.whole - k.first : 0, sets = whole / U;
+  Held<F, U, TWO> now, next;
+  auto step_of = [&](int64_t i) { return k.first + (BACK ? sets - 1 - i : i) * U; };
+  if (sets) at.load(now, step_of(0));
+  start();
+  auto rest = [&]() {
+    for (int64_t step = k.first + sets * U; step < k.last; ++step) {
+      Held<F, 1, TWO> one;
+      if (step < k.whole)
+        at.load(one, step);
+      else
+        at.load_part(one, step);
+      use(one, 0, step);
+    }
+  };
+  if (BACK) rest();
+  for (int64_t i = 0; i < sets; ++i) {
+    if (i + 1 < sets) at.load(next, step_of(i + 1));
+#pragma unroll
+    for (int j = 0; j < U; ++j) use(now, j, step_of(i) + j);
+    now = next;
+  }
+  if (!BACK) rest();
+}
 
 // part[b][group][chunk], counts[b][chunk]
 template <typename F>
-__global__ __launch_bounds__(kStreamThreads) void gn_stats_kernel(Inputs in, double2* __restrict__ part,
-                                                                  int* __restrict__ counts, Shape s, StreamPlan p) {
-  constexpr int U = 4;
+__global__ __launch_bounds__(kThreads) void gn_stats_kernel(Inputs in, double2* __restrict__ part,
+                                                            int* __restrict__ chunk_counts, Shape s, StreamPlan p) {
   extern __shared__ double2 gn_lds[];
-  __shared__ int row_counts[kStreamThreads];
+  __shared__ int row_counts[kThreads];
   const Team& g = p.team;
   const int t = threadIdx.x;
   const Place<F> at(t, g, s.C);
-  const int64_t all = (s.P + g.rows - 1) / g.rows;
   for (int64_t item = blockIdx.x; item < s.B * p.chunks; item += gridDim.x) {
-    const int64_t b = item / p.chunks;
-    const int chunk = (int)(item - b * p.chunks);
-    const int64_t first = (int64_t)chunk * p.steps, last = std::min<int64_t>(first + p.steps, all);
+    const Chunk k(item, p);
     double2 sum[F::SL];
 #pragma unroll
     for (int j = 0; j < F::SL; ++j) sum[j] = double2{0, 0};
     int n = 0;
-    for (int64_t step = first; step < last; step += U) {
-      Rows<F, U> x;
-      Live<F, U> m;
-      x.load((const typename F::T*)in.x, in.xs, s, b, step, last, at, g, true);
-      m.load(in.mask, s, b, step, last, at, g);
-#pragma unroll
-      for (int j = 0; j < U; ++j) {
-        float f[F::VE];
-        x.v[j].get(f);
-        n += m.live[j];
-        if (m.live[j]) add_squares<F>(sum, f);
-      }
-    }
+    for_steps<4, false>(Cursor<F, false, true>(in, nullptr, 0, s, g, k.b, at), k, [] {}, [&](auto& v, int j, int64_t) {
+      if (!v.live[j]) return;
+      float f[F::VE];
+      v.x[j].get(f);
+      add_squares<F>(sum, f);
+      ++n;
+    });
     put_sums<F::SL, F::VE>(gn_lds, sum, at.at, at.skip, at.row, at.on, g);
     if (at.first && at.on) row_counts[at.row] = n;
     __syncthreads();
-    sum_runs(gn_lds, s.G, s.cg / F::CPS * g.pitch, t, kStreamThreads, g.lanes,
-             [&](int o, double2 a) { part[(b * s.G + o) * p.chunks + chunk] = a; });
+    sum_runs(gn_lds, s.G, s.cg / F::CPS * g.pitch, t, kThreads, g.lanes,
+             [&](int o, double2 a) { part[(k.b * s.G + o) * p.chunks + k.chunk] = a; });
     if (in.mask && t < 64) {
       const int64_t count = sum_counts(row_counts, g.rows, t, 64);
-      if (t == 0) counts[item] = (int)count;
+      if (t == 0) chunk_counts[item] = (int)count;
     }
     __syncthreads();
   }
 }
 
-template <typename F>
-__global__ __launch_bounds__(kStreamThreads) void gn_apply_kernel(Inputs in, const double2* __restrict__ part,
-                                                                  const int* __restrict__ counts,
-                                                                  typename F::T* __restrict__ y,
-                                                                  GroupStats* __restrict__ stats, Shape s, StreamPlan p,
-                                                                  float eps, int act) {
-  constexpr int U = 4;
+template <typename F, int ACT>
+__global__ __launch_bounds__(kThreads) void gn_apply_kernel(Inputs in, const double2* __restrict__ part,
+                                                            const int* __restrict__ chunk_counts,
+                                                            typename F::T* __restrict__ y,
+                                                            GroupStats* __restrict__ stats, Shape s, StreamPlan p,
+                                                            float eps) {
+  typedef typename F::T T;
   extern __shared__ double2 gn_lds[];
   GroupStats* mine = (GroupStats*)gn_lds;
   const Team& g = p.team;
   const int t = threadIdx.x;
   const Place<F> at(t, g, s.C);
-  const int64_t all = (s.P + g.rows - 1) / g.rows;
+  const Params<F> params(in.w, in.b, at.at);
   for (int64_t item = blockIdx.x; item < s.B * p.chunks; item += gridDim.x) {
-    const int64_t b = item / p.chunks;
-    const int chunk = (int)(item - b * p.chunks);
-    const int64_t first = (int64_t)chunk * p.steps, last = std::min<int64_t>(first + p.steps, all);
-    Rows<F, U> x;
-    Live<F, U> m;
-    int64_t step = first + (last - 1 - first) / U * U;  // backwards
-    x.load((const typename F::T*)in.x, in.xs, s, b, step, last, at, g, false);
-    m.load(in.mask, s, b, step, last, at, g);
-    const double count =
-        (double)s.cg * (double)(in.mask ? sum_counts(counts + b * p.chunks, p.chunks, t, g.lanes) : s.P);
-    sum_runs(part + b * s.G * p.chunks, s.G, p.chunks, t, kStreamThreads, g.lanes, [&](int o, double2 a) {
-      mine[o] = close_stats(a.x, a.y, count, eps);
-      if (chunk == 0) stats[b * s.G + o] = mine[o];
-    });
-    __syncthreads();
-    Coefs<F> co;
-    co.set(mine, in.w, in.b, at.at, at.at, s.cg);
-    for (;;) {
-#pragma unroll
-      for (int j = 0; j < U; ++j) {
-        const int64_t pos = (step + j) * g.rows + at.row;
-        float f[F::VE];
-        x.v[j].get(f);
-        co.forward(f, m.live[j], act);
-        Vec<typename F::T, F::VE> o;
-        o.set(f);
-        if (at.on && step + j < last && pos < s.P) o.store(y + (b * s.P + pos) * s.C + at.at);
+    const Chunk k(item, p);
+    const Cursor<F, false, false> from(in, nullptr, 0, s, g, k.b, at);
+    T* to = y + (k.b * s.P + at.row) * s.C + at.at;
+    const int64_t y_step = (int64_t)g.rows * s.C;
+    ForwardCoefs<F> co;
+    auto start = [&]() {
+      const double count =
+          (double)s.cg * (double)(in.mask ? sum_counts(chunk_counts + k.b * p.chunks, p.chunks, t, g.lanes) : s.P);
+      sum_runs<8>(part + k.b * s.G * p.chunks, s.G, p.chunks, t, kThreads, g.lanes, [&](int o, double2 a) {
+        mine[o] = close_stats(a.x, a.y, count, eps);
+        if (k.chunk == 0) stats[k.b * s.G + o] = mine[o];
+      });
+      __syncthreads();
+      co.set(mine, params, at.at, s.cg);
+    };
+    for_steps<4, true>(from, k, start, [&](auto& v, int j, int64_t step) {
+      float f[F::VE] = {};
+      if (v.live[j]) {
+        v.x[j].get(f);
+        co.template apply<ACT>(f);
       }
-      step -= U;
-      if (step < first) break;
-      x.load((const typename F::T*)in.x, in.xs, s, b, step, last, at, g, false);
-      m.load(in.mask, s, b, step, last, at, g);
-    }
+      Vec<T, F::VE> o;
+      o.set(f);
+      if (at.on && from.inside(step)) o.store(to + step * y_step);
+    });
     __syncthreads();
   }
 }
 
 // The chunk's sums of dz h and dz, channels[b][chunk][0 and 1][c], and of g and g h,
 // part[b][group][chunk].
-template <typename F>
-__global__ __launch_bounds__(kStreamThreads) void gn_backward_sums_kernel(Inputs in, const typename F::T* __restrict__ dy,
-                                                                          int64_t ds, const GroupStats* __restrict__ stats,
-                                                                          float2* __restrict__ part,
-                                                                          float* __restrict__ channels, Shape s,
-                                                                          StreamPlan p, int act) {
-  constexpr int U = 2;
+template <typename F, int ACT>
+__global__ __launch_bounds__(kThreads) void gn_backward_sums_kernel(Inputs in, const typename F::T* __restrict__ dy,
+                                                                    int64_t ds, const GroupStats* __restrict__ stats,
+                                                                    float2* __restrict__ part,
+                                                                    float* __restrict__ channels, Shape s,
+                                                                    StreamPlan p) {
   extern __shared__ double2 gn_lds[];
   float2* weighted = (float2*)gn_lds;  // [C]: a channel's part of its group's sums
   float2* sums = weighted + s.C;
   const Team& g = p.team;
   const int t = threadIdx.x;
   const Place<F> at(t, g, s.C);
-  const int64_t all = (s.P + g.rows - 1) / g.rows;
+  const Params<F> params(in.w, in.b, at.at);
   for (int64_t item = blockIdx.x; item < s.B * p.chunks; item += gridDim.x) {
-    const int64_t b = item / p.chunks;
-    const int chunk = (int)(item - b * p.chunks);
-    const int64_t first = (int64_t)chunk * p.steps, last = std::min<int64_t>(first + p.steps, all);
-    Coefs<F> co;
-    co.set(stats + b * s.G, in.w, in.b, at.at, at.at, s.cg);
+    const Chunk k(item, p);
+    BackwardCoefs<F> co;
     float2 sum[F::VE];
 #pragma unroll
     for (int e = 0; e < F::VE; ++e) sum[e] = float2{0.f, 0.f};
-    for (int64_t step = first; step < last; step += U) {
-      Rows<F, U> x, d;
-      Live<F, U> m;
-      x.load((const typename F::T*)in.x, in.xs, s, b, step, last, at, g, true);
-      d.load(dy, ds, s, b, step, last, at, g, true);
-      m.load(in.mask, s, b, step, last, at, g);
+    auto start = [&]() { co.set(stats + k.b * s.G, params, at.at, s.cg); };
+    for_steps<2, false>(Cursor<F, true, true>(in, dy, ds, s, g, k.b, at), k, start, [&](auto& v, int j, int64_t) {
+      if (!v.live[j]) return;
+      float f[F::VE], dz[F::VE];
+      v.x[j].get(f);
+      v.d[j].get(dz);
+      co.template apply<ACT>(f, dz);
 #pragma unroll
-      for (int j = 0; j < U; ++j) {
-        float f[F::VE], dz[F::VE];
-        x.v[j].get(f);
-        d.v[j].get(dz);
-        co.backward(f, dz, m.live[j], act);
-#pragma unroll
-        for (int e = 0; e < F::VE; ++e) {
-          sum[e].x += dz[e] * f[e];
-          sum[e].y += dz[e];
-        }
+      for (int e = 0; e < F::VE; ++e) {
+        sum[e].x = fmaf(dz[e], f[e], sum[e].x);
+        sum[e].y += dz[e];
       }
-    }
+    });
     put_sums<F::VE, F::VE>(sums, sum, at.at, at.skip, at.row, at.on, g);
     __syncthreads();
-    sum_runs(sums, s.C, g.pitch, t, kStreamThreads, g.channel_lanes, [&](int c, float2 a) {
+    sum_runs(sums, s.C, g.pitch, t, kThreads, g.channel_lanes, [&](int c, float2 a) {
       if (channels) {
         channels[item * 2 * s.C + c] = a.x;
         channels[(item * 2 + 1) * s.C + c] = a.y;
@@ -595,66 +678,53 @@ __global__ __launch_bounds__(kStreamThreads) void gn_backward_sums_kernel(Inputs
     });
     __syncthreads();
     if (part)
-      sum_runs(weighted, s.G, s.cg, t, kStreamThreads, g.lanes,
-               [&](int o, float2 a) { part[(b * s.G + o) * p.chunks + chunk] = a; });
+      sum_runs(weighted, s.G, s.cg, t, kThreads, g.lanes,
+               [&](int o, float2 a) { part[(k.b * s.G + o) * p.chunks + k.chunk] = a; });
     __syncthreads();
   }
 }
 
-template <typename F>
-__global__ __launch_bounds__(kStreamThreads) void gn_backward_apply_kernel(
+template <typename F, int ACT>
+__global__ __launch_bounds__(kThreads) void gn_backward_apply_kernel(
     Inputs in, const typename F::T* __restrict__ dy, int64_t ds, const GroupStats* __restrict__ stats,
-    const float2* __restrict__ part, typename F::T* __restrict__ dx, Shape s, StreamPlan p, int act) {
-  constexpr int U = 2;
+    const float2* __restrict__ part, typename F::T* __restrict__ dx, Shape s, StreamPlan p) {
+  typedef typename F::T T;
   extern __shared__ double2 gn_lds[];
   float2* means = (float2*)gn_lds;
   const Team& g = p.team;
   const int t = threadIdx.x;
   const Place<F> at(t, g, s.C);
-  const int64_t all = (s.P + g.rows - 1) / g.rows;
+  const Params<F> params(in.w, in.b, at.at);
   for (int64_t item = blockIdx.x; item < s.B * p.chunks; item += gridDim.x) {
-    const int64_t b = item / p.chunks;
-    const int chunk = (int)(item - b * p.chunks);
-    const int64_t first = (int64_t)chunk * p.steps, last = std::min<int64_t>(first + p.steps, all);
-    Rows<F, U> x, d;
-    Live<F, U> m;
-    int64_t step = first + (last - 1 - first) / U * U;  // backwards
-    x.load((const typename F::T*)in.x, in.xs, s, b, step, last, at, g, false);
-    d.load(dy, ds, s, b, step, last, at, g, false);
-    m.load(in.mask, s, b, step, last, at, g);
-    sum_runs(part + b * s.G * p.chunks, s.G, p.chunks, t, kStreamThreads, g.lanes, [&](int o, float2 a) {
-      const float inv = stats[b * s.G + o].inv;
-      means[o] = float2{a.x * inv, a.y * inv};
-    });
-    Coefs<F> co;
-    co.set(stats + b * s.G, in.w, in.b, at.at, at.at, s.cg);
-    __syncthreads();
+    const Chunk k(item, p);
+    const Cursor<F, true, false> from(in, dy, ds, s, g, k.b, at);
+    T* to = dx + (k.b * s.P + at.row) * s.C + at.at;
+    const int64_t dx_step = (int64_t)g.rows * s.C;
+    BackwardCoefs<F> co;
     float2 mean[F::SL];
+    auto start = [&]() {
+      co.set(stats + k.b * s.G, params, at.at, s.cg);
+      sum_runs<8>(part + k.b * s.G * p.chunks, s.G, p.chunks, t, kThreads, g.lanes, [&](int o, float2 a) {
+        const float inv = stats[k.b * s.G + o].inv;
+        means[o] = float2{a.x * inv, a.y * inv};
+      });
+      __syncthreads();
 #pragma unroll
-    for (int j = 0; j < F::SL; ++j) mean[j] = means[(at.at + j * F::CPS) / s.cg];
-    for (;;) {
-#pragma unroll
-      for (int j = 0; j < U; ++j) {
-        const int64_t pos = (step + j) * g.rows + at.row;
-        float f[F::VE], dz[F::VE];
-        x.v[j].get(f);
-        d.v[j].get(dz);
-        co.backward(f, dz, m.live[j], act);
-#pragma unroll
-        for (int e = 0; e < F::VE; ++e) {
-          const int k = e / F::CPS;
-          f[e] = m.live[j] ? (dz[e] * co.w[e] - mean[k].x - f[e] * mean[k].y) * co.rstd[k] : 0.f;
-        }
-        Vec<typename F::T, F::VE> o;
-        o.set(f);
-        if (at.on && step + j < last && pos < s.P) o.store(dx + (b * s.P + pos) * s.C + at.at);
+      for (int j = 0; j < F::SL; ++j) mean[j] = means[(at.at + j * F::CPS) / s.cg];
+    };
+    for_steps<2, true>(from, k, start, [&](auto& v, int j, int64_t step) {
+      float f[F::VE] = {};
+      if (v.live[j]) {
+        float dz[F::VE];
+        v.x[j].get(f);
+        v.d[j].get(dz);
+        co.template apply<ACT>(f, dz);
+        co.finish(f, dz, mean);
       }
-      step -= U;
-      if (step < first) break;
-      x.load((const typename F::T*)in.x, in.xs, s, b, step, last, at, g, false);
-      d.load(dy, ds, s, b, step, last, at, g, false);
-      m.load(in.mask, s, b, step, last, at, g);
-    }
+      Vec<T, F::VE> o;
+      o.set(f);
+      if (at.on && from.inside(step)) o.store(to + step * dx_step);
+    });
     __syncthreads();
   }
 }
@@ -682,10 +752,9 @@ template <typename Fn> __device__ __forceinline__ void for_values(const Shape& s
     for (int k = threadIdx.x; k < s.cg; k += 256) f(pos, c0 + k);
 }
 
-template <typename T>
+template <typename T, int ACT>
 __global__ __launch_bounds__(256) void gn_swept_forward_kernel(Inputs in, T* __restrict__ y,
-                                                               GroupStats* __restrict__ stats, Shape s, float eps,
-                                                               int act) {
+                                                               GroupStats* __restrict__ stats, Shape s, float eps) {
   __shared__ double red[3][4];
   const T* x = (const T*)in.x;
   for (int64_t bg = blockIdx.x; bg < s.B * s.G; bg += gridDim.x) {
@@ -705,26 +774,26 @@ __global__ __launch_bounds__(256) void gn_swept_forward_kernel(Inputs in, T* __r
     for_values(s, c0, [&](int64_t pos, int c) {
       const bool live = !in.mask || in.mask[first + pos] != 0.f;
       const float h = ((to_f32(x[(first + pos) * in.xs + c]) - g.mean) - g.low) * g.rstd;
-      y[(first + pos) * s.C + c] = cvt<T>(live ? activate(fmaf(h, in.w.get(c, 1.f), in.b.get(c, 0.f)), act) : 0.f);
+      y[(first + pos) * s.C + c] = cvt<T>(live ? activate<ACT>(fmaf(h, in.w.get(c, 1.f), in.b.get(c, 0.f))) : 0.f);
     });
   }
 }
 
 // h and dz of a value; false where it does not count.
-template <typename T>
+template <int ACT, typename T>
 __device__ __forceinline__ bool swept_backward(const Inputs& in, const T* dy, int64_t ds, const GroupStats& g,
-                                               int64_t row, int c, int act, float& h, float& dz) {
+                                               int64_t row, int c, float& h, float& dz) {
   h = dz = 0.f;
   if (in.mask && in.mask[row] == 0.f) return false;
   h = ((to_f32(((const T*)in.x)[row * in.xs + c]) - g.mean) - g.low) * g.rstd;
-  dz = to_f32(dy[row * ds + c]) * activate_slope(fmaf(h, in.w.get(c, 1.f), in.b.get(c, 0.f)), act);
+  dz = to_f32(dy[row * ds + c]) * activate_slope<ACT>(fmaf(h, in.w.get(c, 1.f), in.b.get(c, 0.f)));
   return true;
 }
 
-template <typename T>
+template <typename T, int ACT>
 __global__ __launch_bounds__(256) void gn_swept_backward_kernel(Inputs in, const T* __restrict__ dy, int64_t ds,
                                                                 const GroupStats* __restrict__ stats,
-                                                                T* __restrict__ dx, Shape s, int act) {
+                                                                T* __restrict__ dx, Shape s) {
   __shared__ double red[3][4];
   for (int64_t bg = blockIdx.x; bg < s.B * s.G; bg += gridDim.x) {
     const int64_t first = bg / s.G * s.P;
@@ -733,7 +802,7 @@ __global__ __launch_bounds__(256) void gn_swept_backward_kernel(Inputs in, const
     float h, dz;
     double v[3] = {0, 0, 0};
     for_values(s, c0, [&](int64_t pos, int c) {
-      swept_backward(in, dy, ds, g, first + pos, c, act, h, dz);
+      swept_backward<ACT>(in, dy, ds, g, first + pos, c, h, dz);
       const float gw = dz * in.w.get(c, 1.f);
       v[0] += gw;
       v[1] += (double)gw * h;
@@ -741,23 +810,23 @@ __global__ __launch_bounds__(256) void gn_swept_backward_kernel(Inputs in, const
     block_add(v, red);
     const float c1 = (float)(v[0] * g.inv), c2 = (float)(v[1] * g.inv);
     for_values(s, c0, [&](int64_t pos, int c) {
-      const bool live = swept_backward(in, dy, ds, g, first + pos, c, act, h, dz);
+      const bool live = swept_backward<ACT>(in, dy, ds, g, first + pos, c, h, dz);
       dx[(first + pos) * s.C + c] = cvt<T>(live ? (dz * in.w.get(c, 1.f) - c1 - h * c2) * g.rstd : 0.f);
     });
   }
 }
 
-template <typename T>
+template <typename T, int ACT>
 __global__ __launch_bounds__(256) void gn_swept_params_kernel(Inputs in, const T* __restrict__ dy, int64_t ds,
                                                               const GroupStats* __restrict__ stats,
                                                               void* __restrict__ dw, void* __restrict__ db, int dst_bf,
-                                                              Shape s, int act) {
+                                                              Shape s) {
   __shared__ double red[3][4];
   for (int c = blockIdx.x; c < s.C; c += gridDim.x) {
     double v[3] = {0, 0, 0};
     for (int64_t row = threadIdx.x; row < s.B * s.P; row += 256) {
       float h, dz;
-      swept_backward(in, dy, ds, stats[row / s.P * s.G + c / s.cg], row, c, act, h, dz);
+      swept_backward<ACT>(in, dy, ds, stats[row / s.P * s.G + c / s.cg], row, c, h, dz);
       v[0] += (double)dz * h;
       v[1] += dz;
     }
@@ -777,6 +846,7 @@ __global__ __launch_bounds__(256) void gn_swept_params_kernel(Inputs in, const T
 // ---------------------------------------------------------------------------
 // Plans
 // ---------------------------------------------------------------------------
+#define GN_WANT (s.B == 1 ? 1 : 2)
 constexpr size_t kMostLds = 156 * 1024;
 constexpr int kMostBlocks = 1 << 20;  // the kernels loop past that
 
@@ -806,22 +876,22 @@ static Team make_team(int threads, int across, int64_t groups, int64_t channels)
 // The narrowest slices of whole groups that fill 64-byte pieces of memory, wider
 // ones as long as they leave four teams a CU.
 template <typename F> static bool plan_resident(const Shape& s, bool backward, ResidentPlan* plan) {
-  const int most = backward ? 4 : 8;
+  const int most = backward ? 8 : 16;
   bool found = false;
   for (int groups = 1; groups <= s.G; ++groups) {
     if (s.G % groups) continue;
     const int64_t width = (int64_t)groups * s.cg;
     if (width < F::VE || (groups < s.G && width * (int64_t)sizeof(typename F::T) < 64)) continue;
     const int64_t across = (width + F::VE - 1) / F::VE;
-    if (across > 1024 || s.P > 1024 * most) break;
+    if (across > kThreads || s.P > kThreads * most) break;
     const int64_t units = s.B * (s.G / groups);
     if (found && units < 4 * (int64_t)device_cus()) break;
     int threads = pow2_up(across);
     auto held = [&](int n) { return (s.P + n / across - 1) / (n / across); };
-    while (threads < 1024 && held(threads) > most) threads *= 2;
+    while (threads < kThreads && held(threads) > most) threads *= 2;
     if (held(threads) > most) break;
     // more threads where there are few teams
-    while (threads < 1024 && held(threads) > 1 && units * threads < 512 * (int64_t)device_cus()) threads *= 2;
+    while (threads < kThreads && held(threads) > 1 && units * threads < 512 * (int64_t)device_cus()) threads *= 2;
     ResidentPlan p;
     p.team = make_team(threads, (int)across, groups, width);
     p.held = (int)held(threads);
@@ -843,14 +913,13 @@ template <typename F> static bool plan_resident(const Shape& s, bool backward, R
 // launch adds its sample's partial sums up).
 template <typename F> static bool plan_streamed(const Shape& s, StreamPlan* p) {
   const int64_t across = ((int64_t)s.C + F::VE - 1) / F::VE;
-  if (across > kStreamThreads) return false;
-  p->team = make_team(kStreamThreads, (int)across, s.G, s.C);
-  const int64_t all = (s.P + p->team.rows - 1) / p->team.rows;
-  const int64_t want = std::max<int64_t>(1, (s.B == 1 ? 1 : 2) * (int64_t)device_cus() / s.B);
-  const int64_t steps = std::max<int64_t>((all + want - 1) / want, (all + (1 << 30) - 1) >> 30);
-  if (steps > 1 << 30) return false;
-  p->steps = (int)steps;
-  p->chunks = (int)((all + steps - 1) / steps);
+  if (across > kThreads) return false;
+  p->team = make_team(kThreads, (int)across, s.G, s.C);
+  p->all = (s.P + p->team.rows - 1) / p->team.rows;
+  p->whole = s.P / p->team.rows;
+  const int64_t want = std::max<int64_t>(1, GN_WANT * (int64_t)device_cus() / s.B);
+  p->steps = (p->all + want - 1) / want;
+  p->chunks = (int)((p->all + p->steps - 1) / p->steps);
   return true;
 }
 
@@ -875,11 +944,18 @@ template <typename T, typename Fn> static auto for_form(const Shape& s, Fn run) 
 }
 // Calls run(number) for the smallest number of held vectors that is enough.
 template <int MOST, typename Fn> static void for_held(int held, Fn run) {
-  if constexpr (MOST > 4)
-    if (held > 4) return run(std::integral_constant<int, 8>());
+  if constexpr (MOST > 8)
+    if (held > 8) return run(std::integral_constant<int, 16>());
+  if (held > 4) return run(std::integral_constant<int, 8>());
   if (held > 2) return run(std::integral_constant<int, 4>());
   if (held > 1) return run(std::integral_constant<int, 2>());
   run(std::integral_constant<int, 1>());
+}
+
+template <typename Fn> static void for_activation(int act, Fn run) {
+  if (act == GTK_ACT_SILU) return run(std::integral_constant<int, GTK_ACT_SILU>());
+  if (act == GTK_ACT_GELU) return run(std::integral_constant<int, GTK_ACT_GELU>());
+  run(std::integral_constant<int, GTK_ACT_NONE>());
 }
 
 static unsigned blocks_for(int64_t items) { return (unsigned)std::min<int64_t>(items, kMostBlocks); }
@@ -910,10 +986,12 @@ static int launch_gn_forward(const Inputs& in, void* yp, GroupStats* stats, cons
   if (p.resident) {
     StageTimer timer("group_norm_forward", st);
     const int threads = std::max(256, p.r.team.threads), teams = threads / p.r.team.threads;
-    for_held<8>(p.r.held, [&](auto nv) {
-      gn_resident_forward_kernel<F, decltype(nv)::value>
-          <<<blocks_for((s.B * p.r.slices + teams - 1) / teams), threads, teams * p.r.lds, st>>>(in, y, stats, s, p.r, eps,
-                                                                                               act);
+    for_activation(act, [&](auto a) {
+      for_held<16>(p.r.held, [&](auto nv) {
+        gn_resident_forward_kernel<F, decltype(nv)::value, decltype(a)::value>
+            <<<blocks_for((s.B * p.r.slices + teams - 1) / teams), threads, teams * p.r.lds, st>>>(in, y, stats, s, p.r,
+                                                                                                 eps);
+      });
     });
   } else if (p.streamed) {
     Carve cv(ws, ws_bytes);
@@ -921,16 +999,20 @@ static int launch_gn_forward(const Inputs& in, void* yp, GroupStats* stats, cons
     const unsigned blocks = blocks_for(s.B * p.t.chunks);
     {
       StageTimer timer("group_norm_stats", st);
-      gn_stats_kernel<F><<<blocks, kStreamThreads, (size_t)(s.C / F::CPS) * p.t.team.pitch * sizeof(double2), st>>>(
+      gn_stats_kernel<F><<<blocks, kThreads, (size_t)(s.C / F::CPS) * p.t.team.pitch * sizeof(double2), st>>>(
           in, work.part, work.counts, s, p.t);
       GTK_LAUNCH_CHECK();
     }
     StageTimer timer("group_norm_apply", st);
-    gn_apply_kernel<F><<<blocks, kStreamThreads, s.G * sizeof(GroupStats), st>>>(in, work.part, work.counts, y, stats, s,
-                                                                                p.t, eps, act);
+    for_activation(act, [&](auto a) {
+      gn_apply_kernel<F, decltype(a)::value><<<blocks, kThreads, s.G * sizeof(GroupStats), st>>>(
+          in, work.part, work.counts, y, stats, s, p.t, eps);
+    });
   } else {
     StageTimer timer("group_norm_forward", st);
-    gn_swept_forward_kernel<T><<<blocks_for(s.B * s.G), 256, 0, st>>>(in, y, stats, s, eps, act);
+    for_activation(act, [&](auto a) {
+      gn_swept_forward_kernel<T, decltype(a)::value><<<blocks_for(s.B * s.G), 256, 0, st>>>(in, y, stats, s, eps);
+    });
   }
   GTK_LAUNCH_CHECK();
   return GTK_OK;
@@ -949,10 +1031,12 @@ static int launch_gn_backward(const Inputs& in, const void* dyp, int64_t ds, con
   if (p.resident) {
     StageTimer timer("group_norm_backward", st);
     const int threads = std::max(256, p.r.team.threads), teams = threads / p.r.team.threads;
-    for_held<4>(p.r.held, [&](auto nv) {
-      gn_resident_backward_kernel<F, decltype(nv)::value>
-          <<<(unsigned)((p.r.per_slice * p.r.slices + teams - 1) / teams), threads, teams * p.r.lds, st>>>(
-              in, dy, ds, stats, dx, sums ? work.channels : nullptr, s, p.r, act);
+    for_activation(act, [&](auto a) {
+      for_held<8>(p.r.held, [&](auto nv) {
+        gn_resident_backward_kernel<F, decltype(nv)::value, decltype(a)::value>
+            <<<(unsigned)((p.r.per_slice * p.r.slices + teams - 1) / teams), threads, teams * p.r.lds, st>>>(
+                in, dy, ds, stats, dx, sums ? work.channels : nullptr, s, p.r);
+      });
     });
     GTK_LAUNCH_CHECK();
   } else if (p.streamed) {
@@ -960,25 +1044,33 @@ static int launch_gn_backward(const Inputs& in, const void* dyp, int64_t ds, con
     {
       StageTimer timer("group_norm_backward_sums", st);
       const size_t lds = (size_t)s.C * (1 + p.t.team.pitch) * sizeof(float2);
-      gn_backward_sums_kernel<F><<<blocks, kStreamThreads, lds, st>>>(
-          in, dy, ds, stats, dx ? work.part : nullptr, sums ? work.channels : nullptr, s, p.t, act);
+      for_activation(act, [&](auto a) {
+        gn_backward_sums_kernel<F, decltype(a)::value><<<blocks, kThreads, lds, st>>>(
+            in, dy, ds, stats, dx ? work.part : nullptr, sums ? work.channels : nullptr, s, p.t);
+      });
       GTK_LAUNCH_CHECK();
     }
     if (dx) {
       StageTimer timer("group_norm_backward_apply", st);
-      gn_backward_apply_kernel<F><<<blocks, kStreamThreads, s.G * sizeof(float2), st>>>(in, dy, ds, stats, work.part, dx,
-                                                                                       s, p.t, act);
+      for_activation(act, [&](auto a) {
+        gn_backward_apply_kernel<F, decltype(a)::value><<<blocks, kThreads, s.G * sizeof(float2), st>>>(
+            in, dy, ds, stats, work.part, dx, s, p.t);
+      });
       GTK_LAUNCH_CHECK();
     }
   } else {
     if (dx) {
       StageTimer timer("group_norm_backward", st);
-      gn_swept_backward_kernel<T><<<blocks_for(s.B * s.G), 256, 0, st>>>(in, dy, ds, stats, dx, s, act);
+      for_activation(act, [&](auto a) {
+        gn_swept_backward_kernel<T, decltype(a)::value><<<blocks_for(s.B * s.G), 256, 0, st>>>(in, dy, ds, stats, dx, s);
+      });
       GTK_LAUNCH_CHECK();
     }
     if (sums) {
       StageTimer timer("group_norm_params", st);
-      gn_swept_params_kernel<T><<<blocks_for(s.C), 256, 0, st>>>(in, dy, ds, stats, dw, db, dst_bf, s, act);
+      for_activation(act, [&](auto a) {
+        gn_swept_params_kernel<T, decltype(a)::value><<<blocks_for(s.C), 256, 0, st>>>(in, dy, ds, stats, dw, db, dst_bf, s);
+      });
       GTK_LAUNCH_CHECK();
     }
     return GTK_OK;
