@@ -32,16 +32,17 @@ struct GroupStats {
   float mean, low, rstd, inv;
 };
 
-__device__ __forceinline__ GroupStats close_stats(double s, double q, double count, float eps) {
+// From the sums of the values and of their squares; inv: 1 / their number, 0 without.
+// v_rsq_f64 has 24 bits or more, what the result keeps.
+__device__ __forceinline__ GroupStats close_stats(double s, double q, double inv, float eps) {
   GroupStats g{0.f, 0.f, 0.f, 0.f};
-  if (count > 0) {
-    const double mean = s / count, var = fmax(q / count - mean * mean, 0.0);
+  if (inv > 0) {
+    const double mean = s * inv, var = fma(-mean, mean, q * inv);
     g.mean = (float)mean;
     g.low = (float)(mean - (double)g.mean);
-    g.rstd = (float)(1.0 / sqrt(var + (double)eps));
-    g.inv = (float)(1.0 / count);
-    // fmax takes the other operand of a NaN
-    if (!(q - q == 0.0)) g.mean = g.low = g.rstd = __builtin_nanf("");
+    // a NaN stays one (fmax would drop it)
+    g.rstd = (float)__builtin_amdgcn_rsq((var < 0 ? 0.0 : var) + (double)eps);
+    g.inv = (float)inv;
   }
   return g;
 }
@@ -53,43 +54,55 @@ __device__ __forceinline__ GroupStats close_stats(double s, double q, double cou
 __device__ __forceinline__ float logistic(float z) { return __builtin_amdgcn_rcpf(1.f + __expf(-z)); }
 
 // The standard normal distribution's function below -|z| is e^(-z^2/2) t P(t) with t =
-// 1 / (1 + 0.3 |z|), which keeps its relative accuracy to the end; P was fitted to
-// erfcx (weighted least squares on |z| <= 14, iterated towards equal errors): 1.5e-7
-// of the value, 4.4e-7 with fp32's roundings.
-struct Tail {
+// 1 / (1 + k |z|), which keeps its relative accuracy to the end; P was fitted to
+// erfcx (weighted least squares on |z| <= 14, iterated towards equal errors).  FINE:
+// 1.5e-7 of the value, 4.4e-7 with fp32's roundings.  For bf16 results, which round by
+// 3.9e-3, three terms fewer are 3.5e-5 off: gelu binds the kernels by its
+// instructions (2^20 positions of 128 channels, training: 433 us with all terms, 407
+// with these).
+template <bool FINE> struct Tail {
   float e, tp;  // e^(-z^2/2), t P(t)
   __device__ __forceinline__ explicit Tail(float z) {
     e = __builtin_amdgcn_exp2f(z * z * -0.7213475204f);  // log2(e) / 2
-    const float t = __builtin_amdgcn_rcpf(fmaf(0.3f, fabsf(z), 1.f));
-    float p = 0.03567477342812997f;
-    p = fmaf(p, t, -0.1572030800704706f);
-    p = fmaf(p, t, 0.20635350232969402f);
-    p = fmaf(p, t, -0.05368364104385134f);
-    p = fmaf(p, t, 0.1285616251824942f);
-    p = fmaf(p, t, 0.09991349247240931f);
-    p = fmaf(p, t, 0.12075395598321578f);
-    p = fmaf(p, t, 0.11962929883230777f);
+    const float t = __builtin_amdgcn_rcpf(fmaf(FINE ? 0.3f : 0.38f, fabsf(z), 1.f));
+    float p;
+    if constexpr (FINE) {
+      p = 0.03567477342812997f;
+      p = fmaf(p, t, -0.1572030800704706f);
+      p = fmaf(p, t, 0.20635350232969402f);
+      p = fmaf(p, t, -0.05368364104385134f);
+      p = fmaf(p, t, 0.1285616251824942f);
+      p = fmaf(p, t, 0.09991349247240931f);
+      p = fmaf(p, t, 0.12075395598321578f);
+      p = fmaf(p, t, 0.11962929883230777f);
+    } else {
+      p = -0.08992832869603486f;
+      p = fmaf(p, t, 0.18887642422770945f);
+      p = fmaf(p, t, 0.09197977584781399f);
+      p = fmaf(p, t, 0.157829463361757f);
+      p = fmaf(p, t, 0.15122513768077908f);
+    }
     tp = t * p;
   }
 };
 
 // silu(z) = z s(z); gelu(z) = z Phi(z) = max(z, 0) - |z| Phi(-|z|)
-template <int ACT> __device__ __forceinline__ float activate(float z) {
+template <int ACT, bool FINE> __device__ __forceinline__ float activate(float z) {
   if constexpr (ACT == GTK_ACT_SILU) return z * logistic(z);
   if constexpr (ACT == GTK_ACT_GELU) {
-    const Tail a(z);
+    const Tail<FINE> a(z);
     return fmaf(-fabsf(z), a.e * a.tp, fmaxf(z, 0.f));
   }
   return z;
 }
 // silu' = s + z s (1 - s); gelu' = Phi(z) + z phi(z), 1 - that of -z
-template <int ACT> __device__ __forceinline__ float activate_slope(float z) {
+template <int ACT, bool FINE> __device__ __forceinline__ float activate_slope(float z) {
   if constexpr (ACT == GTK_ACT_SILU) {
     const float s = logistic(z);
     return s * fmaf(z, 1.f - s, 1.f);
   }
   if constexpr (ACT == GTK_ACT_GELU) {
-    const Tail a(z);
+    const Tail<FINE> a(z);
     const float below = a.e * fmaf(-fabsf(z), 0.3989422804f, a.tp);
     return z < 0.f ? below : 1.f - below;
   }
@@ -106,6 +119,7 @@ template <int ACT> __device__ __forceinline__ float activate_slope(float z) {
 template <typename T_, int VE_, int SL_> struct Form {
   typedef T_ T;
   static constexpr int VE = VE_, SL = SL_, CPS = VE / SL;  // channels a slot
+  static constexpr bool FINE = sizeof(T) == 4;
 };
 
 struct Team {
@@ -118,6 +132,14 @@ struct Team {
 struct Shape {
   int64_t B, P;
   int C, G, cg;
+  double inv;  // 1 / the values of a group
+
+  static Shape of(int64_t B, int64_t P, int64_t C, int64_t G) {
+    return {B, P, (int)C, (int)G, (int)(C / G), 1.0 / ((double)P * (double)(C / G))};
+  }
+  __device__ __forceinline__ double inverse(int64_t positions) const {
+    return positions ? 1.0 / ((double)positions * (double)cg) : 0.0;
+  }
 };
 
 template <typename F> struct Place {
@@ -174,7 +196,7 @@ __device__ __forceinline__ void sum_runs(const S* sums, int outs, int len, int t
   }
 }
 
-// Positions that count, of `n` counts; the sum in each lane.
+// The sum of `n` counts, in each lane.
 __device__ __forceinline__ int64_t sum_counts(const int* counts, int n, int t, int lanes) {
   int64_t a = 0;
   for (int e = t & (lanes - 1); e < n; e += lanes) a += counts[e];
@@ -227,7 +249,7 @@ template <typename F> struct ForwardCoefs {
   }
   template <int ACT> __device__ __forceinline__ void apply(float* f) const {
 #pragma unroll
-    for (int e = 0; e < F::VE; ++e) f[e] = activate<ACT>(fmaf(f[e] - mean[e / F::CPS], a[e], b[e]));
+    for (int e = 0; e < F::VE; ++e) f[e] = activate<ACT, F::FINE>(fmaf(f[e] - mean[e / F::CPS], a[e], b[e]));
   }
 };
 template <typename F> struct BackwardCoefs {
@@ -252,7 +274,7 @@ template <typename F> struct BackwardCoefs {
     for (int e = 0; e < F::VE; ++e) {
       const int j = e / F::CPS;
       f[e] = fmaf(f[e] - mean[j], rstd[j], shift[j]);
-      g[e] *= activate_slope<ACT>(fmaf(f[e], w[e], b[e]));
+      g[e] *= activate_slope<ACT, F::FINE>(fmaf(f[e], w[e], b[e]));
     }
   }
   // f = dL/dx of h = f and dz = g; means: of g w and g w h over the group
@@ -280,8 +302,10 @@ struct ResidentPlan {
   int held;    // vectors a thread
   int groups;  // a slice
   int slices;
-  int64_t per_slice;  // teams of a slice in the backward pass: each takes several samples
-  size_t lds;         // of a team
+  size_t lds;  // of a team
+  // backward: blocks of a slice (each team takes several samples), and the block's
+  // partial sums of a channel in LDS
+  int teams, blocks, pitch, lanes;
 };
 
 constexpr int kThreads = 512;  // of a block, at most: 256 registers a thread
@@ -293,7 +317,7 @@ __global__ __launch_bounds__(kThreads) void gn_resident_forward_kernel(Inputs in
   typedef typename F::T T;
   extern __shared__ double2 gn_lds[];
   const Team& g = p.team;
-  const int t = threadIdx.x % g.threads, team = threadIdx.x / g.threads, teams = blockDim.x / g.threads;
+  const int t = threadIdx.x % g.threads, team = threadIdx.x / g.threads, teams = p.teams;
   const int width = p.groups * s.cg;
   const Place<F> at(t, g, width);
   char* lds = (char*)gn_lds + team * p.lds;
@@ -332,9 +356,9 @@ __global__ __launch_bounds__(kThreads) void gn_resident_forward_kernel(Inputs in
     put_sums<F::SL, F::VE>(sums, sum, at.at, at.skip, at.row, at.on, g);
     if (at.first && at.on) row_counts[at.row] = n;
     __syncthreads();
-    const double count = (double)s.cg * (double)(in.mask ? sum_counts(row_counts, g.rows, t, g.lanes) : s.P);
+    const double inv = in.mask ? s.inverse(sum_counts(row_counts, g.rows, t, g.lanes)) : s.inv;
     sum_runs(sums, p.groups, s.cg / F::CPS * g.pitch, t, g.threads, g.lanes, [&](int o, double2 a) {
-      mine[o] = close_stats(a.x, a.y, count, eps);
+      mine[o] = close_stats(a.x, a.y, inv, eps);
       if (any) stats[b * s.G + slice * p.groups + o] = mine[o];
     });
     __syncthreads();
@@ -355,7 +379,8 @@ __global__ __launch_bounds__(kThreads) void gn_resident_forward_kernel(Inputs in
   }
 }
 
-// dx, and this team's sums of dz h and dz over its samples, part[team][0 and 1][c].
+// dx, and the block's sums of dz h and dz over its samples, part[block of the
+// slice][0 and 1][c].
 template <typename F, int NV, int ACT>
 __global__ __launch_bounds__(kThreads) void gn_resident_backward_kernel(Inputs in, const typename F::T* __restrict__ dy,
                                                                     int64_t ds, const GroupStats* __restrict__ stats,
@@ -364,20 +389,20 @@ __global__ __launch_bounds__(kThreads) void gn_resident_backward_kernel(Inputs i
   typedef typename F::T T;
   extern __shared__ double2 gn_lds[];
   const Team& g = p.team;
-  const int t = threadIdx.x % g.threads, team = threadIdx.x / g.threads, teams = blockDim.x / g.threads;
+  const int t = threadIdx.x % g.threads, team = threadIdx.x / g.threads;
   const int width = p.groups * s.cg;
   const Place<F> at(t, g, width);
-  char* lds = (char*)gn_lds + team * p.lds;
-  float2* means = (float2*)lds;
+  float2* means = (float2*)((char*)gn_lds + team * p.lds);
   float2* sums = means + p.groups;
-  const int64_t id = xcd_remap_any(blockIdx.x, gridDim.x) * teams + team, index = id / p.slices;
-  const int slice = (int)(id - index * p.slices), c = slice * width + at.at;
+  // slices of a sample share lines of memory: on one die
+  const int id = (int)xcd_remap_any(blockIdx.x, gridDim.x), index = id / p.slices;
+  const int slice = id - index * p.slices, c = slice * width + at.at;
   float2 channel[F::VE];
 #pragma unroll
   for (int e = 0; e < F::VE; ++e) channel[e] = float2{0.f, 0.f};
-  for (int64_t b0 = 0; b0 < s.B; b0 += p.per_slice) {
-    const bool any = index < p.per_slice && b0 + index < s.B;
-    const int64_t b = any ? b0 + index : s.B - 1;
+  for (int64_t b0 = (int64_t)index * p.teams; b0 < s.B; b0 += (int64_t)p.blocks * p.teams) {
+    const bool any = b0 + team < s.B;
+    const int64_t b = any ? b0 + team : s.B - 1;
     const int P = (int)s.P;
     Vec<T, F::VE> x[NV], d[NV];
     bool live[NV];
@@ -440,12 +465,14 @@ __global__ __launch_bounds__(kThreads) void gn_resident_backward_kernel(Inputs i
     }
   }
   if (!part) return;
+  // the rows of all teams
+  float2* channels = (float2*)gn_lds;
+  const Team block{0, 0, g.rows * p.teams, p.pitch, 0, 0};
   __syncthreads();
-  put_sums<F::VE, F::VE>(sums, channel, at.at, at.skip, at.row, at.on, g);
+  put_sums<F::VE, F::VE>(channels, channel, at.at, at.skip, team * g.rows + at.row, at.on, block);
   __syncthreads();
-  float* dst = part + index * 2 * s.C + slice * width;
-  sum_runs(sums, width, g.pitch, t, g.threads, g.channel_lanes, [&](int o, float2 a) {
-    if (index >= p.per_slice) return;
+  float* dst = part + (int64_t)index * 2 * s.C + slice * width;
+  sum_runs(channels, width, p.pitch, threadIdx.x, blockDim.x, p.lanes, [&](int o, float2 a) {
     dst[o] = a.x;
     dst[s.C + o] = a.y;
   });
@@ -497,59 +524,71 @@ template <typename F, bool TWO, bool KEEP> struct Cursor {
     d = TWO ? dy + (b * s.P + at.row) * ds + at.at : nullptr;
     mask = in.mask ? in.mask + b * s.P + at.row : nullptr;
   }
-  template <int U> __device__ __forceinline__ void load(Held<F, U, TWO>& v, int64_t step) const {
+  template <int U> __device__ __forceinline__ void load_live(bool (&live)[U], int64_t step) const {
 #pragma unroll
-    for (int j = 0; j < U; ++j) {
-      get(v.x[j], x + (step + j) * x_step);
-      if constexpr (TWO) get(v.d[j], d + (step + j) * d_step);
-    }
-#pragma unroll
-    for (int j = 0; j < U; ++j) v.live[j] = !mask || mask[(step + j) * rows] != 0.f;
+    for (int j = 0; j < U; ++j) live[j] = !mask || mask[(step + j) * rows] != 0.f;
   }
-  // The sample's last step, which not all threads have a position in: the others
-  // read the last one.
-  __device__ __forceinline__ void load_part(Held<F, 1, TWO>& v, int64_t step) const {
-    const int64_t over = step * rows + row - (left - 1), back = over > 0 ? over : 0;
-    get(v.x[0], x + step * x_step - back * (x_step / rows));
-    if constexpr (TWO) get(v.d[0], d + step * d_step - back * (d_step / rows));
-    v.live[0] = over <= 0 && (!mask || mask[step * rows] != 0.f);
+  // what does not count is not read
+  template <int U> __device__ __forceinline__ void load(Held<F, U, TWO>& v, int64_t step) const {
+    if (!mask) {
+#pragma unroll
+      for (int j = 0; j < U; ++j) get(v, j, step + j);
+    } else {
+#pragma unroll
+      for (int j = 0; j < U; ++j)
+        if (v.live[j]) get(v, j, step + j);
+    }
+  }
+  // One step, which not all threads may have a position in.
+  __device__ __forceinline__ void load_one(Held<F, 1, TWO>& v, int64_t step) const {
+    v.live[0] = inside(step) && (!mask || mask[step * rows] != 0.f);
+    if (v.live[0]) get(v, 0, step);
   }
   __device__ __forceinline__ bool inside(int64_t step) const { return step * rows + row < left; }
 
  private:
-  static __device__ __forceinline__ void get(Vec<T, F::VE>& v, const T* p) {
-    if constexpr (KEEP)
-      v.load_plain(p);
-    else
-      v.load(p);
+  template <int U> __device__ __forceinline__ void get(Held<F, U, TWO>& v, int j, int64_t step) const {
+    if constexpr (KEEP) {
+      v.x[j].load_plain(x + step * x_step);
+      if constexpr (TWO) v.d[j].load_plain(d + step * d_step);
+    } else {
+      v.x[j].load(x + step * x_step);
+      if constexpr (TWO) v.d[j].load(d + step * d_step);
+    }
   }
 };
 
 // Calls use(held, j, step) for the chunk's steps, forwards or backwards, U whole ones at
-// a time while the next U are on their way; start() runs behind the first loads.
+// a time while the next U are on their way, and the mask of those behind them;
+// start() runs behind the first loads.
 template <int U, bool BACK, typename F, bool TWO, bool KEEP, typename Start, typename Use>
 __device__ __forceinline__ void for_steps(const Cursor<F, TWO, KEEP>& at, const Chunk& k, Start start, Use use) {
   const int64_t whole = k.whole > k.first ? k.whole - k.first : 0, sets = whole / U;
   Held<F, U, TWO> now, next;
   auto step_of = [&](int64_t i) { return k.first + (BACK ? sets - 1 - i : i) * U; };
-  if (sets) at.load(now, step_of(0));
+  if (sets) {
+    at.load_live(now.live, step_of(0));
+    if (sets > 1) at.load_live(next.live, step_of(1));
+    at.load(now, step_of(0));
+  }
   start();
   auto rest = [&]() {
     for (int64_t step = k.first + sets * U; step < k.last; ++step) {
       Held<F, 1, TWO> one;
-      if (step < k.whole)
-        at.load(one, step);
-      else
-        at.load_part(one, step);
+      at.load_one(one, step);
       use(one, 0, step);
     }
   };
   if (BACK) rest();
   for (int64_t i = 0; i < sets; ++i) {
+    bool ahead[U];
     if (i + 1 < sets) at.load(next, step_of(i + 1));
+    if (i + 2 < sets) at.load_live(ahead, step_of(i + 2));
 #pragma unroll
     for (int j = 0; j < U; ++j) use(now, j, step_of(i) + j);
     now = next;
+#pragma unroll
+    for (int j = 0; j < U; ++j) next.live[j] = ahead[j];
   }
   if (!BACK) rest();
 }
@@ -609,10 +648,10 @@ __global__ __launch_bounds__(kThreads) void gn_apply_kernel(Inputs in, const dou
     const int64_t y_step = (int64_t)g.rows * s.C;
     ForwardCoefs<F> co;
     auto start = [&]() {
-      const double count =
-          (double)s.cg * (double)(in.mask ? sum_counts(chunk_counts + k.b * p.chunks, p.chunks, t, g.lanes) : s.P);
+      const double inv =
+          in.mask ? s.inverse(sum_counts(chunk_counts + k.b * p.chunks, p.chunks, t, g.lanes)) : s.inv;
       sum_runs<8>(part + k.b * s.G * p.chunks, s.G, p.chunks, t, kThreads, g.lanes, [&](int o, double2 a) {
-        mine[o] = close_stats(a.x, a.y, count, eps);
+        mine[o] = close_stats(a.x, a.y, inv, eps);
         if (k.chunk == 0) stats[k.b * s.G + o] = mine[o];
       });
       __syncthreads();
@@ -643,6 +682,7 @@ __global__ __launch_bounds__(kThreads) void gn_backward_sums_kernel(Inputs in, c
   extern __shared__ double2 gn_lds[];
   float2* weighted = (float2*)gn_lds;  // [C]: a channel's part of its group's sums
   float2* sums = weighted + s.C;
+  float* weight = (float*)(sums + (int64_t)s.C * p.team.pitch);
   const Team& g = p.team;
   const int t = threadIdx.x;
   const Place<F> at(t, g, s.C);
@@ -653,7 +693,12 @@ __global__ __launch_bounds__(kThreads) void gn_backward_sums_kernel(Inputs in, c
     float2 sum[F::VE];
 #pragma unroll
     for (int e = 0; e < F::VE; ++e) sum[e] = float2{0.f, 0.f};
-    auto start = [&]() { co.set(stats + k.b * s.G, params, at.at, s.cg); };
+    auto start = [&]() {
+      co.set(stats + k.b * s.G, params, at.at, s.cg);
+#pragma unroll
+      for (int e = 0; e < F::VE; ++e)
+        if (at.row == 0) weight[at.at + e] = params.w[e];
+    };
     for_steps<2, false>(Cursor<F, true, true>(in, dy, ds, s, g, k.b, at), k, start, [&](auto& v, int j, int64_t) {
       if (!v.live[j]) return;
       float f[F::VE], dz[F::VE];
@@ -673,7 +718,7 @@ __global__ __launch_bounds__(kThreads) void gn_backward_sums_kernel(Inputs in, c
         channels[item * 2 * s.C + c] = a.x;
         channels[(item * 2 + 1) * s.C + c] = a.y;
       }
-      const float w = in.w.get(c, 1.f);
+      const float w = weight[c];
       weighted[c] = float2{a.y * w, a.x * w};
     });
     __syncthreads();
@@ -687,15 +732,20 @@ __global__ __launch_bounds__(kThreads) void gn_backward_sums_kernel(Inputs in, c
 template <typename F, int ACT>
 __global__ __launch_bounds__(kThreads) void gn_backward_apply_kernel(
     Inputs in, const typename F::T* __restrict__ dy, int64_t ds, const GroupStats* __restrict__ stats,
-    const float2* __restrict__ part, typename F::T* __restrict__ dx, Shape s, StreamPlan p) {
+    const float2* __restrict__ part, typename F::T* __restrict__ dx, ColumnSums close, int blocks, Shape s,
+    StreamPlan p) {
   typedef typename F::T T;
   extern __shared__ double2 gn_lds[];
+  if ((int)blockIdx.x >= blocks) {  // the parameters' gradients
+    close_columns<16, kThreads / 16>(close, (int)blockIdx.x - blocks, (float*)gn_lds);
+    return;
+  }
   float2* means = (float2*)gn_lds;
   const Team& g = p.team;
   const int t = threadIdx.x;
   const Place<F> at(t, g, s.C);
   const Params<F> params(in.w, in.b, at.at);
-  for (int64_t item = blockIdx.x; item < s.B * p.chunks; item += gridDim.x) {
+  for (int64_t item = blockIdx.x; item < s.B * p.chunks; item += blocks) {
     const Chunk k(item, p);
     const Cursor<F, true, false> from(in, dy, ds, s, g, k.b, at);
     T* to = dx + (k.b * s.P + at.row) * s.C + at.at;
@@ -769,12 +819,12 @@ __global__ __launch_bounds__(256) void gn_swept_forward_kernel(Inputs in, T* __r
       v[2] += 1;
     });
     block_add(v, red);
-    const GroupStats g = close_stats(v[0], v[1], v[2], eps);
+    const GroupStats g = close_stats(v[0], v[1], v[2] > 0 ? 1.0 / v[2] : 0.0, eps);
     if (threadIdx.x == 0) stats[bg] = g;
     for_values(s, c0, [&](int64_t pos, int c) {
       const bool live = !in.mask || in.mask[first + pos] != 0.f;
       const float h = ((to_f32(x[(first + pos) * in.xs + c]) - g.mean) - g.low) * g.rstd;
-      y[(first + pos) * s.C + c] = cvt<T>(live ? activate<ACT>(fmaf(h, in.w.get(c, 1.f), in.b.get(c, 0.f))) : 0.f);
+      y[(first + pos) * s.C + c] = cvt<T>(live ? activate<ACT, sizeof(T) == 4>(fmaf(h, in.w.get(c, 1.f), in.b.get(c, 0.f))) : 0.f);
     });
   }
 }
@@ -786,7 +836,7 @@ __device__ __forceinline__ bool swept_backward(const Inputs& in, const T* dy, in
   h = dz = 0.f;
   if (in.mask && in.mask[row] == 0.f) return false;
   h = ((to_f32(((const T*)in.x)[row * in.xs + c]) - g.mean) - g.low) * g.rstd;
-  dz = to_f32(dy[row * ds + c]) * activate_slope<ACT>(fmaf(h, in.w.get(c, 1.f), in.b.get(c, 0.f)));
+  dz = to_f32(dy[row * ds + c]) * activate_slope<ACT, sizeof(T) == 4>(fmaf(h, in.w.get(c, 1.f), in.b.get(c, 0.f)));
   return true;
 }
 
@@ -846,7 +896,6 @@ __global__ __launch_bounds__(256) void gn_swept_params_kernel(Inputs in, const T
 // ---------------------------------------------------------------------------
 // Plans
 // ---------------------------------------------------------------------------
-#define GN_WANT (s.B == 1 ? 1 : 2)
 constexpr size_t kMostLds = 156 * 1024;
 constexpr int kMostBlocks = 1 << 20;  // the kernels loop past that
 
@@ -873,51 +922,65 @@ static Team make_team(int threads, int across, int64_t groups, int64_t channels)
   return t;
 }
 
-// The narrowest slices of whole groups that fill 64-byte pieces of memory, wider
-// ones as long as they leave four teams a CU.
+static size_t block_lds(const ResidentPlan& p, int64_t width, bool backward) {
+  const size_t sums = p.lds * p.teams;
+  return backward ? std::max(sums, (size_t)width * p.pitch * sizeof(float2)) : sums;
+}
+
+// Slices whose rows fill 64-byte pieces of memory (8 samples of 4096 positions and 256
+// bf16 channels in 16-byte pieces: 31 + 36 us, streamed 17 + 24), wider ones as long as
+// they leave four teams a CU.
 template <typename F> static bool plan_resident(const Shape& s, bool backward, ResidentPlan* plan) {
-  const int most = backward ? 8 : 16;
+  const int most = backward ? 8 : 16, cus = device_cus();
+  if (s.P > (int64_t)kThreads * most) return false;
   bool found = false;
   for (int groups = 1; groups <= s.G; ++groups) {
-    if (s.G % groups) continue;
     const int64_t width = (int64_t)groups * s.cg;
-    if (width < F::VE || (groups < s.G && width * (int64_t)sizeof(typename F::T) < 64)) continue;
-    const int64_t across = (width + F::VE - 1) / F::VE;
-    if (across > kThreads || s.P > kThreads * most) break;
-    const int64_t units = s.B * (s.G / groups);
-    if (found && units < 4 * (int64_t)device_cus()) break;
+    if (s.G % groups || width < F::VE || (groups < s.G && width * (int64_t)sizeof(typename F::T) < 64)) continue;
+    const int64_t across = (width + F::VE - 1) / F::VE, units = s.B * (s.G / groups);
+    if (across > kThreads || (found && units < 4 * (int64_t)cus)) break;
     int threads = pow2_up(across);
     auto held = [&](int n) { return (s.P + n / across - 1) / (n / across); };
     while (threads < kThreads && held(threads) > most) threads *= 2;
     if (held(threads) > most) break;
+    // A CU takes some 0.25 ns a value (twice that backward): few teams of many values
+    // are slower than two launches over all CUs (1024 positions of 128 bf16 channels in
+    // four teams 10 + 16 us, streamed 9 + 12).
+    if (units < 2 * (int64_t)cus && s.P * width > 32768) break;
     // more threads where there are few teams
-    while (threads < kThreads && held(threads) > 1 && units * threads < 512 * (int64_t)device_cus()) threads *= 2;
+    while (threads < kThreads && held(threads) > 1 && units * threads < 512 * (int64_t)cus) threads *= 2;
     ResidentPlan p;
     p.team = make_team(threads, (int)across, groups, width);
     p.held = (int)held(threads);
     p.groups = groups;
     p.slices = s.G / groups;
-    p.per_slice = std::min<int64_t>(s.B, std::max<int64_t>(1, 2048 * (int64_t)device_cus() / threads / p.slices));
-    p.lds = backward ? groups * sizeof(float2) + width * p.team.pitch * sizeof(float2)
+    p.lds = backward ? (groups + width / F::CPS * p.team.pitch) * sizeof(float2)
                      : width / F::CPS * p.team.pitch * sizeof(double2) + groups * sizeof(GroupStats) +
                            p.team.rows * sizeof(int);
     p.lds = (p.lds + 15) & ~size_t(15);
-    if (p.lds * std::max(1, 256 / threads) > kMostLds) break;
+    p.teams = (backward ? kThreads : std::max(256, threads)) / threads;
+    // two blocks a CU: each leaves 2 C partial sums
+    p.blocks = (int)std::min<int64_t>((s.B + p.teams - 1) / p.teams, std::max(1, 2 * cus / p.slices));
+    p.pitch = p.team.rows * p.teams | 1;
+    p.lanes = lanes_for(kThreads, width);
+    if (block_lds(p, width, backward) > kMostLds) break;
     *plan = p;
     found = true;
   }
   return found;
 }
 
-// A chunk a CU, two where there are several samples (each block of the second
-// launch adds its sample's partial sums up).
+// A chunk a CU, or two of them where they are long: each block of the second launch
+// adds its sample's partial sums up (2^18 positions of 128 bf16 channels 113 us, with
+// two chunks a CU 123; 2^20 of them 454 and 444).
 template <typename F> static bool plan_streamed(const Shape& s, StreamPlan* p) {
   const int64_t across = ((int64_t)s.C + F::VE - 1) / F::VE;
   if (across > kThreads) return false;
   p->team = make_team(kThreads, (int)across, s.G, s.C);
   p->all = (s.P + p->team.rows - 1) / p->team.rows;
   p->whole = s.P / p->team.rows;
-  const int64_t want = std::max<int64_t>(1, GN_WANT * (int64_t)device_cus() / s.B);
+  const int64_t cus = device_cus();
+  const int64_t want = std::max<int64_t>(1, (p->all * s.B >= 32 * 2 * cus ? 2 * cus : cus) / s.B);
   p->steps = (p->all + want - 1) / want;
   p->chunks = (int)((p->all + p->steps - 1) / p->steps);
   return true;
@@ -931,7 +994,7 @@ template <typename F> struct Plan {
     resident = plan_resident<F>(s, backward, &r);
     streamed = !resident && plan_streamed<F>(s, &t);
   }
-  int64_t parts(const Shape& s) const { return resident ? r.per_slice : streamed ? s.B * t.chunks : 0; }
+  int64_t parts(const Shape& s) const { return resident ? r.blocks : streamed ? s.B * t.chunks : 0; }
 };
 
 // Calls run(Form) for the types and the width of a slot.
@@ -985,12 +1048,12 @@ static int launch_gn_forward(const Inputs& in, void* yp, GroupStats* stats, cons
   const Plan<F> p(s, false);
   if (p.resident) {
     StageTimer timer("group_norm_forward", st);
-    const int threads = std::max(256, p.r.team.threads), teams = threads / p.r.team.threads;
+    const unsigned blocks = blocks_for((s.B * p.r.slices + p.r.teams - 1) / p.r.teams);
     for_activation(act, [&](auto a) {
       for_held<16>(p.r.held, [&](auto nv) {
         gn_resident_forward_kernel<F, decltype(nv)::value, decltype(a)::value>
-            <<<blocks_for((s.B * p.r.slices + teams - 1) / teams), threads, teams * p.r.lds, st>>>(in, y, stats, s, p.r,
-                                                                                                 eps);
+            <<<blocks, p.r.teams * p.r.team.threads, block_lds(p.r, p.r.groups * s.cg, false), st>>>(in, y, stats, s, p.r,
+                                                                                                   eps);
       });
     });
   } else if (p.streamed) {
@@ -1030,11 +1093,10 @@ static int launch_gn_backward(const Inputs& in, const void* dyp, int64_t ds, con
   const bool sums = dw || db;
   if (p.resident) {
     StageTimer timer("group_norm_backward", st);
-    const int threads = std::max(256, p.r.team.threads), teams = threads / p.r.team.threads;
     for_activation(act, [&](auto a) {
       for_held<8>(p.r.held, [&](auto nv) {
         gn_resident_backward_kernel<F, decltype(nv)::value, decltype(a)::value>
-            <<<(unsigned)((p.r.per_slice * p.r.slices + teams - 1) / teams), threads, teams * p.r.lds, st>>>(
+            <<<(unsigned)p.r.blocks * p.r.slices, kThreads, block_lds(p.r, p.r.groups * s.cg, true), st>>>(
                 in, dy, ds, stats, dx, sums ? work.channels : nullptr, s, p.r);
       });
     });
@@ -1043,21 +1105,28 @@ static int launch_gn_backward(const Inputs& in, const void* dyp, int64_t ds, con
     const unsigned blocks = blocks_for(s.B * p.t.chunks);
     {
       StageTimer timer("group_norm_backward_sums", st);
-      const size_t lds = (size_t)s.C * (1 + p.t.team.pitch) * sizeof(float2);
+      const size_t lds = (size_t)s.C * ((1 + p.t.team.pitch) * sizeof(float2) + sizeof(float));
       for_activation(act, [&](auto a) {
         gn_backward_sums_kernel<F, decltype(a)::value><<<blocks, kThreads, lds, st>>>(
             in, dy, ds, stats, dx ? work.part : nullptr, sums ? work.channels : nullptr, s, p.t);
       });
       GTK_LAUNCH_CHECK();
     }
+    const ColumnSums close{work.channels, (int)p.parts(s), s.C, dw, db, dst_bf};
+    const unsigned more = sums ? (2 * s.C + 15) / 16 : 0;
     if (dx) {
       StageTimer timer("group_norm_backward_apply", st);
+      const size_t lds = std::max(s.G * sizeof(float2), sums ? kThreads * sizeof(float) : 0);
       for_activation(act, [&](auto a) {
-        gn_backward_apply_kernel<F, decltype(a)::value><<<blocks, kThreads, s.G * sizeof(float2), st>>>(
-            in, dy, ds, stats, work.part, dx, s, p.t);
+        gn_backward_apply_kernel<F, decltype(a)::value><<<blocks + more, kThreads, lds, st>>>(
+            in, dy, ds, stats, work.part, dx, close, (int)blocks, s, p.t);
       });
-      GTK_LAUNCH_CHECK();
+    } else {  // in the same order
+      StageTimer timer("group_norm_close", st);
+      column_close_kernel<16, kThreads / 16><<<more, kThreads, 0, st>>>(close);
     }
+    GTK_LAUNCH_CHECK();
+    return GTK_OK;
   } else {
     if (dx) {
       StageTimer timer("group_norm_backward", st);
@@ -1111,7 +1180,7 @@ using namespace gtk;
 
 extern "C" size_t gtk_group_norm_workspace_size(int64_t B, int64_t positions, int64_t c, int64_t groups, int dtype) {
   if (!gn_shape_ok(B, positions, c, groups, dtype) || B == 0) return 0;
-  return work_size<ForwardWork>(Shape{B, positions, (int)c, (int)groups, (int)(c / groups)}, dtype, false);
+  return work_size<ForwardWork>(Shape::of(B, positions, c, groups), dtype, false);
 }
 
 extern "C" int gtk_group_norm_forward(const void* x, int64_t x_stride, const float* mask, void* y, float* stats,
@@ -1126,7 +1195,7 @@ extern "C" int gtk_group_norm_forward(const void* x, int64_t x_stride, const flo
               "gtk_group_norm_forward: workspace %zu < %zu bytes", workspace ? workspace_bytes : 0, need);
   const int pbf = param_dtype == GTK_BF16;
   const Inputs in{x, x_stride, mask, {weight, pbf}, {bias, pbf}};
-  const Shape s{B, positions, (int)c, (int)groups, (int)(c / groups)};
+  const Shape s = Shape::of(B, positions, c, groups);
   auto run = [&](auto form) {
     return launch_gn_forward<decltype(form)>(in, y, (GroupStats*)stats, s, eps, activation, workspace, workspace_bytes,
                                              (hipStream_t)stream);
@@ -1137,7 +1206,7 @@ extern "C" int gtk_group_norm_forward(const void* x, int64_t x_stride, const flo
 extern "C" size_t gtk_group_norm_backward_workspace_size(int64_t B, int64_t positions, int64_t c, int64_t groups,
                                                          int dtype) {
   if (!gn_shape_ok(B, positions, c, groups, dtype) || B == 0) return 0;
-  return work_size<BackwardWork>(Shape{B, positions, (int)c, (int)groups, (int)(c / groups)}, dtype, true);
+  return work_size<BackwardWork>(Shape::of(B, positions, c, groups), dtype, true);
 }
 
 extern "C" int gtk_group_norm_backward(const void* x, int64_t x_stride, const float* mask, const void* dy,
@@ -1158,7 +1227,7 @@ extern "C" int gtk_group_norm_backward(const void* x, int64_t x_stride, const fl
                ? launch_column_close("group_norm_close", nullptr, 0, (int)c, dweight, dbias, pbf, (hipStream_t)stream)
                : GTK_OK;
   const Inputs in{x, x_stride, mask, {weight, pbf}, {bias, pbf}};
-  const Shape s{B, positions, (int)c, (int)groups, (int)(c / groups)};
+  const Shape s = Shape::of(B, positions, c, groups);
   auto run = [&](auto form) {
     return launch_gn_backward<decltype(form)>(in, dy, dy_stride, (const GroupStats*)stats, dx, dweight, dbias, pbf, s,
                                               activation, workspace, workspace_bytes, (hipStream_t)stream);
