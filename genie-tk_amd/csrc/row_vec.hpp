@@ -26,6 +26,7 @@ template <typename T, int VE> struct Vec {
   __device__ __forceinline__ void load(const T* p) { raw = __builtin_nontemporal_load((const u32x4_any*)p); }
   __device__ __forceinline__ void store(T* p) const { __builtin_nontemporal_store(raw, (u32x4_any*)p); }
   __device__ __forceinline__ void load_plain(const T* p) { raw = *(const u32x4_any*)p; }
+  __device__ __forceinline__ void zero() { raw = u32x4{0, 0, 0, 0}; }
   // What was unpacked before is unpacked again, and need not be kept in registers.
   __device__ __forceinline__ void forget_unpacked() { asm volatile("" : "+v"(raw)); }
   __device__ __forceinline__ void store_plain(T* p) const { *(u32x4_any*)p = raw; }
@@ -56,6 +57,7 @@ template <typename T> struct Vec<T, 1> {
   __device__ __forceinline__ void load(const T* p) { v = *p; }
   __device__ __forceinline__ void store(T* p) const { *p = v; }
   __device__ __forceinline__ void load_plain(const T* p) { v = *p; }
+  __device__ __forceinline__ void zero() { v = cvt<T>(0.f); }
   __device__ __forceinline__ void forget_unpacked() {}
   __device__ __forceinline__ void store_plain(T* p) const { *p = v; }
   __device__ __forceinline__ void get(float* f) const { f[0] = to_f32(v); }
