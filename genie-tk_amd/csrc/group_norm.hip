@@ -488,23 +488,26 @@ __global__ __launch_bounds__(kThreads) void gn_resident_backward_kernel(Inputs i
 }
 
 // ---------------------------------------------------------------------------
-// Streamed: a team is a block, and has a chunk of a sample's positions: `steps` times
-// the team's rows.
+// Streamed: a team is a block, and has a chunk of a sample's positions (`steps` times
+// the team's rows) in a slice of `groups` whole groups: all of them, unless they are
+// more than 512 vectors wide.
 // ---------------------------------------------------------------------------
 struct StreamPlan {
   Team team;
-  int chunks;
+  int groups, slices, chunks;
   int64_t steps, all, whole;  // of a chunk; of a sample; those of them that have all their rows
 };
 
 // A block's chunk: steps [first, last) of sample b, of which those before `whole` have
-// all their rows.
+// all their rows, in the slice that starts at group g0.
 struct Chunk {
-  int64_t b, first, last, whole;
-  int chunk;
+  int64_t index, b, first, last, whole;  // index: of (sample, chunk)
+  int chunk, g0;
   __device__ __forceinline__ Chunk(int64_t item, const StreamPlan& p) {
-    b = item / p.chunks;
-    chunk = (int)(item - b * p.chunks);
+    index = p.slices == 1 ? item : item / p.slices;
+    g0 = (int)(item - index * p.slices) * p.groups;
+    b = index / p.chunks;
+    chunk = (int)(index - b * p.chunks);
     first = chunk * p.steps;
     last = first + p.steps < p.all ? first + p.steps : p.all;
     whole = last < p.whole ? last : p.whole;
@@ -527,10 +530,10 @@ template <typename F, bool TWO, bool KEEP, bool MASKED> struct Cursor {
   int rows, row;
   int64_t left;  // positions behind the sample's first one
   __device__ __forceinline__ Cursor(const Inputs& in, const T* dy, int64_t ds, const Shape& s, const Team& g, int64_t b,
-                                    const Place<F>& at)
+                                    int c, const Place<F>& at)
       : x_step(g.rows * in.xs), d_step(g.rows * ds), rows(g.rows), row(at.row), left(s.P) {
-    x = (const T*)in.x + (b * s.P + at.row) * in.xs + at.at;
-    d = TWO ? dy + (b * s.P + at.row) * ds + at.at : nullptr;
+    x = (const T*)in.x + (b * s.P + at.row) * in.xs + c;
+    d = TWO ? dy + (b * s.P + at.row) * ds + c : nullptr;
     mask = MASKED ? in.mask + b * s.P + at.row : nullptr;
   }
   template <int U> __device__ __forceinline__ void load_live(Held<F, U, TWO>& v, int64_t step) const {
@@ -605,14 +608,16 @@ __global__ __launch_bounds__(kThreads) void gn_stats_kernel(Inputs in, double2* 
   __shared__ int row_counts[kThreads];
   const Team& g = p.team;
   const int t = threadIdx.x;
-  const Place<F> at(t, g, s.C);
-  for (int64_t item = blockIdx.x; item < s.B * p.chunks; item += gridDim.x) {
+  const int width = p.groups * s.cg;
+  const Place<F> at(t, g, width);
+  for (int64_t item = blockIdx.x; item < s.B * p.chunks * p.slices; item += gridDim.x) {
     const Chunk k(item, p);
+    const int c = k.g0 * s.cg + at.at;
     double2 sum[F::SL];
 #pragma unroll
     for (int j = 0; j < F::SL; ++j) sum[j] = double2{0, 0};
     int n = 0;
-    for_steps<4, false>(Cursor<F, false, true, MASKED>(in, nullptr, 0, s, g, k.b, at), k, [] {}, [&](auto& v, int j, int64_t) {
+    for_steps<4, false>(Cursor<F, false, true, MASKED>(in, nullptr, 0, s, g, k.b, c, at), k, [] {}, [&](auto& v, int j, int64_t) {
       if (!v.live[j]) return;
       float f[F::VE];
       v.x[j].get(f);
@@ -622,11 +627,11 @@ __global__ __launch_bounds__(kThreads) void gn_stats_kernel(Inputs in, double2* 
     put_sums<F::SL, F::VE>(gn_lds, sum, at.at, at.skip, at.row, at.on, g);
     if (at.first && at.on) row_counts[at.row] = n;
     __syncthreads();
-    sum_runs(gn_lds, s.G, s.cg / F::CPS * g.pitch, t, kThreads, g.lanes,
-             [&](int o, double2 a) { part[(k.b * s.G + o) * p.chunks + k.chunk] = a; });
-    if (MASKED && t < 64) {
+    sum_runs(gn_lds, p.groups, s.cg / F::CPS * g.pitch, t, kThreads, g.lanes,
+             [&](int o, double2 a) { part[(k.b * s.G + k.g0 + o) * p.chunks + k.chunk] = a; });
+    if (MASKED && t < 64 && k.g0 == 0) {
       const int64_t count = sum_counts(row_counts, g.rows, t, 64);
-      if (t == 0) chunk_counts[item] = (int)count;
+      if (t == 0) chunk_counts[k.index] = (int)count;
     }
     __syncthreads();
   }
@@ -643,20 +648,22 @@ __global__ __launch_bounds__(kThreads) void gn_apply_kernel(Inputs in, const dou
   GroupStats* mine = (GroupStats*)gn_lds;
   const Team& g = p.team;
   const int t = threadIdx.x;
-  const Place<F> at(t, g, s.C);
-  for (int64_t item = blockIdx.x; item < s.B * p.chunks; item += gridDim.x) {
+  const int width = p.groups * s.cg;
+  const Place<F> at(t, g, width);
+  for (int64_t item = blockIdx.x; item < s.B * p.chunks * p.slices; item += gridDim.x) {
     const Chunk k(item, p);
-    const Cursor<F, false, false, MASKED> from(in, nullptr, 0, s, g, k.b, at);
-    T* to = y + (k.b * s.P + at.row) * s.C + at.at;
+    const int c = k.g0 * s.cg + at.at;
+    const Cursor<F, false, false, MASKED> from(in, nullptr, 0, s, g, k.b, c, at);
+    T* to = y + (k.b * s.P + at.row) * s.C + c;
     const int64_t y_step = (int64_t)g.rows * s.C;
     ForwardCoefs<F> co;
     auto start = [&]() {
-      const Params<F> params(in.w, in.b, at.at);
+      const Params<F> params(in.w, in.b, c);
       const double inv =
           MASKED ? s.inverse(sum_counts(chunk_counts + k.b * p.chunks, p.chunks, t, g.lanes)) : s.inv;
-      sum_runs<8>(part + k.b * s.G * p.chunks, s.G, p.chunks, t, kThreads, g.lanes, [&](int o, double2 a) {
+      sum_runs<8>(part + (k.b * s.G + k.g0) * p.chunks, p.groups, p.chunks, t, kThreads, g.lanes, [&](int o, double2 a) {
         mine[o] = close_stats(a.x, a.y, inv, eps);
-        if (k.chunk == 0) stats[k.b * s.G + o] = mine[o];
+        if (k.chunk == 0) stats[k.b * s.G + k.g0 + o] = mine[o];
       });
       __syncthreads();
       co.set(mine, params, at.at, s.cg);
@@ -685,26 +692,28 @@ __global__ __launch_bounds__(kThreads) void gn_backward_sums_kernel(Inputs in, c
                                                                     float* __restrict__ channels, Shape s,
                                                                     StreamPlan p) {
   extern __shared__ double2 gn_lds[];
-  float2* weighted = (float2*)gn_lds;  // [C]: a channel's part of its group's sums
-  float2* sums = weighted + s.C;
-  float* weight = (float*)(sums + (int64_t)s.C * p.team.pitch);
+  float2* weighted = (float2*)gn_lds;  // [width]: a channel's part of its group's sums
+  const int width = p.groups * s.cg;
+  float2* sums = weighted + width;
+  float* weight = (float*)(sums + (int64_t)width * p.team.pitch);
   const Team& g = p.team;
   const int t = threadIdx.x;
-  const Place<F> at(t, g, s.C);
-  for (int64_t item = blockIdx.x; item < s.B * p.chunks; item += gridDim.x) {
+  const Place<F> at(t, g, width);
+  for (int64_t item = blockIdx.x; item < s.B * p.chunks * p.slices; item += gridDim.x) {
     const Chunk k(item, p);
+    const int c = k.g0 * s.cg + at.at;
     BackwardCoefs<F, ACT> co;
     float2 sum[F::VE];
 #pragma unroll
     for (int e = 0; e < F::VE; ++e) sum[e] = float2{0.f, 0.f};
     auto start = [&]() {
-      const Params<F> params(in.w, in.b, at.at);
-      co.set(stats + k.b * s.G, params, at.at, s.cg);
+      const Params<F> params(in.w, in.b, c);
+      co.set(stats + k.b * s.G + k.g0, params, at.at, s.cg);
 #pragma unroll
       for (int e = 0; e < F::VE; ++e)
         if (at.row == 0) weight[at.at + e] = params.w[e];
     };
-    for_steps<2, false>(Cursor<F, true, true, MASKED>(in, dy, ds, s, g, k.b, at), k, start, [&](auto& v, int j, int64_t) {
+    for_steps<2, false>(Cursor<F, true, true, MASKED>(in, dy, ds, s, g, k.b, c, at), k, start, [&](auto& v, int j, int64_t) {
       if (!v.live[j]) return;
       float f[F::VE], dz[F::VE];
       v.x[j].get(f);
@@ -718,18 +727,19 @@ __global__ __launch_bounds__(kThreads) void gn_backward_sums_kernel(Inputs in, c
     });
     put_sums<F::VE, F::VE>(sums, sum, at.at, at.skip, at.row, at.on, g);
     __syncthreads();
-    sum_runs(sums, s.C, g.pitch, t, kThreads, g.channel_lanes, [&](int c, float2 a) {
-      if (channels) {
-        channels[item * 2 * s.C + c] = a.x;
-        channels[(item * 2 + 1) * s.C + c] = a.y;
+    float* to = channels ? channels + k.index * 2 * s.C + k.g0 * s.cg : nullptr;
+    sum_runs(sums, width, g.pitch, t, kThreads, g.channel_lanes, [&](int o, float2 a) {
+      if (to) {
+        to[o] = a.x;
+        to[s.C + o] = a.y;
       }
-      const float w = weight[c];
-      weighted[c] = float2{a.y * w, a.x * w};
+      const float w = weight[o];
+      weighted[o] = float2{a.y * w, a.x * w};
     });
     __syncthreads();
     if (part)
-      sum_runs(weighted, s.G, s.cg, t, kThreads, g.lanes,
-               [&](int o, float2 a) { part[(k.b * s.G + o) * p.chunks + k.chunk] = a; });
+      sum_runs(weighted, p.groups, s.cg, t, kThreads, g.lanes,
+               [&](int o, float2 a) { part[(k.b * s.G + k.g0 + o) * p.chunks + k.chunk] = a; });
     __syncthreads();
   }
 }
@@ -748,18 +758,21 @@ __global__ __launch_bounds__(kThreads) void gn_backward_apply_kernel(
   float2* means = (float2*)gn_lds;
   const Team& g = p.team;
   const int t = threadIdx.x;
-  const Place<F> at(t, g, s.C);
-  for (int64_t item = blockIdx.x; item < s.B * p.chunks; item += blocks) {
+  const int width = p.groups * s.cg;
+  const Place<F> at(t, g, width);
+  for (int64_t item = blockIdx.x; item < s.B * p.chunks * p.slices; item += blocks) {
     const Chunk k(item, p);
-    const Cursor<F, true, false, MASKED> from(in, dy, ds, s, g, k.b, at);
-    T* to = dx + (k.b * s.P + at.row) * s.C + at.at;
+    const int c = k.g0 * s.cg + at.at;
+    const Cursor<F, true, false, MASKED> from(in, dy, ds, s, g, k.b, c, at);
+    T* to = dx + (k.b * s.P + at.row) * s.C + c;
     const int64_t dx_step = (int64_t)g.rows * s.C;
     BackwardCoefs<F, ACT> co;
     float2 mean[F::SL];
     auto start = [&]() {
-      co.set(stats + k.b * s.G, Params<F>(in.w, in.b, at.at), at.at, s.cg);
-      sum_runs<8>(part + k.b * s.G * p.chunks, s.G, p.chunks, t, kThreads, g.lanes, [&](int o, float2 a) {
-        const float inv = stats[k.b * s.G + o].inv;
+      const GroupStats* of = stats + k.b * s.G + k.g0;
+      co.set(of, Params<F>(in.w, in.b, c), at.at, s.cg);
+      sum_runs<8>(part + (k.b * s.G + k.g0) * p.chunks, p.groups, p.chunks, t, kThreads, g.lanes, [&](int o, float2 a) {
+        const float inv = of[o].inv;
         means[o] = float2{a.x * inv, a.y * inv};
       });
       __syncthreads();
@@ -784,8 +797,8 @@ __global__ __launch_bounds__(kThreads) void gn_backward_apply_kernel(
 }
 
 // ---------------------------------------------------------------------------
-// Swept: rows of channels that a block's threads do not span.  A block a sample's
-// group, and for the parameters a block a channel.
+// Swept: groups that are wider than a block's threads span.  A block a sample's group,
+// and for the parameters a block a channel.
 // ---------------------------------------------------------------------------
 template <typename T> __device__ __forceinline__ void block_add(T (&v)[3], T (*red)[4]) {
   __syncthreads();
@@ -926,6 +939,9 @@ static Team make_team(int threads, int across, int64_t groups, int64_t channels)
   return t;
 }
 
+// Vectors a thread holds at most: what 256 registers take.
+template <typename F> constexpr int most_held(bool backward) { return !backward ? 16 : F::SL > 2 ? 4 : 8; }
+
 static size_t block_lds(const ResidentPlan& p, int64_t width, bool backward) {
   const size_t sums = p.lds * p.teams;
   return backward ? std::max(sums, (size_t)width * p.pitch * sizeof(float2)) : sums;
@@ -935,7 +951,7 @@ static size_t block_lds(const ResidentPlan& p, int64_t width, bool backward) {
 // bf16 channels in 16-byte pieces: 31 + 36 us, streamed 17 + 24), wider ones as long as
 // they leave four teams a CU.
 template <typename F> static bool plan_resident(const Shape& s, bool backward, ResidentPlan* plan) {
-  const int most = backward ? 8 : 16, cus = device_cus();
+  const int most = most_held<F>(backward), cus = device_cus();
   if (s.P > (int64_t)kThreads * most) return false;
   bool found = false;
   for (int groups = 1; groups <= s.G; ++groups) {
@@ -978,13 +994,19 @@ template <typename F> static bool plan_resident(const Shape& s, bool backward, R
 // adds its sample's partial sums up (2^18 positions of 128 bf16 channels 113 us, with
 // two chunks a CU 123; 2^20 of them 454 and 444).
 template <typename F> static bool plan_streamed(const Shape& s, StreamPlan* p) {
-  const int64_t across = ((int64_t)s.C + F::VE - 1) / F::VE;
-  if (across > kThreads) return false;
-  p->team = make_team(kThreads, (int)across, s.G, s.C);
+  int slices = 1;
+  auto across = [&] { return ((int64_t)(s.G / slices) * s.cg + F::VE - 1) / F::VE; };
+  while (slices < s.G && (s.G % slices || across() > kThreads)) ++slices;
+  const int64_t width = (int64_t)(s.G / slices) * s.cg;
+  if (across() > kThreads || width < F::VE) return false;
+  p->slices = slices;
+  p->groups = s.G / slices;
+  p->team = make_team(kThreads, (int)across(), p->groups, width);
   p->all = (s.P + p->team.rows - 1) / p->team.rows;
   p->whole = s.P / p->team.rows;
   const int64_t cus = device_cus();
-  const int64_t want = std::max<int64_t>(1, (p->all * s.B >= 32 * 2 * cus ? 2 * cus : cus) / s.B);
+  const int64_t samples = s.B * slices;
+  const int64_t want = std::max<int64_t>(1, (p->all * samples >= 32 * 2 * cus ? 2 * cus : cus) / samples);
   p->steps = (p->all + want - 1) / want;
   // whole sets of four steps: what is left over is read step by step (301 x 301
   // positions of 100 fp32 channels, forward: 29 us, with 18 steps instead of 16 31)
@@ -1016,7 +1038,8 @@ template <typename T, typename Fn> static auto for_form(const Shape& s, Fn run) 
 template <int MOST, typename Fn> static void for_held(int held, Fn run) {
   if constexpr (MOST > 8)
     if (held > 8) return run(std::integral_constant<int, 16>());
-  if (held > 4) return run(std::integral_constant<int, 8>());
+  if constexpr (MOST > 4)
+    if (held > 4) return run(std::integral_constant<int, 8>());
   if (held > 2) return run(std::integral_constant<int, 4>());
   if (held > 1) return run(std::integral_constant<int, 2>());
   run(std::integral_constant<int, 1>());
@@ -1062,7 +1085,7 @@ static int launch_gn_forward(const Inputs& in, void* yp, GroupStats* stats, cons
     StageTimer timer("group_norm_forward", st);
     const unsigned blocks = blocks_for((s.B * p.r.slices + p.r.teams - 1) / p.r.teams);
     for_activation(act, [&](auto a) {
-      for_held<16>(p.r.held, [&](auto nv) {
+      for_held<most_held<F>(false)>(p.r.held, [&](auto nv) {
         gn_resident_forward_kernel<F, decltype(nv)::value, decltype(a)::value>
             <<<blocks, p.r.teams * p.r.team.threads, block_lds(p.r, p.r.groups * s.cg, false), st>>>(in, y, stats, s, p.r,
                                                                                                    eps);
@@ -1071,10 +1094,10 @@ static int launch_gn_forward(const Inputs& in, void* yp, GroupStats* stats, cons
   } else if (p.streamed) {
     Carve cv(ws, ws_bytes);
     const ForwardWork<F> work(cv, s, p);
-    const unsigned blocks = blocks_for(s.B * p.t.chunks);
+    const unsigned blocks = blocks_for(s.B * p.t.chunks * p.t.slices);
     {
       StageTimer timer("group_norm_stats", st);
-      const size_t lds = (size_t)(s.C / F::CPS) * p.t.team.pitch * sizeof(double2);
+      const size_t lds = (size_t)(p.t.groups * s.cg / F::CPS) * p.t.team.pitch * sizeof(double2);
       for_mask(in, [&](auto m) {
         gn_stats_kernel<F, decltype(m)::value><<<blocks, kThreads, lds, st>>>(in, work.part, work.counts, s, p.t);
       });
@@ -1084,7 +1107,7 @@ static int launch_gn_forward(const Inputs& in, void* yp, GroupStats* stats, cons
     for_activation(act, [&](auto a) {
       for_mask(in, [&](auto m) {
         gn_apply_kernel<F, decltype(a)::value, decltype(m)::value>
-            <<<blocks, kThreads, s.G * sizeof(GroupStats), st>>>(in, work.part, work.counts, y, stats, s, p.t, eps);
+            <<<blocks, kThreads, p.t.groups * sizeof(GroupStats), st>>>(in, work.part, work.counts, y, stats, s, p.t, eps);
       });
     });
   } else {
@@ -1110,7 +1133,7 @@ static int launch_gn_backward(const Inputs& in, const void* dyp, int64_t ds, con
   if (p.resident) {
     StageTimer timer("group_norm_backward", st);
     for_activation(act, [&](auto a) {
-      for_held<8>(p.r.held, [&](auto nv) {
+      for_held<most_held<F>(true)>(p.r.held, [&](auto nv) {
         gn_resident_backward_kernel<F, decltype(nv)::value, decltype(a)::value>
             <<<(unsigned)p.r.blocks * p.r.slices, kThreads, block_lds(p.r, p.r.groups * s.cg, true), st>>>(
                 in, dy, ds, stats, dx, sums ? work.channels : nullptr, s, p.r);
@@ -1118,10 +1141,10 @@ static int launch_gn_backward(const Inputs& in, const void* dyp, int64_t ds, con
     });
     GTK_LAUNCH_CHECK();
   } else if (p.streamed) {
-    const unsigned blocks = blocks_for(s.B * p.t.chunks);
+    const unsigned blocks = blocks_for(s.B * p.t.chunks * p.t.slices);
     {
       StageTimer timer("group_norm_backward_sums", st);
-      const size_t lds = (size_t)s.C * ((1 + p.t.team.pitch) * sizeof(float2) + sizeof(float));
+      const size_t lds = (size_t)p.t.groups * s.cg * ((1 + p.t.team.pitch) * sizeof(float2) + sizeof(float));
       for_activation(act, [&](auto a) {
         for_mask(in, [&](auto m) {
           gn_backward_sums_kernel<F, decltype(a)::value, decltype(m)::value><<<blocks, kThreads, lds, st>>>(
@@ -1134,7 +1157,7 @@ static int launch_gn_backward(const Inputs& in, const void* dyp, int64_t ds, con
     const unsigned more = sums ? (2 * s.C + 15) / 16 : 0;
     if (dx) {
       StageTimer timer("group_norm_backward_apply", st);
-      const size_t lds = std::max(s.G * sizeof(float2), sums ? kThreads * sizeof(float) : 0);
+      const size_t lds = std::max(p.t.groups * sizeof(float2), sums ? kThreads * sizeof(float) : 0);
       for_activation(act, [&](auto a) {
         for_mask(in, [&](auto m) {
           gn_backward_apply_kernel<F, decltype(a)::value, decltype(m)::value><<<blocks + more, kThreads, lds, st>>>(

@@ -313,7 +313,8 @@ SHAPES = [((1, 1, 1024), 16), ((5, 1, 512), 8), ((3, 1, 7), 1), ((2, 3, 1), 1), 
           ((2, 40, 12), 4), ((3, 64, 16), 16), ((2, 301, 20), 4), ((1, 1000, 32), 32), ((2, 256, 320), 32),
           ((1, 500, 128), 32), ((2, 777, 100), 20), ((1, 900, 1023), 33), ((3, 33, 1030), 2), ((2, 130, 2048), 32),
           ((1, 21, 8), 8), ((2, 1111, 24), 3), ((70, 16, 64), 8), ((1, 5003, 64), 1), ((2, 3001, 40), 5),
-          ((1, 9001, 100), 20), ((1, 4097, 9), 3), ((300, 7, 96), 6)]
+          ((1, 9001, 100), 20), ((1, 4097, 9), 3), ((300, 7, 96), 6), ((1, 600, 5000), 5), ((2, 130, 12288), 64),
+          ((1, 70, 9002), 2), ((1, 3, 20000), 1), ((40, 1, 16384), 16)]
 
 
 @gpu
