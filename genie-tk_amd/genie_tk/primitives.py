@@ -11,6 +11,7 @@ forward and the backward pass on the HIP kernels.  So are ``GroupNorm`` and
 from __future__ import annotations
 
 import math
+import operator
 from typing import List, Optional, Union
 
 import torch
@@ -307,7 +308,7 @@ _U64 = 0xFFFFFFFFFFFFFFFF
 
 def _signed(value: int) -> int:
     """The int64 with the low 64 bits of ``value``."""
-    value &= _U64
+    value = operator.index(value) & _U64
     return value - (1 << 64) if value >> 63 else value
 
 
@@ -337,6 +338,7 @@ def dropout_mask(shape, p: float, seed: Union[int, Tensor], offset: int = 0, sha
     c0 = torch.arange(outer * blocks, device=device)
     c1 = c0 >> 32
     c0 = c0 & _U32
+    offset = operator.index(offset)
     c2, c3 = torch.full_like(c0, offset & _U32), torch.full_like(c0, offset >> 32 & _U32)
     k0, k1 = key & _U32, key >> 32 & _U32
     for _ in range(10):  # products wrap at 64 bits, whose halves are those of unsigned ones
@@ -384,12 +386,14 @@ def dropout(x: Tensor, p: float, seed: Union[int, Tensor], offset: int = 0, shar
         elif (x.dtype in _dispatch.SUPPORTED_DTYPES
               and (residual is None or residual.dtype in _dispatch.SUPPORTED_DTYPES)):
             wide = None if residual is None else residual.to(kind)
-            y = _ext.C.dropout(x, p, 0 if drawn else seed & _U64, offset & _U64, shared_dim, wide,
-                               seed if drawn else None, False)
+            key = 0 if drawn else operator.index(seed) & _U64
+            y = _ext.C.dropout(x, p, key, operator.index(offset) & _U64, shared_dim, wide, seed if drawn else None,
+                               False)
             if y is not None:
                 return y
     wide = torch.promote_types(kind, torch.float32)
     t = round(65536 * p)
     keep = dropout_mask(x.shape, p, seed, offset, shared_dim, x.device)
-    y = torch.where(keep, x.to(wide) * (65536 / (65536 - t) if t < 65536 else 0.0), torch.zeros((), dtype=wide, device=x.device))
+    scaled = x.to(wide) * (65536 / (65536 - t) if t < 65536 else 0.0)
+    y = torch.where(keep, scaled, scaled.new_zeros(()))
     return (y if residual is None else y + residual.to(wide)).to(kind)

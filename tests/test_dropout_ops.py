@@ -487,3 +487,15 @@ def test_pair_stack_trains_with_a_seed(dt):
         # a tie that was broken the other way, carried through the layers
         tol = (2 * half(DT[dt]) if dt == "bf16" else 64 * U) * b.float().abs().max()
         assert (a.float() - b.float()).abs().max() <= tol
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+def test_seeds_and_offsets_of_numpy(device):
+    x = values((6, 5, 24), 31, torch.float32, device)
+    for seed, offset in ((np.int64(-3), np.int32(7)), (np.uint64(SEED), np.uint64(2 ** 63 + 1)), (np.uint8(200), 0)):
+        y = dropout(x, 0.3, seed, offset, 1)
+        assert torch.equal(y, dropout(x, 0.3, int(seed), int(offset), 1))
+        check(y, x, 0.3, int(seed) % 2 ** 64, int(offset), 1)
+    for seed, offset in ((1.5, 0), (1, 0.5), (None, 0)):
+        with pytest.raises(TypeError):
+            dropout(x, 0.3, seed, offset)
