@@ -877,7 +877,8 @@ struct GroupNormArgs {
                                    : GTK_F32;
     if (m.defined()) {
       TORCH_CHECK(m.sizes() == in.sizes().slice(0, in.dim() - 1), "mask must be x's shape without its channels");
-      mask = f32c(m);
+      // what is not 0 stays so
+      mask = f32c(m.scalar_type() == at::kDouble ? m.ne(0) : m);
     }
     x = as_rows(in, &stride);
   }

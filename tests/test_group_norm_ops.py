@@ -619,3 +619,24 @@ def test_captured_step_and_a_run_of_the_operators(shape, G):
             torch.cuda.synchronize()
             assert all(torch.equal(p, q) for p, q in zip(got, refs[k])), k
         values((1000,), 3, torch.float32, "cuda").square().sum().item()
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+def test_a_64_bit_mask_counts_what_is_not_zero(device):
+    """1e-300 is 0 in fp32."""
+    x = values((3, 40, 24), 61, torch.float32, device)
+    mask = some_mask((3, 40), 62, device).double()
+    w, b = params(24, 63, torch.float32, device)
+    y = group_norm(x, 4, w, b, EPS, "silu", mask * 1e-300)
+    assert torch.equal(y, group_norm(x, 4, w, b, EPS, "silu", mask))
+    assert y.count_nonzero() > 0
+
+
+@gpu
+@pytest.mark.parametrize("shape,G", [((2, 3, 10007), 10007), ((2, 700, 10007), 10007), ((1, 5, 20014), 10007),
+                                     ((2, 65, 4099), 1), ((1, 300, 8198), 2)], ids=str)
+def test_prime_numbers_of_groups_and_of_channels(shape, G):
+    x, dy = values(shape, 71, torch.bfloat16, "cuda"), values(shape, 72, torch.bfloat16, "cuda", 0.0)
+    w, b = params(shape[-1], 73, torch.float32, "cuda")
+    y, *grads = run(x, G, w, b, dy, "silu")
+    check_all(x, dy, G, w, b, "silu", None, y, *grads)
