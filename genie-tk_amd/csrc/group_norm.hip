@@ -963,10 +963,11 @@ template <typename F> static bool plan_resident(const Shape& s, bool backward, R
     auto held = [&](int n) { return (s.P + n / across - 1) / (n / across); };
     while (threads < kThreads && held(threads) > most) threads *= 2;
     if (held(threads) > most) break;
-    // A CU takes some 0.25 ns a value (twice that backward): few teams of many values
-    // are slower than two launches over all CUs (1024 positions of 128 bf16 channels in
-    // four teams 10 + 16 us, streamed 9 + 12).
-    if (units < 2 * (int64_t)cus && s.P * width > 32768) break;
+    // A CU takes some 0.15 ns a value (backward 0.4): few teams of many values are slower
+    // than two launches over all CUs.  128 bf16 channels in four teams, backward with the
+    // closing launch: 256 positions 11.4 us, streamed 12.7; 400 positions 13.7, 12.9; 1024
+    // positions 18.7, 12.8, and forward 9.0, 9.5.
+    if (units < 2 * (int64_t)cus && s.P * width > (backward ? 8192 : 32768)) break;
     // more threads where there are few teams
     while (threads < kThreads && held(threads) > 1 && units * threads < 512 * (int64_t)cus) threads *= 2;
     ResidentPlan p;
@@ -994,14 +995,15 @@ template <typename F> static bool plan_resident(const Shape& s, bool backward, R
 // adds its sample's partial sums up (2^18 positions of 128 bf16 channels 113 us, with
 // two chunks a CU 123; 2^20 of them 454 and 444).
 template <typename F> static bool plan_streamed(const Shape& s, StreamPlan* p) {
-  int slices = 1;
-  auto across = [&] { return ((int64_t)(s.G / slices) * s.cg + F::VE - 1) / F::VE; };
-  while (slices < s.G && (s.G % slices || across() > kThreads)) ++slices;
-  const int64_t width = (int64_t)(s.G / slices) * s.cg;
-  if (across() > kThreads || width < F::VE) return false;
+  // the most groups that a block's threads span
+  int64_t groups = std::min<int64_t>(s.G, (int64_t)kThreads * F::VE / s.cg);
+  while (groups > 1 && s.G % groups) --groups;
+  const int64_t width = groups * s.cg;
+  if (groups < 1 || width < F::VE) return false;
+  const int slices = (int)(s.G / groups);
   p->slices = slices;
-  p->groups = s.G / slices;
-  p->team = make_team(kThreads, (int)across(), p->groups, width);
+  p->groups = (int)groups;
+  p->team = make_team(kThreads, (int)((width + F::VE - 1) / F::VE), p->groups, width);
   p->all = (s.P + p->team.rows - 1) / p->team.rows;
   p->whole = s.P / p->team.rows;
   const int64_t cus = device_cus();
