@@ -16,7 +16,8 @@ struct ColumnSums {
 // dst[c] = sum over the partials (c < D: the weight's, else the bias'): the block'th
 // OUTS of the 2 D sums, by CHUNKS threads each, eight loads in flight; red:
 // OUTS * CHUNKS floats.
-template <int OUTS, int CHUNKS> __device__ __forceinline__ void close_columns(const ColumnSums& s, int block, float* red) {
+template <int OUTS, int CHUNKS>
+__device__ __forceinline__ void close_columns(const ColumnSums& s, int block, float* red) {
   const int o = threadIdx.x % OUTS, ch = threadIdx.x / OUTS;
   const int64_t i = (int64_t)block * OUTS + o, n = 2 * (int64_t)s.D;
   void* dst = i < s.D ? s.dw : s.db;

@@ -254,8 +254,8 @@ __global__ __launch_bounds__(256) void dropout_shared_kernel(const typename Y::T
 template <typename Y>
 __global__ __launch_bounds__(256) void dropout_narrow_kernel(const typename Y::TX* __restrict__ x,
                                                              const typename Y::TR* __restrict__ residual,
-                                                             typename Y::TO* __restrict__ out, int64_t shared, int inner,
-                                                             int64_t n, Key key,
+                                                             typename Y::TO* __restrict__ out, int64_t shared,
+                                                             int inner, int64_t n, Key key,
                                                              const uint64_t* __restrict__ seed_device, float scale) {
   constexpr int N = Y::N, K = 8 / N;
   if (seed_device) key.seed = *seed_device;
@@ -366,8 +366,8 @@ extern "C" int gtk_dropout(const void* x, int dtype, const void* residual, int r
   const Key key = Key::of(seed, offset, t);
   auto run = [&](auto res, auto tx, auto to) {
     typedef decltype(to) TO;
-    return launch_dropout<Types<decltype(res)::value, decltype(tx), TO, TO>>(x, residual, out, outer, shared, inner, key,
-                                                                             seed_device, scale, (hipStream_t)stream);
+    return launch_dropout<Types<decltype(res)::value, decltype(tx), TO, TO>>(
+        x, residual, out, outer, shared, inner, key, seed_device, scale, (hipStream_t)stream);
   };
   const std::true_type with;
   const std::false_type without;

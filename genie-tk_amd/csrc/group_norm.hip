@@ -321,8 +321,8 @@ constexpr int kThreads = 512;  // of a block, at most: 256 registers a thread
 
 template <typename F, int NV, int ACT>
 __global__ __launch_bounds__(kThreads) void gn_resident_forward_kernel(Inputs in, typename F::T* __restrict__ y,
-                                                                   GroupStats* __restrict__ stats, Shape s,
-                                                                   ResidentPlan p, float eps) {
+                                                                       GroupStats* __restrict__ stats, Shape s,
+                                                                       ResidentPlan p, float eps) {
   typedef typename F::T T;
   extern __shared__ double2 gn_lds[];
   const Team& g = p.team;
@@ -391,10 +391,9 @@ __global__ __launch_bounds__(kThreads) void gn_resident_forward_kernel(Inputs in
 // dx, and the block's sums of dz h and dz over its samples, part[block of the
 // slice][0 and 1][c].
 template <typename F, int NV, int ACT>
-__global__ __launch_bounds__(kThreads) void gn_resident_backward_kernel(Inputs in, const typename F::T* __restrict__ dy,
-                                                                    int64_t ds, const GroupStats* __restrict__ stats,
-                                                                    typename F::T* __restrict__ dx,
-                                                                    float* __restrict__ part, Shape s, ResidentPlan p) {
+__global__ __launch_bounds__(kThreads) void gn_resident_backward_kernel(
+    Inputs in, const typename F::T* __restrict__ dy, int64_t ds, const GroupStats* __restrict__ stats,
+    typename F::T* __restrict__ dx, float* __restrict__ part, Shape s, ResidentPlan p) {
   typedef typename F::T T;
   extern __shared__ double2 gn_lds[];
   const Team& g = p.team;
@@ -569,7 +568,8 @@ template <typename F, bool TWO, bool KEEP, bool MASKED> struct Cursor {
 // a time while the next U are on their way, and the mask of those behind them;
 // start() runs behind the first loads.
 template <int U, bool BACK, typename F, bool TWO, bool KEEP, bool MASKED, typename Start, typename Use>
-__device__ __forceinline__ void for_steps(const Cursor<F, TWO, KEEP, MASKED>& at, const Chunk& k, Start start, Use use) {
+__device__ __forceinline__ void for_steps(const Cursor<F, TWO, KEEP, MASKED>& at, const Chunk& k, Start start,
+                                          Use use) {
   const int64_t whole = k.whole > k.first ? k.whole - k.first : 0, sets = whole / U;
   Held<F, U, TWO> now, next;
   auto step_of = [&](int64_t i) { return k.first + (BACK ? sets - 1 - i : i) * U; };
@@ -617,7 +617,8 @@ __global__ __launch_bounds__(kThreads) void gn_stats_kernel(Inputs in, double2* 
 #pragma unroll
     for (int j = 0; j < F::SL; ++j) sum[j] = double2{0, 0};
     int n = 0;
-    for_steps<4, false>(Cursor<F, false, true, MASKED>(in, nullptr, 0, s, g, k.b, c, at), k, [] {}, [&](auto& v, int j, int64_t) {
+    const Cursor<F, false, true, MASKED> from(in, nullptr, 0, s, g, k.b, c, at);
+    for_steps<4, false>(from, k, [] {}, [&](auto& v, int j, int64_t) {
       if (!v.live[j]) return;
       float f[F::VE];
       v.x[j].get(f);
@@ -661,7 +662,8 @@ __global__ __launch_bounds__(kThreads) void gn_apply_kernel(Inputs in, const dou
       const Params<F> params(in.w, in.b, c);
       const double inv =
           MASKED ? s.inverse(sum_counts(chunk_counts + k.b * p.chunks, p.chunks, t, g.lanes)) : s.inv;
-      sum_runs<8>(part + (k.b * s.G + k.g0) * p.chunks, p.groups, p.chunks, t, kThreads, g.lanes, [&](int o, double2 a) {
+      const double2* sums = part + (k.b * s.G + k.g0) * p.chunks;
+      sum_runs<8>(sums, p.groups, p.chunks, t, kThreads, g.lanes, [&](int o, double2 a) {
         mine[o] = close_stats(a.x, a.y, inv, eps);
         if (k.chunk == 0) stats[k.b * s.G + k.g0 + o] = mine[o];
       });
@@ -713,7 +715,8 @@ __global__ __launch_bounds__(kThreads) void gn_backward_sums_kernel(Inputs in, c
       for (int e = 0; e < F::VE; ++e)
         if (at.row == 0) weight[at.at + e] = params.w[e];
     };
-    for_steps<2, false>(Cursor<F, true, true, MASKED>(in, dy, ds, s, g, k.b, c, at), k, start, [&](auto& v, int j, int64_t) {
+    const Cursor<F, true, true, MASKED> from(in, dy, ds, s, g, k.b, c, at);
+    for_steps<2, false>(from, k, start, [&](auto& v, int j, int64_t) {
       if (!v.live[j]) return;
       float f[F::VE], dz[F::VE];
       v.x[j].get(f);
@@ -771,7 +774,8 @@ __global__ __launch_bounds__(kThreads) void gn_backward_apply_kernel(
     auto start = [&]() {
       const GroupStats* of = stats + k.b * s.G + k.g0;
       co.set(of, Params<F>(in.w, in.b, c), at.at, s.cg);
-      sum_runs<8>(part + (k.b * s.G + k.g0) * p.chunks, p.groups, p.chunks, t, kThreads, g.lanes, [&](int o, float2 a) {
+      const float2* sums = part + (k.b * s.G + k.g0) * p.chunks;
+      sum_runs<8>(sums, p.groups, p.chunks, t, kThreads, g.lanes, [&](int o, float2 a) {
         const float inv = of[o].inv;
         means[o] = float2{a.x * inv, a.y * inv};
       });
@@ -841,7 +845,8 @@ __global__ __launch_bounds__(256) void gn_swept_forward_kernel(Inputs in, T* __r
     for_values(s, c0, [&](int64_t pos, int c) {
       const bool live = !in.mask || in.mask[first + pos] != 0.f;
       const float h = ((to_f32(x[(first + pos) * in.xs + c]) - g.mean) - g.low) * g.rstd;
-      y[(first + pos) * s.C + c] = cvt<T>(live ? activate<ACT, sizeof(T) == 4>(fmaf(h, in.w.get(c, 1.f), in.b.get(c, 0.f))) : 0.f);
+      const float z = fmaf(h, in.w.get(c, 1.f), in.b.get(c, 0.f));
+      y[(first + pos) * s.C + c] = cvt<T>(live ? activate<ACT, sizeof(T) == 4>(z) : 0.f);
     });
   }
 }
@@ -853,7 +858,8 @@ __device__ __forceinline__ bool swept_backward(const Inputs& in, const T* dy, in
   h = dz = 0.f;
   if (in.mask && in.mask[row] == 0.f) return false;
   h = ((to_f32(((const T*)in.x)[row * in.xs + c]) - g.mean) - g.low) * g.rstd;
-  dz = to_f32(dy[row * ds + c]) * activate_slope<ACT, sizeof(T) == 4>(Slope<ACT>::kScale * fmaf(h, in.w.get(c, 1.f), in.b.get(c, 0.f)));
+  const float z = fmaf(h, in.w.get(c, 1.f), in.b.get(c, 0.f));
+  dz = to_f32(dy[row * ds + c]) * activate_slope<ACT, sizeof(T) == 4>(Slope<ACT>::kScale * z);
   return true;
 }
 
@@ -1081,8 +1087,8 @@ template <typename F> struct BackwardWork {
 };
 
 template <typename F>
-static int launch_gn_forward(const Inputs& in, void* yp, GroupStats* stats, const Shape& s, float eps, int act, void* ws,
-                             size_t ws_bytes, hipStream_t st) {
+static int launch_gn_forward(const Inputs& in, void* yp, GroupStats* stats, const Shape& s, float eps, int act,
+                             void* ws, size_t ws_bytes, hipStream_t st) {
   typedef typename F::T T;
   T* y = (T*)yp;
   const Plan<F> p(s, false);
@@ -1092,8 +1098,8 @@ static int launch_gn_forward(const Inputs& in, void* yp, GroupStats* stats, cons
     for_activation(act, [&](auto a) {
       for_held<most_held<F>(false)>(p.r.held, [&](auto nv) {
         gn_resident_forward_kernel<F, decltype(nv)::value, decltype(a)::value>
-            <<<blocks, p.r.teams * p.r.team.threads, block_lds(p.r, p.r.groups * s.cg, false), st>>>(in, y, stats, s, p.r,
-                                                                                                   eps);
+            <<<blocks, p.r.teams * p.r.team.threads, block_lds(p.r, p.r.groups * s.cg, false), st>>>(in, y, stats, s,
+                                                                                                     p.r, eps);
       });
     });
   } else if (p.streamed) {
@@ -1112,7 +1118,8 @@ static int launch_gn_forward(const Inputs& in, void* yp, GroupStats* stats, cons
     for_activation(act, [&](auto a) {
       for_mask(in, [&](auto m) {
         gn_apply_kernel<F, decltype(a)::value, decltype(m)::value>
-            <<<blocks, kThreads, p.t.groups * sizeof(GroupStats), st>>>(in, work.part, work.counts, y, stats, s, p.t, eps);
+            <<<blocks, kThreads, p.t.groups * sizeof(GroupStats), st>>>(in, work.part, work.counts, y, stats, s, p.t,
+                                                                        eps);
       });
     });
   } else {
@@ -1126,8 +1133,9 @@ static int launch_gn_forward(const Inputs& in, void* yp, GroupStats* stats, cons
 }
 
 template <typename F>
-static int launch_gn_backward(const Inputs& in, const void* dyp, int64_t ds, const GroupStats* stats, void* dxp, void* dw,
-                              void* db, int dst_bf, const Shape& s, int act, void* ws, size_t ws_bytes, hipStream_t st) {
+static int launch_gn_backward(const Inputs& in, const void* dyp, int64_t ds, const GroupStats* stats, void* dxp,
+                              void* dw, void* db, int dst_bf, const Shape& s, int act, void* ws, size_t ws_bytes,
+                              hipStream_t st) {
   typedef typename F::T T;
   const T* dy = (const T*)dyp;
   T* dx = (T*)dxp;
@@ -1179,20 +1187,23 @@ static int launch_gn_backward(const Inputs& in, const void* dyp, int64_t ds, con
     if (dx) {
       StageTimer timer("group_norm_backward", st);
       for_activation(act, [&](auto a) {
-        gn_swept_backward_kernel<T, decltype(a)::value><<<blocks_for(s.B * s.G), 256, 0, st>>>(in, dy, ds, stats, dx, s);
+        gn_swept_backward_kernel<T, decltype(a)::value>
+            <<<blocks_for(s.B * s.G), 256, 0, st>>>(in, dy, ds, stats, dx, s);
       });
       GTK_LAUNCH_CHECK();
     }
     if (sums) {
       StageTimer timer("group_norm_params", st);
       for_activation(act, [&](auto a) {
-        gn_swept_params_kernel<T, decltype(a)::value><<<blocks_for(s.C), 256, 0, st>>>(in, dy, ds, stats, dw, db, dst_bf, s);
+        gn_swept_params_kernel<T, decltype(a)::value>
+            <<<blocks_for(s.C), 256, 0, st>>>(in, dy, ds, stats, dw, db, dst_bf, s);
       });
       GTK_LAUNCH_CHECK();
     }
     return GTK_OK;
   }
-  return sums ? launch_column_close("group_norm_close", work.channels, (int)p.parts(s), s.C, dw, db, dst_bf, st) : GTK_OK;
+  if (!sums) return GTK_OK;
+  return launch_column_close("group_norm_close", work.channels, (int)p.parts(s), s.C, dw, db, dst_bf, st);
 }
 
 static bool gn_shape_ok(int64_t B, int64_t P, int64_t C, int64_t G, int dtype) {

@@ -801,7 +801,8 @@ struct DropoutFn : public torch::autograd::Function<DropoutFn> {
     const auto seed = ctx->get_saved_variables()[0];
     torch::autograd::variable_list out(5);
     if (ctx->needs_input_grad(0))
-      out[0] = dropout_or_grad(dy, c10::nullopt, (at::ScalarType)v[5], seed.defined() ? MaybeTensor(seed) : c10::nullopt, k);
+      out[0] = dropout_or_grad(dy, c10::nullopt, (at::ScalarType)v[5],
+                               seed.defined() ? MaybeTensor(seed) : c10::nullopt, k);
     // an absent residual has no edge to ask about
     const bool residual = ctx->saved_data["has_residual"].toBool();
     if (residual && ctx->needs_input_grad(1))

@@ -640,3 +640,15 @@ def test_prime_numbers_of_groups_and_of_channels(shape, G):
     w, b = params(shape[-1], 73, torch.float32, "cuda")
     y, *grads = run(x, G, w, b, dy, "silu")
     check_all(x, dy, G, w, b, "silu", None, y, *grads)
+
+
+@gpu
+@pytest.mark.parametrize("dt", ["bf16", "fp32"])
+@pytest.mark.parametrize("shape,G", [((3, 5, 4096), 4096), ((2, 900, 4096), 16), ((2, 700, 512), 512),
+                                     ((1, 1200, 4096), 4096), ((2, 16, 2048), 2048), ((2, 700, 4095), 819)], ids=str)
+def test_most_shared_memory(shape, G, dt):
+    """Slices as wide as a block's threads span, groups of one channel: up to 128 KB."""
+    x, dy = values(shape, 81, DT[dt], "cuda"), values(shape, 82, DT[dt], "cuda", 0.0)
+    w, b = params(shape[-1], 83, torch.float32, "cuda")
+    y, *grads = run(x, G, w, b, dy, "silu")
+    check_all(x, dy, G, w, b, "silu", None, y, *grads)
