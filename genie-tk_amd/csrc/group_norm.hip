@@ -15,6 +15,11 @@
 // holds it from its one load to its one store.  Larger samples are streamed twice:
 // one launch sums, the next one applies, in the opposite order, so that what was read
 // last, and is still in the caches, comes first.
+// On MI355X, inputs in rotation, forward and backward with both parameters: 4096 rows of
+// 512 bf16 channels 7 + 18 us, launches' latency; 16 x 256 x 320 fp32 7 + 15; 8 x 4096 x
+// 256 bf16 15 + 24; 2^18 x 128 bf16, a mask of 0.8 of the positions, 39 + 59; 2^20 x 128
+// bf16 with gelu 145 + 260, of which memory takes 131 + 223 (without an activation;
+// twice over 268 MB a tensor at 6 TB/s, the sums' first reading at 5.6).
 #include <math.h>
 
 #include <algorithm>
@@ -493,7 +498,8 @@ __global__ __launch_bounds__(kThreads) void gn_resident_backward_kernel(
 // ---------------------------------------------------------------------------
 struct StreamPlan {
   Team team;
-  int groups, slices, chunks;
+  int groups, slices;
+  int chunks, parts;          // of this launch; of the one that summed
   int64_t steps, all, whole;  // of a chunk; of a sample; those of them that have all their rows
 };
 
@@ -661,9 +667,9 @@ __global__ __launch_bounds__(kThreads) void gn_apply_kernel(Inputs in, const dou
     auto start = [&]() {
       const Params<F> params(in.w, in.b, c);
       const double inv =
-          MASKED ? s.inverse(sum_counts(chunk_counts + k.b * p.chunks, p.chunks, t, g.lanes)) : s.inv;
-      const double2* sums = part + (k.b * s.G + k.g0) * p.chunks;
-      sum_runs<8>(sums, p.groups, p.chunks, t, kThreads, g.lanes, [&](int o, double2 a) {
+          MASKED ? s.inverse(sum_counts(chunk_counts + k.b * p.parts, p.parts, t, g.lanes)) : s.inv;
+      const double2* sums = part + (k.b * s.G + k.g0) * p.parts;
+      sum_runs<8>(sums, p.groups, p.parts, t, kThreads, g.lanes, [&](int o, double2 a) {
         mine[o] = close_stats(a.x, a.y, inv, eps);
         if (k.chunk == 0) stats[k.b * s.G + k.g0 + o] = mine[o];
       });
@@ -774,8 +780,8 @@ __global__ __launch_bounds__(kThreads) void gn_backward_apply_kernel(
     auto start = [&]() {
       const GroupStats* of = stats + k.b * s.G + k.g0;
       co.set(of, Params<F>(in.w, in.b, c), at.at, s.cg);
-      const float2* sums = part + (k.b * s.G + k.g0) * p.chunks;
-      sum_runs<8>(sums, p.groups, p.chunks, t, kThreads, g.lanes, [&](int o, float2 a) {
+      const float2* sums = part + (k.b * s.G + k.g0) * p.parts;
+      sum_runs<8>(sums, p.groups, p.parts, t, kThreads, g.lanes, [&](int o, float2 a) {
         const float inv = of[o].inv;
         means[o] = float2{a.x * inv, a.y * inv};
       });
@@ -954,7 +960,7 @@ static size_t block_lds(const ResidentPlan& p, int64_t width, bool backward) {
 }
 
 // Slices whose rows fill 64-byte pieces of memory (8 samples of 4096 positions and 256
-// bf16 channels in 16-byte pieces: 31 + 36 us, streamed 17 + 24), wider ones as long as
+// bf16 channels forward in 16-byte pieces: 34 us, streamed 15), wider ones as long as
 // they leave four teams a CU.
 template <typename F> static bool plan_resident(const Shape& s, bool backward, ResidentPlan* plan) {
   const int most = most_held<F>(backward), cus = device_cus();
@@ -997,10 +1003,10 @@ template <typename F> static bool plan_resident(const Shape& s, bool backward, R
   return found;
 }
 
-// A chunk a CU, or two of them where they are long: each block of the second launch
-// adds its sample's partial sums up (2^18 positions of 128 bf16 channels 113 us, with
-// two chunks a CU 123; 2^20 of them 454 and 444).
-template <typename F> static bool plan_streamed(const Shape& s, StreamPlan* p) {
+// The launch that sums has a chunk a CU, the one that applies two of them where they are
+// long: each of its blocks adds its sample's partial sums up (2^20 positions of 128 bf16
+// channels 91 + 129 us, with one chunk 94 + 131; 2^18 of them 24 + 34, with two 25 + 37).
+template <typename F> static bool plan_streamed(const Shape& s, bool backward, StreamPlan* p, StreamPlan* apply) {
   // the most groups that a block's threads span
   int64_t groups = std::min<int64_t>(s.G, (int64_t)kThreads * F::VE / s.cg);
   while (groups > 1 && s.G % groups) --groups;
@@ -1014,25 +1020,30 @@ template <typename F> static bool plan_streamed(const Shape& s, StreamPlan* p) {
   p->whole = s.P / p->team.rows;
   const int64_t cus = device_cus();
   const int64_t samples = s.B * slices;
-  const bool lengthy = p->all * samples >= 32 * 2 * cus;
-  const int64_t want = std::max<int64_t>(1, (lengthy ? 2 : 1) * cus / samples);
-  p->steps = (p->all + want - 1) / want;
-  // whole sets of four steps: what is left over is read step by step (301 x 301
-  // positions of 100 fp32 channels, forward: 29 us, with 18 steps instead of 16 31).
-  // Not more blocks than two a CU where that would begin another round (13 samples
-  // of 190 x 190 positions and 169 bf16 channels in 520 blocks 306 us, in 468 250).
-  if (p->steps >= 12) p->steps = lengthy ? (p->steps + 3) / 4 * 4 : p->steps / 4 * 4;
-  p->chunks = (int)((p->all + p->steps - 1) / p->steps);
+  auto split = [&](StreamPlan* p, int64_t blocks) {
+    const int64_t want = std::max<int64_t>(1, blocks / samples);
+    p->steps = (p->all + want - 1) / want;
+    // whole sets of the kernels' steps, the rest is read step by step: more steps, not
+    // fewer, or some CUs would have a chunk more (640 x 640 positions of 128 bf16
+    // channels, 52 + 50 steps a chunk: 155 us in four launches; 48 steps: 214)
+    const int64_t set = backward ? 2 : 4;
+    if (p->steps >= 12) p->steps = (p->steps + set - 1) / set * set;
+    p->chunks = (int)((p->all + p->steps - 1) / p->steps);
+  };
+  split(p, cus);
+  p->parts = p->chunks;
+  *apply = *p;
+  if (p->all * samples >= 64 * cus) split(apply, 2 * cus);
   return true;
 }
 
 template <typename F> struct Plan {
   bool resident, streamed;
   ResidentPlan r;
-  StreamPlan t;
+  StreamPlan t, apply;
   Plan(const Shape& s, bool backward) {
     resident = plan_resident<F>(s, backward, &r);
-    streamed = !resident && plan_streamed<F>(s, &t);
+    streamed = !resident && plan_streamed<F>(s, backward, &t, &apply);
   }
   int64_t parts(const Shape& s) const { return resident ? r.blocks : streamed ? s.B * t.chunks : 0; }
 };
@@ -1115,11 +1126,12 @@ static int launch_gn_forward(const Inputs& in, void* yp, GroupStats* stats, cons
       GTK_LAUNCH_CHECK();
     }
     StageTimer timer("group_norm_apply", st);
+    const unsigned behind = blocks_for(s.B * p.apply.chunks * p.apply.slices);
     for_activation(act, [&](auto a) {
       for_mask(in, [&](auto m) {
         gn_apply_kernel<F, decltype(a)::value, decltype(m)::value>
-            <<<blocks, kThreads, p.t.groups * sizeof(GroupStats), st>>>(in, work.part, work.counts, y, stats, s, p.t,
-                                                                        eps);
+            <<<behind, kThreads, p.t.groups * sizeof(GroupStats), st>>>(in, work.part, work.counts, y, stats, s,
+                                                                        p.apply, eps);
       });
     });
   } else {
@@ -1170,11 +1182,12 @@ static int launch_gn_backward(const Inputs& in, const void* dyp, int64_t ds, con
     const unsigned more = sums ? (2 * s.C + 15) / 16 : 0;
     if (dx) {
       StageTimer timer("group_norm_backward_apply", st);
+      const unsigned behind = blocks_for(s.B * p.apply.chunks * p.apply.slices);
       const size_t lds = std::max(p.t.groups * sizeof(float2), sums ? kThreads * sizeof(float) : 0);
       for_activation(act, [&](auto a) {
         for_mask(in, [&](auto m) {
-          gn_backward_apply_kernel<F, decltype(a)::value, decltype(m)::value><<<blocks + more, kThreads, lds, st>>>(
-              in, dy, ds, stats, work.part, dx, close, (int)blocks, s, p.t);
+          gn_backward_apply_kernel<F, decltype(a)::value, decltype(m)::value><<<behind + more, kThreads, lds, st>>>(
+              in, dy, ds, stats, work.part, dx, close, (int)behind, s, p.apply);
         });
       });
     } else {  // in the same order
