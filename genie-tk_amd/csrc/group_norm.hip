@@ -18,8 +18,8 @@
 // On MI355X, inputs in rotation, forward and backward with both parameters: 4096 rows of
 // 512 bf16 channels 7 + 18 us, launches' latency; 16 x 256 x 320 fp32 7 + 15; 8 x 4096 x
 // 256 bf16 15 + 24; 2^18 x 128 bf16, a mask of 0.8 of the positions, 39 + 59; 2^20 x 128
-// bf16 with gelu 145 + 260, of which memory takes 131 + 223 (without an activation;
-// twice over 268 MB a tensor at 6 TB/s, the sums' first reading at 5.6).
+// bf16 with gelu 139 + 243 to 149 + 268 from card to card, without an activation 131 +
+// 223, memory's time (each tensor of 268 MB twice, at 5.6 to 6.4 TB/s).
 #include <math.h>
 
 #include <algorithm>
