@@ -59,44 +59,34 @@ __device__ __forceinline__ GroupStats close_stats(double s, double q, double inv
 __device__ __forceinline__ float logistic(float z) { return __builtin_amdgcn_rcpf(1.f + __expf(-z)); }
 
 // The standard normal distribution's function below -|z| is e^(-z^2/2) t P(t) with t =
-// 1 / (1 + k |z|), which keeps its relative accuracy to the end; P was fitted to
-// erfcx (weighted least squares on |z| <= 14, iterated towards equal errors).  FINE:
-// 1.5e-7 of the value, 4.4e-7 with fp32's roundings.  For bf16 results, which round by
-// 3.9e-3, three terms fewer are 3.5e-5 off: gelu binds the kernels by its
-// instructions (some 80 % of the cycles issue one).
-template <bool FINE> struct Tail {
+// 1 / (1 + 0.3 |z|), which keeps its relative accuracy to the end; P was fitted to
+// erfcx (weighted least squares on |z| <= 14, iterated towards equal errors): 1.5e-7 of
+// the value, 4.4e-7 with fp32's roundings.  Inputs of bf16 take the same: the
+// parameters' gradients may be fp32 beside them.
+struct Tail {
   float e, tp;  // e^(-z^2/2), t P(t)
-  static constexpr float k = FINE ? 0.3f : 0.38f;
+  static constexpr float k = 0.3f;
   // k |z|, and -z^2 log2(e) / 2
   __device__ __forceinline__ Tail(float size, float power) {
     e = __builtin_amdgcn_exp2f(power);
     const float t = __builtin_amdgcn_rcpf(size + 1.f);
-    float p;
-    if constexpr (FINE) {
-      p = 0.03567477342812997f;
-      p = fmaf(p, t, -0.1572030800704706f);
-      p = fmaf(p, t, 0.20635350232969402f);
-      p = fmaf(p, t, -0.05368364104385134f);
-      p = fmaf(p, t, 0.1285616251824942f);
-      p = fmaf(p, t, 0.09991349247240931f);
-      p = fmaf(p, t, 0.12075395598321578f);
-      p = fmaf(p, t, 0.11962929883230777f);
-    } else {
-      p = -0.08992832869603486f;
-      p = fmaf(p, t, 0.18887642422770945f);
-      p = fmaf(p, t, 0.09197977584781399f);
-      p = fmaf(p, t, 0.157829463361757f);
-      p = fmaf(p, t, 0.15122513768077908f);
-    }
+    float p = 0.03567477342812997f;
+    p = fmaf(p, t, -0.1572030800704706f);
+    p = fmaf(p, t, 0.20635350232969402f);
+    p = fmaf(p, t, -0.05368364104385134f);
+    p = fmaf(p, t, 0.1285616251824942f);
+    p = fmaf(p, t, 0.09991349247240931f);
+    p = fmaf(p, t, 0.12075395598321578f);
+    p = fmaf(p, t, 0.11962929883230777f);
     tp = t * p;
   }
 };
 
 // silu(z) = z s(z); gelu(z) = z Phi(z) = max(z, 0) - |z| Phi(-|z|)
-template <int ACT, bool FINE> __device__ __forceinline__ float activate(float z) {
+template <int ACT> __device__ __forceinline__ float activate(float z) {
   if constexpr (ACT == GTK_ACT_SILU) return z * logistic(z);
   if constexpr (ACT == GTK_ACT_GELU) {
-    const Tail<FINE> a(Tail<FINE>::k * fabsf(z), z * z * -0.7213475204f);
+    const Tail a(Tail::k * fabsf(z), z * z * -0.7213475204f);
     return fmaf(-fabsf(z), a.e * a.tp, fmaxf(z, 0.f));
   }
   return z;
@@ -107,7 +97,7 @@ template <int ACT> struct Slope {
   static constexpr float kScale =
       ACT == GTK_ACT_SILU ? 1.4426950409f : ACT == GTK_ACT_GELU ? 0.8493218003f : 1.f;  // log2(e); sqrt(log2(e) / 2)
 };
-template <int ACT, bool FINE> __device__ __forceinline__ float activate_slope(float u) {
+template <int ACT> __device__ __forceinline__ float activate_slope(float u) {
   if constexpr (ACT == GTK_ACT_SILU) {
     constexpr float ln2 = 0.6931471806f;
     const float s = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-u));
@@ -115,7 +105,7 @@ template <int ACT, bool FINE> __device__ __forceinline__ float activate_slope(fl
   }
   if constexpr (ACT == GTK_ACT_GELU) {
     constexpr float back = 1.f / Slope<ACT>::kScale;
-    const Tail<FINE> a(Tail<FINE>::k * back * fabsf(u), -(u * u));
+    const Tail a(Tail::k * back * fabsf(u), -(u * u));
     const float below = a.e * fmaf(-fabsf(u), 0.3989422804f * back, a.tp);
     return u < 0.f ? below : 1.f - below;
   }
@@ -132,7 +122,6 @@ template <int ACT, bool FINE> __device__ __forceinline__ float activate_slope(fl
 template <typename T_, int VE_, int SL_> struct Form {
   typedef T_ T;
   static constexpr int VE = VE_, SL = SL_, CPS = VE / SL;  // channels a slot
-  static constexpr bool FINE = sizeof(T) == 4;
 };
 
 struct Team {
@@ -262,7 +251,7 @@ template <typename F> struct ForwardCoefs {
   }
   template <int ACT> __device__ __forceinline__ void apply(float* f) const {
 #pragma unroll
-    for (int e = 0; e < F::VE; ++e) f[e] = activate<ACT, F::FINE>(fmaf(f[e] - mean[e / F::CPS], a[e], b[e]));
+    for (int e = 0; e < F::VE; ++e) f[e] = activate<ACT>(fmaf(f[e] - mean[e / F::CPS], a[e], b[e]));
   }
 };
 template <typename F, int ACT> struct BackwardCoefs {
@@ -288,7 +277,7 @@ template <typename F, int ACT> struct BackwardCoefs {
     for (int e = 0; e < F::VE; ++e) {
       const int j = e / F::CPS;
       f[e] = fmaf(f[e] - mean[j], rstd[j], shift[j]);
-      g[e] *= activate_slope<ACT, F::FINE>(fmaf(f[e], a[e], b[e]));
+      g[e] *= activate_slope<ACT>(fmaf(f[e], a[e], b[e]));
     }
   }
   // f = dL/dx of h = f and dz = g; means: of g w and g w h over the group
@@ -852,7 +841,7 @@ __global__ __launch_bounds__(256) void gn_swept_forward_kernel(Inputs in, T* __r
       const bool live = !in.mask || in.mask[first + pos] != 0.f;
       const float h = ((to_f32(x[(first + pos) * in.xs + c]) - g.mean) - g.low) * g.rstd;
       const float z = fmaf(h, in.w.get(c, 1.f), in.b.get(c, 0.f));
-      y[(first + pos) * s.C + c] = cvt<T>(live ? activate<ACT, sizeof(T) == 4>(z) : 0.f);
+      y[(first + pos) * s.C + c] = cvt<T>(live ? activate<ACT>(z) : 0.f);
     });
   }
 }
@@ -865,7 +854,7 @@ __device__ __forceinline__ bool swept_backward(const Inputs& in, const T* dy, in
   if (in.mask && in.mask[row] == 0.f) return false;
   h = ((to_f32(((const T*)in.x)[row * in.xs + c]) - g.mean) - g.low) * g.rstd;
   const float z = fmaf(h, in.w.get(c, 1.f), in.b.get(c, 0.f));
-  dz = to_f32(dy[row * ds + c]) * activate_slope<ACT, sizeof(T) == 4>(Slope<ACT>::kScale * z);
+  dz = to_f32(dy[row * ds + c]) * activate_slope<ACT>(Slope<ACT>::kScale * z);
   return true;
 }
 

@@ -652,3 +652,22 @@ def test_most_shared_memory(shape, G, dt):
     w, b = params(shape[-1], 83, torch.float32, "cuda")
     y, *grads = run(x, G, w, b, dy, "silu")
     check_all(x, dy, G, w, b, "silu", None, y, *grads)
+
+
+@gpu
+@pytest.mark.parametrize("dt", ["bf16", "fp32"])
+@pytest.mark.parametrize("shape,G", [((1, 1, 4096), 16), ((1, 5003, 64), 4), ((3, 300, 96), 8), ((1, 3, 20000), 1)], ids=str)
+def test_gelu_is_as_exact_for_bf16_inputs(shape, G, dt):
+    """bounds() without its allowance for a shorter polynomial.  One position a
+    channel: dbias is one value of dL/dz, with the slope's error and no sum's."""
+    x, dy = values(shape, 91, DT[dt], "cuda"), values(shape, 92, DT[dt], "cuda", 0.0)
+    w, b = params(shape[-1], 93, torch.float32, "cuda")
+    y, dx, dw, db = run(x, G, w, b, dy, "gelu")
+    arg = (np64(x), np64(dy), G, np64(w), np64(b))
+    ey, edx, ew, eb = bounds(*arg, "gelu", None)
+    check(y, train_ops.group_norm(arg[0], *arg[2:], EPS, "gelu")[0], ey, "y")
+    dxr, dwr, dbr, dz = train_ops.group_norm_grads(*arg, EPS, "gelu")
+    if shape[1] == 1:  # without the sum's share
+        eb = eb - CHAIN * U * np.abs(dz).sum((0, 1))
+    for got, ref, err, what in ((dx, dxr, edx, "dx"), (dw, dwr, ew, "dweight"), (db, dbr, eb, "dbias")):
+        check(got, ref, err, what)
