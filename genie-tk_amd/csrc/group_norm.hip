@@ -4,10 +4,11 @@
 // mean(d^2) with d = x - mean, r = 1 / sqrt(var + eps), h = d r, z = h w + b and
 // y = act(z).  Backward, with dz = dy act'(z) and g = dz w:
 //   dx = r (g - mean(g) - h mean(g h)),  dw = sum dz h,  db = sum dz
-// The statistics are sums of x and x^2 in 64 bits: a product of two 32-bit values
-// is exact there, so far from zero as a value lies, the variance loses nothing
-// that matters.  The mean is kept as a sum of two floats, so that d is off by its
-// own rounding only.
+// The statistics are sums of x - x0 and (x - x0)^2 in 64 bits around a value x0 that a
+// thread has itself; threads and chunks are joined by their means and their sums of
+// squares around them.  So the variance is off by 2^-53 of its root times the values'
+// distance from zero, where sums of x^2 lose the square of that distance.  The mean is
+// kept as a sum of two floats, so that d is off by its own rounding only.
 //
 // Memory bounds it: some 15 to 40 operations a value of 2 or 4 bytes.  A sample's
 // group has to be read whole before its first result.  Where a slice of a sample
@@ -37,14 +38,23 @@ struct GroupStats {
   float mean, low, rstd, inv;
 };
 
-// From the sums of the values and of their squares; inv: 1 / their number, 0 without.
-// v_rsq_f64 has 24 bits or more, what the result keeps.
-__device__ __forceinline__ GroupStats close_stats(double s, double q, double inv, float eps) {
+// Some of a group's values: their mean x, and the sum y of their squared distances from it.
+typedef double2 Moments;
+
+// Of n values, from the sums of their distances from x0 and of those squared; inv = 1 / n,
+// or 0 without.
+__device__ __forceinline__ Moments around(double x0, double s, double q, double inv) {
+  const double d = s * inv;
+  return {x0 + d, fma(-d, s, q)};
+}
+
+// inv: as there.  v_rsq_f64 has 24 bits or more, what the result keeps.
+__device__ __forceinline__ GroupStats close_stats(const Moments& m, double inv, float eps) {
   GroupStats g{0.f, 0.f, 0.f, 0.f};
   if (inv > 0) {
-    const double mean = s * inv, var = fma(-mean, mean, q * inv);
-    g.mean = (float)mean;
-    g.low = (float)(mean - (double)g.mean);
+    const double var = m.y * inv;
+    g.mean = (float)m.x;
+    g.low = (float)(m.x - (double)g.mean);
     // a NaN stays one (fmax would drop it)
     g.rstd = (float)__builtin_amdgcn_rsq((var < 0 ? 0.0 : var) + (double)eps);
     g.inv = (float)inv;
@@ -172,6 +182,13 @@ __device__ __forceinline__ void put_sums(S* sums, const S (&v)[N], int at, int s
   }
 }
 
+// The positions that a row of the team counts: its first thread's.
+template <typename P> __device__ __forceinline__ void put_count(int* counts, int n, const P& at, const Team& g) {
+  if (!at.first || !at.on) return;
+  counts[at.row] = n;
+  if (at.row == g.rows - 1 && g.pitch > g.rows) counts[g.rows] = 0;
+}
+
 template <typename S> __device__ __forceinline__ S lanes_sum(S a, int lanes) {
   for (int off = lanes / 2; off; off /= 2) {
     a.x += __shfl_xor(a.x, off, 64);
@@ -198,12 +215,47 @@ __device__ __forceinline__ void sum_runs(const S* sums, int outs, int len, int t
   }
 }
 
-// The sum of `n` counts, in each lane.
-__device__ __forceinline__ int64_t sum_counts(const int* counts, int n, int t, int lanes) {
-  int64_t a = 0;
-  for (int e = t & (lanes - 1); e < n; e += lanes) a += counts[e];
-  for (int off = lanes / 2; off; off /= 2) a += __shfl_xor(a, off, 64);
-  return a;
+// How many positions n entries count, and the first entry that counts any (0 without).
+struct Counted {
+  int64_t positions;
+  int first;
+  // the same in each lane
+  static __device__ __forceinline__ Counted of(const int* counts, int n, int t, int lanes) {
+    Counted a{0, n};
+    for (int e = t & (lanes - 1); e < n; e += lanes) {
+      const int here = counts[e];
+      a.positions += here;
+      if (here && e < a.first) a.first = e;
+    }
+    for (int off = lanes / 2; off; off /= 2) {
+      a.positions += __shfl_xor(a.positions, off, 64);
+      a.first = min(a.first, __shfl_xor(a.first, off, 64));
+    }
+    if (a.first == n) a.first = 0;
+    return a;
+  }
+};
+
+// f(o, the o-th `len` entries joined) for o < outs, as sum_runs, around the mean of entry
+// `first`, which has values (if any has).  of(e): the number of them in entry e.
+template <int U = 4, typename Of, typename Fn>
+__device__ __forceinline__ void join_runs(const Moments* entries, int outs, int len, int first, double inv, int t,
+                                          int threads, int lanes, Of of, Fn f) {
+  const int l = t & (lanes - 1);
+  for (int o = t / lanes; o < outs; o += threads / lanes) {
+    const Moments* from = entries + (int64_t)o * len;
+    const double x0 = from[first].x;
+    double2 a{0, 0};
+#pragma unroll U
+    for (int e = l; e < len; e += lanes) {
+      const Moments m = from[e];
+      const double d = m.x - x0, nd = of(e) * d;
+      a.x += nd;
+      a.y += fma(nd, d, m.y);
+    }
+    a = lanes_sum(a, lanes);
+    if (l == 0) f(o, around(x0, a.x, a.y, inv));
+  }
 }
 
 template <typename F> __device__ __forceinline__ void load_params(float* f, const ParamVec& p, int c, float none) {
@@ -215,22 +267,45 @@ template <typename F> __device__ __forceinline__ void load_params(float* f, cons
   }
 }
 
-// sum += (f, f^2), slot by slot
-template <typename F> __device__ __forceinline__ void add_squares(double2 (&sum)[F::SL], const float* f) {
+// A thread's values, slot by slot, around the first one of each.
+template <typename F> struct Running {
+  float x0[F::SL];
+  double2 sum[F::SL];
+  int n;  // vectors
+  __device__ __forceinline__ Running() : n(0) {
 #pragma unroll
-  for (int e = 0; e < F::VE; ++e) {
-    const double v = f[e];
-    sum[e / F::CPS].x += v;
-    sum[e / F::CPS].y = fma(v, v, sum[e / F::CPS].y);
+    for (int j = 0; j < F::SL; ++j) {
+      x0[j] = 0.f;
+      sum[j] = double2{0, 0};
+    }
   }
-}
+  __device__ __forceinline__ void add(const float* f) {
+#pragma unroll
+    for (int j = 0; j < F::SL; ++j) x0[j] = n ? x0[j] : f[j * F::CPS];
+#pragma unroll
+    for (int e = 0; e < F::VE; ++e) {
+      double2& s = sum[e / F::CPS];
+      const double v = (double)f[e] - (double)x0[e / F::CPS];
+      s.x += v;
+      s.y = fma(v, v, s.y);
+    }
+    ++n;
+  }
+  __device__ __forceinline__ void close(Moments (&m)[F::SL]) const {
+    const double inv = n ? 1.0 / ((double)n * F::CPS) : 0.0;
+#pragma unroll
+    for (int j = 0; j < F::SL; ++j) m[j] = around(x0[j], sum[j].x, sum[j].y, inv);
+  }
+};
 
 // What a thread needs of its groups and channels.  With d = x - mean, exact where x
 // is near the mean: z = d (r w) + (b - low r w), and in the backward pass h = d r -
 // low r, z = h w + b.
 template <typename F> struct Params {
   float w[F::VE], b[F::VE];
-  __device__ __forceinline__ Params(const ParamVec& wp, const ParamVec& bp, int c) {
+  Params() = default;
+  __device__ __forceinline__ Params(const ParamVec& wp, const ParamVec& bp, int c) { load(wp, bp, c); }
+  __device__ __forceinline__ void load(const ParamVec& wp, const ParamVec& bp, int c) {
     load_params<F>(w, wp, c, 1.f);
     load_params<F>(b, bp, c, 0.f);
   }
@@ -324,7 +399,7 @@ __global__ __launch_bounds__(kThreads) void gn_resident_forward_kernel(Inputs in
   const int width = p.groups * s.cg;
   const Place<F> at(t, g, width);
   char* lds = (char*)gn_lds + team * p.lds;
-  double2* sums = (double2*)lds;
+  Moments* sums = (Moments*)lds;
   GroupStats* mine = (GroupStats*)(sums + (int64_t)width / F::CPS * g.pitch);
   int* row_counts = (int*)(mine + p.groups);
   const int64_t units = s.B * p.slices, steps = (units + teams - 1) / teams;
@@ -337,34 +412,39 @@ __global__ __launch_bounds__(kThreads) void gn_resident_forward_kernel(Inputs in
     const int P = (int)s.P;
     Vec<T, F::VE> x[NV];
     bool live[NV];
-    int n = 0;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {  // past the last position that one again
       const int pos = at.row + k * g.rows;
       const int64_t row = b * P + (pos < P ? pos : P - 1);
       x[k].load((const T*)in.x + row * in.xs + c);
       live[k] = at.on && pos < P && (!in.mask || in.mask[row] != 0.f);
-      n += live[k];
     }
-    const Params<F> params(in.w, in.b, c);
-    double2 sum[F::SL];
-#pragma unroll
-    for (int j = 0; j < F::SL; ++j) sum[j] = double2{0, 0};
+    constexpr bool LATE = F::SL > 4 && NV > 8;  // 256 registers do not hold them beside the sums
+    Params<F> params;
+    if (!LATE) params.load(in.w, in.b, c);
+    Running<F> sum;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
       float f[F::VE];
       x[k].get(f);
-      if (live[k]) add_squares<F>(sum, f);
+      if (live[k]) sum.add(f);
     }
-    put_sums<F::SL, F::VE>(sums, sum, at.at, at.skip, at.row, at.on, g);
-    if (at.first && at.on) row_counts[at.row] = n;
+    Moments own[F::SL];
+    sum.close(own);
+    put_sums<F::SL, F::VE>(sums, own, at.at, at.skip, at.row, at.on, g);
+    put_count(row_counts, sum.n, at, g);
     __syncthreads();
-    const double inv = in.mask ? s.inverse(sum_counts(row_counts, g.rows, t, g.lanes)) : s.inv;
-    sum_runs(sums, p.groups, s.cg / F::CPS * g.pitch, t, g.threads, g.lanes, [&](int o, double2 a) {
-      mine[o] = close_stats(a.x, a.y, inv, eps);
-      if (any) stats[b * s.G + slice * p.groups + o] = mine[o];
-    });
+    Counted counted{P, 0};
+    if (in.mask) counted = Counted::of(row_counts, g.rows, t, g.lanes);
+    const double inv = in.mask ? s.inverse(counted.positions) : s.inv;
+    join_runs(sums, p.groups, s.cg / F::CPS * g.pitch, counted.first, inv, t, g.threads, g.lanes,
+              [&](int e) { return (double)row_counts[(unsigned)e % (unsigned)g.pitch] * F::CPS; },
+              [&](int o, const Moments& m) {
+                mine[o] = close_stats(m, inv, eps);
+                if (any) stats[b * s.G + slice * p.groups + o] = mine[o];
+              });
     __syncthreads();
+    if (LATE) params.load(in.w, in.b, c);
     ForwardCoefs<F> co;
     co.set(mine, params, at.at, s.cg);
 #pragma unroll
@@ -597,10 +677,10 @@ __device__ __forceinline__ void for_steps(const Cursor<F, TWO, KEEP, MASKED>& at
 
 // part[b][group][chunk], counts[b][chunk]
 template <typename F, bool MASKED>
-__global__ __launch_bounds__(kThreads) void gn_stats_kernel(Inputs in, double2* __restrict__ part,
+__global__ __launch_bounds__(kThreads) void gn_stats_kernel(Inputs in, Moments* __restrict__ part,
                                                             int* __restrict__ chunk_counts, Shape s, StreamPlan p) {
   extern __shared__ double2 gn_lds[];
-  __shared__ int row_counts[kThreads];
+  __shared__ int row_counts[kThreads + 1];
   const Team& g = p.team;
   const int t = threadIdx.x;
   const int width = p.groups * s.cg;
@@ -608,33 +688,30 @@ __global__ __launch_bounds__(kThreads) void gn_stats_kernel(Inputs in, double2* 
   for (int64_t item = blockIdx.x; item < s.B * p.chunks * p.slices; item += gridDim.x) {
     const Chunk k(item, p);
     const int c = k.g0 * s.cg + at.at;
-    double2 sum[F::SL];
-#pragma unroll
-    for (int j = 0; j < F::SL; ++j) sum[j] = double2{0, 0};
-    int n = 0;
+    Running<F> sum;
     const Cursor<F, false, true, MASKED> from(in, nullptr, 0, s, g, k.b, c, at);
     for_steps<4, false>(from, k, [] {}, [&](auto& v, int j, int64_t) {
       if (!v.live[j]) return;
       float f[F::VE];
       v.x[j].get(f);
-      add_squares<F>(sum, f);
-      ++n;
+      sum.add(f);
     });
-    put_sums<F::SL, F::VE>(gn_lds, sum, at.at, at.skip, at.row, at.on, g);
-    if (at.first && at.on) row_counts[at.row] = n;
+    Moments own[F::SL];
+    sum.close(own);
+    put_sums<F::SL, F::VE>(gn_lds, own, at.at, at.skip, at.row, at.on, g);
+    put_count(row_counts, sum.n, at, g);
     __syncthreads();
-    sum_runs(gn_lds, p.groups, s.cg / F::CPS * g.pitch, t, kThreads, g.lanes,
-             [&](int o, double2 a) { part[(k.b * s.G + k.g0 + o) * p.chunks + k.chunk] = a; });
-    if (MASKED && t < 64 && k.g0 == 0) {
-      const int64_t count = sum_counts(row_counts, g.rows, t, 64);
-      if (t == 0) chunk_counts[k.index] = (int)count;
-    }
+    const Counted counted = Counted::of(row_counts, g.rows, t, g.lanes);
+    join_runs(gn_lds, p.groups, s.cg / F::CPS * g.pitch, counted.first, s.inverse(counted.positions), t, kThreads,
+              g.lanes, [&](int e) { return (double)row_counts[(unsigned)e % (unsigned)g.pitch] * F::CPS; },
+              [&](int o, const Moments& m) { part[(k.b * s.G + k.g0 + o) * p.chunks + k.chunk] = m; });
+    if (t == 0 && k.g0 == 0) chunk_counts[k.index] = (int)counted.positions;
     __syncthreads();
   }
 }
 
 template <typename F, int ACT, bool MASKED>
-__global__ __launch_bounds__(kThreads) void gn_apply_kernel(Inputs in, const double2* __restrict__ part,
+__global__ __launch_bounds__(kThreads) void gn_apply_kernel(Inputs in, const Moments* __restrict__ part,
                                                             const int* __restrict__ chunk_counts,
                                                             typename F::T* __restrict__ y,
                                                             GroupStats* __restrict__ stats, Shape s, StreamPlan p,
@@ -655,13 +732,16 @@ __global__ __launch_bounds__(kThreads) void gn_apply_kernel(Inputs in, const dou
     ForwardCoefs<F> co;
     auto start = [&]() {
       const Params<F> params(in.w, in.b, c);
-      const double inv =
-          MASKED ? s.inverse(sum_counts(chunk_counts + k.b * p.parts, p.parts, t, g.lanes)) : s.inv;
-      const double2* sums = part + (k.b * s.G + k.g0) * p.parts;
-      sum_runs<8>(sums, p.groups, p.parts, t, kThreads, g.lanes, [&](int o, double2 a) {
-        mine[o] = close_stats(a.x, a.y, inv, eps);
-        if (k.chunk == 0) stats[k.b * s.G + k.g0 + o] = mine[o];
-      });
+      const int* counts = chunk_counts + k.b * p.parts;
+      Counted counted{s.P, 0};
+      if (MASKED) counted = Counted::of(counts, p.parts, t, g.lanes);
+      const double inv = MASKED ? s.inverse(counted.positions) : s.inv;
+      join_runs<8>(part + (k.b * s.G + k.g0) * p.parts, p.groups, p.parts, counted.first, inv, t, kThreads, g.lanes,
+                   [&](int e) { return (double)counts[e] * s.cg; },
+                   [&](int o, const Moments& m) {
+                     mine[o] = close_stats(m, inv, eps);
+                     if (k.chunk == 0) stats[k.b * s.G + k.g0 + o] = mine[o];
+                   });
       __syncthreads();
       co.set(mine, params, at.at, s.cg);
     };
@@ -827,15 +907,20 @@ __global__ __launch_bounds__(256) void gn_swept_forward_kernel(Inputs in, T* __r
     const int64_t first = bg / s.G * s.P;
     const int c0 = (int)(bg % s.G) * s.cg;
     double v[3] = {0, 0, 0};
+    float x0 = 0.f;  // the first channel's value at the first position that counts
     for_values(s, c0, [&](int64_t pos, int c) {
       if (in.mask && in.mask[first + pos] == 0.f) return;
-      const double f = to_f32(x[(first + pos) * in.xs + c]);
-      v[0] += f;
-      v[1] += f * f;
+      const T* row = x + (first + pos) * in.xs;
+      if (v[2] == 0) x0 = to_f32(row[c0]);
+      const double d = (double)to_f32(row[c]) - (double)x0;
+      v[0] += d;
+      v[1] = fma(d, d, v[1]);
       v[2] += 1;
     });
     block_add(v, red);
-    const GroupStats g = close_stats(v[0], v[1], v[2] > 0 ? 1.0 / v[2] : 0.0, eps);
+    const double inv = v[2] > 0 ? 1.0 / v[2] : 0.0;
+    // threads without a channel have no x0, nor a use for it
+    const GroupStats g = close_stats(around(x0, v[0], v[1], inv), inv, eps);
     if (threadIdx.x == 0) stats[bg] = g;
     for_values(s, c0, [&](int64_t pos, int c) {
       const bool live = !in.mask || in.mask[first + pos] != 0.f;
@@ -977,8 +1062,8 @@ template <typename F> static bool plan_resident(const Shape& s, bool backward, R
     p.groups = groups;
     p.slices = s.G / groups;
     p.lds = backward ? (groups + width / F::CPS * p.team.pitch) * sizeof(float2)
-                     : width / F::CPS * p.team.pitch * sizeof(double2) + groups * sizeof(GroupStats) +
-                           p.team.rows * sizeof(int);
+                     : width / F::CPS * p.team.pitch * sizeof(Moments) + groups * sizeof(GroupStats) +
+                           p.team.pitch * sizeof(int);
     p.lds = (p.lds + 15) & ~size_t(15);
     p.teams = (backward ? kThreads : std::max(256, threads)) / threads;
     // two blocks a CU: each leaves 2 C partial sums
@@ -1070,10 +1155,10 @@ template <typename Fn> static void for_activation(int act, Fn run) {
 static unsigned blocks_for(int64_t items) { return (unsigned)std::min<int64_t>(items, kMostBlocks); }
 
 template <typename F> struct ForwardWork {
-  double2* part;
+  Moments* part;
   int* counts;
   ForwardWork(Carve& cv, const Shape& s, const Plan<F>& p) {
-    part = cv.take<double2>(p.streamed ? s.B * s.G * p.t.chunks : 0);
+    part = cv.take<Moments>(p.streamed ? s.B * s.G * p.t.chunks : 0);
     counts = cv.take<int>(p.streamed ? s.B * p.t.chunks : 0);
   }
 };
@@ -1108,7 +1193,7 @@ static int launch_gn_forward(const Inputs& in, void* yp, GroupStats* stats, cons
     const unsigned blocks = blocks_for(s.B * p.t.chunks * p.t.slices);
     {
       StageTimer timer("group_norm_stats", st);
-      const size_t lds = (size_t)(p.t.groups * s.cg / F::CPS) * p.t.team.pitch * sizeof(double2);
+      const size_t lds = (size_t)(p.t.groups * s.cg / F::CPS) * p.t.team.pitch * sizeof(Moments);
       for_mask(in, [&](auto m) {
         gn_stats_kernel<F, decltype(m)::value><<<blocks, kThreads, lds, st>>>(in, work.part, work.counts, s, p.t);
       });

@@ -671,3 +671,93 @@ def test_gelu_is_as_exact_for_bf16_inputs(shape, G, dt):
         eb = eb - CHAIN * U * np.abs(dz).sum((0, 1))
     for got, ref, err, what in ((dx, dxr, edx, "dx"), (dw, dwr, ew, "dweight"), (db, dbr, eb, "dbias")):
         check(got, ref, err, what)
+
+
+def plain_reference(x, dy, G, w, b, mask=None, narrow=False):
+    """(y, dx, dweight, dbias) without an activation in 64 bits, on x's device, and
+    their bounds: those of the module's first lines, but that the statistics are joined
+    from sums around values of the group itself.  With M the group's largest |x| and
+    s = 1 / r its spread, the mean is then off by CHAIN 2^-53 M and the variance by
+    CHAIN 2^-53 (s^2 + s M), so h by eh = 8 u |h| + k (1 + |h|), k = (4 u^2 + CHAIN
+    2^-53) M r: of the first order in M, not of the second.  narrow: sums of 32 bits
+    over x - m1, m1 the mean in 32 bits (off by CHAIN u M, which leaves CHAIN u^2 M in
+    the differences' rounding), and again over what is left: k = CHAIN u (1 + u M r)."""
+    B, C = x.shape[0], x.shape[-1]
+    split = (B, -1, G, C // G)
+    xd, dyd = x.double().reshape(split), dy.double().reshape(split)
+    live = torch.ones_like(xd[..., :1, :1], dtype=torch.bool) if mask is None else (mask != 0).reshape(B, -1, 1, 1)
+    zero = torch.zeros((), dtype=torch.float64, device=x.device)
+    only = lambda t: torch.where(live, t, zero)  # noqa: E731
+    xd, dyd = only(xd), only(dyd)
+    count = (live.sum(1, keepdim=True) * (C // G)).clamp(min=1)
+    mean = lambda t: t.sum((1, 3), keepdim=True) / count  # noqa: E731
+    d = only(xd - mean(xd))
+    d = only(d - mean(d))
+    r = (mean(d * d) + EPS).rsqrt()
+    h = d * r
+    wd, bd = w.double().view(G, -1), b.double().view(G, -1)
+    M = xd.abs().amax((1, 3), keepdim=True)
+    k = CHAIN * U * (1 + U * M * r) if narrow else (4 * U * U + CHAIN * 2.0 ** -53) * M * r
+    eh = only(8 * U * h.abs() + k * (1 + h.abs()))
+    y = only(h * wd + bd)
+    ey = wd.abs() * eh + 2 * U * (h.abs() * wd.abs() + bd.abs())
+    g = dyd * wd
+    eg = 2 * U * g.abs()
+    c1, c2 = mean(g), mean(g * h)
+    ec1 = mean(eg) + CHAIN * U * mean(g.abs())
+    ec2 = mean(eg * h.abs() + g.abs() * eh) + CHAIN * U * mean((g * h).abs())
+    er = 2 * U + k
+    dx = only(r * (g - c1 - h * c2))
+    edx = r * (eg + ec1 + h.abs() * ec2 + eh * c2.abs() + (er + 4 * U) * (g.abs() + c1.abs() + h.abs() * c2.abs()))
+    dw, db = (dyd * h).sum((0, 1)), dyd.sum((0, 1))
+    ew = (dyd.abs() * eh).sum((0, 1)) + CHAIN * U * (dyd * h).abs().sum((0, 1))
+    eb = CHAIN * U * dyd.abs().sum((0, 1))
+    return (y, dx, dw, db), (ey, edx, ew, eb)
+
+
+def check_plain(got, refs, errs, what):
+    for name, t, ref, err in zip(("y", "dx", "dweight", "dbias"), got, refs, errs):
+        t64 = t.detach().double().reshape(ref.shape)
+        excess = (t64 - ref).abs() - (half(t.dtype) * ref.abs() + (1 + half(t.dtype)) * err + 1e-36)
+        assert bool((excess <= 0).all()), (what, name, int((excess > 0).sum()), excess.numel(), excess.max().item())
+
+
+@gpu
+@pytest.mark.parametrize("shape,G", [((3, 60, 24), 4), ((2, 6000, 64), 8), ((2, 3001, 20), 4), ((70, 1, 512), 8),
+                                     ((1, 33, 4101), 1), ((2, 3, 5), 5)], ids=str)
+def test_values_far_from_zero(shape, G):
+    """The statistics do not lose what the values' distance from zero takes of the
+    squares, whatever part is masked, the first positions among it."""
+    C = shape[-1]
+    w, b = params(C, 102, torch.float32, "cuda")
+    dy = values(shape, 101, torch.float32, "cuda", 0.0)
+    late = some_mask(shape[:2], 103, "cuda")
+    late[:, :shape[1] // 3] = 0
+    for mean, spread in ((1e5, 0.01), (1e6, 0.1), (1e6, 1.0), (-1e3, 1e-3), (9.5e4, 0.0), (8.4e5, 0.0), (0.0, 1.0)):
+        x = (mean + spread * values(shape, 100, torch.float64, mean=0.0)).float().cuda()
+        for mask in (None, late):
+            case = (shape, G, mean, spread, mask is not None)
+            print("far from zero", *case, flush=True)
+            if mask is None:
+                seen = x
+            else:
+                seen = torch.where(mask.unsqueeze(-1) != 0, x, float("nan"))
+            check_plain(run(seen, G, w, b, dy, None, mask), *plain_reference(x, dy, G, w, b, mask), case)
+    # a constant in bf16, and one value far from the others in the first place
+    x = torch.full(shape, 94720.0, dtype=torch.bfloat16, device="cuda")
+    check_plain(run(x, G, w, b, dy.bfloat16()), *plain_reference(x, dy.bfloat16(), G, w, b), "constant")
+    x = values(shape, 100, torch.float32, "cuda")
+    x[:, 0] = 1e4
+    check_plain(run(x, G, w, b, dy), *plain_reference(x, dy, G, w, b), "first")
+
+
+@gpu
+@pytest.mark.parametrize("dt", ["bf16", "fp32"])
+@pytest.mark.parametrize("shape,G", [((20000, 40, 40), 8), ((9000, 100, 24), 3), ((30001, 12, 33), 11)], ids=str)
+def test_many_small_samples(shape, G, dt):
+    """Teams of a few threads with up to 16 vectors each, also of eight groups' channels."""
+    x, dy = values(shape, 105, DT[dt], "cuda"), values(shape, 106, DT[dt], "cuda", 0.0)
+    w, b = params(shape[-1], 107, torch.float32, "cuda")
+    for mask in (None, some_mask(shape[:2], 108, "cuda", empty=True)):
+        got = run(x, G, w, b, dy, None, mask)
+        check_plain(got, *plain_reference(x, dy, G, w, b, mask), (shape, G, dt, mask is not None))
