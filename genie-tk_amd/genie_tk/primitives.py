@@ -209,25 +209,29 @@ def _group_norm_pytorch(x: Tensor, num_groups: int, weight: Optional[Tensor], bi
     P = math.prod(x.shape[1:-1])  # also where another size is 0
     xf = x.to(wide).reshape(B, P, num_groups, C // num_groups)
     if mask is None:
-        var, mean = torch.var_mean(xf, (1, 3), correction=0, keepdim=True)
-        d = xf - mean
+        live, count = None, max(P * xf.shape[3], 1)
     else:
         live = (mask != 0).reshape(B, P, 1, 1)
-        zero = xf.new_zeros(())
-        xf = torch.where(live, xf, zero)
-        count = (live.sum((1, 2, 3), keepdim=True) * xf.shape[3]).clamp(min=1).to(wide)
-        d = torch.where(live, xf - xf.sum((1, 3), keepdim=True) / count, zero)
-        var = d.square().sum((1, 3), keepdim=True) / count
-    y = d * torch.rsqrt(var + eps)
+        count = (live.sum((1, 2, 3), keepdim=True) * xf.shape[3]).clamp(min=1)
+
+    def only(v: Tensor) -> Tensor:
+        return v if live is None else torch.where(live, v, v.new_zeros(()))
+
+    def mean(v: Tensor) -> Tensor:
+        return (v.sum((1, 3), keepdim=True, dtype=torch.float64) / count).to(wide)
+
+    # the mean is rounded by its own size; what is left of it, by the values' spread
+    d = only(xf)
+    d = only(d - mean(d))
+    d = only(d - mean(d))
+    y = d * torch.rsqrt(mean(d.square()) + eps)
     if weight is not None:
         y = y * weight.to(wide).view(num_groups, -1)
     if bias is not None:
         y = y + bias.to(wide).view(num_groups, -1)
     if activation is not None:
         y = F.silu(y) if activation == "silu" else F.gelu(y)
-    if mask is not None:
-        y = torch.where(live, y, zero)
-    return y.to(x.dtype).reshape(x.shape)
+    return only(y).to(x.dtype).reshape(x.shape)
 
 
 def group_norm(x: Tensor, num_groups: int, weight: Optional[Tensor] = None, bias: Optional[Tensor] = None,

@@ -761,3 +761,18 @@ def test_many_small_samples(shape, G, dt):
     for mask in (None, some_mask(shape[:2], 108, "cuda", empty=True)):
         got = run(x, G, w, b, dy, None, mask)
         check_plain(got, *plain_reference(x, dy, G, w, b, mask), (shape, G, dt, mask is not None))
+
+
+@pytest.mark.parametrize("masked", [False, True])
+@pytest.mark.parametrize("far", [10.0, 100.0, 1e4])
+def test_pytorch_path_far_from_zero(far, masked):
+    """A mean that is rounded to fp32 once is off by u of itself; what is left of it in
+    x - mean is taken off there."""
+    shape = (1, 20000, 8)
+    x, dy = values(shape, 110, torch.float32, mean=0.0) + far, values(shape, 111, torch.float32, mean=0.0)
+    w, b = params(8, 112, torch.float32)
+    mask = None
+    if masked:
+        mask = some_mask(shape[:2], 113)
+        mask[:, :500] = 0
+    check_plain(run(x, 2, w, b, dy, None, mask), *plain_reference(x, dy, 2, w, b, mask, True), far)
