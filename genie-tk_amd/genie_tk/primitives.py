@@ -139,6 +139,14 @@ class Attention(nn.Module):
         return self.linear_o(o)
 
 
+def _autocast_fp32(x: Tensor, *params: Optional[Tensor]) -> List[Optional[Tensor]]:
+    """What torch's autocast makes of a norm's arguments on the GPU."""
+    if not (x.is_cuda and torch.is_autocast_enabled("cuda")):
+        return [x, *params]
+    return [t.float() if t is not None and t.is_floating_point() and t.dtype != torch.float64 else t
+            for t in (x, *params)]
+
+
 def layer_norm(x: Tensor, weight: Optional[Tensor] = None, bias: Optional[Tensor] = None,
                eps: float = 1e-5) -> Tensor:
     """LayerNorm over the last dimension of ``x`` with optional ``weight`` and
@@ -153,9 +161,7 @@ def layer_norm(x: Tensor, weight: Optional[Tensor] = None, bias: Optional[Tensor
     forward-mode tangent, run torch's LayerNorm.  Under autocast GPU tensors
     narrower than fp32 are taken to fp32 first, as torch's LayerNorm takes them,
     and so is the output."""
-    if x.is_cuda and torch.is_autocast_enabled("cuda"):
-        x, weight, bias = (t.float() if t is not None and t.is_floating_point() and t.dtype != torch.float64 else t
-                           for t in (x, weight, bias))
+    x, weight, bias = _autocast_fp32(x, weight, bias)
     params = [p for p in (weight, bias) if p is not None]
     if x.is_cuda:
         if _ext.C is None or not torch.cuda.is_available():
@@ -266,9 +272,7 @@ def group_norm(x: Tensor, num_groups: int, weight: Optional[Tensor] = None, bias
             raise ValueError(f"group_norm: {name} must be [{C}], got {tuple(p.shape)}")
     if mask is not None:
         mask = mask.detach().expand(x.shape[:-1])
-    if x.is_cuda and torch.is_autocast_enabled("cuda"):
-        x, weight, bias = (t.float() if t is not None and t.is_floating_point() and t.dtype != torch.float64 else t
-                           for t in (x, weight, bias))
+    x, weight, bias = _autocast_fp32(x, weight, bias)
     if x.is_cuda:
         if _ext.C is None or not torch.cuda.is_available():
             _ext.missing("group_norm")
@@ -303,7 +307,8 @@ class GroupNorm(nn.GroupNorm):
             return group_norm(x, self.num_groups, self.weight, self.bias, self.eps, self.activation, mask)
         if mask is not None:
             mask = mask.detach().expand(x.shape[:-1])
-        return _group_norm_pytorch(x, self.num_groups, self.weight, self.bias, self.eps, self.activation, mask)
+        x, weight, bias = _autocast_fp32(x, self.weight, self.bias)
+        return _group_norm_pytorch(x, self.num_groups, weight, bias, self.eps, self.activation, mask)
 
 
 _U32 = 0xFFFFFFFF

@@ -776,3 +776,20 @@ def test_pytorch_path_far_from_zero(far, masked):
         mask = some_mask(shape[:2], 113)
         mask[:, :500] = 0
     check_plain(run(x, 2, w, b, dy, None, mask), *plain_reference(x, dy, 2, w, b, mask, True), far)
+
+
+@gpu
+def test_autocast_without_the_kernels():
+    """use_fused_kernel=False changes the path, not the type."""
+    x = values((2, 30, 24), 121, torch.bfloat16, "cuda")
+    mask = some_mask((2, 30), 122, "cuda")
+    for dtype in (torch.float32, torch.bfloat16):
+        m = GroupNorm(4, 24, activation="silu", device="cuda", dtype=dtype)
+        u = GroupNorm(4, 24, activation="silu", device="cuda", dtype=dtype, use_fused_kernel=False)
+        u.load_state_dict(m.state_dict())
+        for live in (None, mask):
+            with torch.autocast("cuda", dtype=torch.bfloat16):
+                one, two = m(x, live), u(x, live)
+            assert one.dtype == two.dtype == torch.float32
+            torch.testing.assert_close(one, two, rtol=1e-5, atol=1e-5)
+            assert u(x, live).dtype == torch.bfloat16
