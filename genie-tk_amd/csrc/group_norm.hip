@@ -1040,11 +1040,13 @@ template <typename F> static bool plan_resident(const Shape& s, bool backward, R
   const int most = most_held<F>(backward), cus = device_cus();
   if (s.P > (int64_t)kThreads * most) return false;
   bool found = false;
-  for (int groups = 1; groups <= s.G; ++groups) {
+  // the most groups that a block's threads span
+  const int64_t span = std::min<int64_t>(s.G, (int64_t)kThreads * F::VE / s.cg);
+  for (int groups = 1; groups <= span; ++groups) {
     const int64_t width = (int64_t)groups * s.cg;
     if (s.G % groups || width < F::VE || (groups < s.G && width * (int64_t)sizeof(typename F::T) < 64)) continue;
     const int64_t across = (width + F::VE - 1) / F::VE, units = s.B * (s.G / groups);
-    if (across > kThreads || (found && units < 4 * (int64_t)cus)) break;
+    if (found && units < 4 * (int64_t)cus) break;
     int threads = pow2_up(across);
     auto held = [&](int n) { return (s.P + n / across - 1) / (n / across); };
     while (threads < kThreads && held(threads) > most) threads *= 2;

@@ -793,3 +793,18 @@ def test_autocast_without_the_kernels():
             assert one.dtype == two.dtype == torch.float32
             torch.testing.assert_close(one, two, rtol=1e-5, atol=1e-5)
             assert u(x, live).dtype == torch.bfloat16
+
+
+def test_plans_of_many_groups_are_found_at_once(lib):
+    """Each call plans anew: no walk over all of 2^24 numbers of groups."""
+    import time
+    for name in ("gtk_group_norm_workspace_size", "gtk_group_norm_backward_workspace_size"):
+        for groups in (16777213, 1 << 24, 10007, 3):  # prime, a power of two, prime
+            size = getattr(lib, name)
+            size(2, 3, groups, groups, 1)
+            times = []
+            for _ in range(5):
+                t = time.perf_counter()
+                size(2, 3, groups, groups, 1)
+                times.append(time.perf_counter() - t)
+            assert min(times) < 2e-3, (name, groups, times)
