@@ -202,6 +202,7 @@ class LayerNorm(nn.LayerNorm):
 
 # the codes of genie_tk._C's group norm
 _ACTIVATIONS = {None: 0, "silu": 1, "gelu": 2}
+_GROUP_NORM_CHANNELS = 1 << 24  # what its kernels take
 
 
 def _group_norm_pytorch(x: Tensor, num_groups: int, weight: Optional[Tensor], bias: Optional[Tensor], eps: float,
@@ -253,11 +254,11 @@ def group_norm(x: Tensor, num_groups: int, weight: Optional[Tensor] = None, bias
     count: elsewhere the output and dL/dx are 0, whatever x and dL/dy hold there.  A
     sample without any is all 0.
 
-    Kernel path (bf16 or fp32 GPU tensor, parameters in bf16 or fp32, also mixed):
-    ``genie_tk._C.group_norm``.  The output and dL/dx have the type of ``x``, the
-    parameters' gradients their own; sums and statistics are held in fp32 or more.
-    Positions that lie one stride apart (a slice of wider channels) are read as they
-    are.  Other tensors, and those with a forward-mode tangent, run the same formula
+    Kernel path (bf16 or fp32 GPU tensor of up to 2^24 channels, parameters in bf16 or
+    fp32, also mixed): ``genie_tk._C.group_norm``.  The output and dL/dx have the type
+    of ``x``, the parameters' gradients their own; sums and statistics are held in fp32
+    or more.  Positions that lie one stride apart (a slice of wider channels) are read
+    as they are.  Other tensors, and those with a forward-mode tangent, run the same formula
     in PyTorch.  Under autocast GPU tensors narrower than fp32 are taken to fp32
     first, as torch's group norm takes them, and so is the output."""
     if x.dim() < 2:
@@ -276,7 +277,7 @@ def group_norm(x: Tensor, num_groups: int, weight: Optional[Tensor] = None, bias
     if x.is_cuda:
         if _ext.C is None or not torch.cuda.is_available():
             _ext.missing("group_norm")
-        elif (x.dtype in _dispatch.SUPPORTED_DTYPES
+        elif (x.dtype in _dispatch.SUPPORTED_DTYPES and C <= _GROUP_NORM_CHANNELS
               and all(p is None or p.dtype in _dispatch.SUPPORTED_DTYPES for p in (weight, bias))):
             y = _ext.C.group_norm(x, num_groups, weight, bias, eps, _ACTIVATIONS[activation], mask, False)
             if y is not None:

@@ -808,3 +808,18 @@ def test_plans_of_many_groups_are_found_at_once(lib):
                 size(2, 3, groups, groups, 1)
                 times.append(time.perf_counter() - t)
             assert min(times) < 2e-3, (name, groups, times)
+
+
+@gpu
+def test_more_channels_than_the_kernels_take():
+    """They run the PyTorch path, as layer_norm's do."""
+    C = (1 << 24) + 2
+    x = values((1, 2, C), 131, torch.bfloat16, "cuda", 0.0).requires_grad_(True)
+    y = group_norm(x, 3, activation="silu")
+    dx, = torch.autograd.grad(y, x, torch.ones_like(y))
+    with torch.no_grad():
+        xf = x.double().view(2, 3, -1)
+        d = xf - xf.mean((0, 2), keepdim=True)
+        ref = F.silu(d * (d.square().mean((0, 2), keepdim=True) + EPS).rsqrt()).view(1, 2, C)
+    assert y.dtype == dx.dtype == torch.bfloat16 and torch.isfinite(dx).all()
+    assert ((y.double() - ref).abs() <= half(y.dtype) * ref.abs() + 1e-5 * (1 + ref.abs())).all()
