@@ -92,17 +92,21 @@ struct Tail {
   }
 };
 
-// silu(z) = z s(z); gelu(z) = z Phi(z) = max(z, 0) - |z| Phi(-|z|)
+constexpr float kLargest = 3.402823466e38f;
+
+// silu(z) = z s(z); gelu(z) = z Phi(z) = max(z, 0) - |z| Phi(-|z|), whose last product is 0
+// at an infinite z too
 template <int ACT> __device__ __forceinline__ float activate(float z) {
   if constexpr (ACT == GTK_ACT_SILU) return z * logistic(z);
   if constexpr (ACT == GTK_ACT_GELU) {
     const Tail a(Tail::k * fabsf(z), z * z * -0.7213475204f);
-    return fmaf(-fabsf(z), a.e * a.tp, fmaxf(z, 0.f));
+    return fmaf(-fminf(fabsf(z), kLargest), a.e * a.tp, fmaxf(z, 0.f));
   }
   return z;
 }
 // silu' = s + z s (1 - s); gelu' = Phi(z) + z phi(z), 1 - that of -z.  The argument is
-// kScale z, which the coefficients of z carry: one product less a value.
+// kScale z, which the coefficients of z carry: one product less a value.  Of SiLU's it may
+// be infinite where z is not.
 template <int ACT> struct Slope {
   static constexpr float kScale =
       ACT == GTK_ACT_SILU ? 1.4426950409f : ACT == GTK_ACT_GELU ? 0.8493218003f : 1.f;  // log2(e); sqrt(log2(e) / 2)
@@ -111,7 +115,7 @@ template <int ACT> __device__ __forceinline__ float activate_slope(float u) {
   if constexpr (ACT == GTK_ACT_SILU) {
     constexpr float ln2 = 0.6931471806f;
     const float s = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-u));
-    return s * fmaf(u, fmaf(-s, ln2, ln2), 1.f);
+    return s * fmaf(__builtin_amdgcn_fmed3f(u, -kLargest, kLargest), fmaf(-s, ln2, ln2), 1.f);
   }
   if constexpr (ACT == GTK_ACT_GELU) {
     constexpr float back = 1.f / Slope<ACT>::kScale;

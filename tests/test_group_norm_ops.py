@@ -823,3 +823,29 @@ def test_more_channels_than_the_kernels_take():
         ref = F.silu(d * (d.square().mean((0, 2), keepdim=True) + EPS).rsqrt()).view(1, 2, C)
     assert y.dtype == dx.dtype == torch.bfloat16 and torch.isfinite(dx).all()
     assert ((y.double() - ref).abs() <= half(y.dtype) * ref.abs() + 1e-5 * (1 + ref.abs())).all()
+
+
+@gpu
+@pytest.mark.parametrize("dt", ["bf16", "fp32"])
+@pytest.mark.parametrize("P", [30, 5000])
+def test_activations_of_the_largest_arguments(P, dt):
+    """gelu(inf) = inf, as silu's and torch's; and the slope of a finite z is finite."""
+    C = 16
+    x, dy = values((2, P, C), 141, DT[dt], "cuda"), values((2, P, C), 142, DT[dt], "cuda")
+    w, b = params(C, 143, torch.float32, "cuda")
+    far = b.clone()
+    far[3] = float("inf")
+    for act in ("silu", "gelu"):
+        y = group_norm(x, 4, w, far, EPS, act)
+        rest = torch.arange(C, device="cuda") != 3
+        assert (y[..., 3] == float("inf")).all()
+        assert torch.equal(y[..., rest], group_norm(x, 4, w, b, EPS, act)[..., rest])
+    for value in (3e38, -3e38):
+        far[3] = value
+        for act in ("silu", "gelu"):
+            y, dx, dw, db = run(x, 4, w, far, dy, act)
+            slope = 1.0 if value > 0 else 0.0
+            assert torch.equal(y[..., 3], torch.full_like(y[..., 3], max(value, 0.0)))
+            assert torch.isfinite(dx).all() and torch.isfinite(dw).all() and torch.isfinite(db).all()
+            ref = slope * np64(dy)[..., 3].sum()
+            assert abs(db[3].item() - ref) <= (half(torch.float32) + CHAIN * U) * np.abs(np64(dy)[..., 3]).sum()
