@@ -343,7 +343,8 @@ def dropout_mask(shape, p: float, seed: Union[int, Tensor], offset: int = 0, sha
         device = seed.device if device is None else device
         key = seed.detach().reshape(1).to(device)
     else:
-        key = torch.tensor([_signed(seed)], device=device)
+        # a fill, which a captured graph may hold
+        key = torch.full((1,), _signed(seed), dtype=torch.int64, device=device)
     blocks = (inner + 7) // 8
     c0 = torch.arange(outer * blocks, device=device)
     c1 = c0 >> 32

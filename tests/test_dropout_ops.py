@@ -499,3 +499,20 @@ def test_seeds_and_offsets_of_numpy(device):
     for seed, offset in ((1.5, 0), (1, 0.5), (None, 0)):
         with pytest.raises(TypeError):
             dropout(x, 0.3, seed, offset)
+
+
+@gpu
+def test_the_pytorch_path_in_a_captured_step():
+    """64-bit values have no kernel; a seed that is a number is no copy from the host."""
+    x = values((4, 30), 51, torch.float64, "cuda")
+    ref = dropout(x, 0.25, 9, 1)
+    assert torch.equal(ref.cpu(), dropout(x.cpu(), 0.25, 9, 1))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = dropout(x, 0.25, 9, 1)
+    for _ in range(3):
+        y.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, ref)
+        values((1000,), 3, torch.float32, "cuda").square().sum().item()
