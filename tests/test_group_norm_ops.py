@@ -849,3 +849,90 @@ def test_activations_of_the_largest_arguments(P, dt):
             assert torch.isfinite(dx).all() and torch.isfinite(dw).all() and torch.isfinite(db).all()
             ref = slope * np64(dy)[..., 3].sum()
             assert abs(db[3].item() - ref) <= (half(torch.float32) + CHAIN * U) * np.abs(np64(dy)[..., 3]).sum()
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+@pytest.mark.parametrize("act", [None, "silu", "gelu"])
+@pytest.mark.parametrize("shape,G", [((2, 400, 24), 4), ((1, 6000, 16), 2)], ids=str)
+def test_gradients_against_differences_along_themselves(shape, G, act, device):
+    """Along the signs of a gradient nothing cancels: the derivative is sum |g|, and
+    what differences leave open is a small part of it.  With D(t) the central difference
+    at step t, off by c t^2 + O(t^4), (4 D(t / 2) - D(t)) / 3 is off by O(t^4), below
+    |D(t) - D(t / 2)|; the losses' roundings (y is off by 16 u (1 + |y|) or less) add their sum over t."""
+    x, dy = values(shape, 151, torch.float32, device, 0.0), values(shape, 152, torch.float32, device, 0.0)
+    w, b = params(shape[-1], 153, torch.float32, device)
+    mask = some_mask(shape[:2], 154, device)
+    y, *grads = run(x, G, w, b, dy, act, mask)
+    y = y.detach()
+    loss = lambda *a: float((group_norm(a[0], G, *a[1:], EPS, act, mask).double() * dy.double()).sum())  # noqa: E731
+    round_off = 16 * U * float((dy.double().abs() * (1 + y.double().abs())).sum())
+    t = 2.0 ** -5
+    for k, g in enumerate(grads):
+        def central(step):
+            at = [[s * step * g.sign() if j == k else 0.0 for j in range(3)] for s in (1, -1)]
+            hi, lo = (loss(*(p + d for p, d in zip((x, w, b), ds))) for ds in at)
+            return (hi - lo) / (2 * step)
+        whole, halved = central(t), central(t / 2)
+        size = float(g.double().abs().sum())
+        allowed = abs(whole - halved) + 2 * round_off / t + CHAIN * U * size
+        assert allowed < 0.03 * size, (k, allowed, size)
+        assert abs((4 * halved - whole) / 3 - size) <= allowed, (k, whole, halved, size)
+
+
+@gpu
+@pytest.mark.parametrize("masked", [False, True])
+@pytest.mark.parametrize("shape,G,dt", [((1, 17000 * 32 + 5, 128), 32, "bf16"), ((2, 8300 * 32 + 7, 128), 8, "bf16"),
+                                        ((1, 16500 * 81 + 80, 24), 4, "fp32"), ((3, 5600 * 34 + 33, 60), 12, "fp32")], ids=str)
+def test_second_launches_with_chunks_of_their_own(shape, G, dt, masked):
+    """Long samples: the launch that applies has more chunks than the one that sums, at
+    512 threads and 256 CUs from 16384 steps of 512 / (vectors of a row) positions on."""
+    x = torch.empty(shape, device="cuda")
+    x.normal_(generator=torch.Generator("cuda").manual_seed(161)).mul_(1.5).add_(0.5)
+    dy = torch.empty(shape, device="cuda").normal_(generator=torch.Generator("cuda").manual_seed(162))
+    x, dy = x.to(DT[dt]), dy.to(DT[dt])
+    w, b = params(shape[-1], 163, torch.float32, "cuda")
+    mask = None
+    if masked:
+        mask = (torch.rand(shape[:2], device="cuda", generator=torch.Generator("cuda").manual_seed(164)) < 0.8).float()
+        mask[:, shape[1] * 9 // 10:] = 0
+        mask[0, :70000] = 0
+    got = run(x, G, w, b, dy, None, mask)
+    check_plain(got, *plain_reference(x, dy, G, w, b, mask), (shape, dt, masked))
+    again = run(x, G, w, b, dy, None, mask)
+    assert all(torch.equal(p, q) for p, q in zip(got, again))
+
+
+@gpu
+def test_gradients_of_more_than_2_to_the_31_values():
+    """[1, P, 64] with 2^31 + 64 * 999 values: x and dL/dy have a period of 4096 positions
+    and a tail of ones and zeros, so one period gives every sum."""
+    P, C, G, many = (1 << 25) + 999, 64, 4, 1 << 13
+    period, up = (values((4096, C), k, torch.bfloat16, "cuda", m) for k, m in ((171, 1.0), (172, 0.0)))
+    w, b = params(C, 173, torch.float32, "cuda")
+    x = torch.ones(1, P, C, dtype=torch.bfloat16, device="cuda")
+    dy = torch.zeros(1, P, C, dtype=torch.bfloat16, device="cuda")
+    for t, one in ((x, period), (dy, up)):
+        t[0, :1 << 25].view(many, 4096, C).copy_(one)
+    _, dx, dw, db = run(x, G, w, b, dy)
+    n, d, wn = np64(period), np64(up), np64(w)
+    cg, total = C // G, P * (C // G)
+    spread = lambda t: np.repeat(t, cg)  # noqa: E731
+    grouped = lambda t: t.reshape(-1, G, cg).sum((0, 2))  # noqa: E731
+    mean = (grouped(n) * many + 999 * cg) / total
+    var = (grouped((n - spread(mean)) ** 2) * many + 999 * cg * (1 - mean) ** 2) / total
+    r = spread(1 / np.sqrt(var + EPS))
+    h, tail = (n - spread(mean)) * r, (1 - spread(mean)) * r
+    g = d * wn
+    c1, c2 = spread(grouped(g) * many / total), spread(grouped(g * h) * many / total)
+    # a thread adds some 2^25 / 64 / 256 positions up, one behind the other
+    chain = 2048 + CHAIN
+    ec1 = spread(grouped(np.abs(g)) * many / total) * chain * U
+    ec2 = spread(grouped(np.abs(g * h)) * many / total) * chain * U
+    for at in (0, 1 << 24, (1 << 25) - 4096):
+        ref = r * (g - c1 - h * c2)
+        err = r * (ec1 + np.abs(h) * ec2 + 32 * U * (np.abs(g) + np.abs(c1) + np.abs(h * c2)))
+        check(dx[0, at:at + 4096], ref, err, ("dx", at))
+    ref = np.broadcast_to(r * (-c1 - tail * c2), (999, C))
+    check(dx[0, 1 << 25:], ref, r * (ec1 + np.abs(tail) * ec2 + 32 * U * (np.abs(c1) + np.abs(tail * c2))), "the tail")
+    check(dw, (d * h).sum(0) * many, (chain + 16) * U * np.abs(d * h).sum(0) * many, "dweight")
+    check(db, d.sum(0) * many, chain * U * np.abs(d).sum(0) * many, "dbias")
