@@ -17,10 +17,11 @@
 // one launch sums, the next one applies, in the opposite order, so that what was read
 // last, and is still in the caches, comes first.
 // On MI355X, inputs in rotation, forward and backward with both parameters: 4096 rows of
-// 512 bf16 channels 7 + 18 us, launches' latency; 16 x 256 x 320 fp32 7 + 15; 8 x 4096 x
-// 256 bf16 15 + 24; 2^18 x 128 bf16, a mask of 0.8 of the positions, 39 + 59; 2^20 x 128
-// bf16 with gelu 139 + 243 to 149 + 268 from card to card, without an activation 131 +
-// 223, memory's time (each tensor of 268 MB twice, at 5.6 to 6.4 TB/s).
+// 512 bf16 channels 8 + 19 us, of which a launch by itself is 3.4 (two block barriers a
+// row, the backward pass' partial sums); 16 x 256 x 320 fp32 8 + 14; 8 x 4096 x 256 bf16
+// 17 + 24; 2^18 x 128 bf16, 36 % of the positions masked, 41 + 61; 2^20 x 128 bf16 with
+// gelu 161 + 274, without an activation 138 + 219, memory's time (each tensor of 268 MB
+// twice, at 5.1 to 6.6 TB/s).
 #include <math.h>
 
 #include <algorithm>
@@ -1038,7 +1039,7 @@ static size_t block_lds(const ResidentPlan& p, int64_t width, bool backward) {
 }
 
 // Slices whose rows fill 64-byte pieces of memory (8 samples of 4096 positions and 256
-// bf16 channels forward in 16-byte pieces: 34 us, streamed 15), wider ones as long as
+// bf16 channels forward in 16-byte pieces: 33 us, streamed 17), wider ones as long as
 // they leave four teams a CU.
 template <typename F> static bool plan_resident(const Shape& s, bool backward, ResidentPlan* plan) {
   const int most = most_held<F>(backward), cus = device_cus();
@@ -1058,7 +1059,7 @@ template <typename F> static bool plan_resident(const Shape& s, bool backward, R
     // A CU takes some 0.15 ns a value (backward 0.4): few teams of many values are slower
     // than two launches over all CUs.  128 bf16 channels in four teams, backward with the
     // closing launch: 256 positions 11.4 us, streamed 12.7; 400 positions 13.7, 12.9; 1024
-    // positions 18.7, 12.8, and forward 9.0, 9.5.
+    // positions 18.7, 12.8, and forward 10.2, 10.6.
     if (units < 2 * (int64_t)cus && s.P * width > (backward ? 8192 : 32768)) break;
     // more threads where there are few teams
     while (threads < kThreads && held(threads) > 1 && units * threads < 512 * (int64_t)cus) threads *= 2;
@@ -1085,7 +1086,8 @@ template <typename F> static bool plan_resident(const Shape& s, bool backward, R
 
 // The launch that sums has a chunk a CU, the one that applies two of them where they are
 // long: each of its blocks adds its sample's partial sums up (2^20 positions of 128 bf16
-// channels 91 + 129 us, with one chunk 94 + 131; 2^18 of them 24 + 34, with two 25 + 37).
+// channels without an activation 85 + 123 us, with one chunk 81 + 131; 2^18 of them with
+// silu 24 + 36, with two 25 + 38).
 template <typename F> static bool plan_streamed(const Shape& s, bool backward, StreamPlan* p, StreamPlan* apply) {
   // the most groups that a block's threads span
   int64_t groups = std::min<int64_t>(s.G, (int64_t)kThreads * F::VE / s.cg);
@@ -1105,7 +1107,7 @@ template <typename F> static bool plan_streamed(const Shape& s, bool backward, S
     p->steps = (p->all + want - 1) / want;
     // whole sets of the kernels' steps, the rest is read step by step: more steps, not
     // fewer, or some CUs would have a chunk more (640 x 640 positions of 128 bf16
-    // channels, 52 + 50 steps a chunk: 155 us in four launches; 48 steps: 214)
+    // channels forward, 52 steps a chunk: 60 us in two launches; 48 steps: 80)
     const int64_t set = backward ? 2 : 4;
     if (p->steps >= 12) p->steps = (p->steps + set - 1) / set * set;
     p->chunks = (int)((p->all + p->steps - 1) / p->steps);

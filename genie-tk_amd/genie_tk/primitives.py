@@ -379,8 +379,9 @@ def dropout(x: Tensor, p: float, seed: Union[int, Tensor], offset: int = 0, shar
 
     Kernel path (bf16 and fp32 GPU tensors): ``genie_tk._C.dropout``, differentiable
     any number of times.  Other tensors, and those with a forward-mode tangent, run
-    the same formula in PyTorch.  Whether a module is training is the caller's to
-    ask."""
+    the same formula in PyTorch, where the product is rounded to fp32 before the sum:
+    the kernel has one fused multiply-add, so a sum in the middle between two results
+    may go to the other one.  Whether a module is training is the caller's to ask."""
     if not 0.0 <= p <= 1.0:
         raise ValueError(f"dropout probability has to be between 0 and 1, but got {p}")
     if shared_dim is not None and not -x.dim() <= shared_dim < x.dim():

@@ -453,8 +453,9 @@ int gtk_grad_clip_with_norm(const gtk_tensor_list* grads, const gtk_tensor_list*
  * and `offset` (high 64 bits) under the key `seed`.  So p is taken to a multiple
  * of 2^-16, and the scale is that multiple's; t = 65536 drops everything.  A
  * dropped value counts for nothing, also where it is not finite.  The product
- * and the sum are fp32, rounded once to out's type.  The backward pass is the
- * same call without residual on dL/dout.
+ * (with the scale in fp32) and the sum are one fused multiply-add in fp32, whose
+ * result is rounded to out's type.  The backward pass is the same call without
+ * residual on dL/dout.
  * seed_device: NULL, or one value on the device that replaces `seed` when the
  * kernel runs (a captured graph draws a new mask at each replay).
  * Types (x, residual, out): without residual any pair of GTK_F32 and GTK_BF16;
